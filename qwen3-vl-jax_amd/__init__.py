@@ -8,8 +8,8 @@ from . import capi
 from .vision import (GridMetadata, Qwen3VisionTransformer, Qwen3VLModel, Qwen3VLSpec, VisionBackboneSpec,
                      VisionEmbeddings, attention_worklist_split, grid_metadata, random_params, spec_2b, spec_8b,
                      spec_from_config, vision_spec_from_config)
-from . import decoder_io, preprocess, vision, weights
+from . import decoder_attn, decoder_io, preprocess, vision, weights
 
 __all__ = ["capi", "GridMetadata", "Qwen3VisionTransformer", "Qwen3VLModel", "Qwen3VLSpec", "VisionBackboneSpec",
            "VisionEmbeddings", "attention_worklist_split", "grid_metadata", "random_params", "spec_2b", "spec_8b",
-           "spec_from_config", "vision_spec_from_config", "decoder_io", "preprocess", "weights"]
+           "spec_from_config", "vision_spec_from_config", "decoder_attn", "decoder_io", "preprocess", "weights"]

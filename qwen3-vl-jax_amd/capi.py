@@ -1,4 +1,5 @@
-"""ctypes binding of libqvl.so (the C ABI declared in include/qvl_vision.h).
+"""ctypes binding of libqvl.so (the C ABI declared in include/qvl_vision.h and
+include/qvl_decoder.h).
 
 Loading fails loudly when the library was not built: there is no CPU or eager fallback.
 """
@@ -81,7 +82,10 @@ class VisionMetadataDev(C.Structure):
                 ("n_positions", _i64)]
 
 
-# name -> (restype, argtypes); every function in include/qvl_vision.h
+_view = [_p, _i64, _i64]   # a [rows, heads, head_dim] view: pointer, row and head stride
+_pi64 = C.POINTER(_i64)
+
+# name -> (restype, argtypes); every function in include/qvl_vision.h and include/qvl_decoder.h
 SIGNATURES = {
     "qvl_last_error": (C.c_char_p, []),
     "qvl_status_string": (C.c_char_p, [C.c_int]),
@@ -146,6 +150,16 @@ SIGNATURES = {
     "qvl_vision_positions": (C.c_int, [_p, _p, _i64, _i64, _i32, _i64, _p, _p]),
     "qvl_scatter_vision_rows": (C.c_int, [_p, _i32, _i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _i64, _p, _p]),
     "qvl_scatter_flagged_rows": (C.c_int, [_p, _i32, _i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _i64, _i32, _p, _i32]),
+    "qvl_text_rotary_table": (C.c_int, [_i32, C.c_double, _pi32, _i32, _p]),
+    "qvl_qk_norm_rotary": (C.c_int, [_p, _i32, *_view, *_view, *_view, _p, _p, _f32, _p, _i64, _p, _p, _i64, *_view,
+                                     *_view, *_view, _i64, _i32, _i32, _i32]),
+    "qvl_causal_worklist": (C.c_int, [_i64, _pi64, _pi64, _pi64, _i32, _i32, _i32, _i32, _i32, _pi32, _i64, _pi64, _pi64]),
+    "qvl_causal_workspace_size": (C.c_int, [_i32, _i64, _i64, C.POINTER(_sz)]),
+    "qvl_causal_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _p, _i64, _i64, _f32, *_view, _i64, _i32,
+                                       _i32, _i32, _p, _sz]),
+    "qvl_decode_workspace_size": (C.c_int, [_i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "qvl_decode_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
+                                       _i64, _f32, *_view, _i64, _i32, _i32, _i32, _p, _sz]),
 }
 
 

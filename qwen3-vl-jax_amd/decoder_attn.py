@@ -1,0 +1,313 @@
+"""What a text decoder layer computes between its qkv Dense and its output Dense, on the GPU.
+
+After `decoder_io.inject_vision` a prompt's hidden rows go through the decoder's layers. In each of them, on torch device
+tensors [rows, heads, head_dim] (any row and head strides of whole 16 bytes), float32 or bfloat16:
+
+    rotary = TextRotary.from_spec(spec.text)                             # once
+    plan = CausalPlan(q_lens, k_lens, k_starts, num_heads=..., ...)      # once per prefill, for all layers
+    q, k_cache, v_cache = qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary, k_cache=k_cache, v_cache=v_cache,
+                                         rows=rows)
+    out = causal_attention(q, k_cache, v_cache, plan)                    # the prompt
+    out = decode_attention(q, k_cache, v_cache, k_start, k_len, max_len=...)       # then token by token
+    out = prefix_attention(q, k_cache, v_cache, k_start, k_len, prefix_start, prefix_len, cu_groups, max_len=...,
+                           max_prefix=...)                               # where sequences share an image's tokens
+
+Everything runs on the tensors' device and its current stream; nothing synchronises. Workspaces come from torch's
+allocator with every call, so calls on several streams and captured graphs share none.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+import numpy as np
+
+from . import capi
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _qdtype(dtype):
+    torch = _torch()
+    if dtype == torch.bfloat16:
+        return capi.QVL_DTYPE_BF16
+    if dtype == torch.float32:
+        return capi.QVL_DTYPE_F32
+    raise TypeError(f"unsupported dtype {dtype} (bfloat16 or float32)")
+
+
+def _device(device):
+    torch = _torch()
+    d = torch.device(device)
+    if d.type != "cuda":
+        raise ValueError(f"device {d}: the decoder operators run on the GPU")
+    return torch.device("cuda", torch.cuda.current_device()) if d.index is None else d
+
+
+def _heads_view(t, what: str, like=None, heads: Optional[int] = None, written: bool = False):
+    """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor, checked against `like`."""
+    if t.dim() != 3:
+        raise ValueError(f"{what} must be [rows, heads, head_dim], not {tuple(t.shape)}")
+    rows, n, dim = t.shape
+    row, head, one = t.stride()
+    if dim > 1 and one != 1:
+        raise ValueError(f"{what}: the last axis must be contiguous")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{what} is {t.dtype}, q is {like.dtype}")
+        if t.device != like.device:
+            raise ValueError(f"{what} on {t.device}, q on {like.device}")
+        if dim != like.shape[2]:
+            raise ValueError(f"{what}: head_dim {dim}, q has {like.shape[2]}")
+    if heads is not None and n != heads:
+        raise ValueError(f"{what}: {n} heads, expected {heads}")
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
+    # the stride of an axis of one entry is never used: torch may hold any value there
+    row, head = row if rows > 1 else 0, head if n > 1 else 0
+    if written and rows > 0 and n > 0:
+        inner, outer, count = (head, row, n) if n > 1 and (rows == 1 or head <= row) else (row, head, rows)
+        if (n > 1 or rows > 1) and (inner < dim or (n > 1 and rows > 1 and outer < inner * (count - 1) + dim)):
+            raise ValueError(f"{what}: its rows and heads lie over one another (strides {t.stride()})")
+    return t.data_ptr(), row, head
+
+
+def _word(t, what: str, q, dtype, shape):
+    """Pointer of a contiguous device tensor of whole numbers beside q."""
+    if t.dtype != dtype:
+        raise TypeError(f"{what} is {t.dtype}, expected {dtype}")
+    if t.device != q.device:
+        raise ValueError(f"{what} on {t.device}, q on {q.device}")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class _On:
+    """The tensors' device made current for a launch (a kernel goes to the current device's stream)."""
+
+    def __init__(self, device):
+        torch = _torch()
+        if device.type != "cuda":
+            raise ValueError(f"tensors on {device}: the decoder operators run on the GPU")
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.device = device
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _torch().cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+class TextRotary:
+    """The rotation of `qk_norm_rotary`: frequencies theta^(-2j/head_dim), j < head_dim/2, each following the t, h or w
+    position (`section`: how many follow which, one axis after the other or interleaved)."""
+
+    def __init__(self, head_dim: int, theta: float, section: Sequence[int], interleaved: bool = True, device="cuda"):
+        torch = _torch()
+        if len(section) != 3:
+            raise ValueError(f"section {tuple(section)}: expected the counts of t, h and w")
+        self.head_dim, self.theta = int(head_dim), float(theta)
+        self.section, self.interleaved = tuple(int(s) for s in section), bool(interleaved)
+        table = np.zeros((max(self.head_dim // 2, 0), 2), np.uint64)
+        sec = (C.c_int32 * 3)(*self.section)
+        capi.check(capi.load().qvl_text_rotary_table(self.head_dim, self.theta, sec, int(self.interleaved),
+                                                     table.ctypes.data), "qvl_text_rotary_table")
+        self.table = torch.from_numpy(table.view(np.int64)).to(_device(device))
+
+    @classmethod
+    def from_spec(cls, text, device="cuda"):
+        """The rotation of a TextBackboneSpec (model.py:67-81)."""
+        if text.rope_scaling_factor not in (None, 1, 1.0):
+            raise ValueError(f"rope_scaling factor {text.rope_scaling_factor} is not supported")
+        return cls(text.head_dim, text.rope_theta, tuple(text.rope_section), text.mrope_interleaved, device)
+
+
+def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, eps: float = 1e-6, k_cache=None,
+                   v_cache=None, rows=None, q_out=None):
+    """Per-head RMSNorm of q [N, Hq, D] and k [N, Hkv, D] (weights q_norm, k_norm float32 [D]) and the rotation by
+    `positions` (int32 [3, N] for t, h, w, or [N] for text), one pass. Returns (q, k, v): without a cache new tensors q
+    and k and v itself; with k_cache, v_cache [R, Hkv, D] and rows (int64 [N]), token n's key and value go to row
+    rows[n] of the caches, which are returned (a row outside [0, R) is dropped; rows should differ). q_out, if given,
+    takes q (it may be q itself)."""
+    torch = _torch()
+    N, Hq, D = (int(s) for s in q.shape)
+    Hkv = int(k.shape[1])
+    if int(k.shape[0]) != N or (v is not None and int(v.shape[0]) != N):
+        raise ValueError(f"q has {N} tokens, k {int(k.shape[0])}" + ("" if v is None else f", v {int(v.shape[0])}"))
+    if D != rotary.head_dim:
+        raise ValueError(f"head_dim {D}, the rotation is made for {rotary.head_dim}")
+    if rotary.table.device != q.device:
+        raise ValueError(f"the rotation on {rotary.table.device}, q on {q.device}")
+    qv = _heads_view(q, "q")
+    kv = _heads_view(k, "k", q)
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous() or w.device != q.device:
+            raise ValueError(f"{name} must be a contiguous float32 [{D}] on {q.device}")
+    if positions.dim() == 1:
+        pos, pos_stride = _word(positions, "positions", q, torch.int32, (N,)), 0
+    else:
+        pos, pos_stride = _word(positions, "positions", q, torch.int32, (3, N)), N
+    if q_out is None:
+        q_out = torch.empty((N, Hq, D), dtype=q.dtype, device=q.device)
+    elif int(q_out.shape[0]) != N:
+        raise ValueError(f"q_out has {int(q_out.shape[0])} rows for {N} tokens")
+    qo = _heads_view(q_out, "q_out", q, Hq, True)
+    if (k_cache is None) != (v_cache is None) or (k_cache is None) != (rows is None):
+        raise ValueError("k_cache, v_cache and rows come together")
+    if k_cache is None:
+        k_cache, out_rows, prow = torch.empty((N, Hkv, D), dtype=q.dtype, device=q.device), N, None
+        vv = vo = (None, 0, 0)
+    else:
+        if v is None:
+            raise ValueError("v_cache without v")
+        vv = _heads_view(v, "v", q, Hkv)
+        vo = _heads_view(v_cache, "v_cache", q, Hkv, True)
+        out_rows, prow = int(k_cache.shape[0]), _word(rows, "rows", q, torch.int64, (N,))
+        if int(v_cache.shape[0]) != out_rows:
+            raise ValueError(f"k_cache has {out_rows} rows, v_cache {int(v_cache.shape[0])}")
+        if out_rows == 0:
+            raise ValueError("the caches have no rows")
+    ko = _heads_view(k_cache, "k_cache", q, Hkv, True)
+    with _On(q.device) as st:
+        capi.check(capi.load().qvl_qk_norm_rotary(
+            st, _qdtype(q.dtype), *qv, *kv, *vv, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), pos, pos_stride,
+            rotary.table.data_ptr(), prow, out_rows, *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
+    return q_out, k_cache, v if v_cache is None else v_cache
+
+
+class CausalPlan:
+    """The work list of `causal_attention` for one packed prefill: sequence i brings q_lens[i] new tokens and has k_lens[i]
+    keys (default q_lens), the new ones among them, in cache rows from k_starts[i] (default: one sequence after the other).
+    Made on the host once and used by every layer."""
+
+    def __init__(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None,
+                 k_starts: Optional[Sequence[int]] = None, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype,
+                 device="cuda"):
+        torch = _torch()
+        device = _device(device)
+        new = np.ascontiguousarray(q_lens, np.int64).reshape(-1)
+        keys = new if k_lens is None else np.ascontiguousarray(k_lens, np.int64).reshape(-1)
+        first = (np.concatenate([[0], np.cumsum(keys)[:-1]]).astype(np.int64) if k_starts is None and len(keys) else
+                 np.ascontiguousarray([] if k_starts is None else k_starts, np.int64).reshape(-1))
+        if not len(new) == len(keys) == len(first):
+            raise ValueError(f"{len(new)} query lengths, {len(keys)} key lengths, {len(first)} starts")
+        self.num_heads, self.num_kv_heads, self.head_dim = int(num_heads), int(num_kv_heads), int(head_dim)
+        self.dtype, self.device = dtype, device
+        self.n_tokens = int(new.sum())
+        self.kv_rows = int((first + keys).max()) if len(keys) else 0     # rows the caches must have
+        lib = capi.load()
+        n_cus = torch.cuda.get_device_properties(device).multi_processor_count
+        p64 = lambda a: a.ctypes.data_as(C.POINTER(C.c_int64))
+        n, whole = C.c_int64(), C.c_int64()
+
+        def build(items, capacity):
+            capi.check(lib.qvl_causal_worklist(len(new), p64(new), p64(keys), p64(first), self.num_heads, self.num_kv_heads,
+                                               self.head_dim, _qdtype(dtype), n_cus, items, capacity, C.byref(n),
+                                               C.byref(whole)), "qvl_causal_worklist")
+
+        build(None, 0)
+        items = np.zeros((max(n.value, 1), 8), np.int32)
+        build(items.ctypes.data_as(C.POINTER(C.c_int32)), n.value)
+        self.n_items, self.n_whole = n.value, whole.value
+        nb = C.c_size_t()
+        capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.n_items, self.n_whole, C.byref(nb)),
+                   "qvl_causal_workspace_size")
+        self.workspace_bytes = nb.value
+        self.items = torch.from_numpy(items).to(device)
+
+
+def _attention_views(q, k, v, out):
+    torch = _torch()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out {tuple(out.shape)}, q {tuple(q.shape)}")
+    qv, kv = _heads_view(q, "q"), _heads_view(k, "k", q)
+    vv = _heads_view(v, "v", q, int(k.shape[1]))
+    if k.shape[0] != v.shape[0]:
+        raise ValueError(f"k has {int(k.shape[0])} rows, v {int(v.shape[0])}")
+    return qv, kv, vv, _heads_view(out, "out", q, int(q.shape[1]), True), out
+
+
+def _workspace(nbytes: int, device):
+    return _torch().empty(nbytes, dtype=_torch().uint8, device=device) if nbytes else None
+
+
+def _scale(scale, head_dim: int) -> float:
+    return float(head_dim) ** -0.5 if scale is None else float(scale)
+
+
+def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None, out=None):
+    """softmax(scale q k^T) v of a packed prefill: q [N, Hq, D] holds the plan's new tokens one sequence after the other
+    (rows past them are left as they are in `out`), k and v [R, Hkv, D] the caches (or the prompt's own keys and values).
+    Token t of a sequence sees its keys up to itself; scale defaults to D^-0.5."""
+    qv, kv, vv, ov, out = _attention_views(q, k, v, out)
+    N, Hq, D = (int(s) for s in q.shape)
+    if (Hq, int(k.shape[1]), D) != (plan.num_heads, plan.num_kv_heads, plan.head_dim) or q.dtype != plan.dtype:
+        raise ValueError(f"q of {Hq} heads, k of {int(k.shape[1])}, head_dim {D}, {q.dtype}: the plan is for "
+                         f"{plan.num_heads}, {plan.num_kv_heads}, {plan.head_dim}, {plan.dtype}")
+    if q.device != plan.device:
+        raise ValueError(f"q on {q.device}, the plan on {plan.device}")
+    if N < plan.n_tokens or int(k.shape[0]) < plan.kv_rows:
+        raise ValueError(f"{N} tokens and {int(k.shape[0])} cache rows; the plan needs {plan.n_tokens} and {plan.kv_rows}")
+    ws = _workspace(plan.workspace_bytes, q.device)
+    with _On(q.device) as st:
+        capi.check(capi.load().qvl_causal_attention(
+            st, _qdtype(q.dtype), *qv, *kv, *vv, int(k.shape[0]), plan.items.data_ptr(), plan.n_items, plan.n_whole,
+            _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
+            plan.workspace_bytes), "qvl_causal_attention")
+    return out
+
+
+def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
+    torch = _torch()
+    qv, kv, vv, ov, out = _attention_views(q, k, v, out)
+    N, Hq, D = (int(s) for s in q.shape)
+    Hkv, n_seqs = int(k.shape[1]), int(k_start.shape[0])
+    ks = _word(k_start, "k_start", q, torch.int64, (n_seqs,))
+    kl = _word(k_len, "k_len", q, torch.int32, (n_seqs,))
+    cq = None if cu_q is None else _word(cu_q, "cu_q", q, torch.int32, (n_seqs + 1,))
+    cg = ps = pl = None
+    n_groups = max_prefix = 0
+    if groups is not None:
+        prefix_start, prefix_len, cu_groups, max_prefix = groups
+        n_groups = int(prefix_start.shape[0])
+        ps = _word(prefix_start, "prefix_start", q, torch.int64, (n_groups,))
+        pl = _word(prefix_len, "prefix_len", q, torch.int32, (n_groups,))
+        cg = _word(cu_groups, "cu_groups", q, torch.int32, (n_groups + 1,))
+    dt = _qdtype(q.dtype)
+    lib = capi.load()
+    nb = C.c_size_t()
+    with _On(q.device) as st:
+        capi.check(lib.qvl_decode_workspace_size(N, n_seqs, int(max_len), n_groups, int(max_prefix), Hq, Hkv, D, dt,
+                                                 C.byref(nb)), "qvl_decode_workspace_size")
+        ws = _workspace(nb.value, q.device)
+        capi.check(lib.qvl_decode_attention(
+            st, dt, *qv, *kv, *vv, int(k.shape[0]), cq, n_seqs, ks, kl, int(max_len), cg, n_groups, ps, pl,
+            int(max_prefix), _scale(scale, D), *ov, N, Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb.value),
+            "qvl_decode_attention")
+    return out
+
+
+def decode_attention(q, k, v, k_start, k_len, *, max_len: int, cu_q=None, scale: Optional[float] = None, out=None):
+    """Attention of new tokens over the caches k, v [R, Hkv, D]: sequence i's keys are the k_len[i] (int32) rows from
+    k_start[i] (int64), its new tokens' own at their end. q [N, Hq, D] holds one token per sequence, or tokens
+    cu_q[i]..cu_q[i+1] (int32 [n + 1]). The lengths are read on the device; max_len, the longest the launch is laid out
+    for, only sets how far the keys are split over the GPU."""
+    return _decode(q, k, v, k_start, k_len, max_len, cu_q, None, scale, out)
+
+
+def prefix_attention(q, k, v, k_start, k_len, prefix_start, prefix_len, cu_groups, *, max_len: int, max_prefix: int,
+                     cu_q=None, scale: Optional[float] = None, out=None):
+    """`decode_attention` of sequences that share prefixes: every token of sequences cu_groups[g]..cu_groups[g+1] (int32
+    [G + 1], from 0 to the number of sequences) also sees the prefix_len[g] (int32) cache rows from prefix_start[g]
+    (int64), which lie in the cache once and are read once for the group."""
+    return _decode(q, k, v, k_start, k_len, max_len, cu_q, (prefix_start, prefix_len, cu_groups, max_prefix), scale, out)

@@ -1,0 +1,232 @@
+"""CPU checks of the decoder operators: the rotation table, the causal work list and every refusal of the C entries and of
+the Python layer that needs no GPU."""
+import ctypes as C
+import math
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+FAKE = 1 << 20   # never dereferenced: validation fails first
+
+
+def table(pkg, head_dim, theta, section, interleaved):
+    out = np.zeros((head_dim // 2, 2), np.uint64)
+    sec = (C.c_int32 * 3)(*section)
+    pkg.capi.check(pkg.capi.load().qvl_text_rotary_table(head_dim, theta, sec, interleaved, out.ctypes.data))
+    return out
+
+
+@pytest.mark.parametrize("head_dim,theta,section,interleaved", [
+    (128, 5e6, (24, 20, 20), 1), (128, 5e6, (24, 20, 20), 0), (64, 1e4, (12, 10, 10), 1), (64, 1e4, (32, 0, 0), 0)])
+def test_rotary_table(pkg, head_dim, theta, section, interleaved):
+    t = table(pkg, head_dim, theta, section, interleaved)
+    half = head_dim // 2
+    for j in range(half):
+        want = theta ** (-2.0 * j / head_dim) / (2 * math.pi)
+        # the reference itself is a double: 2^-50 covers its power, division and pi; the entry is rounded to 2^-64
+        # turns, off by up to half of that (one unit where the long double power ends near a tie)
+        assert abs(float(Fraction(int(t[j, 0]), 2 ** 64)) - want) < 2.0 ** -50 * want + 2.0 ** -64
+        if interleaved:
+            axis = 1 if j % 3 == 1 and j < 3 * section[1] else 2 if j % 3 == 2 and j < 3 * section[2] else 0
+        else:
+            axis = 0 if j < section[0] else 1 if j < section[0] + section[1] else 2
+        assert int(t[j, 1]) == axis
+
+
+def test_rotary_table_refusals(pkg):
+    f = pkg.capi.load().qvl_text_rotary_table
+    out = np.zeros((128, 2), np.uint64)
+    sec = lambda *s: (C.c_int32 * 3)(*s)
+    for hd, theta, s in [(0, 1e4, sec(0, 0, 0)), (130, 1e4, sec(65, 0, 0)), (260, 1e4, sec(130, 0, 0)), (64, 1.0, sec(32, 0, 0)),
+                         (64, float("inf"), sec(32, 0, 0)), (64, float("nan"), sec(32, 0, 0)), (64, 1e4, sec(12, 10, 9)),
+                         (64, 1e4, sec(-1, 23, 10)), (64, 1e4, sec(33, 0, 0))]:
+        assert f(hd, theta, s, 0, out.ctypes.data) == -1
+    assert f(64, 1e4, None, 0, out.ctypes.data) == -1
+    assert f(64, 1e4, sec(32, 0, 0), 0, None) == -1
+
+
+def worklist(pkg, new, length, start, hq, hkv, hd=128, dtype=1, n_cus=256):
+    lib = pkg.capi.load()
+    a = [np.array(v, np.int64) for v in (new, length, start)]
+    p = [v.ctypes.data_as(C.POINTER(C.c_int64)) for v in a]
+    n, w = C.c_int64(), C.c_int64()
+    pkg.capi.check(lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, None, 0, C.byref(n), C.byref(w)))
+    items = np.zeros((n.value, 8), np.int32)
+    ptr = items.ctypes.data_as(C.POINTER(C.c_int32))
+    pkg.capi.check(lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, ptr, n.value, C.byref(n), C.byref(w)))
+    if n.value > 0:
+        assert lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, ptr, n.value - 1, C.byref(n), C.byref(w)) == -1
+    return items, w.value
+
+
+@pytest.mark.parametrize("new,old,hq,hkv,hd,dtype", [
+    ([1], [0], 16, 8, 128, 1), ([300, 0, 1, 129], [0, 5, 77, 4000], 16, 8, 128, 1), ([2048], [0], 32, 8, 128, 1),
+    ([40], [24000], 32, 8, 128, 1), ([1181, 317, 5], [0, 64, 0], 14, 2, 64, 0), ([7] * 40, [0] * 40, 4, 1, 64, 1),
+    ([513], [1000], 6, 2, 128, 0)])
+def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtype):
+    length = [a + b for a, b in zip(new, old)]
+    start = [(1 << 33) + 17 * i for i in range(len(new))]
+    items, n_whole = worklist(pkg, new, length, start, hq, hkv, hd, dtype)
+    group = hq // hkv
+    q0 = np.concatenate([[0], np.cumsum(new)])
+    seen = {}
+    slots = []
+    for k, it in enumerate(items.tolist()):
+        first, n_new, n_keys, row0, head, slot, lo, hi = it
+        if n_new == 0:          # padding of a short queue
+            continue
+        i = [j for j in range(len(new)) if q0[j] == first and new[j] == n_new][0]
+        assert n_keys == length[i] and (hi << 32 | lo & 0xffffffff) == start[i]
+        part, parts = head >> 12 & 0xff, head >> 20 & 0xff
+        assert (parts >= 2 and part < parts and k >= n_whole) if parts else k < n_whole
+        if parts:
+            slots.append(slot)
+        assert row0 % 128 == 0 and 0 <= row0 < n_new * group
+        seen.setdefault((i, row0, head & 0xfff), []).append((part, max(parts, 1)))
+    want = {(i, r, h) for i in range(len(new)) for r in range(0, new[i] * group, 128) for h in range(hkv)}
+    assert set(seen) == want
+    for got in seen.values():
+        assert sorted(p for p, _ in got) == list(range(got[0][1])) and len({n for _, n in got}) == 1
+    assert sorted(slots) == list(range(len(items) - n_whole))
+
+
+def test_worklist_refusals(pkg):
+    f = pkg.capi.load().qvl_causal_worklist
+    n, w = C.c_int64(), C.c_int64()
+    one = lambda v: (C.c_int64 * 1)(v)
+    ok = dict(new=4, length=9, start=0, hq=8, hkv=2, hd=128, dt=1, cus=256)
+
+    def rc(**k):
+        a = dict(ok, **k)
+        return f(1, one(a["new"]), one(a["length"]), one(a["start"]), a["hq"], a["hkv"], a["hd"], a["dt"], a["cus"], None, 0,
+                 C.byref(n), C.byref(w))
+
+    assert rc() == 0
+    for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57)):
+        assert rc(**bad) == -1, bad
+    for bad in (dict(hd=96), dict(dt=2), dict(hq=8192, hkv=8192), dict(length=1 << 30), dict(new=1 << 29)):
+        assert rc(**bad) == -2, bad
+    assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, None, 0, C.byref(n), C.byref(w)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, None, 0, None, C.byref(w)) == -1
+
+
+def rotary_args(**change):
+    a = dict(stream=None, dtype=1, q=FAKE, q_row=2048, q_head=128, k=FAKE, k_row=2048, k_head=128, v=FAKE, v_row=2048,
+             v_head=128, qw=FAKE, kw=FAKE, eps=1e-6, pos=FAKE, pos_stride=4, table=FAKE, rows=FAKE, out_rows=9, qo=FAKE,
+             qo_row=2048, qo_head=128, ko=FAKE, ko_row=2048, ko_head=128, vo=FAKE, vo_row=2048, vo_head=128, n=4, hq=16,
+             hkv=8, hd=128)
+    assert not set(change) - set(a)
+    a.update(change)
+    return list(a.values())
+
+
+def test_qk_norm_rotary_refusals(pkg):
+    f = pkg.capi.load().qvl_qk_norm_rotary
+    for want, bad in [(-2, dict(dtype=2)), (-2, dict(hd=96)), (-1, dict(n=-1)), (-1, dict(hq=0)), (-1, dict(hkv=0)),
+                      (-1, dict(eps=-1.0)), (-1, dict(eps=float("nan"))), (-1, dict(rows=None, out_rows=3)), (-1, dict(v=None)),
+                      (-1, dict(vo=None)), (-1, dict(q=None)), (-1, dict(k=None)), (-1, dict(qw=None)), (-1, dict(kw=None)),
+                      (-1, dict(pos=None)), (-1, dict(table=None)), (-1, dict(qo=None)), (-1, dict(ko=None)),
+                      (-1, dict(q_row=-8)), (-1, dict(k_head=1 << 31)), (-3, dict(q=FAKE + 8)), (-3, dict(v_row=2044)),
+                      (-3, dict(ko_head=132)), (-3, dict(rows=FAKE + 4)), (-3, dict(kw=FAKE + 4)), (-1, dict(pos_stride=-1)),
+                      (-2, dict(hq=4097)), (-2, dict(n=1 << 30)), (-1, dict(out_rows=-1))]:
+        assert f(*rotary_args(**bad)) == want, bad
+    assert f(*rotary_args(n=0, q=None)) == 0      # nothing to do
+
+
+def attn_common(**change):
+    a = dict(stream=None, dtype=1, q=FAKE, q_row=2048, q_head=128, k=FAKE, k_row=1024, k_head=128, v=FAKE, v_row=1024,
+             v_head=128, kv_rows=100)
+    a.update({k: v for k, v in change.items() if k in a})
+    return list(a.values())
+
+
+def attn_tail(**change):
+    a = dict(scale=0.1, out=FAKE, out_row=2048, out_head=128, n=4, hq=16, hkv=8, hd=128, ws=FAKE, ws_bytes=1 << 40)
+    a.update({k: v for k, v in change.items() if k in a})
+    return list(a.values())
+
+
+ATTN_BAD = [(-2, dict(dtype=3)), (-2, dict(hd=80)), (-1, dict(hq=12)), (-1, dict(hkv=0)), (-1, dict(n=-1)), (-1, dict(kv_rows=-1)),
+            (-1, dict(scale=0.0)), (-1, dict(scale=-1.0)), (-1, dict(scale=float("inf"))), (-1, dict(scale=float("nan"))),
+            (-1, dict(q=None)), (-1, dict(k=None)), (-1, dict(v=None)), (-1, dict(out=None)), (-1, dict(q_head=-128)),
+            (-1, dict(k_row=1 << 31)), (-3, dict(q=FAKE + 2)), (-3, dict(k_row=1020)), (-3, dict(out_head=4)),
+            (-2, dict(hq=8192, hkv=8192)), (-2, dict(n=1 << 30))]
+
+
+def test_causal_attention_refusals(pkg):
+    f = pkg.capi.load().qvl_causal_attention
+
+    def rc(items=FAKE, n_items=3, n_whole=3, **k):
+        return f(*attn_common(**k), items, n_items, n_whole, *attn_tail(**k))
+
+    for want, bad in ATTN_BAD + [(-1, dict(items=None)), (-3, dict(items=FAKE + 4)), (-1, dict(n_whole=4)), (-1, dict(n_whole=-1)),
+                                 (-1, dict(n_items=1 << 31))]:
+        assert rc(**bad) == want, bad
+    assert rc(n=0, q=None) == 0 and rc(items=None, n_items=0, n_whole=0) == 0
+    nb = C.c_size_t()
+    size = pkg.capi.load().qvl_causal_workspace_size
+    assert size(128, 4, 4, C.byref(nb)) == 0 and nb.value == 0
+    assert size(96, 4, 4, C.byref(nb)) == -2 and size(128, 3, 4, C.byref(nb)) == -1 and size(128, 4, 4, None) == -1
+
+
+def test_decode_attention_refusals(pkg):
+    f = pkg.capi.load().qvl_decode_attention
+
+    def rc(cu_q=None, n_seqs=4, ks=FAKE, kl=FAKE, max_len=100, cg=None, groups=0, ps=None, pl=None, max_prefix=0, **k):
+        return f(*attn_common(**k), cu_q, n_seqs, ks, kl, max_len, cg, groups, ps, pl, max_prefix, *attn_tail(**k))
+
+    for want, bad in ATTN_BAD[:-1] + [
+            (-1, dict(n_seqs=-1)), (-1, dict(n_seqs=5)), (-1, dict(ks=None)), (-1, dict(kl=None)), (-1, dict(max_len=-1)),
+            (-1, dict(groups=1)), (-1, dict(groups=1, cg=FAKE, ps=FAKE)), (-1, dict(groups=-1)), (-1, dict(max_prefix=-1)),
+            (-3, dict(ks=FAKE + 4)), (-3, dict(kl=FAKE + 2)), (-3, dict(cu_q=FAKE + 1)),
+            (-3, dict(groups=1, cg=FAKE, ps=FAKE + 4, pl=FAKE)), (-2, dict(n=70000, n_seqs=70000))]:
+        assert rc(**bad) == want, bad
+    assert rc(n=0, n_seqs=0, q=None) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# the Python layer's own checks (tensors on the CPU: every call ends before a launch)
+# ---------------------------------------------------------------------------------------------
+def test_python_refusals_on_the_cpu(pkg):
+    torch = pytest.importorskip("torch")
+    ops = pkg.decoder_attn
+    q, k = torch.zeros(3, 8, 64), torch.zeros(9, 2, 64)
+    ks, kl = torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int32)
+    dec = lambda **a: ops.decode_attention(a.get("q", q), a.get("k", k), a.get("v", k), a.get("ks", ks), a.get("kl", kl),
+                                           max_len=9, **{n: a[n] for n in ("cu_q", "out") if n in a})
+    with pytest.raises(ValueError, match="run on the GPU"):
+        dec()
+    with pytest.raises(ValueError, match="run on the GPU"):
+        ops.TextRotary(64, 1e4, (32, 0, 0), False, device="cpu")
+    with pytest.raises(ValueError, match="rows, heads, head_dim"):
+        dec(q=q[0])
+    with pytest.raises(ValueError, match="head_dim 32"):
+        dec(k=k[..., :32], v=k[..., :32])
+    with pytest.raises(ValueError, match="last axis"):
+        dec(k=k[..., ::2], v=k[..., ::2])
+    with pytest.raises(TypeError, match="bfloat16"):
+        dec(k=k.bfloat16())
+    with pytest.raises(ValueError, match="rows"):
+        dec(v=k[:8])
+    with pytest.raises(ValueError, match="heads"):
+        dec(v=torch.zeros(9, 4, 64))
+    with pytest.raises(TypeError, match="k_len"):
+        dec(kl=kl.long())
+    with pytest.raises(ValueError, match="k_len"):
+        dec(kl=kl[:2])
+    with pytest.raises(ValueError, match="cu_q"):
+        dec(cu_q=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="out"):
+        dec(out=torch.zeros(2, 8, 64))
+    with pytest.raises(ValueError, match="over one another"):
+        dec(out=torch.zeros(1, 8, 64).expand(3, 8, 64))
+    with pytest.raises(ValueError, match="gradient"):
+        dec(q=q.clone().requires_grad_())
+    spec = pkg.spec_from_config({"text_config": {"hidden_size": 2048, "num_attention_heads": 16, "num_hidden_layers": 28,
+                                                 "num_key_value_heads": 8, "head_dim": 128, "intermediate_size": 6144,
+                                                 "rms_norm_eps": 1e-6, "vocab_size": 151936, "rope_theta": 5e6,
+                                                 "rope_scaling": {"mrope_section": [24, 20, 20], "mrope_interleaved": True,
+                                                                  "factor": 2.0}}})
+    with pytest.raises(ValueError, match="factor"):
+        ops.TextRotary.from_spec(spec.text, device="cpu")
