@@ -30,104 +30,779 @@ struct AttnParams {
   const int64_t* prefix_start;
   const int32_t* prefix_len;
   int n_seqs, n_groups;
+  // Partial results: per part and row the unnormalised output and (m, l). causal: [slot][128 rows], slots of the items
+  // from n_whole on; decode: [part][token][head], prefix parts first.
+  float* part_o;
+  f32x2* part_ml;
+  int n_whole;
+  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // parts of so many keys each
 };
 
-template <typename T> __device__ __forceinline__ float load_one(const char* p, int i) {
-  return (float)reinterpret_cast<const T*>(p)[i];
-}
+template <int V> using int_c = std::integral_constant<int, V>;
 
-// One row over up to two runs of cache rows (start, keys), by one wave: 64 keys at a time, a lane's score each; then a
-// lane holds D / 64 of the output's dims. `q` is the row in LDS, fp32.
-template <typename T, int D>
-__device__ __forceinline__ void attend_row(const AttnParams& P, const float* q, int kvh, const int64_t (&start)[2],
-                                           const int64_t (&keys)[2], char* out) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY, l = 0.f, o[E] = {};
-  for (int run = 0; run < 2; ++run) {
-    const char* kb = P.k.p + start[run] * P.k.row + kvh * P.k.head;
-    const char* vb = P.v.p + start[run] * P.v.row + kvh * P.v.head;
-    for (int64_t j0 = 0; j0 < keys[run]; j0 += 64) {
-      float s = -INFINITY;
-      if (j0 + lane < keys[run]) {
-        const char* kr = kb + (j0 + lane) * P.k.row;
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = __builtin_fmaf(q[d], load_one<T>(kr, d), s);
-        s *= P.scale;
+// What one wave does with 32 rows and a block of 32 keys in LDS. S^T = K Q^T puts a row in a lane (column lane % 32) with
+// 16 of the block's keys: register r is key 8 (r / 4) + 4 (lane / 32) + r % 4. The second product O^T = V^T P^T takes P as
+// it lies in those registers, as its B operand; only V has to come transposed.
+//
+// bf16: v_mfma_f32_32x32x16. K and V lie in LDS row by row as they come from memory. A lane's 8 keys of a 16-key group
+// are two runs of 4, so V^T is read by two transposing reads of 4 keys (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16
+// values, and each gets a column). The row sums add the rounded weights that multiply V, two to an instruction.
+// 16-byte chunks are XOR-swizzled by the row so that neither read meets a bank twice: 16 rows of one chunk for K, 4 rows
+// of 64 bytes for V.
+template <typename T, int D> struct Core;
+
+template <int D> struct Core<bf16, D> {
+  static constexpr int kRowBytes = D * 2, kDB = D / 32;
+  static constexpr int kChunks = kRowBytes / 16;
+  bf16x8 q[D / 16];
+  f32x16 o[kDB];
+  float l;
+
+  static __device__ __forceinline__ int k_swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int v_swz(int row) { return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
+
+  __device__ __forceinline__ void init(const char* qrow) {
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const bf16x8*>(qrow + (ks * 16 + hh * 8) * 2);
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) o[db] = f32x16{};
+    l = 0.f;
+  }
+  // keys block b of the tile at `lds`
+  __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+    f32x16 s = f32x16{};
+    const char* row = lds + (b * 32 + l32) * kRowBytes;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const bf16x8 k = *reinterpret_cast<const bf16x8*>(row + (((ks * 2 + hh) ^ k_swz(l32)) << 4));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[ks], s, 0, 0, 0);
+    }
+    return s;
+  }
+  // V^T rows 32 db + lane % 32, the lane's 8 keys of 16-key group g (keys 16 g on)
+  __device__ __forceinline__ bf16x8 v_frag(const char* lds, int db, int g) const {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    const int lane = threadIdx.x & 63, hh = lane >> 5, i = lane & 15;
+    const int r = 4 * hh + (i >> 2);                       // row of the first run; the second is 8 rows on (same swizzle)
+    const int c = db * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+    const char* p = lds + (16 * g + r) * kRowBytes + ((c ^ v_swz(r)) << 4) + (i & 1) * 8;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * kRowBytes));
+    return __builtin_bit_cast(bf16x8, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+  }
+  __device__ __forceinline__ void pv(const char* lds, int b, const f32x16& p) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u32x4 pw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pw[j] = pack_bf16x2(p[8 * e + 2 * j], p[8 * e + 2 * j + 1]);
+      add_weights(pw);
+      const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(lds, db, 2 * b + e), pf, o[db], 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void add_weights(const u32x4& pw) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = pw[j];   // a copy: __builtin_bit_cast of a vector's element takes element 0 here
+      t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), t, false);
+    }
+    l += t;
+  }
+  // The same where some rows do not see all of the block's keys and V may hold infinities or NaN, which a weight of zero
+  // does not silence: V's non-finite values are left out of the product and counted, row by row, among the keys that the
+  // row sees (+inf as 1, -inf as 2^8, NaN as 2^16: sums of 16 keys stay exact), and the counts put back what they stand for.
+  __device__ __forceinline__ void pv_safe(const char* lds, int b, const f32x16& p, uint32_t seen) {
+    for (int e = 0; e < 2; ++e) {
+      u32x4 pw, sw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 8 * e + 2 * j;
+        pw[j] = pack_bf16x2(p[r], p[r + 1]);
+        sw[j] = ((seen >> r) & 1 ? 0x3f80u : 0u) | ((seen >> (r + 1)) & 1 ? 0x3f800000u : 0u);
       }
-      float mx = s;
-      for (int w = 1; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-      const float mn = fmaxf(m, mx), shift = mn == -INFINITY ? 0.f : mn;
-      const float a = __builtin_amdgcn_exp2f(m - shift), p = __builtin_amdgcn_exp2f(s - shift);
-      m = mn;
-      l *= a;
-      for (int e = 0; e < E; ++e) o[e] *= a;
-      const int n = (int)min((int64_t)64, keys[run] - j0);
-      for (int j = 0; j < n; ++j) {
-        const float pj = __shfl(p, j);
-        l += pj;
-        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(pj, load_one<T>(vb + (j0 + j) * P.v.row, lane * E + e), o[e]);
+      add_weights(pw);
+      const bf16x8 pf = __builtin_bit_cast(bf16x8, pw), sf = __builtin_bit_cast(bf16x8, sw);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        u32x4 v = __builtin_bit_cast(u32x4, v_frag(lds, db, 2 * b + e)), bad;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t clean = 0, mark = 0;
+#pragma unroll
+          for (int h = 0; h < 32; h += 16) {
+            const uint32_t x = (v[j] >> h) & 0xffffu;
+            const bool ok = (x & 0x7f80u) != 0x7f80u;
+            clean |= (ok ? x : 0u) << h;
+            mark |= (ok ? 0u : x == 0x7f80u ? 0x3f80u : x == 0xff80u ? 0x4380u : 0x4780u) << h;
+          }
+          v[j] = clean;
+          bad[j] = mark;
+        }
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pf, o[db], 0, 0, 0);
+        const f32x16 n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bad), sf, f32x16{}, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t c = (uint32_t)n[r];
+          if (c & 0xffu) o[db][r] += INFINITY;
+          if (c & 0xff00u) o[db][r] -= INFINITY;
+          if (c >> 16) o[db][r] = NAN;
+        }
       }
     }
   }
-  const bool none = keys[0] + keys[1] <= 0;
-  for (int e = 0; e < E; ++e) reinterpret_cast<T*>(out)[lane * E + e] = (T)(none ? 0.f : o[e] / l);
+  __device__ __forceinline__ void rescale(float a) {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) o[db] *= a;
+    l *= a;
+  }
+  // the row's sum, in both of its lanes
+  __device__ __forceinline__ float row_sum() const { return l + __shfl_xor(l, 32); }
+  // f(first dim, 4 values) for each run of 4 dims this lane holds of its row
+  template <typename F> __device__ __forceinline__ void each4(F&& f) const {
+    const int hh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int db = 0; db < kDB; ++db)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        f(db * 32 + 8 * k + 4 * hh, f32x4{o[db][4 * k], o[db][4 * k + 1], o[db][4 * k + 2], o[db][4 * k + 3]});
+  }
+};
+
+// fp32: v_mfma_f32_32x32x2_f32, one value a lane and operand. The two lanes of a row take dims (or keys) 4 apart, so that K
+// is read 16 bytes at a time; a lane of V^T takes the dims kDB i + db of its row i, which lie together in V's row: one
+// read serves all of a key's output blocks. P needs no packing.
+template <int D> struct Core<float, D> {
+  static constexpr int kRowBytes = D * 4, kDB = D / 32;
+  static constexpr int kChunks = kRowBytes / 16;
+  f32x4 q[D / 8];
+  f32x16 o[kDB];
+  float l;
+
+  static __device__ __forceinline__ int k_swz(int row) { return row & 15; }
+  static __device__ __forceinline__ int v_swz(int) { return 0; }
+
+  __device__ __forceinline__ void init(const char* qrow) {
+    const int hh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) q[j] = *reinterpret_cast<const f32x4*>(qrow + (j * 8 + hh * 4) * 4);
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) o[db] = f32x16{};
+    l = 0.f;
+  }
+  __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+    f32x16 s = f32x16{};
+    const char* row = lds + (b * 32 + l32) * kRowBytes;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      const f32x4 k = *reinterpret_cast<const f32x4*>(row + (((j * 2 + hh) ^ k_swz(l32)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[j][e], s, 0, 0, 0);
+    }
+    return s;
+  }
+  // dims kDB (lane % 32) + db of the lane's key in register r of block b
+  __device__ __forceinline__ void v_frag(const char* lds, int b, int r, float (&v)[kDB]) const {
+    const int lane = threadIdx.x & 63;
+    const char* p = lds + (b * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * kRowBytes + (lane & 31) * kDB * 4;
+    if constexpr (kDB == 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) v[db] = x[db];
+    } else {
+      const f32x2 x = *reinterpret_cast<const f32x2*>(p);
+      v[0] = x[0];
+      v[1] = x[1];
+    }
+  }
+  __device__ __forceinline__ void pv(const char* lds, int b, const f32x16& p) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float v[kDB];
+      v_frag(lds, b, r, v);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[db], p[r], o[db], 0, 0, 0);
+      l += p[r];
+    }
+  }
+  __device__ __forceinline__ void pv_safe(const char* lds, int b, const f32x16& p, uint32_t seen) {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      f32x16 n = f32x16{};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float v[kDB];
+        v_frag(lds, b, r, v);
+        const bool ok = fabsf(v[db]) < INFINITY;
+        const float mark = ok ? 0.f : v[db] == INFINITY ? 1.f : v[db] == -INFINITY ? 256.f : 65536.f;
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(ok ? v[db] : 0.f, p[r], o[db], 0, 0, 0);
+        n = __builtin_amdgcn_mfma_f32_32x32x2f32(mark, (seen >> r) & 1 ? 1.f : 0.f, n, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t c = (uint32_t)n[r];
+        if (c & 0xffu) o[db][r] += INFINITY;
+        if (c & 0xff00u) o[db][r] -= INFINITY;
+        if (c >> 16) o[db][r] = NAN;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) l += p[r];
+  }
+  __device__ __forceinline__ void rescale(float a) {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) o[db] *= a;
+    l *= a;
+  }
+  __device__ __forceinline__ float row_sum() const { return l + __shfl_xor(l, 32); }
+  template <typename F> __device__ __forceinline__ void each4(F&& f) const {
+    const int hh = (threadIdx.x & 63) >> 5;
+    if constexpr (kDB == 4) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) f(4 * (8 * (r >> 2) + 4 * hh + (r & 3)), f32x4{o[0][r], o[1][r], o[2][r], o[3][r]});
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        f(2 * (8 * (r >> 2) + 4 * hh + (r & 3)), f32x4{o[0][r], o[1][r], o[0][r + 1], o[1][r + 1]});
+    }
+  }
+};
+
+// 4 values rounded to T at dim d of a row.
+template <typename T> __device__ __forceinline__ void store4(char* row, int d, const f32x4& x) {
+  if constexpr (std::is_same<T, float>::value) *reinterpret_cast<f32x4*>(row + 4 * d) = x;
+  else *reinterpret_cast<u32x2*>(row + 2 * d) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+}
+
+// Keys of one unit of work for one key/value head: cache rows from `k`, `v`, rows of the unit [row0, rows) as (token, head)
+// pairs, token by token; token t sees keys below lim0 + t, and never more than `len`.
+struct Unit {
+  const char *k, *v;
+  int len, lim0;       // lim0 + t: keys that token t sees (len - 1 and more: all of them)
+  int64_t token0;      // the sequence's (or group's) first token
+  int rows, row0, kvh;
+};
+
+// The online softmax of one wave: 32 rows over the keys it is given.
+template <typename T, int D> struct Wave {
+  Core<T, D> core;
+  float m;             // running maximum of the lane's row, in powers of two; -inf before the first key it sees
+  int lim, lim_lo;     // keys the lane's row sees; the fewest any row of the wave does
+  int lim_hi;          // the most
+
+  __device__ __forceinline__ void init(const AttnParams& P, const Unit& u, int first_row) {
+    const int row = min(first_row + (int)(threadIdx.x & 31), u.rows - 1);
+    const int t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
+    const char* q = P.q.p + (u.token0 + t) * P.q.row + (int64_t)(u.kvh * P.group + g) * P.q.head;
+    lim = max(min(u.lim0 + t, u.len), 0);
+    const int lo = min(first_row, u.rows - 1), hi = min(first_row + 31, u.rows - 1);
+    lim_lo = max(min(u.lim0 + (int)((uint32_t)lo / (uint32_t)P.group), u.len), 0);
+    lim_hi = max(min(u.lim0 + (int)((uint32_t)hi / (uint32_t)P.group), u.len), 0);
+    m = -INFINITY;
+    core.init(q);
+  }
+  // NB blocks of 32 keys from key kb on; K and V tiles in LDS. `between` runs once the scores are read out of K's tile,
+  // `before_v` before V's is read.
+  template <int NB, typename F, typename G>
+  __device__ __forceinline__ void step(const char* klds, const char* vlds, int kb, float scale, bool safe, F&& between, G&& before_v) {
+    f32x16 s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = core.scores(klds, b);
+    between();
+    const bool edge = kb + 32 * NB > lim_lo;
+    uint32_t seen[NB];
+    if (edge) {
+      const int base = lim - kb - 4 * (int)((threadIdx.x & 63) >> 5);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        seen[b] = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool in = 32 * b + 8 * (r >> 2) + (r & 3) < base;
+          seen[b] |= (in ? 1u : 0u) << r;
+          s[b][r] = in ? s[b][r] : -INFINITY;
+        }
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
+    // A row's maximum moves only where it grew by more than 2^8: until then weights of up to 2^8 lose nothing (fp32 sums,
+    // and bf16 weights of the same relative rounding), and the accumulators need no pass. Row by row, so that a row's result
+    // does not depend on the others of its wave.
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+      const float mn = mx > m + 8.f ? mx : m;
+      core.rescale(__builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn)));
+      m = mn;
+    }
+    const float shift = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], scale, shift));
+    before_v();
+    if (edge && safe) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) core.pv_safe(vlds, b, s[b], seen[b]);
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) core.pv(vlds, b, s[b]);
+    }
+  }
+  __device__ __forceinline__ bool finite() const {
+    bool ok = true;
+    core.each4([&](int, const f32x4& x) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ok = ok & (fabsf(x[e]) < INFINITY);
+    });
+    return ok;
+  }
+};
+
+// The rows of a [rows, heads, dim] view as a buffer that ends after `rows` of them: loads past it give zeros.
+__device__ __forceinline__ u32x4 rows_rsrc(const char* base, int64_t stride, int rows, int row_bytes) {
+  return rsrc_words(base, rows > 0 ? (uint32_t)((int64_t)(min(rows, 64) - 1) * stride + row_bytes) : 0u);
+}
+
+// Where a lane's 16 bytes of row i of a DMA of 1 KiB come from: lane j fills chunk j % kChunks of row j / kChunks, which
+// holds the logical chunk the swizzle maps there.
+template <typename T, int D> struct Loader {
+  using C = Core<T, D>;
+  static constexpr int kRowsPerDma = 1024 / C::kRowBytes;
+
+  // rows [r0, r0 + n) of the tile that starts at key kb, by one wave; n a multiple of kRowsPerDma
+  template <bool V>
+  static __device__ __forceinline__ void rows(const u32x4& rsrc, int64_t stride, int r0, int n, uint32_t lds) {
+    const int lane = threadIdx.x & 63;
+    for (int r = r0; r < r0 + n; r += kRowsPerDma) {
+      const int row = r + lane / C::kChunks;
+      const int c = (lane % C::kChunks) ^ (V ? C::v_swz(row) : C::k_swz(row & 31));
+      dma16(rsrc, (uint32_t)(row * (uint32_t)stride) + (uint32_t)(c << 4), 0, lds + r * C::kRowBytes);
+    }
+  }
+};
+
+// A row's result: rounded to its place, or unnormalised with (m, l) into a partial buffer.
+template <typename T, int D>
+__device__ __forceinline__ char* out_row(const AttnParams& P, const Unit& u, int row) {
+  const int t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
+  return const_cast<char*>(P.out.p) + (u.token0 + t) * P.out.row + (int64_t)(u.kvh * P.group + g) * P.out.head;
+}
+
+// 128 rows a workgroup, 32 a wave; the four waves share each tile of 64 (fp32: 32) keys, which comes by LDS DMA into one of
+// two stages while the other is computed on.
+template <typename T, int D> struct RowsUnit {
+  static constexpr int kNB = std::is_same<T, float>::value ? 1 : 2, kBN = 32 * kNB;
+  static constexpr int kTile = kBN * Core<T, D>::kRowBytes, kLds = 4 * kTile;
+
+  // tiles [t0, t1) of the unit; true where the whole workgroup's rows are done
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1, bool safe) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lds0 = lds_addr_of(smem);
+    auto load = [&](int t, int stage) {
+      const int kb = t * kBN;
+      const u32x4 rk = rows_rsrc(u.k + (int64_t)kb * P.k.row, P.k.row, u.len - kb, Core<T, D>::kRowBytes);
+      const u32x4 rv = rows_rsrc(u.v + (int64_t)kb * P.v.row, P.v.row, u.len - kb, Core<T, D>::kRowBytes);
+      const uint32_t l = lds0 + stage * 2 * kTile;
+      Loader<T, D>::template rows<false>(rk, P.k.row, wave * (kBN / 4), kBN / 4, l);
+      Loader<T, D>::template rows<true>(rv, P.v.row, wave * (kBN / 4), kBN / 4, l + kTile);
+    };
+    if (t0 < t1) load(t0, 0);
+    wait_dma();
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int stage = (t - t0) & 1;
+      if (t + 1 < t1) load(t + 1, stage ^ 1);
+      const char* k = smem + stage * 2 * kTile;
+      if (t * kBN < w.lim_hi) w.template step<kNB>(k, k + kTile, t * kBN, P.scale, safe, [] {}, [] {});
+      wait_dma();
+      __syncthreads();
+    }
+  }
+};
+
+// Up to 32 rows a workgroup; the four waves take every fourth block of 32 keys, each through LDS of its own: while a block's
+// weights are formed the next block's keys arrive, while its scores are formed the next values do. Joined in LDS at the end.
+template <typename T, int D> struct KeysUnit {
+  static constexpr int kTile = 32 * Core<T, D>::kRowBytes, kLds = 4 * 2 * kTile;
+  static constexpr int kDmas = kTile / 1024;
+
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const char* k = smem + wave * 2 * kTile;
+    const uint32_t kl = lds_addr_of(k), vl = kl + kTile;
+    auto load_k = [&](int t) {
+      Loader<T, D>::template rows<false>(rows_rsrc(u.k + (int64_t)(t * 32) * P.k.row, P.k.row, u.len - t * 32, Core<T, D>::kRowBytes),
+                                         P.k.row, 0, 32, kl);
+    };
+    auto load_v = [&](int t) {
+      Loader<T, D>::template rows<true>(rows_rsrc(u.v + (int64_t)(t * 32) * P.v.row, P.v.row, u.len - t * 32, Core<T, D>::kRowBytes),
+                                        P.v.row, 0, 32, vl);
+    };
+    t0 += wave;
+    if (t0 >= t1) return;
+    load_k(t0);
+    load_v(t0);
+    // In flight, oldest first: K(t), V(t) at the top; V(t), K(t + 1) before V is read.
+    const bool safe = w.lim_lo < u.len;
+    for (int t = t0; t < t1; t += 4) {
+      const bool more = t + 4 < t1;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDmas) : "memory");
+      w.template step<1>(k, k + kTile, t * 32, P.scale, safe,
+                         [&] {
+                           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                           if (more) load_k(t + 4);
+                         },
+                         [&] {
+                           if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDmas) : "memory");
+                           else wait_dma();
+                         });
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) load_v(t + 4);
+    }
+  }
+};
+
+
+// (m, l) of a part as the combine reads it: no key seen (-inf, 0), only keys of score -inf (-inf, -0).
+__device__ __forceinline__ f32x2 part_state(float m, float l, bool sees) { return f32x2{m, l == 0.f && sees ? -0.f : l}; }
+
+// One wave writes its 32 rows: to the output, or as a part.
+template <typename T, int D>
+__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, int row, float* po, f32x2* pml, bool sees) {
+  const float l = w.core.row_sum();
+  if (row >= u.rows) return;
+  if (po) {
+    w.core.each4([&](int d, const f32x4& x) { *reinterpret_cast<f32x4*>(po + d) = x; });
+    if ((threadIdx.x & 63) < 32) *pml = part_state(w.m, l, sees);
+  } else {
+    const float inv = 1.0f / l;
+    char* out = out_row<T, D>(P, u, row);
+    w.core.each4([&](int d, const f32x4& x) { store4<T>(out, d, sees ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f}); });
+  }
 }
 
 template <typename T, int D>
-__device__ __forceinline__ const float* row_to_lds(const AttnParams& P, float (*lds)[D], int64_t token, int head) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const char* q = P.q.p + token * P.q.row + head * P.q.head;
-  __builtin_amdgcn_wave_barrier();
-  for (int d = lane; d < D; d += 64) lds[wave][d] = load_one<T>(q, d);
-  __builtin_amdgcn_wave_barrier();
-  return lds[wave];
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(256) void causal_kernel(AttnParams P) {
-  __shared__ float lds[4][D];
+__global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P) {
+  using R = RowsUnit<T, D>;
+  __shared__ __attribute__((aligned(16))) char smem[R::kLds];
   const int32_t* it = P.items + 8 * (int64_t)blockIdx.x;
   const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
+  const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
   const int64_t start = (int64_t)(((uint64_t)(uint32_t)it[7] << 32) | (uint32_t)it[6]);
   if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 || start < 0 ||
-      start + len > P.kv_rows) return;
-  for (int r = row0 + (threadIdx.x >> 6); r < min(row0 + kItemRows, n_new * P.group); r += 4) {
-    const int t = r / P.group, head = kvh * P.group + r % P.group;
-    const int64_t starts[2] = {start, 0}, keys[2] = {max(len - n_new + t + 1, 0), 0};
-    const float* q = row_to_lds<T, D>(P, lds, q0 + t, head);
-    attend_row<T, D>(P, q, kvh, starts, keys, const_cast<char*>(P.out.p) + (q0 + t) * P.out.row + head * P.out.head);
+      start > P.kv_rows - len || row0 >= n_new * P.group || (parts && (part >= parts || slot != (int)blockIdx.x - P.n_whole))) return;
+  const Unit u{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
+               n_new * P.group, row0, kvh};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int last = min(row0 + kItemRows, u.rows) - 1;
+  const int k_hi = max(min(u.lim0 + (int)((uint32_t)last / (uint32_t)P.group), len), 0);
+  const int n_t = (k_hi + R::kBN - 1) / R::kBN;
+  const int t0 = parts ? (int)((int64_t)n_t * part / parts) : 0, t1 = parts ? (int)((int64_t)n_t * (part + 1) / parts) : n_t;
+  Wave<T, D> w;
+  w.init(P, u, row0 + wave * 32);
+  R::run(P, u, w, smem, t0, t1, false);
+  // A value that is not finite may come from a key that its row does not see: once more, telling them apart.
+  if (__syncthreads_or(!w.finite())) {
+    w.core.clear();
+    w.m = -INFINITY;
+    R::run(P, u, w, smem, t0, t1, true);
+  }
+  const int r = wave * 32 + (threadIdx.x & 31);
+  const int64_t at = (int64_t)slot * kItemRows + r;
+  write_rows<T, D>(P, u, w, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * R::kBN);
+}
+
+// One row's parts joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, in part order. One wave; part p's state is
+// ml[p * stride], its output o[p * stride * D].
+template <typename T, int D>
+__device__ __forceinline__ void combine_row(const f32x2* ml, const float* o, int64_t stride, int parts, char* out) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  float M = -INFINITY;
+  for (int p = lane; p < parts; p += 64) M = fmaxf(M, ml[p * stride].x);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+  const float shift = M == -INFINITY ? 0.f : M;
+  float l = 0.f, acc[E] = {};
+  bool sees = false;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    const f32x2 st = p0 + lane < parts ? ml[(p0 + lane) * stride] : f32x2{-INFINITY, 0.f};
+    const float wt = __builtin_amdgcn_exp2f(st.x - shift);
+    sees = sees || __builtin_amdgcn_ballot_w64(__float_as_uint(st.y) != 0) != 0;
+    const int n = min(64, parts - p0);
+    for (int p = 0; p < n; ++p) {
+      const float w = __shfl(wt, p), lp = __shfl(st.y, p);
+      l += w * lp;
+      if (w == 0.f) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(w, o[(p0 + p) * stride * D + lane * E + e], acc[e]);
+    }
+  }
+  const float inv = 1.0f / l;
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(out)[lane * E + e] = sees ? acc[e] * inv : 0.f;
+  } else {
+    uint32_t w = 0;
+    if constexpr (E == 2) {
+      w = sees ? pack_bf16x2(acc[0] * inv, acc[1] * inv) : 0u;
+      reinterpret_cast<uint32_t*>(out)[lane] = w;
+    } else {
+      reinterpret_cast<bf16*>(out)[lane] = (bf16)(sees ? acc[0] * inv : 0.f);
+    }
+  }
+}
+
+// The rows of split tiles: the workgroup of a part joins its share of the tile's 128 rows.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void causal_combine_kernel(AttnParams P) {
+  const int32_t* it = P.items + 8 * ((int64_t)P.n_whole + blockIdx.x);
+  const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
+  const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
+  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || part >= parts ||
+      slot != (int)blockIdx.x || part > slot || slot - part + parts > (int)gridDim.x) return;
+  const Unit u{nullptr, nullptr, len, 0, q0, n_new * P.group, row0, kvh};
+  const int r1 = min(kItemRows * (part + 1) / parts, u.rows - row0);
+  for (int r = kItemRows * part / parts + (threadIdx.x >> 6); r < r1; r += 4) {
+    const int64_t at = (int64_t)(slot - part) * kItemRows + r;
+    combine_row<T, D>(P.part_ml + at, P.part_o + at * D, kItemRows, parts, out_row<T, D>(P, u, row0 + r));
+  }
+}
+
+
+// The four waves' results of the same rows joined in LDS (free by then), and written: to the output, or as a part.
+template <typename T, int D>
+__device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int part, int ka) {
+  constexpr int kC = D / 4;                    // 16-byte chunks of a row, XOR-swizzled by the row
+  __shared__ float sm[4][32], sl[4][32];
+  __shared__ int slim[32];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = min(32, u.rows - first_row);
+  const float lw = w.core.row_sum();
+  if (lane < 32) {
+    sm[wave][l32] = w.m;
+    sl[wave][l32] = lw;
+    slim[l32] = w.lim;
+  }
+  __syncthreads();                             // every wave is past its tiles
+  float* const so = reinterpret_cast<float*>(smem);
+  if (l32 < n)
+    w.core.each4([&](int d, const f32x4& x) {
+      *reinterpret_cast<f32x4*>(so + ((wave * 32 + l32) * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 4) = x;
+    });
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * kC; i += 256) {
+    const int r = i / kC, c = i % kC;
+    float M = sm[0][r];
+#pragma unroll
+    for (int x = 1; x < 4; ++x) M = fmaxf(M, sm[x][r]);
+    const float shift = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sm[x][r] - shift);
+      l += f * sl[x][r];
+      // a wave that saw none of the row's keys has zeros; one whose maximum is far below the others' may hold infinities
+      const f32x4 o = *reinterpret_cast<const f32x4*>(so + ((x * 32 + r) * kC + (c ^ (r & (kC - 1)))) * 4);
+      if (f != 0.f) acc += f * o;
+    }
+    const int row = first_row + r, t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
+    const bool sees = slim[r] > ka;
+    if (P.part_o) {
+      const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + g;
+      *reinterpret_cast<f32x4*>(P.part_o + at * D + c * 4) = acc;
+      if (c == 0) P.part_ml[at] = part_state(M, l, sees);
+    } else {
+      const float inv = 1.0f / l;
+      store4<T>(out_row<T, D>(P, u, row), c * 4, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+  __syncthreads();                             // the tiles may be written again
+}
+
+// A row of no keys in this part (l = 0), or of keys that may not be read (NaN).
+template <typename T, int D>
+__device__ __forceinline__ void write_fixed(const AttnParams& P, const Unit& u, int part, float value) {
+  for (int row = threadIdx.x; row < u.rows; row += 256) {
+    const int t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
+    if (P.part_o) {
+      const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + g;
+      P.part_ml[at] = f32x2{value == 0.f ? -INFINITY : value, value};
+    } else {
+      char* out = out_row<T, D>(P, u, row);
+      for (int d = 0; d < D; d += 4) store4<T>(out, d, f32x4{value, value, value, value});
+    }
+  }
+}
+
+// The token range of sequences [s0, s1), empty where it is none of [0, n_tokens).
+__device__ __forceinline__ int64_t tokens_of(const AttnParams& P, int s0, int s1, int64_t& first) {
+  const int64_t a = P.cu_q ? P.cu_q[s0] : s0, b = P.cu_q ? P.cu_q[s1] : s1;
+  first = a;
+  return a < 0 || b > P.n_tokens || b < a ? 0 : b - a;
+}
+
+// Workgroups [0, prefix units): a part of a group's prefix for a tile of the group's rows (ROWS: tiles of 128, else of 32);
+// the others: a part of a sequence's own keys for its rows. The key/value head runs fastest, then the part, so that the
+// tiles of one part of the prefix meet in one L2 where heads x parts fill the 8 XCDs evenly.
+template <typename T, int D, bool ROWS>
+__device__ __forceinline__ void decode_unit(const AttnParams& P) {
+  using R = RowsUnit<T, D>;
+  using K = KeysUnit<T, D>;
+  __shared__ __attribute__((aligned(16))) char smem[K::kLds > R::kLds ? K::kLds : R::kLds];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int prefix_units = P.hkv * P.prefix_parts * P.prefix_tiles * P.n_groups;
+  Unit u;
+  u.kvh = id % P.hkv;
+  if (id < prefix_units) {
+    id /= P.hkv;
+    const int part = id % P.prefix_parts, tile0 = id / P.prefix_parts % P.prefix_tiles, g = id / P.prefix_parts / P.prefix_tiles;
+    const int s0 = min(max(P.cu_groups[g], 0), P.n_seqs), s1 = min(max(P.cu_groups[g + 1], 0), P.n_seqs);
+    u.rows = s1 > s0 ? (int)tokens_of(P, s0, s1, u.token0) * P.group : 0;
+    if (u.rows == 0) return;
+    const int64_t start = P.prefix_start[g];
+    u.len = P.prefix_len[g];
+    u.lim0 = u.len;
+    if (u.len < 0 || u.len > kItemMaxLen || start < 0 || start > P.kv_rows - u.len) {
+      write_fixed<T, D>(P, u, part, NAN);
+      return;
+    }
+    const int ka = min((int64_t)part * P.prefix_chunk, (int64_t)u.len);
+    const int kb = part + 1 == P.prefix_parts ? u.len : min((int64_t)ka + P.prefix_chunk, (int64_t)u.len);
+    if (ka >= kb) {
+      write_fixed<T, D>(P, u, part, 0.f);
+      return;
+    }
+    u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
+    u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
+    if constexpr (ROWS) {
+      for (int row0 = tile0 * kItemRows; row0 < u.rows; row0 += P.prefix_tiles * kItemRows) {
+        Wave<T, D> w;
+        w.init(P, u, row0 + wave * 32);
+        R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN, false);
+        const int row = row0 + wave * 32 + (threadIdx.x & 31);
+        const int t = (int)((uint32_t)min(row, u.rows - 1) / (uint32_t)P.group), h = min(row, u.rows - 1) - t * P.group;
+        const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + h;
+        write_rows<T, D>(P, u, w, row, P.part_o + at * D, P.part_ml + at, true);
+      }
+    } else {
+      for (int row0 = tile0 * 32; row0 < u.rows; row0 += P.prefix_tiles * 32) {
+        Wave<T, D> w;
+        w.init(P, u, row0);
+        K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
+        join_waves<T, D>(P, u, w, smem, row0, part, ka);
+      }
+    }
+    return;
+  }
+  id = (id - prefix_units) / P.hkv;
+  u.kvh = (blockIdx.x - prefix_units) % P.hkv;
+  const int own = id % P.own_parts, seq = id / P.own_parts, part = P.prefix_parts + own;
+  const int n_new = (int)tokens_of(P, seq, seq + 1, u.token0);
+  u.rows = n_new * P.group;
+  if (u.rows == 0) return;
+  const int64_t start = P.k_start[seq];
+  u.len = P.k_len[seq];
+  if (u.len < 0 || u.len > kItemMaxLen || start < 0 || start > P.kv_rows - u.len) {
+    write_fixed<T, D>(P, u, part, NAN);
+    return;
+  }
+  u.lim0 = u.len - n_new + 1;
+  const int ka = min((int64_t)own * P.own_chunk, (int64_t)u.len);
+  const int kb = own + 1 == P.own_parts ? u.len : min((int64_t)ka + P.own_chunk, (int64_t)u.len);
+  if (ka >= kb) {
+    write_fixed<T, D>(P, u, part, 0.f);
+    return;
+  }
+  u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
+  u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
+  for (int row0 = 0; row0 < u.rows; row0 += 32) {
+    Wave<T, D> w;
+    w.init(P, u, row0);
+    K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
+    join_waves<T, D>(P, u, w, smem, row0, part, ka);
   }
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void decode_kernel(AttnParams P) {
-  __shared__ float lds[4][D];
-  const int seq = blockIdx.x, kvh = blockIdx.y;
-  const int64_t q0 = P.cu_q ? P.cu_q[seq] : seq, q1 = P.cu_q ? P.cu_q[seq + 1] : seq + 1;
-  if (q0 < 0 || q1 > P.n_tokens) return;
-  int64_t starts[2] = {0, P.k_start[seq]};
-  int64_t len = P.k_len[seq], prefix = 0;
-  for (int g = 0; g < P.n_groups; ++g)
-    if (P.cu_groups[g] <= seq && seq < P.cu_groups[g + 1]) {
-      starts[0] = P.prefix_start[g];
-      prefix = P.prefix_len[g];
-    }
-  const bool bad = len < 0 || starts[1] < 0 || starts[1] > P.kv_rows - len || prefix < 0 || starts[0] < 0 ||
-                   starts[0] > P.kv_rows - prefix;
-  const int64_t rows = (q1 - q0) * P.group;
-  for (int64_t r = threadIdx.x >> 6; r < rows; r += 4) {
-    const int64_t t = r / P.group;
-    const int head = kvh * P.group + (int)(r % P.group);
-    char* out = const_cast<char*>(P.out.p) + (q0 + t) * P.out.row + head * P.out.head;
-    if (bad) {
-      for (int d = threadIdx.x & 63; d < D; d += 64) reinterpret_cast<T*>(out)[d] = (T)NAN;
-      continue;
-    }
-    const int64_t keys[2] = {prefix, max(len - (q1 - q0) + t + 1, (int64_t)0)};
-    const float* q = row_to_lds<T, D>(P, lds, q0 + t, head);
-    attend_row<T, D>(P, q, kvh, starts, keys, out);
+__global__ __launch_bounds__(256, 2) void decode_rows_kernel(AttnParams P) { decode_unit<T, D, true>(P); }
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void decode_keys_kernel(AttnParams P) { decode_unit<T, D, false>(P); }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void decode_combine_kernel(AttnParams P) {
+  const int64_t heads = P.hkv * P.group, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t end = P.cu_q ? min((int64_t)P.cu_q[P.n_seqs], P.n_tokens) : P.n_tokens;
+  const int64_t token = row / heads, first = P.cu_q ? max(P.cu_q[0], 0) : 0;
+  if (token >= end || token < first) return;
+  combine_row<T, D>(P.part_ml + row, P.part_o + row * D, P.n_tokens * heads, P.prefix_parts + P.own_parts,
+                    const_cast<char*>(P.out.p) + token * P.out.row + (row - token * heads) * P.out.head);
+}
+
+// How a decode launch is laid out: from the sizes alone, so that the workspace can be told beforehand.
+struct DecodePlan {
+  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;
+  bool prefix_rows;
+  int64_t units;
+  size_t part_rows;      // 0: no parts, the kernel writes the output
+};
+
+// Parts of at least 128 keys (a block of 32 a wave), as many as fill the workgroup slots once.
+static int split_parts(int64_t keys, int64_t units, int64_t slots, int64_t least, int& chunk) {
+  int64_t parts = std::max(slots / std::max<int64_t>(units, 1), least);
+  parts = std::min({parts, (keys + 127) / 128, (int64_t)64});
+  parts = std::max<int64_t>(parts, 1);
+  const int64_t c = round_up(std::max<int64_t>((keys + parts - 1) / parts, 1), 64);
+  chunk = (int)std::min<int64_t>(c, kItemMaxLen);
+  return (int)std::max<int64_t>((keys + c - 1) / c, 1);
+}
+
+static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
+                       int32_t num_heads, int32_t num_kv_heads, int32_t dtype, DecodePlan& D) {
+  if (n_tokens < 0 || n_seqs < 0 || n_groups < 0 || max_len < 0 || max_prefix < 0) return set_error(QVL_ERR_INVALID_ARG, "%s: bad sizes", what);
+  if (n_seqs > 65535 || n_groups > 65535) return set_error(QVL_ERR_UNSUPPORTED, "%s: more than 65535 sequences or groups", what);
+  if (max_len > kItemMaxLen || max_prefix > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: lengths", what);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
+    return set_error(QVL_ERR_INVALID_ARG, "%s: %d heads over %d key/value heads", what, num_heads, num_kv_heads);
+  if (num_heads > kItemHeadMask || n_tokens > kItemMaxLen || n_tokens * (num_heads / num_kv_heads) > kItemMaxLen)
+    return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  const int64_t slots = (int64_t)gemm_device_cus() * (dtype == QVL_DTYPE_BF16 ? 2 : 1), rows = n_tokens * (num_heads / num_kv_heads);
+  D = DecodePlan{};
+  // sequences of unlike lengths: parts of at most 1024 keys even out what the workgroups do
+  D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, n_seqs > 1 ? (max_len + 1023) / 1024 : 1, D.own_chunk);
+  if (n_groups > 0) {
+    const int64_t mean = (rows + n_groups - 1) / n_groups;
+    D.prefix_rows = mean > 32;
+    const int64_t tile = D.prefix_rows ? kItemRows : 32;
+    D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
+    D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, slots, 1, D.prefix_chunk);
+  } else {
+    D.prefix_tiles = 1;
   }
+  D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
+  if (D.units > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  D.part_rows = n_groups > 0 || D.own_parts > 1 ? (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads : 0;
+  return QVL_OK;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -154,6 +829,8 @@ static int attn_params(const char* what, int32_t dtype, const void* q, int64_t q
       return set_error(QVL_ERR_INVALID_ARG, "%s: %s is NULL", what, w.name);
     if (w.row < 0 || w.head < 0 || w.row > 0x7fffffffLL || w.head > 0x7fffffffLL)
       return set_error(QVL_ERR_INVALID_ARG, "%s: strides of %s", what, w.name);
+    if ((w.to == &P.k || w.to == &P.v) && w.row * size > (int64_t)1 << 26)   // a tile's 64 rows are addressed in 32 bits
+      return set_error(QVL_ERR_UNSUPPORTED, "%s: rows of %s are more than 64 MiB apart", what, w.name);
     if ((uintptr_t)w.p % 16 || w.row * size % 16 || w.head * size % 16)
       return set_error(QVL_ERR_MISALIGNED, "%s: %s and its strides must be multiples of 16 bytes", what, w.name);
     *w.to = AttnView{(const char*)w.p, w.row * size, w.head * size};
@@ -188,7 +865,7 @@ int qvl_causal_workspace_size(int32_t head_dim, int64_t n_items, int64_t n_whole
   if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: bytes is NULL");
   if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "causal_workspace_size: head_dim=%d", head_dim);
   if (n_whole < 0 || n_items < n_whole) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: items");
-  *bytes = 0;
+  *bytes = (size_t)(n_items - n_whole) * kItemRows * ((size_t)head_dim + 2) * sizeof(float);
   return QVL_OK;
 }
 
@@ -204,15 +881,30 @@ int qvl_causal_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
   if (n_tokens == 0 || n_items == 0) return QVL_OK;
   if (!items) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: items is NULL");
   if ((uintptr_t)items % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: items");
+  size_t need = 0;
+  QVL_TRY_RC(qvl_causal_workspace_size(head_dim, n_items, n_whole, &need));
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(QVL_ERR_WORKSPACE, "causal_attention: workspace %zu < %zu", workspace_bytes, need);
+  if (need && (uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: workspace");
   P.items = items;
+  P.n_whole = (int)n_whole;
+  P.part_o = need ? (float*)workspace : nullptr;
+  P.part_ml = need ? (f32x2*)((float*)workspace + (n_items - n_whole) * kItemRows * head_dim) : nullptr;
   QVL_ATTN_LAUNCH(causal_kernel, dim3((unsigned)n_items));
-  return check_launch("causal_attention");
+  QVL_TRY_RC(check_launch("causal_attention"));
+  if (!need) return QVL_OK;
+  QVL_ATTN_LAUNCH(causal_combine_kernel, dim3((unsigned)(n_items - n_whole)));
+  return check_launch("causal_combine");
 }
 
 int qvl_decode_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, size_t* bytes) {
   if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "decode_workspace_size: bytes is NULL");
-  *bytes = 0;
+  if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: head_dim=%d", head_dim);
+  if (dtype != QVL_DTYPE_F32 && dtype != QVL_DTYPE_BF16) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: dtype %d", dtype);
+  DecodePlan plan;
+  QVL_TRY_RC(decode_plan("decode_workspace_size", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype, plan));
+  *bytes = plan.part_rows * ((size_t)head_dim + 2) * sizeof(float);
   return QVL_OK;
 }
 
@@ -226,8 +918,8 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
   AttnParams P{};
   QVL_TRY_RC(attn_params("decode_attention", dtype, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, kv_rows, out,
                          out_row, out_head, n_tokens, num_heads, num_kv_heads, head_dim, scale, P));
-  if (n_seqs < 0 || n_groups < 0 || max_len < 0 || max_prefix < 0) return set_error(QVL_ERR_INVALID_ARG, "decode_attention: bad sizes");
-  if (n_seqs > 65535 || n_groups > 65535) return set_error(QVL_ERR_UNSUPPORTED, "decode_attention: more than 65535 sequences or groups");
+  DecodePlan plan;
+  QVL_TRY_RC(decode_plan("decode_attention", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype, plan));
   if (!cu_q && n_tokens != n_seqs) return set_error(QVL_ERR_INVALID_ARG, "decode_attention: %lld tokens of %lld sequences without cu_q", (long long)n_tokens, (long long)n_seqs);
   if (n_tokens == 0 || n_seqs == 0) return QVL_OK;
   if (!k_start || !k_len || (n_groups > 0 && (!cu_groups || !prefix_start || !prefix_len)))
@@ -243,8 +935,24 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
   P.prefix_len = prefix_len;
   P.n_seqs = (int)n_seqs;
   P.n_groups = (int)n_groups;
-  QVL_ATTN_LAUNCH(decode_kernel, dim3((unsigned)n_seqs, (unsigned)num_kv_heads));
-  return check_launch("decode_attention");
+  const size_t need = plan.part_rows * ((size_t)head_dim + 2) * sizeof(float);
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(QVL_ERR_WORKSPACE, "decode_attention: workspace %zu < %zu", workspace_bytes, need);
+  if (need && (uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "decode_attention: workspace");
+  P.part_o = need ? (float*)workspace : nullptr;
+  P.part_ml = need ? (f32x2*)((float*)workspace + plan.part_rows * head_dim) : nullptr;
+  P.own_parts = plan.own_parts;
+  P.own_chunk = plan.own_chunk;
+  P.prefix_parts = plan.prefix_parts;
+  P.prefix_chunk = plan.prefix_chunk;
+  P.prefix_tiles = plan.prefix_tiles;
+  if (plan.prefix_rows) QVL_ATTN_LAUNCH(decode_rows_kernel, dim3((unsigned)plan.units));
+  else QVL_ATTN_LAUNCH(decode_keys_kernel, dim3((unsigned)plan.units));
+  QVL_TRY_RC(check_launch("decode_attention"));
+  if (!need) return QVL_OK;
+  const int64_t blocks = (n_tokens * num_heads + 3) / 4;
+  QVL_ATTN_LAUNCH(decode_combine_kernel, dim3((unsigned)blocks));
+  return check_launch("decode_combine");
 }
 
 }  // extern "C"
