@@ -508,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P) {
   const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
   const int64_t start = (int64_t)(((uint64_t)(uint32_t)it[7] << 32) | (uint32_t)it[6]);
   if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 || start < 0 ||
-      start > P.kv_rows - len || row0 >= n_new * P.group || (parts && (part >= parts || slot != (int)blockIdx.x - P.n_whole))) return;
+      start > P.kv_rows - len || row0 >= n_new * P.group || (parts && (part >= parts || slot < 0 || slot >= (int)gridDim.x - P.n_whole))) return;
   const Unit u{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
                n_new * P.group, row0, kvh};
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256) void causal_combine_kernel(AttnParams P) {
   const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
   const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
   if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || part >= parts ||
-      slot != (int)blockIdx.x || part > slot || slot - part + parts > (int)gridDim.x) return;
+      part > slot || slot - part + parts > (int)gridDim.x) return;
   const Unit u{nullptr, nullptr, len, 0, q0, n_new * P.group, row0, kvh};
   const int r1 = min(kItemRows * (part + 1) / parts, u.rows - row0);
   for (int r = kItemRows * part / parts + (threadIdx.x >> 6); r < r1; r += 4) {

@@ -5,11 +5,157 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
+#include <functional>
+#include <map>
+#include <queue>
 #include <vector>
 
 #include "qvl_decoder_items.h"
 
 using namespace qvl;
+
+namespace {
+
+struct Job {
+  int64_t seq;      // -1: none (padding of a queue)
+  int32_t row0, head, part, parts, slot;
+  int32_t steps;    // key tiles
+};
+
+// Greedy time of jobs, longest first, on `slots` workgroup slots.
+double makespan(std::vector<double> cost, int64_t slots) {
+  std::sort(cost.begin(), cost.end(), std::greater<double>());
+  std::priority_queue<double, std::vector<double>, std::greater<double>> free;
+  for (int64_t s = 0; s < slots; ++s) free.push(0.0);
+  double end = 0;
+  for (double c : cost) {
+    const double t = free.top() + c;
+    free.pop();
+    free.push(t);
+    end = std::max(end, t);
+  }
+  return end;
+}
+
+// Where the jobs do not fill the slots evenly (few rows over many keys, or a prompt of a few tiles whose last one is the
+// longest), long jobs are split along their keys. Candidates are part lengths of the mean load of a slot and fractions of
+// it; the one of least modelled time is taken, unsplit among them. The model's constants, in steps of one tile of 64
+// (fp32: 32) keys by 128 rows with two workgroups a CU: what a job costs beside its steps, a part's written and joined
+// rows, and the join's launch.
+void split_jobs(std::vector<Job>& jobs, std::vector<Job>& parts, int64_t total, int64_t slots, int32_t dtype) {
+  if (jobs.empty() || (int64_t)jobs.size() > 8 * slots) return;
+  const bool half = dtype == QVL_DTYPE_BF16;
+  const double fixed = half ? 1.5 : 0.3, join = half ? 2.5 : 0.6, each = half ? 0.015 : 0.004;
+  const int32_t least = 4;
+  std::vector<double> cost;
+  for (const Job& j : jobs) cost.push_back(j.steps + fixed);
+  double best = makespan(cost, slots);
+  int32_t best_len = 0;
+  const double mean = (double)total / slots;
+  int32_t tried = 0;
+  for (double f : {1.0, 0.75, 0.5, 0.334, 0.25, 0.167, 0.125}) {
+    const int32_t length = std::max((int32_t)std::ceil(mean * f), least);
+    if (length == tried) continue;
+    tried = length;
+    cost.clear();
+    int64_t n_parts = 0;
+    for (const Job& j : jobs) {
+      const int32_t p = std::min<int32_t>((j.steps + length - 1) / length, 255);
+      if (p < 2) {
+        cost.push_back(j.steps + fixed);
+        continue;
+      }
+      for (int32_t k = 0; k < p; ++k) cost.push_back((double)j.steps / p + fixed);
+      n_parts += p;
+    }
+    if (n_parts == 0) continue;
+    const double t = makespan(cost, slots) + join + each * n_parts;
+    if (t < best) {
+      best = t;
+      best_len = length;
+    }
+  }
+  if (best_len == 0) return;
+  std::vector<Job> whole;
+  for (const Job& j : jobs) {
+    const int32_t p = std::min<int32_t>((j.steps + best_len - 1) / best_len, 255);
+    if (p < 2) {
+      whole.push_back(j);
+      continue;
+    }
+    for (int32_t k = 0; k < p; ++k) {
+      Job one = j;
+      one.part = k;
+      one.parts = p;
+      one.slot = (int32_t)parts.size();
+      one.steps = (int32_t)((int64_t)j.steps * (k + 1) / p - (int64_t)j.steps * k / p);
+      parts.push_back(one);
+    }
+  }
+  jobs.swap(whole);
+}
+
+// Jobs dealt to 8 queues, one per XCD (the dispatcher gives workgroup k to XCD k % 8): the jobs of one sequence and
+// key/value head go to one queue, whose L2 then holds their keys, the longest such group to the queue with least to do;
+// where queues come out unlike, jobs of the fullest move to the emptiest. A queue's longest jobs come first; short queues
+// are padded.
+std::vector<Job> deal(const std::vector<Job>& jobs) {
+  if (jobs.empty()) return {};
+  std::map<std::pair<int64_t, int32_t>, std::vector<Job>> by_group;
+  for (const Job& j : jobs) by_group[{j.seq, j.head}].push_back(j);
+  std::vector<std::pair<int64_t, std::vector<Job>*>> groups;
+  for (auto& g : by_group) {
+    int64_t w = 0;
+    for (const Job& j : g.second) w += j.steps + 1;
+    groups.push_back({w, &g.second});
+  }
+  std::stable_sort(groups.begin(), groups.end(),
+                   [](const std::pair<int64_t, std::vector<Job>*>& a, const std::pair<int64_t, std::vector<Job>*>& b) { return a.first > b.first; });
+  std::array<std::vector<Job>, kAttnQueues> queue;
+  std::array<int64_t, kAttnQueues> load{};
+  int64_t all = 0;
+  for (auto& g : groups) {
+    const size_t q = std::min_element(load.begin(), load.end()) - load.begin();
+    load[q] += g.first;
+    all += g.first;
+    queue[q].insert(queue[q].end(), g.second->begin(), g.second->end());
+  }
+  auto longer = [](const Job& a, const Job& b) { return a.steps > b.steps; };
+  for (auto& q : queue) std::stable_sort(q.begin(), q.end(), longer);
+  for (int round = 0; round < 64; ++round) {
+    const size_t hi = std::max_element(load.begin(), load.end()) - load.begin();
+    const size_t lo = std::min_element(load.begin(), load.end()) - load.begin();
+    const int64_t half = (load[hi] - load[lo]) / 2;
+    if (half <= all / 400) break;
+    // every other job of the fullest queue, so that what is left and what moves are alike, up to half the difference
+    std::vector<Job> keep, move;
+    int64_t moved = 0;
+    for (size_t k = 0; k < queue[hi].size(); ++k) {
+      const Job& j = queue[hi][k];
+      if (k % 2 == 1 && moved + j.steps + 1 <= half) {
+        move.push_back(j);
+        moved += j.steps + 1;
+      } else {
+        keep.push_back(j);
+      }
+    }
+    if (move.empty()) break;
+    queue[hi].swap(keep);
+    queue[lo].insert(queue[lo].end(), move.begin(), move.end());
+    std::stable_sort(queue[lo].begin(), queue[lo].end(), longer);
+    load[hi] -= moved;
+    load[lo] += moved;
+  }
+  size_t longest = 0;
+  for (auto& q : queue) longest = std::max(longest, q.size());
+  std::vector<Job> out(longest * kAttnQueues, Job{-1, 0, 0, 0, 0, -1, 0});
+  for (size_t k = 0; k < out.size(); ++k)
+    if (k / kAttnQueues < queue[k % kAttnQueues].size()) out[k] = queue[k % kAttnQueues][k / kAttnQueues];
+  return out;
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -47,25 +193,53 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
   if (num_heads > kItemHeadMask) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: num_heads=%d", num_heads);
   if (n_cus <= 0) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_cus=%d", n_cus);
   const int64_t group = num_heads / num_kv_heads;
-  std::vector<std::array<int32_t, 8>> list;
-  int64_t q0 = 0;
+  const int64_t step_keys = dtype == QVL_DTYPE_BF16 ? 64 : 32;
+  std::vector<Job> jobs;
+  std::vector<int64_t> q_first;
+  int64_t q0 = 0, total = 0;
   for (int64_t i = 0; i < n_seqs; ++i) {
     if (n_new[i] < 0 || len[i] < 0 || start[i] < 0 || start[i] > (int64_t)1 << 56)
       return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: sequence %lld: %lld new, %lld keys from row %lld", (long long)i,
                        (long long)n_new[i], (long long)len[i], (long long)start[i]);
     if (len[i] > kItemMaxLen || q0 + n_new[i] > kItemMaxLen || n_new[i] * group > kItemMaxLen)
       return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: sequence %lld is too long", (long long)i);
-    for (int64_t r = 0; r < n_new[i] * group; r += kItemRows)
-      for (int32_t h = 0; h < num_kv_heads; ++h)
-        list.push_back({(int32_t)q0, (int32_t)n_new[i], (int32_t)len[i], (int32_t)r, h, -1,
-                        (int32_t)(uint32_t)(start[i] & 0xffffffff), (int32_t)(start[i] >> 32)});
+    q_first.push_back(q0);
+    for (int64_t r = 0; r < n_new[i] * group; r += kItemRows) {
+      const int64_t last = (std::min(r + kItemRows, n_new[i] * group) - 1) / group;
+      const int64_t keys = std::max<int64_t>(std::min(len[i] - n_new[i] + 1 + last, len[i]), 0);
+      const int32_t steps = (int32_t)((keys + step_keys - 1) / step_keys);
+      for (int32_t h = 0; h < num_kv_heads; ++h) jobs.push_back({i, (int32_t)r, h, 0, 0, -1, steps});
+      total += steps * (int64_t)num_kv_heads;
+    }
     q0 += n_new[i];
   }
-  *n_items = *n_whole = (int64_t)list.size();
+  std::vector<Job> parts;
+  split_jobs(jobs, parts, total, (int64_t)n_cus * (head_dim == 64 ? 3 : 2), dtype);
+  std::vector<Job> list = deal(jobs);
+  const std::vector<Job> tail = deal(parts);
+  *n_whole = (int64_t)list.size();
+  for (const Job& j : tail)
+    if (j.seq >= 0) list.push_back(j);
+  *n_items = (int64_t)list.size();
   if (!items) return QVL_OK;
   if (capacity < *n_items)
     return set_error(QVL_ERR_INVALID_ARG, "causal_worklist capacity %lld < %lld", (long long)capacity, (long long)*n_items);
-  for (size_t k = 0; k < list.size(); ++k) std::copy(list[k].begin(), list[k].end(), items + 8 * k);
+  for (size_t k = 0; k < list.size(); ++k) {
+    const Job& j = list[k];
+    int32_t* it = items + 8 * k;
+    if (j.seq < 0) {
+      memset(it, 0, 8 * sizeof(int32_t));
+      continue;
+    }
+    it[0] = (int32_t)q_first[j.seq];
+    it[1] = (int32_t)n_new[j.seq];
+    it[2] = (int32_t)len[j.seq];
+    it[3] = j.row0;
+    it[4] = j.head | j.part << kItemPartShift | j.parts << kItemPartsShift;
+    it[5] = j.slot;
+    it[6] = (int32_t)(uint32_t)(start[j.seq] & 0xffffffff);
+    it[7] = (int32_t)(start[j.seq] >> 32);
+  }
   return QVL_OK;
 }
 
