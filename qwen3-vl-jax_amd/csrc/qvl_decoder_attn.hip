@@ -40,6 +40,12 @@ struct AttnParams {
 
 template <int V> using int_c = std::integral_constant<int, V>;
 
+// The larger of the two lanes of a row.
+__device__ __forceinline__ float across_halves(float x) {
+  const u32x2 p = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
 // What one wave does with 32 rows and a block of 32 keys in LDS. S^T = K Q^T puts a row in a lane (column lane % 32) with
 // 16 of the block's keys: register r is key 8 (r / 4) + 4 (lane / 32) + r % 4. The second product O^T = V^T P^T takes P as
 // it lies in those registers, as its B operand; only V has to come transposed.
@@ -65,6 +71,9 @@ template <int D> struct Core<bf16, D> {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const bf16x8*>(qrow + (ks * 16 + hh * 8) * 2);
+    // used here, so that the wait for these loads stands before the loop: inside it, it would be one for the DMA in flight
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
     clear();
   }
   __device__ __forceinline__ void clear() {
@@ -111,13 +120,76 @@ template <int D> struct Core<bf16, D> {
   }
   __device__ __forceinline__ void add_weights(const u32x4& pw) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    float t = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t w = pw[j];   // a copy: __builtin_bit_cast of a vector's element takes element 0 here
-      t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), t, false);
+      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);
     }
-    l += t;
+  }
+  // The scores of both blocks of a tile of 64 keys: a block's fragments are read ahead of its products.
+  // `beside(i)`, i < 8, runs among the products.
+  template <typename F> __device__ __forceinline__ void scores2(const char* lds, f32x16 (&s)[2], F&& beside) const {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+    const char* row = lds + l32 * kRowBytes;
+    bf16x8 a[D / 16], c[D / 16];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) a[ks] = *reinterpret_cast<const bf16x8*>(row + (((ks * 2 + hh) ^ k_swz(l32)) << 4));
+    __builtin_amdgcn_sched_barrier(0);
+    s[0] = f32x16{};
+    s[1] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      c[ks] = *reinterpret_cast<const bf16x8*>(row + 32 * kRowBytes + (((ks * 2 + hh) ^ k_swz(l32)) << 4));
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks], q[ks], s[0], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (ks % (D / 64) == D / 64 - 1) beside(ks / (D / 64));
+    }
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[ks], q[ks], s[1], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (ks % (D / 64) == D / 64 - 1) beside(4 + ks / (D / 64));
+    }
+  }
+  __device__ __forceinline__ void v_group(const char* lds, int g, bf16x8 (&v)[kDB]) const {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) v[db] = v_frag(lds, db, g);
+  }
+  static __device__ __forceinline__ u32x4 pack8(const f32x16& s, int e, float scale, float shift) {
+    float p[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * e + r], scale, shift));
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
+    return w;
+  }
+  // Weights and their product with V, 16 keys at a time: a group's weights are formed and its V read beside the products of
+  // the group before. v0: V's first group.
+  __device__ __forceinline__ void pv2(const char* lds, bf16x8 (&v0)[kDB], const f32x16 (&s)[2], float scale, float shift) {
+    u32x4 pw = pack8(s[0], 0, scale, shift);
+    bf16x8 v1[kDB];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 (&now)[kDB] = g & 1 ? v1 : v0;
+      bf16x8 (&next)[kDB] = g & 1 ? v0 : v1;
+      if (g < 3) v_group(lds, g + 1, next);
+      add_weights(pw);
+      const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now[db], pf, o[db], 0, 0, 0);
+      if (g < 3) pw = pack8(s[(g + 1) >> 1], (g + 1) & 1, scale, shift);
+      if (g < 3) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * kDB, 0);
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 24 / kDB, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
   // The same where some rows do not see all of the block's keys and V may hold infinities or NaN, which a weight of zero
   // does not silence: V's non-finite values are left out of the product and counted, row by row, among the keys that the
@@ -196,6 +268,8 @@ template <int D> struct Core<float, D> {
     const int hh = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) q[j] = *reinterpret_cast<const f32x4*>(qrow + (j * 8 + hh * 4) * 4);
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) asm volatile("" : "+v"(q[j]));   // as above
     clear();
   }
   __device__ __forceinline__ void clear() {
@@ -315,14 +389,23 @@ template <typename T, int D> struct Wave {
     m = -INFINITY;
     core.init(q);
   }
-  // NB blocks of 32 keys from key kb on; K and V tiles in LDS. `between` runs once the scores are read out of K's tile,
-  // `before_v` before V's is read.
-  template <int NB, typename F, typename G>
-  __device__ __forceinline__ void step(const char* klds, const char* vlds, int kb, float scale, bool safe, F&& between, G&& before_v) {
+  // NB blocks of 32 keys from key kb on; K and V tiles in LDS. `between(i)`, i < 8, runs beside the scores' products, or
+  // after them, once they are read out of K's tile; `before_v` before V's is read.
+  // SAFE: V may hold what is not finite.
+  template <int NB, bool SAFE, typename F, typename G>
+  __device__ __forceinline__ void step(const char* klds, const char* vlds, int kb, float scale, F&& between, G&& before_v) {
     f32x16 s[NB];
+    constexpr bool kAhead = NB == 2 && !SAFE && std::is_same<T, bf16>::value;
+    bf16x8 v0[D / 32];
+    if constexpr (kAhead) {
+      core.scores2(klds, s, between);
+      core.v_group(vlds, 0, v0);
+    } else {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = core.scores(klds, b);
-    between();
+      for (int b = 0; b < NB; ++b) s[b] = core.scores(klds, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) between(i);
+    }
     const bool edge = kb + 32 * NB > lim_lo;
     uint32_t seen[NB];
     if (edge) {
@@ -338,12 +421,16 @@ template <typename T, int D> struct Wave {
         }
       }
     }
-    float mx = s[0][0];
+    float m4[4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int c = 0; c < 4; ++c) {
+      m4[c] = s[0][c];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = b ? 0 : 4; r < 16; r += 4) m4[c] = fmaxf(m4[c], s[b][r + c]);
+    }
+    const float mx = across_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * scale;
     // A row's maximum moves only where it grew by more than 2^8: until then weights of up to 2^8 lose nothing (fp32 sums,
     // and bf16 weights of the same relative rounding), and the accumulators need no pass. Row by row, so that a row's result
     // does not depend on the others of its wave.
@@ -353,12 +440,16 @@ template <typename T, int D> struct Wave {
       m = mn;
     }
     const float shift = m == -INFINITY ? 0.f : -m;
+    if constexpr (kAhead) {
+      core.pv2(vlds, v0, s, scale, shift);
+      return;
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], scale, shift));
     before_v();
-    if (edge && safe) {
+    if (SAFE && edge) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) core.pv_safe(vlds, b, s[b], seen[b]);
     } else {
@@ -376,26 +467,30 @@ template <typename T, int D> struct Wave {
   }
 };
 
-// The rows of a [rows, heads, dim] view as a buffer that ends after `rows` of them: loads past it give zeros.
-__device__ __forceinline__ u32x4 rows_rsrc(const char* base, int64_t stride, int rows, int row_bytes) {
-  return rsrc_words(base, rows > 0 ? (uint32_t)((int64_t)(min(rows, 64) - 1) * stride + row_bytes) : 0u);
-}
-
-// Where a lane's 16 bytes of row i of a DMA of 1 KiB come from: lane j fills chunk j % kChunks of row j / kChunks, which
-// holds the logical chunk the swizzle maps there.
-template <typename T, int D> struct Loader {
+// One DMA fills 1 KiB of a tile: lane j chunk j % kChunks of row j / kChunks, from the logical chunk that the swizzle maps
+// there. A K or V tile takes a whole number of them; `Loader` does the i-th.
+template <typename T, int D, bool V> struct Loader {
   using C = Core<T, D>;
-  static constexpr int kRowsPerDma = 1024 / C::kRowBytes;
+  static constexpr int kRows = 1024 / C::kRowBytes;   // rows of one DMA
+  u32x4 rsrc;
+  uint32_t stride, row_off, chunk;
 
-  // rows [r0, r0 + n) of the tile that starts at key kb, by one wave; n a multiple of kRowsPerDma
-  template <bool V>
-  static __device__ __forceinline__ void rows(const u32x4& rsrc, int64_t stride, int r0, int n, uint32_t lds) {
+  __device__ __forceinline__ Loader(const AttnView& x) {
     const int lane = threadIdx.x & 63;
-    for (int r = r0; r < r0 + n; r += kRowsPerDma) {
-      const int row = r + lane / C::kChunks;
-      const int c = (lane % C::kChunks) ^ (V ? C::v_swz(row) : C::k_swz(row & 31));
-      dma16(rsrc, (uint32_t)(row * (uint32_t)stride) + (uint32_t)(c << 4), 0, lds + r * C::kRowBytes);
-    }
+    stride = (uint32_t)x.row;
+    row_off = (uint32_t)(lane / C::kChunks) * stride;
+    chunk = (uint32_t)((lane % C::kChunks) ^ swz(lane / C::kChunks)) << 4;
+  }
+  static __device__ __forceinline__ int swz(int row) { return V ? C::v_swz(row) : C::k_swz(row); }
+  // `left` rows from `base` on; past them zeros arrive
+  __device__ __forceinline__ void at(const char* base, int left) {
+    rsrc = rsrc_words(base, left > 0 ? (uint32_t)((int64_t)(min(left, 64) - 1) * stride + C::kRowBytes) : 0u);
+  }
+  // rows [kRows i, kRows (i + 1)) of the tile at `lds`. (A DMA's rows lie in one aligned run of kRows, so the swizzle of
+  // row kRows i + r is that of kRows i XOR that of r.)
+  __device__ __forceinline__ void operator()(int i, uint32_t lds) const {
+    const uint32_t r = (uint32_t)(i * kRows);
+    dma16(rsrc, row_off + r * stride + (chunk ^ ((uint32_t)swz(r & 31) << 4)), 0, lds + r * C::kRowBytes);
   }
 };
 
@@ -412,27 +507,59 @@ template <typename T, int D> struct RowsUnit {
   static constexpr int kNB = std::is_same<T, float>::value ? 1 : 2, kBN = 32 * kNB;
   static constexpr int kTile = kBN * Core<T, D>::kRowBytes, kLds = 4 * kTile;
 
-  // tiles [t0, t1) of the unit; true where the whole workgroup's rows are done
-  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1, bool safe) {
+  static constexpr int kDmas = kTile / 1024 / 4;   // of each wave and tile
+
+  // Tiles [t0, t1) of the unit. The next tile's DMAs stand among this one's products: issued together they would hold the
+  // wave for as long as they take to address (8 of them: 900 cycles of 3850 a tile).
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds0 = lds_addr_of(smem);
-    auto load = [&](int t, int stage) {
-      const int kb = t * kBN;
-      const u32x4 rk = rows_rsrc(u.k + (int64_t)kb * P.k.row, P.k.row, u.len - kb, Core<T, D>::kRowBytes);
-      const u32x4 rv = rows_rsrc(u.v + (int64_t)kb * P.v.row, P.v.row, u.len - kb, Core<T, D>::kRowBytes);
-      const uint32_t l = lds0 + stage * 2 * kTile;
-      Loader<T, D>::template rows<false>(rk, P.k.row, wave * (kBN / 4), kBN / 4, l);
-      Loader<T, D>::template rows<true>(rv, P.v.row, wave * (kBN / 4), kBN / 4, l + kTile);
+    Loader<T, D, false> lk(P.k);
+    Loader<T, D, true> lv(P.v);
+    const auto aim = [&](int t) {
+      const int kb = t * kBN, left = t < t1 ? u.len - kb : 0;
+      lk.at(u.k + (int64_t)kb * P.k.row, left);
+      lv.at(u.v + (int64_t)kb * P.v.row, left);
     };
-    if (t0 < t1) load(t0, 0);
+    const auto load = [&](int i, int stage) {   // i < 2 kDmas
+      if (i < kDmas) lk(wave * kDmas + i, lds0 + stage * 2 * kTile);
+      else if (i < 2 * kDmas) lv(wave * kDmas + i - kDmas, lds0 + stage * 2 * kTile + kTile);
+    };
+    aim(t0);
+#pragma unroll
+    for (int i = 0; i < 2 * kDmas; ++i) load(i, 0);
     wait_dma();
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int stage = (t - t0) & 1;
-      if (t + 1 < t1) load(t + 1, stage ^ 1);
       const char* k = smem + stage * 2 * kTile;
-      if (t * kBN < w.lim_hi) w.template step<kNB>(k, k + kTile, t * kBN, P.scale, safe, [] {}, [] {});
+      aim(t + 1);
+      if (t * kBN < w.lim_hi) {
+        w.template step<kNB, false>(k, k + kTile, t * kBN, P.scale, [&](int i) { load(i, stage ^ 1); }, [] {});
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * kDmas; ++i) load(i, stage ^ 1);
+      }
       wait_dma();
+      __syncthreads();
+    }
+  }
+  // The same, telling apart what a row sees where V is not finite; a tile at a time.
+  static __device__ __forceinline__ void run_safe(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lds0 = lds_addr_of(smem);
+    Loader<T, D, false> lk(P.k);
+    Loader<T, D, true> lv(P.v);
+    for (int t = t0; t < t1; ++t) {
+      lk.at(u.k + (int64_t)(t * kBN) * P.k.row, u.len - t * kBN);
+      lv.at(u.v + (int64_t)(t * kBN) * P.v.row, u.len - t * kBN);
+      for (int i = wave * kDmas; i < (wave + 1) * kDmas; ++i) {
+        lk(i, lds0);
+        lv(i, lds0 + kTile);
+      }
+      wait_dma();
+      __syncthreads();
+      if (t * kBN < w.lim_hi) w.template step<kNB, true>(smem, smem + kTile, t * kBN, P.scale, [](int) {}, [] {});
       __syncthreads();
     }
   }
@@ -448,35 +575,45 @@ template <typename T, int D> struct KeysUnit {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const char* k = smem + wave * 2 * kTile;
     const uint32_t kl = lds_addr_of(k), vl = kl + kTile;
-    auto load_k = [&](int t) {
-      Loader<T, D>::template rows<false>(rows_rsrc(u.k + (int64_t)(t * 32) * P.k.row, P.k.row, u.len - t * 32, Core<T, D>::kRowBytes),
-                                         P.k.row, 0, 32, kl);
+    Loader<T, D, false> lk(P.k);
+    Loader<T, D, true> lv(P.v);
+    const auto load_k = [&](int t) {
+      lk.at(u.k + (int64_t)(t * 32) * P.k.row, u.len - t * 32);
+#pragma unroll
+      for (int i = 0; i < kDmas; ++i) lk(i, kl);
     };
-    auto load_v = [&](int t) {
-      Loader<T, D>::template rows<true>(rows_rsrc(u.v + (int64_t)(t * 32) * P.v.row, P.v.row, u.len - t * 32, Core<T, D>::kRowBytes),
-                                        P.v.row, 0, 32, vl);
+    const auto load_v = [&](int t) {
+      lv.at(u.v + (int64_t)(t * 32) * P.v.row, u.len - t * 32);
+#pragma unroll
+      for (int i = 0; i < kDmas; ++i) lv(i, vl);
     };
     t0 += wave;
     if (t0 >= t1) return;
     load_k(t0);
     load_v(t0);
     // In flight, oldest first: K(t), V(t) at the top; V(t), K(t + 1) before V is read.
-    const bool safe = w.lim_lo < u.len;
-    for (int t = t0; t < t1; t += 4) {
+    int t = t0;
+    const auto each = [&](auto safe) {
       const bool more = t + 4 < t1;
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDmas) : "memory");
-      w.template step<1>(k, k + kTile, t * 32, P.scale, safe,
-                         [&] {
-                           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                           if (more) load_k(t + 4);
-                         },
-                         [&] {
-                           if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDmas) : "memory");
-                           else wait_dma();
-                         });
+      w.template step<1, decltype(safe)::value>(k, k + kTile, t * 32, P.scale,
+                                                [&](int i) {
+                                                  if (i) return;
+                                                  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                                                  if (more) load_k(t + 4);
+                                                },
+                                                [&] {
+                                                  if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDmas) : "memory");
+                                                  else wait_dma();
+                                                });
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) load_v(t + 4);
-    }
+      t += 4;
+    };
+    // blocks that every row sees whole, or that only end inside (what lies behind the keys reads as zeros); then the rest
+    const int whole = w.lim_lo < u.len ? min(w.lim_lo / 32, t1) : t1;
+    while (t < whole) each(std::false_type{});
+    while (t < t1) each(std::true_type{});
   }
 };
 
@@ -518,12 +655,12 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P) {
   const int t0 = parts ? (int)((int64_t)n_t * part / parts) : 0, t1 = parts ? (int)((int64_t)n_t * (part + 1) / parts) : n_t;
   Wave<T, D> w;
   w.init(P, u, row0 + wave * 32);
-  R::run(P, u, w, smem, t0, t1, false);
+  R::run(P, u, w, smem, t0, t1);
   // A value that is not finite may come from a key that its row does not see: once more, telling them apart.
-  if (__syncthreads_or(!w.finite())) {
+  if (__builtin_expect(__syncthreads_or(!w.finite()), 0)) {
     w.core.clear();
     w.m = -INFINITY;
-    R::run(P, u, w, smem, t0, t1, true);
+    R::run_safe(P, u, w, smem, t0, t1);
   }
   const int r = wave * 32 + (threadIdx.x & 31);
   const int64_t at = (int64_t)slot * kItemRows + r;
@@ -699,7 +836,7 @@ __device__ __forceinline__ void decode_unit(const AttnParams& P) {
       for (int row0 = tile0 * kItemRows; row0 < u.rows; row0 += P.prefix_tiles * kItemRows) {
         Wave<T, D> w;
         w.init(P, u, row0 + wave * 32);
-        R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN, false);
+        R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN);
         const int row = row0 + wave * 32 + (threadIdx.x & 31);
         const int t = (int)((uint32_t)min(row, u.rows - 1) / (uint32_t)P.group), h = min(row, u.rows - 1) - t * P.group;
         const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + h;
