@@ -18,6 +18,7 @@ allocator with every call, so calls on several streams and captured graphs share
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Sequence
 
 import numpy as np
@@ -25,6 +26,7 @@ import numpy as np
 from . import capi
 
 
+@functools.lru_cache(maxsize=None)
 def _torch():
     import torch
     return torch
@@ -47,41 +49,54 @@ def _device(device):
     return torch.device("cuda", torch.cuda.current_device()) if d.index is None else d
 
 
-def _heads_view(t, what: str, like=None, heads: Optional[int] = None, written: bool = False):
-    """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor, checked against `like`."""
-    if t.dim() != 3:
-        raise ValueError(f"{what} must be [rows, heads, head_dim], not {tuple(t.shape)}")
-    rows, n, dim = t.shape
+def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool = False):
+    """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor, checked against `like`: q's (dtype, device,
+    head_dim)."""
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what} must be [rows, heads, head_dim], not {tuple(shape)}")
+    rows, n, dim = shape
     row, head, one = t.stride()
-    if dim > 1 and one != 1:
+    if one != 1 and dim > 1:
         raise ValueError(f"{what}: the last axis must be contiguous")
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise TypeError(f"{what} is {t.dtype}, q is {like.dtype}")
-        if t.device != like.device:
-            raise ValueError(f"{what} on {t.device}, q on {like.device}")
-        if dim != like.shape[2]:
-            raise ValueError(f"{what}: head_dim {dim}, q has {like.shape[2]}")
+    if t.dtype != like[0]:
+        raise TypeError(f"{what} is {t.dtype}, q is {like[0]}")
+    if t.device != like[1]:
+        raise ValueError(f"{what} on {t.device}, q on {like[1]}")
+    if dim != like[2]:
+        raise ValueError(f"{what}: head_dim {dim}, q has {like[2]}")
     if heads is not None and n != heads:
         raise ValueError(f"{what}: {n} heads, expected {heads}")
     if t.requires_grad and _torch().is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
     # the stride of an axis of one entry is never used: torch may hold any value there
-    row, head = row if rows > 1 else 0, head if n > 1 else 0
-    if written and rows > 0 and n > 0:
+    if rows < 2:
+        row = 0
+    if n < 2:
+        head = 0
+    if written and row < head * n and rows > 0 and n > 0:   # (rows of whole, separate heads need no further look)
         inner, outer, count = (head, row, n) if n > 1 and (rows == 1 or head <= row) else (row, head, rows)
         if (n > 1 or rows > 1) and (inner < dim or (n > 1 and rows > 1 and outer < inner * (count - 1) + dim)):
             raise ValueError(f"{what}: its rows and heads lie over one another (strides {t.stride()})")
+    elif written and (rows > 1 or n > 1) and (head < dim if n > 1 else row < dim):
+        raise ValueError(f"{what}: its rows and heads lie over one another (strides {t.stride()})")
     return t.data_ptr(), row, head
 
 
-def _word(t, what: str, q, dtype, shape):
+def _like(q):
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"q must be [rows, heads, head_dim], not {tuple(shape)}")
+    return q.dtype, q.device, shape[2]
+
+
+def _word(t, what: str, like, dtype, shape):
     """Pointer of a contiguous device tensor of whole numbers beside q."""
     if t.dtype != dtype:
         raise TypeError(f"{what} is {t.dtype}, expected {dtype}")
-    if t.device != q.device:
-        raise ValueError(f"{what} on {t.device}, q on {q.device}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.device != like[1]:
+        raise ValueError(f"{what} on {t.device}, q on {like[1]}")
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -94,12 +109,12 @@ class _On:
         if device.type != "cuda":
             raise ValueError(f"tensors on {device}: the decoder operators run on the GPU")
         self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-        self.device = device
+        self.index = device.index
 
     def __enter__(self):
         if self.guard is not None:
             self.guard.__enter__()
-        return _torch().cuda.current_stream(self.device).cuda_stream
+        return _torch()._C._cuda_getCurrentRawStream(self.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -138,48 +153,48 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
     rows[n] of the caches, which are returned (a row outside [0, R) is dropped; rows should differ). q_out, if given,
     takes q (it may be q itself)."""
     torch = _torch()
-    N, Hq, D = (int(s) for s in q.shape)
-    Hkv = int(k.shape[1])
-    if int(k.shape[0]) != N or (v is not None and int(v.shape[0]) != N):
-        raise ValueError(f"q has {N} tokens, k {int(k.shape[0])}" + ("" if v is None else f", v {int(v.shape[0])}"))
+    like = _like(q)
+    N, Hq, D = q.shape
+    qv = _heads_view(q, "q", like)
+    kv = _heads_view(k, "k", like)
+    Hkv = k.shape[1]
+    if k.shape[0] != N or (v is not None and v.shape[0] != N):
+        raise ValueError(f"q has {N} tokens, k {k.shape[0]}" + ("" if v is None else f", v {v.shape[0]}"))
+    table = rotary.table
     if D != rotary.head_dim:
         raise ValueError(f"head_dim {D}, the rotation is made for {rotary.head_dim}")
-    if rotary.table.device != q.device:
-        raise ValueError(f"the rotation on {rotary.table.device}, q on {q.device}")
-    qv = _heads_view(q, "q")
-    kv = _heads_view(k, "k", q)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous() or w.device != q.device:
-            raise ValueError(f"{name} must be a contiguous float32 [{D}] on {q.device}")
+    if table.device != like[1]:
+        raise ValueError(f"the rotation on {table.device}, q on {q.device}")
+    qw, kw = _word(q_norm, "q_norm", like, torch.float32, (D,)), _word(k_norm, "k_norm", like, torch.float32, (D,))
     if positions.dim() == 1:
-        pos, pos_stride = _word(positions, "positions", q, torch.int32, (N,)), 0
+        pos, pos_stride = _word(positions, "positions", like, torch.int32, (N,)), 0
     else:
-        pos, pos_stride = _word(positions, "positions", q, torch.int32, (3, N)), N
+        pos, pos_stride = _word(positions, "positions", like, torch.int32, (3, N)), N
     if q_out is None:
-        q_out = torch.empty((N, Hq, D), dtype=q.dtype, device=q.device)
-    elif int(q_out.shape[0]) != N:
-        raise ValueError(f"q_out has {int(q_out.shape[0])} rows for {N} tokens")
-    qo = _heads_view(q_out, "q_out", q, Hq, True)
+        q_out = q.new_empty((N, Hq, D))
+    elif q_out.shape[0] != N:
+        raise ValueError(f"q_out has {q_out.shape[0]} rows for {N} tokens")
+    qo = _heads_view(q_out, "q_out", like, Hq, True)
     if (k_cache is None) != (v_cache is None) or (k_cache is None) != (rows is None):
         raise ValueError("k_cache, v_cache and rows come together")
     if k_cache is None:
-        k_cache, out_rows, prow = torch.empty((N, Hkv, D), dtype=q.dtype, device=q.device), N, None
+        k_cache, out_rows, prow = q.new_empty((N, Hkv, D)), N, None
         vv = vo = (None, 0, 0)
     else:
         if v is None:
             raise ValueError("v_cache without v")
-        vv = _heads_view(v, "v", q, Hkv)
-        vo = _heads_view(v_cache, "v_cache", q, Hkv, True)
-        out_rows, prow = int(k_cache.shape[0]), _word(rows, "rows", q, torch.int64, (N,))
-        if int(v_cache.shape[0]) != out_rows:
-            raise ValueError(f"k_cache has {out_rows} rows, v_cache {int(v_cache.shape[0])}")
+        vv = _heads_view(v, "v", like, Hkv)
+        vo = _heads_view(v_cache, "v_cache", like, Hkv, True)
+        out_rows, prow = k_cache.shape[0], _word(rows, "rows", like, torch.int64, (N,))
+        if v_cache.shape[0] != out_rows:
+            raise ValueError(f"k_cache has {out_rows} rows, v_cache {v_cache.shape[0]}")
         if out_rows == 0:
             raise ValueError("the caches have no rows")
-    ko = _heads_view(k_cache, "k_cache", q, Hkv, True)
-    with _On(q.device) as st:
+    ko = _heads_view(k_cache, "k_cache", like, Hkv, True)
+    with _On(like[1]) as st:
         capi.check(capi.load().qvl_qk_norm_rotary(
-            st, _qdtype(q.dtype), *qv, *kv, *vv, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), pos, pos_stride,
-            rotary.table.data_ptr(), prow, out_rows, *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
+            st, _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
+            *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
     return q_out, k_cache, v if v_cache is None else v_cache
 
 
@@ -224,21 +239,20 @@ class CausalPlan:
         self.items = torch.from_numpy(items).to(device)
 
 
-def _attention_views(q, k, v, out):
-    torch = _torch()
+def _attention_views(q, k, v, out, like):
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError(f"out {tuple(out.shape)}, q {tuple(q.shape)}")
-    qv, kv = _heads_view(q, "q"), _heads_view(k, "k", q)
-    vv = _heads_view(v, "v", q, int(k.shape[1]))
+    qv, kv = _heads_view(q, "q", like), _heads_view(k, "k", like)
+    vv = _heads_view(v, "v", like, k.shape[1])
     if k.shape[0] != v.shape[0]:
-        raise ValueError(f"k has {int(k.shape[0])} rows, v {int(v.shape[0])}")
-    return qv, kv, vv, _heads_view(out, "out", q, int(q.shape[1]), True), out
+        raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
+    return qv + kv + vv, _heads_view(out, "out", like, q.shape[1], True), out
 
 
-def _workspace(nbytes: int, device):
-    return _torch().empty(nbytes, dtype=_torch().uint8, device=device) if nbytes else None
+def _workspace(nbytes: int, q):
+    return q.new_empty(nbytes, dtype=_torch().uint8) if nbytes else None
 
 
 def _scale(scale, head_dim: int) -> float:
@@ -249,51 +263,58 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
     """softmax(scale q k^T) v of a packed prefill: q [N, Hq, D] holds the plan's new tokens one sequence after the other
     (rows past them are left as they are in `out`), k and v [R, Hkv, D] the caches (or the prompt's own keys and values).
     Token t of a sequence sees its keys up to itself; scale defaults to D^-0.5."""
-    qv, kv, vv, ov, out = _attention_views(q, k, v, out)
-    N, Hq, D = (int(s) for s in q.shape)
-    if (Hq, int(k.shape[1]), D) != (plan.num_heads, plan.num_kv_heads, plan.head_dim) or q.dtype != plan.dtype:
-        raise ValueError(f"q of {Hq} heads, k of {int(k.shape[1])}, head_dim {D}, {q.dtype}: the plan is for "
+    like = _like(q)
+    views, ov, out = _attention_views(q, k, v, out, like)
+    N, Hq, D = q.shape
+    if (Hq, k.shape[1], D, like[0]) != (plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype):
+        raise ValueError(f"q of {Hq} heads, k of {k.shape[1]}, head_dim {D}, {q.dtype}: the plan is for "
                          f"{plan.num_heads}, {plan.num_kv_heads}, {plan.head_dim}, {plan.dtype}")
-    if q.device != plan.device:
+    if like[1] != plan.device:
         raise ValueError(f"q on {q.device}, the plan on {plan.device}")
-    if N < plan.n_tokens or int(k.shape[0]) < plan.kv_rows:
-        raise ValueError(f"{N} tokens and {int(k.shape[0])} cache rows; the plan needs {plan.n_tokens} and {plan.kv_rows}")
-    ws = _workspace(plan.workspace_bytes, q.device)
-    with _On(q.device) as st:
+    rows = k.shape[0]
+    if N < plan.n_tokens or rows < plan.kv_rows:
+        raise ValueError(f"{N} tokens and {rows} cache rows; the plan needs {plan.n_tokens} and {plan.kv_rows}")
+    ws = _workspace(plan.workspace_bytes, q)
+    with _On(like[1]) as st:
         capi.check(capi.load().qvl_causal_attention(
-            st, _qdtype(q.dtype), *qv, *kv, *vv, int(k.shape[0]), plan.items.data_ptr(), plan.n_items, plan.n_whole,
-            _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
-            plan.workspace_bytes), "qvl_causal_attention")
+            st, _qdtype(like[0]), *views, rows, plan.items.data_ptr(), plan.n_items, plan.n_whole, _scale(scale, D), *ov, N,
+            Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_bytes(device_index, *sizes) -> int:
+    """qvl_decode_workspace_size: the same for the same sizes on the same (current) device."""
+    nb = C.c_size_t()
+    capi.check(capi.load().qvl_decode_workspace_size(*sizes, C.byref(nb)), "qvl_decode_workspace_size")
+    return nb.value
 
 
 def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
     torch = _torch()
-    qv, kv, vv, ov, out = _attention_views(q, k, v, out)
-    N, Hq, D = (int(s) for s in q.shape)
-    Hkv, n_seqs = int(k.shape[1]), int(k_start.shape[0])
-    ks = _word(k_start, "k_start", q, torch.int64, (n_seqs,))
-    kl = _word(k_len, "k_len", q, torch.int32, (n_seqs,))
-    cq = None if cu_q is None else _word(cu_q, "cu_q", q, torch.int32, (n_seqs + 1,))
+    like = _like(q)
+    views, ov, out = _attention_views(q, k, v, out, like)
+    N, Hq, D = q.shape
+    rows, Hkv = k.shape[0], k.shape[1]
+    n_seqs = k_start.shape[0]
+    ks = _word(k_start, "k_start", like, torch.int64, (n_seqs,))
+    kl = _word(k_len, "k_len", like, torch.int32, (n_seqs,))
+    cq = None if cu_q is None else _word(cu_q, "cu_q", like, torch.int32, (n_seqs + 1,))
     cg = ps = pl = None
     n_groups = max_prefix = 0
     if groups is not None:
         prefix_start, prefix_len, cu_groups, max_prefix = groups
-        n_groups = int(prefix_start.shape[0])
-        ps = _word(prefix_start, "prefix_start", q, torch.int64, (n_groups,))
-        pl = _word(prefix_len, "prefix_len", q, torch.int32, (n_groups,))
-        cg = _word(cu_groups, "cu_groups", q, torch.int32, (n_groups + 1,))
-    dt = _qdtype(q.dtype)
-    lib = capi.load()
-    nb = C.c_size_t()
-    with _On(q.device) as st:
-        capi.check(lib.qvl_decode_workspace_size(N, n_seqs, int(max_len), n_groups, int(max_prefix), Hq, Hkv, D, dt,
-                                                 C.byref(nb)), "qvl_decode_workspace_size")
-        ws = _workspace(nb.value, q.device)
-        capi.check(lib.qvl_decode_attention(
-            st, dt, *qv, *kv, *vv, int(k.shape[0]), cq, n_seqs, ks, kl, int(max_len), cg, n_groups, ps, pl,
-            int(max_prefix), _scale(scale, D), *ov, N, Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb.value),
-            "qvl_decode_attention")
+        n_groups = prefix_start.shape[0]
+        ps = _word(prefix_start, "prefix_start", like, torch.int64, (n_groups,))
+        pl = _word(prefix_len, "prefix_len", like, torch.int32, (n_groups,))
+        cg = _word(cu_groups, "cu_groups", like, torch.int32, (n_groups + 1,))
+    dt, max_len, max_prefix = _qdtype(like[0]), int(max_len), int(max_prefix)
+    with _On(like[1]) as st:
+        nb = _decode_bytes(like[1].index, N, n_seqs, max_len, n_groups, max_prefix, Hq, Hkv, D, dt)
+        ws = _workspace(nb, q)
+        capi.check(capi.load().qvl_decode_attention(
+            st, dt, *views, rows, cq, n_seqs, ks, kl, max_len, cg, n_groups, ps, pl, max_prefix, _scale(scale, D), *ov, N,
+            Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb), "qvl_decode_attention")
     return out
 
 
