@@ -1,0 +1,477 @@
+// Attention of a few new tokens of each sequence over a cache, the sequences' state read on the device: bound by reading
+// the keys and values once.
+//
+// Without prefixes one launch streams over all keys of all sequences: their blocks of 32 keys, sequence by sequence, are one
+// line cut into equal runs, each taken by one workgroup a key/value head, so that the lengths need not be known on the
+// host and unlike ones leave no workgroup slot idle. (A workgroup for each part of each sequence: 96 lengths from 1 to 7900,
+// 32/8 heads, bf16: 358 us at best, its slots 58 % occupied; one read of the keys takes 252 us at 6.2 TB/s.) The heads of one
+// run go by neighbouring workgroups: they read the same cache rows at the same time, whole rows and not 256 bytes here and
+// there. (One line over heads too, its runs at unlike places: 438 us.) A job, a tile of a sequence's rows, that lies in one
+// run is finished there; one that crosses runs leaves parts, which a second launch joins.
+//
+// With prefixes the tokens of a group are the rows of one more problem, the prefix's keys for all of them at once, 128 (32)
+// rows a workgroup and the keys in parts; the sequences' own keys are parts beside them, and one join covers both.
+#include "qvl_decoder_core.h"
+
+namespace qvl {
+
+// A job of the streaming launch whose last block lies in this run and whose first does not: what its join needs.
+struct SplitJob {
+  int64_t token0;
+  int rows, row0, first, parts;   // parts == 0: none
+};
+
+struct DecodeState {
+  const int32_t* cu_q;
+  const int64_t* k_start;
+  const int32_t* k_len;
+  const int32_t* cu_groups;
+  const int64_t* prefix_start;
+  const int32_t* prefix_len;
+  int n_seqs, n_groups;
+  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // with prefixes: parts of so many keys each
+  SplitJob* split;                                                      // streaming: [runs]
+  int slot_rows;                                                        // streaming: rows a part's slot has
+};
+
+// The four waves' results of the same rows joined in LDS (free by then), and written: to the output, or as a part, row r of
+// which is row at(r) of the part buffers. `ka`: the first key of the range the waves covered.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int ka,
+                                           bool part, F&& at) {
+  constexpr int kC = D / 4;                    // 16-byte chunks of a row, XOR-swizzled by the row
+  __shared__ float sm[4][32], sl[4][32];
+  __shared__ int slim[32];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = min(32, u.rows - first_row);
+  const float lw = w.core.row_sum();
+  if (lane < 32) {
+    sm[wave][l32] = w.m;
+    sl[wave][l32] = lw;
+    slim[l32] = w.lim;
+  }
+  __syncthreads();                             // every wave is past its tiles
+  float* const so = reinterpret_cast<float*>(smem);
+  if (l32 < n)
+    w.core.each4([&](int d, const f32x4& x) {
+      *reinterpret_cast<f32x4*>(so + ((wave * 32 + l32) * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 4) = x;
+    });
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * kC; i += 256) {
+    const int r = i / kC, c = i % kC;
+    float M = sm[0][r];
+#pragma unroll
+    for (int x = 1; x < 4; ++x) M = fmaxf(M, sm[x][r]);
+    const float shift = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sm[x][r] - shift);
+      l += f * sl[x][r];
+      // a wave that saw none of the row's keys has zeros; one whose maximum is far below the others' may hold infinities
+      const f32x4 o = *reinterpret_cast<const f32x4*>(so + ((x * 32 + r) * kC + (c ^ (r & (kC - 1)))) * 4);
+      if (f != 0.f) acc += f * o;
+    }
+    const bool sees = slim[r] > ka;
+    if (part) {
+      const int64_t a = at(r);
+      *reinterpret_cast<f32x4*>(P.part_o + a * D + c * 4) = acc;
+      if (c == 0) P.part_ml[a] = part_state(M, l, sees);
+    } else {
+      const float inv = 1.0f / l;
+      store4<T>(out_row<T, D>(P, u, first_row + r), c * 4, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+  __syncthreads();                             // the tiles may be written again
+}
+
+// The token range of sequences [s0, s1), empty where it is none of [0, n_tokens).
+__device__ __forceinline__ int64_t tokens_of(const AttnParams& P, const DecodeState& S, int s0, int s1, int64_t& first) {
+  const int64_t a = S.cu_q ? S.cu_q[s0] : s0, b = S.cu_q ? S.cu_q[s1] : s1;
+  first = a;
+  return a < 0 || b > P.n_tokens || b < a ? 0 : b - a;
+}
+
+__device__ __forceinline__ bool bad_keys(const AttnParams& P, int64_t start, int len) {
+  return len < 0 || len > kItemMaxLen || start < 0 || start > P.kv_rows - len;
+}
+
+// ---------------------------------------------------------------------------------------------
+// streaming
+// ---------------------------------------------------------------------------------------------
+// A sequence's jobs (tiles of 32 rows) and each one's blocks of 32 keys: one where there is nothing to read, for the rows'
+// zeros (or NaN).
+__device__ __forceinline__ int64_t jobs_of(const AttnParams& P, const DecodeState& S, int seq, int& blocks) {
+  int64_t first;
+  const int64_t rows = tokens_of(P, S, seq, seq + 1, first) * P.group;
+  const int len = S.k_len[seq];
+  blocks = bad_keys(P, S.k_start[seq], len) ? 1 : max((len + 31) >> 5, 1);
+  return (rows + 31) / 32;
+}
+
+// Exclusive sums of v over the workgroup, in excl[0..256] (excl[256]: the total).
+__device__ __forceinline__ void scan256(int64_t v, int64_t* excl) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ int64_t waves[4];
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) x += waves[i];
+  excl[threadIdx.x + 1] = x;
+  if (threadIdx.x == 0) excl[0] = 0;
+  __syncthreads();
+}
+
+// The sequence that block `pos` of the line belongs to, and the block its first job starts at. `excl`: sums over runs of
+// `per` sequences a thread.
+__device__ __forceinline__ void locate(const AttnParams& P, const DecodeState& S, int64_t pos, int per, const int64_t* excl,
+                                       int64_t* work, int& seq, int64_t& base) {
+  __shared__ int hit;
+  if (excl[threadIdx.x] <= pos && pos < excl[threadIdx.x + 1]) hit = threadIdx.x;
+  __syncthreads();
+  const int run = hit;
+  __syncthreads();
+  seq = run * per;
+  base = excl[run];
+  if (per == 1) return;
+  int blocks = 0;
+  const int s = seq + (int)threadIdx.x;
+  const int64_t jobs = (int)threadIdx.x < per && s < S.n_seqs ? jobs_of(P, S, s, blocks) : 0;
+  scan256(jobs * blocks, work);
+  if (work[threadIdx.x] <= pos - base && pos - base < work[threadIdx.x + 1]) hit = threadIdx.x;
+  __syncthreads();
+  const int in = hit;
+  seq += in;
+  base += work[in];
+  __syncthreads();
+}
+
+// Where run i of n begins: an equal share of the line, moved to a job's end where the job is no longer than a share (or a
+// block for each wave), so that short jobs stay whole.
+__device__ __forceinline__ int64_t share(int64_t total, int i, int n) { return total / n * i + total % n * i / n; }
+__device__ __forceinline__ int64_t run_start(const AttnParams& P, const DecodeState& S, int64_t total, int i, int n, int per,
+                                             const int64_t* excl, int64_t* work, int& seq, int64_t& base) {
+  const int64_t pos = share(total, i, n);
+  if (pos >= total) return total;
+  locate(P, S, pos, per, excl, work, seq, base);
+  int blocks;
+  jobs_of(P, S, seq, blocks);
+  const int64_t in = (pos - base) % blocks;
+  seq = uniform(seq);
+  base = uniform(base);
+  return in == 0 || blocks > max((int64_t)4, total / n) ? pos : pos - in + (2 * in < blocks ? 0 : blocks);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, DecodeState S) {
+  using K = KeysUnit<T, D>;
+  __shared__ __attribute__((aligned(16))) char smem[K::kLds];
+  __shared__ int64_t excl[257], work[257];
+  const int run = blockIdx.x / P.hkv, kvh = blockIdx.x % P.hkv;
+  // this run of the line: [pos, end), pos in sequence `seq` whose jobs begin at `base`
+  const int per = (S.n_seqs + 255) / 256;
+  int64_t mine = 0;
+  for (int s = threadIdx.x * per; s < min((int)(threadIdx.x + 1) * per, S.n_seqs); ++s) {
+    int blocks;
+    const int64_t jobs = jobs_of(P, S, s, blocks);
+    mine += jobs * blocks;
+  }
+  scan256(mine, excl);
+  const int64_t total = uniform(excl[256]);
+  const int n = (int)min((int64_t)(gridDim.x / P.hkv), total);   // no run of a split job is empty
+  if (run >= n) {
+    if (threadIdx.x == 0 && kvh == 0) S.split[run].parts = 0;
+    return;
+  }
+  int seq = 0, seq_end = 0;
+  int64_t base = 0, base_end = 0;
+  int64_t pos = uniform(run_start(P, S, total, run, n, per, excl, work, seq, base));
+  const int64_t end = uniform(run_start(P, S, total, run + 1, n, per, excl, work, seq_end, base_end));
+  SplitJob joined{};
+  while (pos < end) {
+    Unit u;
+    int blocks;
+    const int64_t jobs = uniform(jobs_of(P, S, seq, blocks));
+    blocks = uniform(blocks);
+    if (pos >= base + jobs * blocks) {           // the next sequence (jobs == 0: it has no rows)
+      base += jobs * blocks;
+      ++seq;
+      continue;
+    }
+    const int n_new = uniform((int)tokens_of(P, S, seq, seq + 1, u.token0));
+    const int64_t start = uniform(S.k_start[seq]);
+    u.token0 = uniform(u.token0);
+    u.len = uniform(S.k_len[seq]);
+    const int job = (int)((pos - base) / blocks), b0 = (int)((pos - base) % blocks);
+    const int b1 = (int)min((int64_t)blocks, b0 + (end - pos));
+    u.kvh = kvh;
+    u.row0 = job * 32;
+    u.rows = n_new * P.group;
+    u.lim0 = u.len - n_new + 1;
+    const int n_rows = min(32, u.rows - u.row0);
+    const bool whole = b0 == 0 && b1 == blocks, bad = bad_keys(P, start, u.len);
+    if (bad) {
+      for (int i = threadIdx.x; i < n_rows * (D / 4); i += 256)
+        store4<T>(out_row<T, D>(P, u, u.row0 + i / (D / 4)), i % (D / 4) * 4, f32x4{NAN, NAN, NAN, NAN});
+    } else {
+      u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
+      u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
+      Wave<T, D> w;
+      w.init(P, u, u.row0);
+      K::run(P, u, w, smem, b0, min(b1, (u.len + 31) >> 5));
+      const int64_t slot = ((int64_t)(2 * run + (b0 == 0)) * P.hkv + kvh) * S.slot_rows;
+      join_waves<T, D>(P, u, w, smem, u.row0, b0 * 32, !whole, [&](int r) { return slot + r; });
+    }
+    if (b0 > 0 && b1 == blocks) {
+      // the run that holds the job's first block: the last whose share begins there or before
+      const int64_t first = pos - b0;
+      int w0 = (int)min((int64_t)((double)first / (double)total * n), (int64_t)run);
+      while (w0 > 0 && share(total, w0, n) > first) --w0;
+      while (w0 < run && share(total, w0 + 1, n) <= first) ++w0;
+      joined = SplitJob{u.token0, u.rows, u.row0, w0, run - w0 + 1};
+    }
+    pos += b1 - b0;
+  }
+  if (threadIdx.x == 0 && kvh == 0) S.split[run] = joined;
+}
+
+// Part p of a split job: the second slot of its first run (the job begins inside it), the first slot of each later one.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void decode_stream_join_kernel(AttnParams P, DecodeState S) {
+  const SplitJob j = S.split[blockIdx.x];
+  if (j.parts == 0) return;
+  const int kvh = blockIdx.y;
+  const Unit u{nullptr, nullptr, 0, 0, j.token0, j.rows, j.row0, kvh};
+  const int n = min(32, j.rows - j.row0), per = (n + gridDim.z - 1) / gridDim.z, r0 = blockIdx.z * per;
+  join_parts<T, D>(P, r0, min(r0 + per, n), j.parts,
+                   [&](int r, int p) { return ((int64_t)(2 * (j.first + p) + (p == 0)) * P.hkv + kvh) * S.slot_rows + r; },
+                   [&](int r) { return out_row<T, D>(P, u, j.row0 + r); });
+}
+
+// ---------------------------------------------------------------------------------------------
+// with prefixes
+// ---------------------------------------------------------------------------------------------
+// Row (token, head) of part `part`, for row r of the unit.
+__device__ __forceinline__ int64_t part_row(const AttnParams& P, const Unit& u, int part, int r) {
+  const int t = (int)((uint32_t)r / (uint32_t)P.group), g = r - t * P.group;
+  return ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + g;
+}
+
+// Rows without keys in this part (0), or of keys that may not be read (NaN).
+__device__ __forceinline__ void write_fixed(const AttnParams& P, const Unit& u, int part, float value) {
+  for (int r = threadIdx.x; r < u.rows; r += 256) P.part_ml[part_row(P, u, part, r)] = f32x2{value == 0.f ? -INFINITY : value, value};
+}
+
+// Workgroups [0, prefix units): a part of a group's prefix for a tile of the group's rows (ROWS: tiles of 128, else of 32);
+// the others: a part of a sequence's own keys for its rows. The key/value head runs fastest, then the part, so that the
+// tiles of one part of the prefix meet in one L2 where heads x parts fill the 8 XCDs evenly.
+template <typename T, int D, bool ROWS>
+__device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeState& S) {
+  using R = RowsUnit<T, D>;
+  using K = KeysUnit<T, D>;
+  __shared__ __attribute__((aligned(16))) char smem[ROWS && R::kLds > K::kLds ? R::kLds : K::kLds];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int prefix_units = P.hkv * S.prefix_parts * S.prefix_tiles * S.n_groups;
+  const bool own = (int)blockIdx.x >= prefix_units;
+  int id = own ? blockIdx.x - prefix_units : blockIdx.x;
+  Unit u;
+  u.kvh = id % P.hkv;
+  id /= P.hkv;
+  const int parts = own ? S.own_parts : S.prefix_parts, p = id % parts, chunk = own ? S.own_chunk : S.prefix_chunk;
+  const int part = own ? S.prefix_parts + p : p;
+  id /= parts;
+  const int tile0 = own ? 0 : id % S.prefix_tiles, who = own ? id : id / S.prefix_tiles;   // a sequence, or a group
+  int s0 = who, s1 = who + 1;
+  if (!own) {
+    s0 = min(max(S.cu_groups[who], 0), S.n_seqs);
+    s1 = min(max(S.cu_groups[who + 1], 0), S.n_seqs);
+  }
+  const int tokens = uniform(s1 > s0 ? (int)tokens_of(P, S, s0, s1, u.token0) : 0);
+  u.rows = tokens * P.group;
+  if (u.rows == 0) return;
+  const int64_t start = uniform(own ? S.k_start[who] : S.prefix_start[who]);
+  u.token0 = uniform(u.token0);
+  u.len = uniform(own ? S.k_len[who] : S.prefix_len[who]);
+  if (bad_keys(P, start, u.len)) {
+    write_fixed(P, u, part, NAN);
+    return;
+  }
+  u.lim0 = own ? u.len - tokens + 1 : u.len;
+  const int ka = (int)min((int64_t)p * chunk, (int64_t)u.len);
+  const int kb = p + 1 == parts ? u.len : (int)min((int64_t)ka + chunk, (int64_t)u.len);
+  if (ka >= kb) {
+    write_fixed(P, u, part, 0.f);
+    return;
+  }
+  u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
+  u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
+  if (ROWS && !own) {
+    for (int row0 = tile0 * kItemRows; row0 < u.rows; row0 += S.prefix_tiles * kItemRows) {
+      Wave<T, D> w;
+      w.init(P, u, row0 + wave * 32);
+      R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN);
+      const int row = row0 + wave * 32 + (threadIdx.x & 31);
+      const int64_t at = part_row(P, u, part, min(row, u.rows - 1));
+      write_rows<T, D>(P, u, w, row, P.part_o + at * D, P.part_ml + at, true);
+    }
+  } else {
+    const int step = own ? 32 : S.prefix_tiles * 32;
+    for (int row0 = tile0 * 32; row0 < u.rows; row0 += step) {
+      Wave<T, D> w;
+      w.init(P, u, row0);
+      K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
+      join_waves<T, D>(P, u, w, smem, row0, ka, true, [&](int r) { return part_row(P, u, part, row0 + r); });
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void prefix_rows_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, true>(P, S); }
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void prefix_keys_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, false>(P, S); }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(AttnParams P, DecodeState S) {
+  const int64_t heads = P.hkv * P.group, total = P.n_tokens * heads;
+  const int64_t first = (S.cu_q ? (int64_t)max(S.cu_q[0], 0) : 0) * heads;
+  const int64_t end = (S.cu_q ? min((int64_t)S.cu_q[S.n_seqs], P.n_tokens) : P.n_tokens) * heads;
+  const int parts = S.prefix_parts + S.own_parts;
+  const int64_t per = 256 / (D / 4) / join_split(parts);   // rows a workgroup
+  const int64_t r0 = (int64_t)blockIdx.x * per;
+  const int64_t a = max(r0, first), b = min(r0 + per, end);
+  if (a >= b) return;
+  join_parts<T, D>(P, (int)(a - r0), (int)(b - r0), parts, [&](int r, int p) { return p * total + r0 + r; },
+                   [&](int r) {
+                     const int64_t token = (r0 + r) / heads;
+                     return const_cast<char*>(P.out.p) + token * P.out.row + (r0 + r - token * heads) * P.out.head;
+                   });
+}
+
+// How a launch is laid out: from the sizes alone, so that the workspace can be told beforehand.
+struct DecodePlan {
+  int runs, slot_rows;                                                  // streaming
+  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // with prefixes
+  bool prefix_rows;
+  int64_t units;
+  size_t part_rows, split_bytes;
+};
+
+// Parts of at least 128 keys (a block of 32 a wave), as many as fill the workgroup slots once.
+static int split_parts(int64_t keys, int64_t units, int64_t slots, int& chunk) {
+  int64_t parts = std::min({slots / std::max<int64_t>(units, 1), (keys + 127) / 128, (int64_t)64});
+  parts = std::max<int64_t>(parts, 1);
+  const int64_t c = round_up(std::max<int64_t>((keys + parts - 1) / parts, 1), 64);
+  chunk = (int)std::min<int64_t>(c, kItemMaxLen);
+  return (int)std::max<int64_t>((keys + c - 1) / c, 1);
+}
+
+static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
+                       int32_t num_heads, int32_t num_kv_heads, int32_t dtype, int32_t head_dim, DecodePlan& D) {
+  if (n_tokens < 0 || n_seqs < 0 || n_groups < 0 || max_len < 0 || max_prefix < 0) return set_error(QVL_ERR_INVALID_ARG, "%s: bad sizes", what);
+  if (n_seqs > 65535 || n_groups > 65535) return set_error(QVL_ERR_UNSUPPORTED, "%s: more than 65535 sequences or groups", what);
+  if (max_len > kItemMaxLen || max_prefix > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: lengths", what);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
+    return set_error(QVL_ERR_INVALID_ARG, "%s: %d heads over %d key/value heads", what, num_heads, num_kv_heads);
+  const int64_t rows = n_tokens * (num_heads / num_kv_heads);
+  if (num_heads > kItemHeadMask || n_tokens > kItemMaxLen || rows > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  // workgroups a GPU holds: two a CU, one where the tiles take 128 KB (fp32, head_dim 128)
+  const int64_t slots = (int64_t)gemm_device_cus() * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
+  D = DecodePlan{};
+  if (n_groups == 0) {
+    // a run for each slot, but no more than give each wave a block, nor fewer than there are jobs
+    const int64_t tiles = std::max<int64_t>((rows + 32 * n_seqs - 1) / (32 * std::max<int64_t>(n_seqs, 1)), 1);
+    const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + 31) / 32);
+    D.runs = (int)std::max<int64_t>(std::min(slots / num_kv_heads, std::max((blocks + 3) / 4, jobs)), 1);
+    D.units = (int64_t)D.runs * num_kv_heads;
+    D.slot_rows = (int)std::min<int64_t>(32, std::max<int64_t>(rows, 1));
+    D.part_rows = (size_t)D.units * 2 * D.slot_rows;
+    D.split_bytes = round_up(D.runs * sizeof(SplitJob), 16);
+    return QVL_OK;
+  }
+  const int64_t mean = (rows + n_groups - 1) / n_groups;
+  D.prefix_rows = mean > 32;
+  const int64_t tile = D.prefix_rows ? kItemRows : 32;
+  D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
+  D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
+  D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, slots, D.prefix_chunk);
+  D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
+  if (D.units > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  D.part_rows = (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads;
+  return QVL_OK;
+}
+
+static size_t workspace_bytes_of(const DecodePlan& D, int32_t head_dim) {
+  return D.split_bytes + D.part_rows * ((size_t)head_dim + 2) * sizeof(float);
+}
+
+}  // namespace qvl
+
+using namespace qvl;
+
+extern "C" {
+
+int qvl_decode_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, size_t* bytes) {
+  if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "decode_workspace_size: bytes is NULL");
+  if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: head_dim=%d", head_dim);
+  if (dtype != QVL_DTYPE_F32 && dtype != QVL_DTYPE_BF16) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: dtype %d", dtype);
+  DecodePlan plan;
+  QVL_TRY_RC(decode_plan("decode_workspace_size", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype,
+                         head_dim, plan));
+  *bytes = workspace_bytes_of(plan, head_dim);
+  return QVL_OK;
+}
+
+int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
+                         int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows,
+                         const int32_t* cu_q, int64_t n_seqs, const int64_t* k_start, const int32_t* k_len, int64_t max_len,
+                         const int32_t* cu_groups, int64_t n_groups, const int64_t* prefix_start,
+                         const int32_t* prefix_len, int64_t max_prefix, float scale, void* out, int64_t out_row,
+                         int64_t out_head, int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                         void* workspace, size_t workspace_bytes) {
+  AttnParams P{};
+  QVL_TRY_RC(attn_params("decode_attention", dtype, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, kv_rows, out,
+                         out_row, out_head, n_tokens, num_heads, num_kv_heads, head_dim, scale, P));
+  DecodePlan plan;
+  QVL_TRY_RC(decode_plan("decode_attention", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype,
+                         head_dim, plan));
+  if (!cu_q && n_tokens != n_seqs) return set_error(QVL_ERR_INVALID_ARG, "decode_attention: %lld tokens of %lld sequences without cu_q", (long long)n_tokens, (long long)n_seqs);
+  if (n_tokens == 0 || n_seqs == 0) return QVL_OK;
+  if (!k_start || !k_len || (n_groups > 0 && (!cu_groups || !prefix_start || !prefix_len)))
+    return set_error(QVL_ERR_INVALID_ARG, "decode_attention: NULL pointer");
+  if ((uintptr_t)k_start % 8 || (uintptr_t)k_len % 4 || (uintptr_t)cu_q % 4 || (uintptr_t)cu_groups % 4 ||
+      (uintptr_t)prefix_start % 8 || (uintptr_t)prefix_len % 4)
+    return set_error(QVL_ERR_MISALIGNED, "decode_attention: the sequences' state");
+  const size_t need = workspace_bytes_of(plan, head_dim);
+  if (workspace_bytes < need || !workspace)
+    return set_error(QVL_ERR_WORKSPACE, "decode_attention: workspace %zu < %zu", workspace_bytes, need);
+  if ((uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "decode_attention: workspace");
+  P.part_o = (float*)((char*)workspace + plan.split_bytes);
+  P.part_ml = (f32x2*)(P.part_o + plan.part_rows * head_dim);
+  const DecodeState S{cu_q, k_start, k_len, cu_groups, prefix_start, prefix_len, (int)n_seqs, (int)n_groups, plan.own_parts,
+                      plan.own_chunk, plan.prefix_parts, plan.prefix_chunk, plan.prefix_tiles, (SplitJob*)workspace, plan.slot_rows};
+  const dim3 units((unsigned)plan.units);
+  if (n_groups == 0) {
+    QVL_ATTN_LAUNCH(decode_stream_kernel, units, P, S);
+    QVL_TRY_RC(check_launch("decode_stream"));
+    if (plan.runs == 1) return QVL_OK;
+    // a split job's rows over a few workgroups: they are few, and each reads every part
+    QVL_ATTN_LAUNCH(decode_stream_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)std::min(plan.slot_rows, 8)), P, S);
+    return check_launch("decode_stream_join");
+  }
+  if (plan.prefix_rows) QVL_ATTN_LAUNCH(prefix_rows_kernel, units, P, S);
+  else QVL_ATTN_LAUNCH(prefix_keys_kernel, units, P, S);
+  QVL_TRY_RC(check_launch("prefix_attention"));
+  const int64_t per = 256 / (head_dim / 4) / join_split(plan.prefix_parts + plan.own_parts);
+  QVL_ATTN_LAUNCH(prefix_join_kernel, dim3((unsigned)((n_tokens * num_heads + per - 1) / per)), P, S);
+  return check_launch("prefix_join");
+}
+
+}  // extern "C"

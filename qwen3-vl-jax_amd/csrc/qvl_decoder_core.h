@@ -1,8 +1,9 @@
-// Causal, decode and shared-prefix attention of a text decoder: out = softmax(scale q k^T) v over the keys a token sees,
-// grouped heads, bf16 or fp32, head_dim 64 or 128.
+// Device side shared by the decoder's attention kernels (qvl_causal.hip, qvl_decode.hip): out = softmax(scale q k^T) v over the
+// keys a token sees, grouped heads, bf16 or fp32, head_dim 64 or 128.
 //
 // A row is one (token, query head); the rows of one key/value head that see the same keys are handled together. One
-// pass over the keys holds the running maximum m, the sum l of exp(s - m) and the unnormalised output.
+// pass over the keys holds the running maximum m, the sum l of 2^(s - m) and the unnormalised output.
+#pragma once
 #include <math.h>
 #include <type_traits>
 
@@ -21,24 +22,15 @@ struct AttnParams {
   int64_t kv_rows, n_tokens;
   int hkv, group;          // key/value heads, query heads of each
   float scale;             // of the scores, times log2(e): the softmax runs on powers of two
-  // causal: items; decode: the sequences' state
-  const int32_t* items;
-  const int32_t* cu_q;
-  const int64_t* k_start;
-  const int32_t* k_len;
-  const int32_t* cu_groups;
-  const int64_t* prefix_start;
-  const int32_t* prefix_len;
-  int n_seqs, n_groups;
-  // Partial results: per part and row the unnormalised output and (m, l). causal: [slot][128 rows], slots of the items
-  // from n_whole on; decode: [part][token][head], prefix parts first.
-  float* part_o;
+  float* part_o;           // partial results: unnormalised outputs and (m, l) of rows
   f32x2* part_ml;
-  int n_whole;
-  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // parts of so many keys each
 };
 
-template <int V> using int_c = std::integral_constant<int, V>;
+// A value that is the same in every lane, in scalar registers (a DMA's descriptor and a workgroup's branches have to be).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
+}
 
 // The larger of the two lanes of a row.
 __device__ __forceinline__ float across_halves(float x) {
@@ -71,10 +63,13 @@ template <int D> struct Core<bf16, D> {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const bf16x8*>(qrow + (ks * 16 + hh * 8) * 2);
-    // used here, so that the wait for these loads stands before the loop: inside it, it would be one for the DMA in flight
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
     clear();
+  }
+  // Uses the rows, so that the wait for their loads stands here, behind the first DMAs' issue: at their first use in the loop
+  // it would be a wait for every DMA in flight, tile by tile.
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (auto& x : q) asm volatile("" : "+v"(x));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -221,6 +216,7 @@ template <int D> struct Core<bf16, D> {
           v[j] = clean;
           bad[j] = mark;
         }
+        __builtin_amdgcn_sched_barrier(0);   // one output block at a time: registers
         o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pf, o[db], 0, 0, 0);
         const f32x16 n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bad), sf, f32x16{}, 0, 0, 0);
 #pragma unroll
@@ -268,9 +264,11 @@ template <int D> struct Core<float, D> {
     const int hh = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) q[j] = *reinterpret_cast<const f32x4*>(qrow + (j * 8 + hh * 4) * 4);
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) asm volatile("" : "+v"(q[j]));   // as above
     clear();
+  }
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (auto& x : q) asm volatile("" : "+v"(x));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -528,6 +526,7 @@ template <typename T, int D> struct RowsUnit {
     aim(t0);
 #pragma unroll
     for (int i = 0; i < 2 * kDmas; ++i) load(i, 0);
+    w.core.pin();
     wait_dma();
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -591,6 +590,7 @@ template <typename T, int D> struct KeysUnit {
     if (t0 >= t1) return;
     load_k(t0);
     load_v(t0);
+    w.core.pin();
     // In flight, oldest first: K(t), V(t) at the top; V(t), K(t + 1) before V is read.
     int t = t0;
     const auto each = [&](auto safe) {
@@ -636,460 +636,97 @@ __device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, c
   }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P) {
-  using R = RowsUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[R::kLds];
-  const int32_t* it = P.items + 8 * (int64_t)blockIdx.x;
-  const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
-  const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
-  const int64_t start = (int64_t)(((uint64_t)(uint32_t)it[7] << 32) | (uint32_t)it[6]);
-  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 || start < 0 ||
-      start > P.kv_rows - len || row0 >= n_new * P.group || (parts && (part >= parts || slot < 0 || slot >= (int)gridDim.x - P.n_whole))) return;
-  const Unit u{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
-               n_new * P.group, row0, kvh};
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int last = min(row0 + kItemRows, u.rows) - 1;
-  const int k_hi = max(min(u.lim0 + (int)((uint32_t)last / (uint32_t)P.group), len), 0);
-  const int n_t = (k_hi + R::kBN - 1) / R::kBN;
-  const int t0 = parts ? (int)((int64_t)n_t * part / parts) : 0, t1 = parts ? (int)((int64_t)n_t * (part + 1) / parts) : n_t;
-  Wave<T, D> w;
-  w.init(P, u, row0 + wave * 32);
-  R::run(P, u, w, smem, t0, t1);
-  // A value that is not finite may come from a key that its row does not see: once more, telling them apart.
-  if (__builtin_expect(__syncthreads_or(!w.finite()), 0)) {
-    w.core.clear();
-    w.m = -INFINITY;
-    R::run_safe(P, u, w, smem, t0, t1);
-  }
-  const int r = wave * 32 + (threadIdx.x & 31);
-  const int64_t at = (int64_t)slot * kItemRows + r;
-  write_rows<T, D>(P, u, w, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * R::kBN);
-}
+// Parts of rows joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, in an order that only the number of parts
+// sets. A workgroup takes 256 / (lanes x split) rows at once: D / 4 lanes hold a row, 16 bytes each, and `split` groups of
+// them share its parts, 4 in flight each, so that a row of 32 parts costs one trip to memory and not 32. `at(r, p)` is part
+// p's row index in P.part_ml / P.part_o, `out(r)` where row r goes.
+__device__ __host__ constexpr int join_split(int parts) { return parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8; }
 
-// One row's parts joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, in part order. One wave; part p's state is
-// ml[p * stride], its output o[p * stride * D].
-template <typename T, int D>
-__device__ __forceinline__ void combine_row(const f32x2* ml, const float* o, int64_t stride, int parts, char* out) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  float M = -INFINITY;
-  for (int p = lane; p < parts; p += 64) M = fmaxf(M, ml[p * stride].x);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-  const float shift = M == -INFINITY ? 0.f : M;
-  float l = 0.f, acc[E] = {};
-  bool sees = false;
-  for (int p0 = 0; p0 < parts; p0 += 64) {
-    const f32x2 st = p0 + lane < parts ? ml[(p0 + lane) * stride] : f32x2{-INFINITY, 0.f};
-    const float wt = __builtin_amdgcn_exp2f(st.x - shift);
-    sees = sees || __builtin_amdgcn_ballot_w64(__float_as_uint(st.y) != 0) != 0;
-    const int n = min(64, parts - p0);
-    for (int p = 0; p < n; ++p) {
-      const float w = __shfl(wt, p), lp = __shfl(st.y, p);
-      l += w * lp;
-      if (w == 0.f) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(w, o[(p0 + p) * stride * D + lane * E + e], acc[e]);
-    }
-  }
-  const float inv = 1.0f / l;
-  if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(out)[lane * E + e] = sees ? acc[e] * inv : 0.f;
-  } else {
-    uint32_t w = 0;
-    if constexpr (E == 2) {
-      w = sees ? pack_bf16x2(acc[0] * inv, acc[1] * inv) : 0u;
-      reinterpret_cast<uint32_t*>(out)[lane] = w;
-    } else {
-      reinterpret_cast<bf16*>(out)[lane] = (bf16)(sees ? acc[0] * inv : 0.f);
-    }
-  }
-}
-
-// The rows of split tiles: the workgroup of a part joins its share of the tile's 128 rows.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void causal_combine_kernel(AttnParams P) {
-  const int32_t* it = P.items + 8 * ((int64_t)P.n_whole + blockIdx.x);
-  const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
-  const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
-  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || part >= parts ||
-      part > slot || slot - part + parts > (int)gridDim.x) return;
-  const Unit u{nullptr, nullptr, len, 0, q0, n_new * P.group, row0, kvh};
-  const int r1 = min(kItemRows * (part + 1) / parts, u.rows - row0);
-  for (int r = kItemRows * part / parts + (threadIdx.x >> 6); r < r1; r += 4) {
-    const int64_t at = (int64_t)(slot - part) * kItemRows + r;
-    combine_row<T, D>(P.part_ml + at, P.part_o + at * D, kItemRows, parts, out_row<T, D>(P, u, row0 + r));
-  }
-}
-
-
-// The four waves' results of the same rows joined in LDS (free by then), and written: to the output, or as a part.
-template <typename T, int D>
-__device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int part, int ka) {
-  constexpr int kC = D / 4;                    // 16-byte chunks of a row, XOR-swizzled by the row
-  __shared__ float sm[4][32], sl[4][32];
-  __shared__ int slim[32];
-  const int lane = threadIdx.x & 63, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = min(32, u.rows - first_row);
-  const float lw = w.core.row_sum();
-  if (lane < 32) {
-    sm[wave][l32] = w.m;
-    sl[wave][l32] = lw;
-    slim[l32] = w.lim;
-  }
-  __syncthreads();                             // every wave is past its tiles
-  float* const so = reinterpret_cast<float*>(smem);
-  if (l32 < n)
-    w.core.each4([&](int d, const f32x4& x) {
-      *reinterpret_cast<f32x4*>(so + ((wave * 32 + l32) * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 4) = x;
-    });
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * kC; i += 256) {
-    const int r = i / kC, c = i % kC;
-    float M = sm[0][r];
-#pragma unroll
-    for (int x = 1; x < 4; ++x) M = fmaxf(M, sm[x][r]);
-    const float shift = M == -INFINITY ? 0.f : M;
-    float l = 0.f;
+template <typename T, int D, typename At, typename Out>
+__device__ __forceinline__ void join_parts(const AttnParams& P, int row0, int row1, int parts, At&& at, Out&& out) {
+  constexpr int kLanes = D / 4, kSlots = 256 / kLanes;
+  __shared__ f32x4 so[kSlots][kLanes];
+  __shared__ float sm[kSlots], sl[kSlots];
+  __shared__ int ss[kSlots];
+  const int split = join_split(parts), slot = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, g = slot % split;
+  for (int base = row0; base < row1; base += kSlots / split) {
+    const int r = base + slot / split;
+    float m = -INFINITY, l = 0.f;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool sees = false;
+    if (r < row1) {
+      for (int p0 = g; p0 < parts; p0 += 4 * split) {
+        f32x2 st[4];
+        f32x4 o[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float f = __builtin_amdgcn_exp2f(sm[x][r] - shift);
-      l += f * sl[x][r];
-      // a wave that saw none of the row's keys has zeros; one whose maximum is far below the others' may hold infinities
-      const f32x4 o = *reinterpret_cast<const f32x4*>(so + ((x * 32 + r) * kC + (c ^ (r & (kC - 1)))) * 4);
-      if (f != 0.f) acc += f * o;
+        for (int i = 0; i < 4; ++i) {
+          const int p = p0 + i * split;
+          const int64_t a = at(r, p < parts ? p : p0);
+          st[i] = P.part_ml[a];
+          o[i] = *reinterpret_cast<const f32x4*>(P.part_o + a * D + lane * 4);
+          if (p >= parts) st[i] = f32x2{-INFINITY, 0.f};
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), m), shift = mn == -INFINITY ? 0.f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - shift);
+        l *= a;
+        acc *= a;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = __builtin_amdgcn_exp2f(st[i].x - shift);
+          l += w * st[i].y;
+          sees = sees || __float_as_uint(st[i].y) != 0;
+          if (w != 0.f) acc += w * o[i];   // a part without keys has written no output
+        }
+      }
     }
-    const int row = first_row + r, t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
-    const bool sees = slim[r] > ka;
-    if (P.part_o) {
-      const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + g;
-      *reinterpret_cast<f32x4*>(P.part_o + at * D + c * 4) = acc;
-      if (c == 0) P.part_ml[at] = part_state(M, l, sees);
-    } else {
+    if (split > 1) {
+      __syncthreads();
+      so[slot][lane] = acc;
+      if (lane == 0) {
+        sm[slot] = m;
+        sl[slot] = l;
+        ss[slot] = sees;
+      }
+      __syncthreads();
+      if (g == 0) {
+        for (int x = 1; x < split; ++x) m = fmaxf(m, sm[slot + x]);
+        const float shift = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < split; ++x) {
+          const float w = __builtin_amdgcn_exp2f(sm[slot + x] - shift);
+          l += w * sl[slot + x];
+          sees = sees || ss[slot + x];
+          if (w != 0.f) acc += w * so[slot + x][lane];
+        }
+      }
+    }
+    if (g == 0 && r < row1) {
       const float inv = 1.0f / l;
-      store4<T>(out_row<T, D>(P, u, row), c * 4, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
-    }
-  }
-  __syncthreads();                             // the tiles may be written again
-}
-
-// A row of no keys in this part (l = 0), or of keys that may not be read (NaN).
-template <typename T, int D>
-__device__ __forceinline__ void write_fixed(const AttnParams& P, const Unit& u, int part, float value) {
-  for (int row = threadIdx.x; row < u.rows; row += 256) {
-    const int t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
-    if (P.part_o) {
-      const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + g;
-      P.part_ml[at] = f32x2{value == 0.f ? -INFINITY : value, value};
-    } else {
-      char* out = out_row<T, D>(P, u, row);
-      for (int d = 0; d < D; d += 4) store4<T>(out, d, f32x4{value, value, value, value});
+      store4<T>(out(r), lane * 4, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
     }
   }
 }
 
-// The token range of sequences [s0, s1), empty where it is none of [0, n_tokens).
-__device__ __forceinline__ int64_t tokens_of(const AttnParams& P, int s0, int s1, int64_t& first) {
-  const int64_t a = P.cu_q ? P.cu_q[s0] : s0, b = P.cu_q ? P.cu_q[s1] : s1;
-  first = a;
-  return a < 0 || b > P.n_tokens || b < a ? 0 : b - a;
-}
+// Checks shared by the entries, and the views (qvl_causal.hip).
+int attn_params(const char* what, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows, const void* out,
+                int64_t out_row, int64_t out_head, int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads,
+                int32_t head_dim, float scale, AttnParams& P);
 
-// Workgroups [0, prefix units): a part of a group's prefix for a tile of the group's rows (ROWS: tiles of 128, else of 32);
-// the others: a part of a sequence's own keys for its rows. The key/value head runs fastest, then the part, so that the
-// tiles of one part of the prefix meet in one L2 where heads x parts fill the 8 XCDs evenly.
-template <typename T, int D, bool ROWS>
-__device__ __forceinline__ void decode_unit(const AttnParams& P) {
-  using R = RowsUnit<T, D>;
-  using K = KeysUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[K::kLds > R::kLds ? K::kLds : R::kLds];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int prefix_units = P.hkv * P.prefix_parts * P.prefix_tiles * P.n_groups;
-  Unit u;
-  u.kvh = id % P.hkv;
-  if (id < prefix_units) {
-    id /= P.hkv;
-    const int part = id % P.prefix_parts, tile0 = id / P.prefix_parts % P.prefix_tiles, g = id / P.prefix_parts / P.prefix_tiles;
-    const int s0 = min(max(P.cu_groups[g], 0), P.n_seqs), s1 = min(max(P.cu_groups[g + 1], 0), P.n_seqs);
-    u.rows = s1 > s0 ? (int)tokens_of(P, s0, s1, u.token0) * P.group : 0;
-    if (u.rows == 0) return;
-    const int64_t start = P.prefix_start[g];
-    u.len = P.prefix_len[g];
-    u.lim0 = u.len;
-    if (u.len < 0 || u.len > kItemMaxLen || start < 0 || start > P.kv_rows - u.len) {
-      write_fixed<T, D>(P, u, part, NAN);
-      return;
-    }
-    const int ka = min((int64_t)part * P.prefix_chunk, (int64_t)u.len);
-    const int kb = part + 1 == P.prefix_parts ? u.len : min((int64_t)ka + P.prefix_chunk, (int64_t)u.len);
-    if (ka >= kb) {
-      write_fixed<T, D>(P, u, part, 0.f);
-      return;
-    }
-    u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
-    u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
-    if constexpr (ROWS) {
-      for (int row0 = tile0 * kItemRows; row0 < u.rows; row0 += P.prefix_tiles * kItemRows) {
-        Wave<T, D> w;
-        w.init(P, u, row0 + wave * 32);
-        R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN);
-        const int row = row0 + wave * 32 + (threadIdx.x & 31);
-        const int t = (int)((uint32_t)min(row, u.rows - 1) / (uint32_t)P.group), h = min(row, u.rows - 1) - t * P.group;
-        const int64_t at = ((int64_t)part * P.n_tokens + u.token0 + t) * (P.hkv * P.group) + u.kvh * P.group + h;
-        write_rows<T, D>(P, u, w, row, P.part_o + at * D, P.part_ml + at, true);
-      }
-    } else {
-      for (int row0 = tile0 * 32; row0 < u.rows; row0 += P.prefix_tiles * 32) {
-        Wave<T, D> w;
-        w.init(P, u, row0);
-        K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
-        join_waves<T, D>(P, u, w, smem, row0, part, ka);
-      }
-    }
-    return;
-  }
-  id = (id - prefix_units) / P.hkv;
-  u.kvh = (blockIdx.x - prefix_units) % P.hkv;
-  const int own = id % P.own_parts, seq = id / P.own_parts, part = P.prefix_parts + own;
-  const int n_new = (int)tokens_of(P, seq, seq + 1, u.token0);
-  u.rows = n_new * P.group;
-  if (u.rows == 0) return;
-  const int64_t start = P.k_start[seq];
-  u.len = P.k_len[seq];
-  if (u.len < 0 || u.len > kItemMaxLen || start < 0 || start > P.kv_rows - u.len) {
-    write_fixed<T, D>(P, u, part, NAN);
-    return;
-  }
-  u.lim0 = u.len - n_new + 1;
-  const int ka = min((int64_t)own * P.own_chunk, (int64_t)u.len);
-  const int kb = own + 1 == P.own_parts ? u.len : min((int64_t)ka + P.own_chunk, (int64_t)u.len);
-  if (ka >= kb) {
-    write_fixed<T, D>(P, u, part, 0.f);
-    return;
-  }
-  u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
-  u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
-  for (int row0 = 0; row0 < u.rows; row0 += 32) {
-    Wave<T, D> w;
-    w.init(P, u, row0);
-    K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
-    join_waves<T, D>(P, u, w, smem, row0, part, ka);
-  }
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void decode_rows_kernel(AttnParams P) { decode_unit<T, D, true>(P); }
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void decode_keys_kernel(AttnParams P) { decode_unit<T, D, false>(P); }
-
-template <typename T, int D>
-__global__ __launch_bounds__(256) void decode_combine_kernel(AttnParams P) {
-  const int64_t heads = P.hkv * P.group, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t end = P.cu_q ? min((int64_t)P.cu_q[P.n_seqs], P.n_tokens) : P.n_tokens;
-  const int64_t token = row / heads, first = P.cu_q ? max(P.cu_q[0], 0) : 0;
-  if (token >= end || token < first) return;
-  combine_row<T, D>(P.part_ml + row, P.part_o + row * D, P.n_tokens * heads, P.prefix_parts + P.own_parts,
-                    const_cast<char*>(P.out.p) + token * P.out.row + (row - token * heads) * P.out.head);
-}
-
-// How a decode launch is laid out: from the sizes alone, so that the workspace can be told beforehand.
-struct DecodePlan {
-  int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;
-  bool prefix_rows;
-  int64_t units;
-  size_t part_rows;      // 0: no parts, the kernel writes the output
-};
-
-// Parts of at least 128 keys (a block of 32 a wave), as many as fill the workgroup slots once.
-static int split_parts(int64_t keys, int64_t units, int64_t slots, int64_t least, int& chunk) {
-  int64_t parts = std::max(slots / std::max<int64_t>(units, 1), least);
-  parts = std::min({parts, (keys + 127) / 128, (int64_t)64});
-  parts = std::max<int64_t>(parts, 1);
-  const int64_t c = round_up(std::max<int64_t>((keys + parts - 1) / parts, 1), 64);
-  chunk = (int)std::min<int64_t>(c, kItemMaxLen);
-  return (int)std::max<int64_t>((keys + c - 1) / c, 1);
-}
-
-static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
-                       int32_t num_heads, int32_t num_kv_heads, int32_t dtype, DecodePlan& D) {
-  if (n_tokens < 0 || n_seqs < 0 || n_groups < 0 || max_len < 0 || max_prefix < 0) return set_error(QVL_ERR_INVALID_ARG, "%s: bad sizes", what);
-  if (n_seqs > 65535 || n_groups > 65535) return set_error(QVL_ERR_UNSUPPORTED, "%s: more than 65535 sequences or groups", what);
-  if (max_len > kItemMaxLen || max_prefix > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: lengths", what);
-  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
-    return set_error(QVL_ERR_INVALID_ARG, "%s: %d heads over %d key/value heads", what, num_heads, num_kv_heads);
-  if (num_heads > kItemHeadMask || n_tokens > kItemMaxLen || n_tokens * (num_heads / num_kv_heads) > kItemMaxLen)
-    return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
-  const int64_t slots = (int64_t)gemm_device_cus() * (dtype == QVL_DTYPE_BF16 ? 2 : 1), rows = n_tokens * (num_heads / num_kv_heads);
-  D = DecodePlan{};
-  // sequences of unlike lengths: parts of at most 1024 keys even out what the workgroups do
-  D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, n_seqs > 1 ? (max_len + 1023) / 1024 : 1, D.own_chunk);
-  if (n_groups > 0) {
-    const int64_t mean = (rows + n_groups - 1) / n_groups;
-    D.prefix_rows = mean > 32;
-    const int64_t tile = D.prefix_rows ? kItemRows : 32;
-    D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
-    D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, slots, 1, D.prefix_chunk);
-  } else {
-    D.prefix_tiles = 1;
-  }
-  D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
-  if (D.units > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
-  D.part_rows = n_groups > 0 || D.own_parts > 1 ? (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads : 0;
-  return QVL_OK;
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Checks shared by the two entries, and the views.
-static int attn_params(const char* what, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
-                       int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows,
-                       const void* out, int64_t out_row, int64_t out_head, int64_t n_tokens, int32_t num_heads,
-                       int32_t num_kv_heads, int32_t head_dim, float scale, AttnParams& P) {
-  if (dtype != QVL_DTYPE_F32 && dtype != QVL_DTYPE_BF16) return set_error(QVL_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
-  if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "%s: head_dim=%d (64 or 128)", what, head_dim);
-  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
-    return set_error(QVL_ERR_INVALID_ARG, "%s: %d heads over %d key/value heads", what, num_heads, num_kv_heads);
-  if (num_heads > kItemHeadMask) return set_error(QVL_ERR_UNSUPPORTED, "%s: num_heads=%d", what, num_heads);
-  if (n_tokens < 0 || kv_rows < 0) return set_error(QVL_ERR_INVALID_ARG, "%s: bad sizes", what);
-  if (n_tokens > kItemMaxLen || n_tokens * (num_heads / num_kv_heads) > kItemMaxLen || kv_rows > (int64_t)1 << 56)
-    return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
-  if (!(scale > 0.f) || !isfinite(scale)) return set_error(QVL_ERR_INVALID_ARG, "%s: scale %g", what, (double)scale);
-  const int64_t size = dtype == QVL_DTYPE_BF16 ? 2 : 4;
-  struct { const char* name; const void* p; int64_t row, head; AttnView* to; } views[] = {
-      {"q", q, q_row, q_head, &P.q}, {"k", k, k_row, k_head, &P.k}, {"v", v, v_row, v_head, &P.v}, {"out", out, out_row, out_head, &P.out}};
-  for (auto& w : views) {
-    if (!w.p && n_tokens > 0 && (kv_rows > 0 || w.to == &P.q || w.to == &P.out))
-      return set_error(QVL_ERR_INVALID_ARG, "%s: %s is NULL", what, w.name);
-    if (w.row < 0 || w.head < 0 || w.row > 0x7fffffffLL || w.head > 0x7fffffffLL)
-      return set_error(QVL_ERR_INVALID_ARG, "%s: strides of %s", what, w.name);
-    if ((w.to == &P.k || w.to == &P.v) && w.row * size > (int64_t)1 << 26)   // a tile's 64 rows are addressed in 32 bits
-      return set_error(QVL_ERR_UNSUPPORTED, "%s: rows of %s are more than 64 MiB apart", what, w.name);
-    if ((uintptr_t)w.p % 16 || w.row * size % 16 || w.head * size % 16)
-      return set_error(QVL_ERR_MISALIGNED, "%s: %s and its strides must be multiples of 16 bytes", what, w.name);
-    *w.to = AttnView{(const char*)w.p, w.row * size, w.head * size};
-  }
-  P.kv_rows = kv_rows;
-  P.n_tokens = n_tokens;
-  P.hkv = num_kv_heads;
-  P.group = num_heads / num_kv_heads;
-  P.scale = scale * kLog2e;
-  return QVL_OK;
-}
-
-}  // namespace qvl
-
-using namespace qvl;
-
-#define QVL_ATTN_LAUNCH(KERNEL, GRID)                                                                              \
-  do {                                                                                                             \
-    const dim3 grid = GRID;                                                                                        \
-    if (dtype == QVL_DTYPE_BF16) {                                                                                 \
-      if (head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16, 128>), grid, dim3(256), 0, (hipStream_t)stream, P);    \
-      else hipLaunchKernelGGL((KERNEL<bf16, 64>), grid, dim3(256), 0, (hipStream_t)stream, P);                     \
-    } else {                                                                                                       \
-      if (head_dim == 128) hipLaunchKernelGGL((KERNEL<float, 128>), grid, dim3(256), 0, (hipStream_t)stream, P);   \
-      else hipLaunchKernelGGL((KERNEL<float, 64>), grid, dim3(256), 0, (hipStream_t)stream, P);                    \
-    }                                                                                                              \
+// KERNEL<T, D> of the entry's dtype and head_dim.
+#define QVL_ATTN_LAUNCH(KERNEL, GRID, ...)                                                                              \
+  do {                                                                                                                  \
+    const dim3 grid = GRID;                                                                                             \
+    hipStream_t st = (hipStream_t)stream;                                                                               \
+    if (dtype == QVL_DTYPE_BF16) {                                                                                      \
+      if (head_dim == 128) hipLaunchKernelGGL((KERNEL<bf16, 128>), grid, dim3(256), 0, st, __VA_ARGS__);                \
+      else hipLaunchKernelGGL((KERNEL<bf16, 64>), grid, dim3(256), 0, st, __VA_ARGS__);                                 \
+    } else {                                                                                                            \
+      if (head_dim == 128) hipLaunchKernelGGL((KERNEL<float, 128>), grid, dim3(256), 0, st, __VA_ARGS__);               \
+      else hipLaunchKernelGGL((KERNEL<float, 64>), grid, dim3(256), 0, st, __VA_ARGS__);                                \
+    }                                                                                                                   \
   } while (0)
 
-extern "C" {
-
-int qvl_causal_workspace_size(int32_t head_dim, int64_t n_items, int64_t n_whole, size_t* bytes) {
-  if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: bytes is NULL");
-  if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "causal_workspace_size: head_dim=%d", head_dim);
-  if (n_whole < 0 || n_items < n_whole) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: items");
-  *bytes = (size_t)(n_items - n_whole) * kItemRows * ((size_t)head_dim + 2) * sizeof(float);
-  return QVL_OK;
-}
-
-int qvl_causal_attention(void* stream, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
-                         int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows,
-                         const int32_t* items, int64_t n_items, int64_t n_whole, float scale, void* out, int64_t out_row,
-                         int64_t out_head, int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                         void* workspace, size_t workspace_bytes) {
-  AttnParams P{};
-  QVL_TRY_RC(attn_params("causal_attention", dtype, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, kv_rows, out,
-                         out_row, out_head, n_tokens, num_heads, num_kv_heads, head_dim, scale, P));
-  if (n_whole < 0 || n_items < n_whole || n_items > 0x7fffffffLL) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: items");
-  if (n_tokens == 0 || n_items == 0) return QVL_OK;
-  if (!items) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: items is NULL");
-  if ((uintptr_t)items % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: items");
-  size_t need = 0;
-  QVL_TRY_RC(qvl_causal_workspace_size(head_dim, n_items, n_whole, &need));
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(QVL_ERR_WORKSPACE, "causal_attention: workspace %zu < %zu", workspace_bytes, need);
-  if (need && (uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: workspace");
-  P.items = items;
-  P.n_whole = (int)n_whole;
-  P.part_o = need ? (float*)workspace : nullptr;
-  P.part_ml = need ? (f32x2*)((float*)workspace + (n_items - n_whole) * kItemRows * head_dim) : nullptr;
-  QVL_ATTN_LAUNCH(causal_kernel, dim3((unsigned)n_items));
-  QVL_TRY_RC(check_launch("causal_attention"));
-  if (!need) return QVL_OK;
-  QVL_ATTN_LAUNCH(causal_combine_kernel, dim3((unsigned)(n_items - n_whole)));
-  return check_launch("causal_combine");
-}
-
-int qvl_decode_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
-                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, size_t* bytes) {
-  if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "decode_workspace_size: bytes is NULL");
-  if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: head_dim=%d", head_dim);
-  if (dtype != QVL_DTYPE_F32 && dtype != QVL_DTYPE_BF16) return set_error(QVL_ERR_UNSUPPORTED, "decode_workspace_size: dtype %d", dtype);
-  DecodePlan plan;
-  QVL_TRY_RC(decode_plan("decode_workspace_size", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype, plan));
-  *bytes = plan.part_rows * ((size_t)head_dim + 2) * sizeof(float);
-  return QVL_OK;
-}
-
-int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
-                         int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows,
-                         const int32_t* cu_q, int64_t n_seqs, const int64_t* k_start, const int32_t* k_len, int64_t max_len,
-                         const int32_t* cu_groups, int64_t n_groups, const int64_t* prefix_start,
-                         const int32_t* prefix_len, int64_t max_prefix, float scale, void* out, int64_t out_row,
-                         int64_t out_head, int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                         void* workspace, size_t workspace_bytes) {
-  AttnParams P{};
-  QVL_TRY_RC(attn_params("decode_attention", dtype, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, kv_rows, out,
-                         out_row, out_head, n_tokens, num_heads, num_kv_heads, head_dim, scale, P));
-  DecodePlan plan;
-  QVL_TRY_RC(decode_plan("decode_attention", n_tokens, n_seqs, max_len, n_groups, max_prefix, num_heads, num_kv_heads, dtype, plan));
-  if (!cu_q && n_tokens != n_seqs) return set_error(QVL_ERR_INVALID_ARG, "decode_attention: %lld tokens of %lld sequences without cu_q", (long long)n_tokens, (long long)n_seqs);
-  if (n_tokens == 0 || n_seqs == 0) return QVL_OK;
-  if (!k_start || !k_len || (n_groups > 0 && (!cu_groups || !prefix_start || !prefix_len)))
-    return set_error(QVL_ERR_INVALID_ARG, "decode_attention: NULL pointer");
-  if ((uintptr_t)k_start % 8 || (uintptr_t)k_len % 4 || (uintptr_t)cu_q % 4 || (uintptr_t)cu_groups % 4 ||
-      (uintptr_t)prefix_start % 8 || (uintptr_t)prefix_len % 4)
-    return set_error(QVL_ERR_MISALIGNED, "decode_attention: the sequences' state");
-  P.cu_q = cu_q;
-  P.k_start = k_start;
-  P.k_len = k_len;
-  P.cu_groups = cu_groups;
-  P.prefix_start = prefix_start;
-  P.prefix_len = prefix_len;
-  P.n_seqs = (int)n_seqs;
-  P.n_groups = (int)n_groups;
-  const size_t need = plan.part_rows * ((size_t)head_dim + 2) * sizeof(float);
-  if (workspace_bytes < need || (need && !workspace))
-    return set_error(QVL_ERR_WORKSPACE, "decode_attention: workspace %zu < %zu", workspace_bytes, need);
-  if (need && (uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "decode_attention: workspace");
-  P.part_o = need ? (float*)workspace : nullptr;
-  P.part_ml = need ? (f32x2*)((float*)workspace + plan.part_rows * head_dim) : nullptr;
-  P.own_parts = plan.own_parts;
-  P.own_chunk = plan.own_chunk;
-  P.prefix_parts = plan.prefix_parts;
-  P.prefix_chunk = plan.prefix_chunk;
-  P.prefix_tiles = plan.prefix_tiles;
-  if (plan.prefix_rows) QVL_ATTN_LAUNCH(decode_rows_kernel, dim3((unsigned)plan.units));
-  else QVL_ATTN_LAUNCH(decode_keys_kernel, dim3((unsigned)plan.units));
-  QVL_TRY_RC(check_launch("decode_attention"));
-  if (!need) return QVL_OK;
-  const int64_t blocks = (n_tokens * num_heads + 3) / 4;
-  QVL_ATTN_LAUNCH(decode_combine_kernel, dim3((unsigned)blocks));
-  return check_launch("decode_combine");
-}
-
-}  // extern "C"
+}  // namespace qvl
