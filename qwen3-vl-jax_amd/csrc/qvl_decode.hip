@@ -34,8 +34,11 @@ struct DecodeState {
   int slot_rows;                                                        // streaming: rows a part's slot has
 };
 
-// The four waves' results of the same rows joined in LDS (free by then), and written: to the output, or as a part, row r of
-// which is row at(r) of the part buffers. `ka`: the first key of the range the waves covered.
+// A barrier for what lies in LDS alone: __syncthreads also waits until stores to memory are through (3 us of a launch of 20).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The four waves' results of the same rows joined in LDS, each wave's where its tiles were, and written: to the output, or as
+// a part, row r of which is row at(r) of the part buffers. `ka`: the first key of the range the waves covered.
 template <typename T, int D, typename F>
 __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int ka,
                                            bool part, F&& at) {
@@ -50,13 +53,13 @@ __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W
     sl[wave][l32] = lw;
     slim[l32] = w.lim;
   }
-  __syncthreads();                             // every wave is past its tiles
-  float* const so = reinterpret_cast<float*>(smem);
+  constexpr int kWave = 2 * KeysUnit<T, D>::kTile;
+  static_assert(kWave >= 32 * D * 4, "a wave's rows fit its tiles");
   if (l32 < n)
     w.core.each4([&](int d, const f32x4& x) {
-      *reinterpret_cast<f32x4*>(so + ((wave * 32 + l32) * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 4) = x;
+      *reinterpret_cast<f32x4*>(smem + wave * kWave + (l32 * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 16) = x;
     });
-  __syncthreads();
+  lds_barrier();
   for (int i = threadIdx.x; i < n * kC; i += 256) {
     const int r = i / kC, c = i % kC;
     float M = sm[0][r];
@@ -70,7 +73,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W
       const float f = __builtin_amdgcn_exp2f(sm[x][r] - shift);
       l += f * sl[x][r];
       // a wave that saw none of the row's keys has zeros; one whose maximum is far below the others' may hold infinities
-      const f32x4 o = *reinterpret_cast<const f32x4*>(so + ((x * 32 + r) * kC + (c ^ (r & (kC - 1)))) * 4);
+      const f32x4 o = *reinterpret_cast<const f32x4*>(smem + x * kWave + (r * kC + (c ^ (r & (kC - 1)))) * 16);
       if (f != 0.f) acc += f * o;
     }
     const bool sees = slim[r] > ka;
@@ -83,7 +86,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W
       store4<T>(out_row<T, D>(P, u, first_row + r), c * 4, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
     }
   }
-  __syncthreads();                             // the tiles may be written again
+  lds_barrier();                               // the tiles may be written again
 }
 
 // The token range of sequences [s0, s1), empty where it is none of [0, n_tokens).
@@ -100,14 +103,21 @@ __device__ __forceinline__ bool bad_keys(const AttnParams& P, int64_t start, int
 // ---------------------------------------------------------------------------------------------
 // streaming
 // ---------------------------------------------------------------------------------------------
-// A sequence's jobs (tiles of 32 rows) and each one's blocks of 32 keys: one where there is nothing to read, for the rows'
-// zeros (or NaN).
-__device__ __forceinline__ int64_t jobs_of(const AttnParams& P, const DecodeState& S, int seq, int& blocks) {
-  int64_t first;
-  const int64_t rows = tokens_of(P, S, seq, seq + 1, first) * P.group;
-  const int len = S.k_len[seq];
-  blocks = bad_keys(P, S.k_start[seq], len) ? 1 : max((len + 31) >> 5, 1);
-  return (rows + 31) / 32;
+// What the line holds of a sequence: its jobs (tiles of 32 rows), and the blocks of 32 keys of each, one where there is
+// nothing to read, for the rows' zeros (or NaN).
+struct Sequence {
+  int64_t token0, start;
+  int tokens, len, jobs, blocks;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const AttnParams& P, const DecodeState& S, int seq) {
+  Sequence q;
+  q.tokens = (int)tokens_of(P, S, seq, seq + 1, q.token0);
+  q.start = S.k_start[seq];
+  q.len = S.k_len[seq];
+  q.jobs = (int)(((int64_t)q.tokens * P.group + 31) / 32);
+  q.blocks = bad_keys(P, q.start, q.len) ? 1 : max((q.len + 31) >> 5, 1);
+  return q;
 }
 
 // Exclusive sums of v over the workgroup, in excl[0..256] (excl[256]: the total).
@@ -129,92 +139,143 @@ __device__ __forceinline__ void scan256(int64_t v, int64_t* excl) {
   __syncthreads();
 }
 
-// The sequence that block `pos` of the line belongs to, and the block its first job starts at. `excl`: sums over runs of
-// `per` sequences a thread.
-__device__ __forceinline__ void locate(const AttnParams& P, const DecodeState& S, int64_t pos, int per, const int64_t* excl,
-                                       int64_t* work, int& seq, int64_t& base) {
-  __shared__ int hit;
-  if (excl[threadIdx.x] <= pos && pos < excl[threadIdx.x + 1]) hit = threadIdx.x;
-  __syncthreads();
-  const int run = hit;
-  __syncthreads();
-  seq = run * per;
-  base = excl[run];
-  if (per == 1) return;
-  int blocks = 0;
-  const int s = seq + (int)threadIdx.x;
-  const int64_t jobs = (int)threadIdx.x < per && s < S.n_seqs ? jobs_of(P, S, s, blocks) : 0;
-  scan256(jobs * blocks, work);
-  if (work[threadIdx.x] <= pos - base && pos - base < work[threadIdx.x + 1]) hit = threadIdx.x;
-  __syncthreads();
-  const int in = hit;
-  seq += in;
-  base += work[in];
-  __syncthreads();
+__device__ __forceinline__ Sequence uniform(Sequence q) {
+  q.token0 = uniform(q.token0);
+  q.start = uniform(q.start);
+  q.tokens = uniform(q.tokens);
+  q.len = uniform(q.len);
+  q.jobs = uniform(q.jobs);
+  q.blocks = uniform(q.blocks);
+  return q;
 }
 
 // Where run i of n begins: an equal share of the line, moved to a job's end where the job is no longer than a share (or a
-// block for each wave), so that short jobs stay whole.
+// block for each wave), so that short jobs stay whole. `base`: where the jobs of the sequence that the share begins in do.
 __device__ __forceinline__ int64_t share(int64_t total, int i, int n) { return total / n * i + total % n * i / n; }
-__device__ __forceinline__ int64_t run_start(const AttnParams& P, const DecodeState& S, int64_t total, int i, int n, int per,
-                                             const int64_t* excl, int64_t* work, int& seq, int64_t& base) {
-  const int64_t pos = share(total, i, n);
-  if (pos >= total) return total;
-  locate(P, S, pos, per, excl, work, seq, base);
-  int blocks;
-  jobs_of(P, S, seq, blocks);
-  const int64_t in = (pos - base) % blocks;
-  seq = uniform(seq);
-  base = uniform(base);
+__device__ __forceinline__ int64_t run_start(int64_t total, int64_t pos, int n, int64_t base, int blocks) {
+  const int in = (int)((pos - base) % blocks);
   return in == 0 || blocks > max((int64_t)4, total / n) ? pos : pos - in + (2 * in < blocks ? 0 : blocks);
+}
+
+// The line as one workgroup sees it. Up to 64 sequences: one a lane, and each wave finds its way without the others (a decode
+// step of a few chats is a few microseconds long). More: a run of `per` sequences a thread, summed up in LDS, then one run
+// again.
+struct Line {
+  int64_t excl[257], work[257];
+  int hit;
+};
+
+__device__ __forceinline__ void locate(const AttnParams& P, const DecodeState& S, Line& L, int64_t pos, int per, int& seq, int64_t& base) {
+  if (L.excl[threadIdx.x] <= pos && pos < L.excl[threadIdx.x + 1]) L.hit = threadIdx.x;
+  __syncthreads();
+  const int run = L.hit;
+  seq = run * per;
+  base = L.excl[run];
+  __syncthreads();
+  const int s = seq + (int)threadIdx.x;
+  int64_t mine = 0;
+  if ((int)threadIdx.x < per && s < S.n_seqs) {
+    const Sequence q = sequence_of(P, S, s);
+    mine = (int64_t)q.jobs * q.blocks;
+  }
+  scan256(mine, L.work);
+  if (L.work[threadIdx.x] <= pos - base && pos - base < L.work[threadIdx.x + 1]) L.hit = threadIdx.x;
+  __syncthreads();
+  seq = uniform(seq + L.hit);
+  base = uniform(base + L.work[L.hit]);
+  __syncthreads();
+}
+
+// The run [pos, end) of workgroup `run` of at most `runs`, how many there are (n), and the sequence that pos lies in, whose
+// jobs begin at `base`. pos >= end: nothing to do.
+__device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState& S, Line& L, int run, int runs, int64_t& total, int& n,
+                                         int64_t& pos, int64_t& end, int& seq, int64_t& base, Sequence& q) {
+  const int lane = threadIdx.x & 63;
+  pos = end = 0;
+  if (S.n_seqs <= 64) {
+    Sequence mine{};
+    if (lane < S.n_seqs) mine = sequence_of(P, S, lane);
+    int64_t x = (int64_t)mine.jobs * mine.blocks;
+    const int64_t own = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(x, d);
+      if (lane >= d) x += y;
+    }
+    total = uniform(__shfl(x, 63));
+    n = (int)min((int64_t)runs, total);   // no run of a split job is empty
+    if (run >= n) return;
+    auto start = [&](int i, int& at) {
+      const int64_t p = share(total, i, n);
+      if (p >= total) return total;
+      at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x - own <= p && p < x)) - 1;
+      return run_start(total, p, n, uniform(__shfl(x - own, at)), uniform(__shfl(mine.blocks, at)));
+    };
+    int other = 0;
+    pos = start(run, seq);
+    end = start(run + 1, other);
+    base = uniform(__shfl(x - own, seq));
+    q.token0 = __shfl(mine.token0, seq);
+    q.start = __shfl(mine.start, seq);
+    q.tokens = __shfl(mine.tokens, seq);
+    q.len = __shfl(mine.len, seq);
+    q.jobs = __shfl(mine.jobs, seq);
+    q.blocks = __shfl(mine.blocks, seq);
+    q = uniform(q);
+    return;
+  }
+  const int per = (S.n_seqs + 255) / 256;
+  int64_t mine = 0;
+  for (int s = threadIdx.x * per; s < min((int)(threadIdx.x + 1) * per, S.n_seqs); ++s) {
+    const Sequence one = sequence_of(P, S, s);
+    mine += (int64_t)one.jobs * one.blocks;
+  }
+  scan256(mine, L.excl);
+  total = uniform(L.excl[256]);
+  n = (int)min((int64_t)runs, total);
+  if (run >= n) return;
+  auto start = [&](int i, int& at, int64_t& first) {
+    const int64_t p = share(total, i, n);
+    if (p >= total) return total;
+    locate(P, S, L, p, per, at, first);
+    return run_start(total, p, n, first, uniform(sequence_of(P, S, at).blocks));
+  };
+  int other = 0;
+  int64_t other_base = 0;
+  pos = start(run, seq, base);
+  end = start(run + 1, other, other_base);
+  q = uniform(sequence_of(P, S, seq));
 }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, DecodeState S) {
   using K = KeysUnit<T, D>;
   __shared__ __attribute__((aligned(16))) char smem[K::kLds];
-  __shared__ int64_t excl[257], work[257];
+  __shared__ Line L;
   const int run = blockIdx.x / P.hkv, kvh = blockIdx.x % P.hkv;
-  // this run of the line: [pos, end), pos in sequence `seq` whose jobs begin at `base`
-  const int per = (S.n_seqs + 255) / 256;
-  int64_t mine = 0;
-  for (int s = threadIdx.x * per; s < min((int)(threadIdx.x + 1) * per, S.n_seqs); ++s) {
-    int blocks;
-    const int64_t jobs = jobs_of(P, S, s, blocks);
-    mine += jobs * blocks;
-  }
-  scan256(mine, excl);
-  const int64_t total = uniform(excl[256]);
-  const int n = (int)min((int64_t)(gridDim.x / P.hkv), total);   // no run of a split job is empty
-  if (run >= n) {
-    if (threadIdx.x == 0 && kvh == 0) S.split[run].parts = 0;
-    return;
-  }
-  int seq = 0, seq_end = 0;
-  int64_t base = 0, base_end = 0;
-  int64_t pos = uniform(run_start(P, S, total, run, n, per, excl, work, seq, base));
-  const int64_t end = uniform(run_start(P, S, total, run + 1, n, per, excl, work, seq_end, base_end));
+  int64_t total, pos, end, base = 0;
+  int n, seq = 0;
+  Sequence q;
+  find_run(P, S, L, run, gridDim.x / P.hkv, total, n, pos, end, seq, base, q);
   SplitJob joined{};
   while (pos < end) {
-    Unit u;
-    int blocks;
-    const int64_t jobs = uniform(jobs_of(P, S, seq, blocks));
-    blocks = uniform(blocks);
-    if (pos >= base + jobs * blocks) {           // the next sequence (jobs == 0: it has no rows)
-      base += jobs * blocks;
-      ++seq;
+    const int blocks = q.blocks;
+    const int64_t own = (int64_t)q.jobs * blocks;
+    if (pos >= base + own) {           // the next sequence (jobs == 0: it has no rows)
+      base += own;
+      q = uniform(sequence_of(P, S, ++seq));
       continue;
     }
-    const int n_new = uniform((int)tokens_of(P, S, seq, seq + 1, u.token0));
-    const int64_t start = uniform(S.k_start[seq]);
-    u.token0 = uniform(u.token0);
-    u.len = uniform(S.k_len[seq]);
+    Unit u;
+    const int64_t start = q.start;
+    u.token0 = q.token0;
+    u.len = q.len;
     const int job = (int)((pos - base) / blocks), b0 = (int)((pos - base) % blocks);
     const int b1 = (int)min((int64_t)blocks, b0 + (end - pos));
     u.kvh = kvh;
     u.row0 = job * 32;
-    u.rows = n_new * P.group;
-    u.lim0 = u.len - n_new + 1;
+    u.rows = q.tokens * P.group;
+    u.lim0 = u.len - q.tokens + 1;
     const int n_rows = min(32, u.rows - u.row0);
     const bool whole = b0 == 0 && b1 == blocks, bad = bad_keys(P, start, u.len);
     if (bad) {

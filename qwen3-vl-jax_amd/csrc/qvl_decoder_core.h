@@ -482,7 +482,8 @@ template <typename T, int D, bool V> struct Loader {
   static __device__ __forceinline__ int swz(int row) { return V ? C::v_swz(row) : C::k_swz(row); }
   // `left` rows from `base` on; past them zeros arrive
   __device__ __forceinline__ void at(const char* base, int left) {
-    rsrc = rsrc_words(base, left > 0 ? (uint32_t)((int64_t)(min(left, 64) - 1) * stride + C::kRowBytes) : 0u);
+    rsrc = rsrc_words((const char*)uniform((int64_t)base),
+                      (uint32_t)uniform((int)(left > 0 ? (uint32_t)((int64_t)(min(left, 64) - 1) * stride + C::kRowBytes) : 0u)));
   }
   // rows [kRows i, kRows (i + 1)) of the tile at `lds`. (A DMA's rows lie in one aligned run of kRows, so the swizzle of
   // row kRows i + r is that of kRows i XOR that of r.)
@@ -638,13 +639,13 @@ __device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, c
 
 // Parts of rows joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, in an order that only the number of parts
 // sets. A workgroup takes 256 / (lanes x split) rows at once: D / 4 lanes hold a row, 16 bytes each, and `split` groups of
-// them share its parts, 4 in flight each, so that a row of 32 parts costs one trip to memory and not 32. `at(r, p)` is part
+// them share its parts, 8 in flight each, so that a row of 64 parts costs one trip to memory and not 64. `at(r, p)` is part
 // p's row index in P.part_ml / P.part_o, `out(r)` where row r goes.
-__device__ __host__ constexpr int join_split(int parts) { return parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8; }
+__device__ __host__ constexpr int join_split(int parts) { return parts <= 8 ? 1 : parts <= 16 ? 2 : parts <= 32 ? 4 : 8; }
 
 template <typename T, int D, typename At, typename Out>
 __device__ __forceinline__ void join_parts(const AttnParams& P, int row0, int row1, int parts, At&& at, Out&& out) {
-  constexpr int kLanes = D / 4, kSlots = 256 / kLanes;
+  constexpr int kLanes = D / 4, kSlots = 256 / kLanes, kFlight = 8;
   __shared__ f32x4 so[kSlots][kLanes];
   __shared__ float sm[kSlots], sl[kSlots];
   __shared__ int ss[kSlots];
@@ -655,24 +656,27 @@ __device__ __forceinline__ void join_parts(const AttnParams& P, int row0, int ro
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
     bool sees = false;
     if (r < row1) {
-      for (int p0 = g; p0 < parts; p0 += 4 * split) {
-        f32x2 st[4];
-        f32x4 o[4];
+      for (int p0 = g; p0 < parts; p0 += kFlight * split) {
+        f32x2 st[kFlight];
+        f32x4 o[kFlight];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kFlight; ++i) {
           const int p = p0 + i * split;
           const int64_t a = at(r, p < parts ? p : p0);
           st[i] = P.part_ml[a];
           o[i] = *reinterpret_cast<const f32x4*>(P.part_o + a * D + lane * 4);
           if (p >= parts) st[i] = f32x2{-INFINITY, 0.f};
         }
-        const float mn = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), m), shift = mn == -INFINITY ? 0.f : mn;
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) mn = fmaxf(mn, st[i].x);
+        const float shift = mn == -INFINITY ? 0.f : mn;
         const float a = __builtin_amdgcn_exp2f(m - shift);
         l *= a;
         acc *= a;
         m = mn;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kFlight; ++i) {
           const float w = __builtin_amdgcn_exp2f(st[i].x - shift);
           l += w * st[i].y;
           sees = sees || __float_as_uint(st[i].y) != 0;
