@@ -37,12 +37,17 @@ struct DecodeState {
 // A barrier for what lies in LDS alone: __syncthreads also waits until stores to memory are through (3 us of a launch of 20).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The four waves' results of the same rows joined in LDS, each wave's where its tiles were, and written: to the output, or as
+// LDS of the join below, over the tiles.
+template <typename T, int D> constexpr int kJoinBytes = 4 * 32 * (D * 4 + 16);
+
+// The four waves' results of the same rows joined in LDS and written: to the output, or as
 // a part, row r of which is row at(r) of the part buffers. `ka`: the first key of the range the waves covered.
 template <typename T, int D, typename F>
 __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int ka,
                                            bool part, F&& at) {
-  constexpr int kC = D / 4;                    // 16-byte chunks of a row, XOR-swizzled by the row
+  // Rows of kPitch bytes: 16 more than a row, so that neither rows nor chunks meet in a bank and every address is one lane's
+  // base and a constant (each line of code that runs once costs a workgroup some 800 cycles of fetching it).
+  constexpr int kC = D / 4, kPitch = D * 4 + 16, kWave = kJoinBytes<T, D> / 4;
   __shared__ float sm[4][32], sl[4][32];
   __shared__ int slim[32];
   const int lane = threadIdx.x & 63, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -53,12 +58,11 @@ __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W
     sl[wave][l32] = lw;
     slim[l32] = w.lim;
   }
-  constexpr int kWave = 2 * KeysUnit<T, D>::kTile;
-  static_assert(kWave >= 32 * D * 4, "a wave's rows fit its tiles");
-  if (l32 < n)
-    w.core.each4([&](int d, const f32x4& x) {
-      *reinterpret_cast<f32x4*>(smem + wave * kWave + (l32 * kC + ((d >> 2) ^ (l32 & (kC - 1)))) * 16) = x;
-    });
+  lds_barrier();                               // every wave is past its tiles
+  if (l32 < n) {
+    char* row = smem + wave * kWave + l32 * kPitch;
+    w.core.each4([&](int d, const f32x4& x) { *reinterpret_cast<f32x4*>(row + d * 4) = x; });
+  }
   lds_barrier();
   for (int i = threadIdx.x; i < n * kC; i += 256) {
     const int r = i / kC, c = i % kC;
@@ -73,7 +77,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W
       const float f = __builtin_amdgcn_exp2f(sm[x][r] - shift);
       l += f * sl[x][r];
       // a wave that saw none of the row's keys has zeros; one whose maximum is far below the others' may hold infinities
-      const f32x4 o = *reinterpret_cast<const f32x4*>(smem + x * kWave + (r * kC + (c ^ (r & (kC - 1)))) * 16);
+      const f32x4 o = *reinterpret_cast<const f32x4*>(smem + x * kWave + r * kPitch + c * 16);
       if (f != 0.f) acc += f * o;
     }
     const bool sees = slim[r] > ka;
@@ -157,9 +161,8 @@ __device__ __forceinline__ int64_t run_start(int64_t total, int64_t pos, int n, 
   return in == 0 || blocks > max((int64_t)4, total / n) ? pos : pos - in + (2 * in < blocks ? 0 : blocks);
 }
 
-// The line as one workgroup sees it. Up to 64 sequences: one a lane, and each wave finds its way without the others (a decode
-// step of a few chats is a few microseconds long). More: a run of `per` sequences a thread, summed up in LDS, then one run
-// again.
+// The line as one workgroup sees it. Up to 64 sequences: one a lane, and each wave finds its way without the others. More: a
+// run of `per` sequences a thread, summed up in LDS, then one run again.
 struct Line {
   int64_t excl[257], work[257];
   int hit;
@@ -195,34 +198,45 @@ __device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState&
   if (S.n_seqs <= 64) {
     Sequence mine{};
     if (lane < S.n_seqs) mine = sequence_of(P, S, lane);
-    int64_t x = (int64_t)mine.jobs * mine.blocks;
-    const int64_t own = x;
+    // in 32 bits where the line is that short (2^30 blocks: 2^35 keys): a few instructions for each division, not a hundred,
+    // and code that runs once is paid by its length
+    const int own = (int)min((int64_t)mine.jobs * mine.blocks, (int64_t)1 << 25);
+    int x = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(x, d);
-      if (lane >= d) x += y;
+      const int y = __shfl_up(x, d);
+      x += lane >= d ? y : 0;
     }
-    total = uniform(__shfl(x, 63));
-    n = (int)min((int64_t)runs, total);   // no run of a split job is empty
-    if (run >= n) return;
-    auto start = [&](int i, int& at) {
-      const int64_t p = share(total, i, n);
-      if (p >= total) return total;
-      at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x - own <= p && p < x)) - 1;
-      return run_start(total, p, n, uniform(__shfl(x - own, at)), uniform(__shfl(mine.blocks, at)));
-    };
-    int other = 0;
-    pos = start(run, seq);
-    end = start(run + 1, other);
-    base = uniform(__shfl(x - own, seq));
-    q.token0 = __shfl(mine.token0, seq);
-    q.start = __shfl(mine.start, seq);
-    q.tokens = __shfl(mine.tokens, seq);
-    q.len = __shfl(mine.len, seq);
-    q.jobs = __shfl(mine.jobs, seq);
-    q.blocks = __shfl(mine.blocks, seq);
-    q = uniform(q);
-    return;
+    const uint32_t sum = (uint32_t)__builtin_amdgcn_readlane(x, 63);
+    if (__builtin_amdgcn_ballot_w64((int64_t)mine.jobs * mine.blocks != own) == 0) {
+      total = sum;
+      n = (int)min((uint32_t)runs, sum);   // no run of a split job is empty
+      if (run >= n) return;
+      const uint32_t each = sum / (uint32_t)n, rest = sum - each * (uint32_t)n;
+      auto start = [&](int i, int& at) {
+        const uint32_t p = each * (uint32_t)i + rest * (uint32_t)i / (uint32_t)n;
+        at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64((uint32_t)(x - own) <= p && p < (uint32_t)x)) - 1;
+        if (i == n) return (int64_t)sum;
+        const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane(mine.blocks, at);
+        const uint32_t in = (p - (uint32_t)__builtin_amdgcn_readlane(x - own, at)) % blocks;
+        return (int64_t)(in == 0 || blocks > max(4u, each) ? p : p - in + (2 * in < blocks ? 0 : blocks));
+      };
+      int other = 0;
+      end = start(run + 1, other);
+      pos = start(run, seq);
+      base = __builtin_amdgcn_readlane(x - own, seq);
+      auto lane64 = [&](int64_t v) {
+        return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), seq) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)v, seq));
+      };
+      q.token0 = lane64(mine.token0);
+      q.start = lane64(mine.start);
+      q.tokens = __builtin_amdgcn_readlane(mine.tokens, seq);
+      q.len = __builtin_amdgcn_readlane(mine.len, seq);
+      q.jobs = __builtin_amdgcn_readlane(mine.jobs, seq);
+      q.blocks = __builtin_amdgcn_readlane(mine.blocks, seq);
+      return;
+    }
   }
   const int per = (S.n_seqs + 255) / 256;
   int64_t mine = 0;
@@ -250,7 +264,7 @@ __device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState&
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, DecodeState S) {
   using K = KeysUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[K::kLds];
+  __shared__ __attribute__((aligned(16))) char smem[std::max(K::kLds, kJoinBytes<T, D>)];
   __shared__ Line L;
   const int run = blockIdx.x / P.hkv, kvh = blockIdx.x % P.hkv;
   int64_t total, pos, end, base = 0;
@@ -270,7 +284,12 @@ __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, Dec
     const int64_t start = q.start;
     u.token0 = q.token0;
     u.len = q.len;
-    const int job = (int)((pos - base) / blocks), b0 = (int)((pos - base) % blocks);
+    const int64_t into = pos - base;
+    int job = 0, b0 = (int)into;
+    if (into >= blocks) {
+      job = (int)(into / blocks);
+      b0 = (int)(into % blocks);
+    }
     const int b1 = (int)min((int64_t)blocks, b0 + (end - pos));
     u.kvh = kvh;
     u.row0 = job * 32;
@@ -293,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, Dec
     if (b0 > 0 && b1 == blocks) {
       // the run that holds the job's first block: the last whose share begins there or before
       const int64_t first = pos - b0;
-      int w0 = (int)min((int64_t)((double)first / (double)total * n), (int64_t)run);
+      int w0 = (int)min((int64_t)((float)first / (float)total * n), (int64_t)run);
       while (w0 > 0 && share(total, w0, n) > first) --w0;
       while (w0 < run && share(total, w0 + 1, n) <= first) ++w0;
       joined = SplitJob{u.token0, u.rows, u.row0, w0, run - w0 + 1};
@@ -337,7 +356,7 @@ template <typename T, int D, bool ROWS>
 __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeState& S) {
   using R = RowsUnit<T, D>;
   using K = KeysUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[ROWS && R::kLds > K::kLds ? R::kLds : K::kLds];
+  __shared__ __attribute__((aligned(16))) char smem[std::max({K::kLds, kJoinBytes<T, D>, ROWS ? R::kLds : 0})];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int prefix_units = P.hkv * S.prefix_parts * S.prefix_tiles * S.n_groups;
   const bool own = (int)blockIdx.x >= prefix_units;

@@ -434,7 +434,8 @@ template <typename T, int D> struct Wave {
     // does not depend on the others of its wave.
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
       const float mn = mx > m + 8.f ? mx : m;
-      core.rescale(__builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn)));
+      // (nothing to rescale before a row's first key)
+      if (__builtin_amdgcn_ballot_w64(m != -INFINITY) != 0) core.rescale(__builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn)));
       m = mn;
     }
     const float shift = m == -INFINITY ? 0.f : -m;
