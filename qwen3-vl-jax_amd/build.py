@@ -36,7 +36,10 @@ def common_flags() -> list:
 # Per-file device-code flags. The GEMM file is scheduled with the backend's max-ILP strategy: on
 # MI355X it took fc1 / qkv 1.5-2 % and the config-2 / 3 / 4 forwards 0.5-0.8 % below the default
 # scheduler's (same-call A/B, no spills either way).
-FILE_FLAGS = {"qvl_gemm.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]}
+# The 256-row attention tiles keep every product's result in vector registers and the operands in the accumulation ones; the
+# compiler's own choice copies the accumulators through each other in the loop.
+FILE_FLAGS = {"qvl_gemm.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+              "qvl_causal_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def build(verbose: bool = False, jobs: int = 8) -> Path:

@@ -1,8 +1,10 @@
-// Causal attention of packed prompts over a work list (qvl_causal_worklist): 128 rows a workgroup, long tiles split along
-// their keys and joined.
+// Causal attention of packed prompts over a work list (qvl_causal_worklist): 128 rows a workgroup, or 256 (qvl_causal_wide.hip),
+// long tiles split along their keys and joined.
 #include "qvl_decoder_core.h"
 
 namespace qvl {
+
+void launch_causal_wide(void* stream, int32_t head_dim, const AttnParams& P, const int32_t* items, int64_t n_items, int64_t n_whole);
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P, const int32_t* items, int n_whole) {
@@ -37,16 +39,16 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P, const int3
 
 // The rows of split tiles: the workgroup of a part joins its share of the tile's 128 rows.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void causal_combine_kernel(AttnParams P, const int32_t* items, int n_whole) {
+__global__ __launch_bounds__(256) void causal_combine_kernel(AttnParams P, const int32_t* items, int n_whole, int tile_rows) {
   const int32_t* it = items + 8 * ((int64_t)n_whole + blockIdx.x);
   const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
   const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
   if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || part >= parts ||
       part > slot || slot - part + parts > (int)gridDim.x) return;
   const Unit u{nullptr, nullptr, len, 0, q0, n_new * P.group, row0, kvh};
-  const int64_t first = (int64_t)(slot - part) * kItemRows;
-  join_parts<T, D>(P, kItemRows * part / parts, min(kItemRows * (part + 1) / parts, u.rows - row0), parts,
-                   [&](int r, int p) { return first + (int64_t)p * kItemRows + r; },
+  const int64_t first = (int64_t)(slot - part) * tile_rows;
+  join_parts<T, D>(P, tile_rows * part / parts, min(tile_rows * (part + 1) / parts, u.rows - row0), parts,
+                   [&](int r, int p) { return first + (int64_t)p * tile_rows + r; },
                    [&](int r) { return out_row<T, D>(P, u, row0 + r); });
 }
 
@@ -94,37 +96,40 @@ using namespace qvl;
 
 extern "C" {
 
-int qvl_causal_workspace_size(int32_t head_dim, int64_t n_items, int64_t n_whole, size_t* bytes) {
+int qvl_causal_workspace_size(int32_t head_dim, int32_t tile_rows, int64_t n_items, int64_t n_whole, size_t* bytes) {
   if (!bytes) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: bytes is NULL");
   if (head_dim != 64 && head_dim != 128) return set_error(QVL_ERR_UNSUPPORTED, "causal_workspace_size: head_dim=%d", head_dim);
-  if (n_whole < 0 || n_items < n_whole) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: items");
-  *bytes = (size_t)(n_items - n_whole) * kItemRows * ((size_t)head_dim + 2) * sizeof(float);
+  if (n_whole < 0 || n_items < n_whole || (tile_rows != 128 && tile_rows != 256)) return set_error(QVL_ERR_INVALID_ARG, "causal_workspace_size: items");
+  *bytes = (size_t)(n_items - n_whole) * tile_rows * ((size_t)head_dim + 2) * sizeof(float);
   return QVL_OK;
 }
 
 int qvl_causal_attention(void* stream, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
                          int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows,
-                         const int32_t* items, int64_t n_items, int64_t n_whole, float scale, void* out, int64_t out_row,
+                         int32_t tile_rows, const int32_t* items, int64_t n_items, int64_t n_whole, float scale, void* out, int64_t out_row,
                          int64_t out_head, int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                          void* workspace, size_t workspace_bytes) {
   AttnParams P{};
   QVL_TRY_RC(attn_params("causal_attention", dtype, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, kv_rows, out,
                          out_row, out_head, n_tokens, num_heads, num_kv_heads, head_dim, scale, P));
   if (n_whole < 0 || n_items < n_whole || n_items > 0x7fffffffLL) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: items");
+  if (tile_rows != 128 && tile_rows != 256) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: tile_rows=%d", tile_rows);
+  if (tile_rows == 256 && dtype == QVL_DTYPE_F32) return set_error(QVL_ERR_UNSUPPORTED, "causal_attention: tiles of 256 rows are bf16 only");
   if (n_tokens == 0 || n_items == 0) return QVL_OK;
   if (!items) return set_error(QVL_ERR_INVALID_ARG, "causal_attention: items is NULL");
   if ((uintptr_t)items % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: items");
   size_t need = 0;
-  QVL_TRY_RC(qvl_causal_workspace_size(head_dim, n_items, n_whole, &need));
+  QVL_TRY_RC(qvl_causal_workspace_size(head_dim, tile_rows, n_items, n_whole, &need));
   if (workspace_bytes < need || (need && !workspace))
     return set_error(QVL_ERR_WORKSPACE, "causal_attention: workspace %zu < %zu", workspace_bytes, need);
   if (need && (uintptr_t)workspace % 16) return set_error(QVL_ERR_MISALIGNED, "causal_attention: workspace");
   P.part_o = need ? (float*)workspace : nullptr;
-  P.part_ml = need ? (f32x2*)((float*)workspace + (n_items - n_whole) * kItemRows * head_dim) : nullptr;
-  QVL_ATTN_LAUNCH(causal_kernel, dim3((unsigned)n_items), P, items, (int)n_whole);
+  P.part_ml = need ? (f32x2*)((float*)workspace + (n_items - n_whole) * tile_rows * head_dim) : nullptr;
+  if (tile_rows == 256) launch_causal_wide(stream, head_dim, P, items, n_items, n_whole);
+  else QVL_ATTN_LAUNCH(causal_kernel, dim3((unsigned)n_items), P, items, (int)n_whole);
   QVL_TRY_RC(check_launch("causal_attention"));
   if (!need) return QVL_OK;
-  QVL_ATTN_LAUNCH(causal_combine_kernel, dim3((unsigned)(n_items - n_whole)), P, items, (int)n_whole);
+  QVL_ATTN_LAUNCH(causal_combine_kernel, dim3((unsigned)(n_items - n_whole)), P, items, (int)n_whole, tile_rows);
   return check_launch("causal_combine");
 }
 

@@ -113,13 +113,13 @@ template <int D> struct Core<bf16, D> {
       for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(lds, db, 2 * b + e), pf, o[db], 0, 0, 0);
     }
   }
-  __device__ __forceinline__ void add_weights(const u32x4& pw) {
+  __device__ __forceinline__ void add_pair(uint32_t w) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);
+  }
+  __device__ __forceinline__ void add_weights(const u32x4& pw) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = pw[j];   // a copy: __builtin_bit_cast of a vector's element takes element 0 here
-      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);
-    }
+    for (int j = 0; j < 4; ++j) add_pair(pw[j]);   // by value: __builtin_bit_cast of a vector's element takes element 0 here
   }
   // The scores of both blocks of a tile of 64 keys: a block's fragments are read ahead of its products.
   // `beside(i)`, i < 8, runs among the products.
@@ -387,6 +387,18 @@ template <typename T, int D> struct Wave {
     m = -INFINITY;
     core.init(q);
   }
+  // Scores of 32 keys from kb on that the lane's row does not see become -inf; returns which it sees, a bit per register.
+  __device__ __forceinline__ uint32_t mask(f32x16& s, int kb) const {
+    const int base = lim - kb - 4 * (int)((threadIdx.x & 63) >> 5);
+    uint32_t seen = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool in = 8 * (r >> 2) + (r & 3) < base;
+      seen |= (in ? 1u : 0u) << r;
+      s[r] = in ? s[r] : -INFINITY;
+    }
+    return seen;
+  }
   // NB blocks of 32 keys from key kb on; K and V tiles in LDS. `between(i)`, i < 8, runs beside the scores' products, or
   // after them, once they are read out of K's tile; `before_v` before V's is read.
   // SAFE: V may hold what is not finite.
@@ -407,17 +419,8 @@ template <typename T, int D> struct Wave {
     const bool edge = kb + 32 * NB > lim_lo;
     uint32_t seen[NB];
     if (edge) {
-      const int base = lim - kb - 4 * (int)((threadIdx.x & 63) >> 5);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        seen[b] = 0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool in = 32 * b + 8 * (r >> 2) + (r & 3) < base;
-          seen[b] |= (in ? 1u : 0u) << r;
-          s[b][r] = in ? s[b][r] : -INFINITY;
-        }
-      }
+      for (int b = 0; b < NB; ++b) seen[b] = mask(s[b], kb + 32 * b);
     }
     float m4[4];
 #pragma unroll

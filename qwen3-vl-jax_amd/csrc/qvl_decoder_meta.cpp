@@ -38,48 +38,62 @@ double makespan(std::vector<double> cost, int64_t slots) {
   return end;
 }
 
+// What the kernel of a tile height does with key tiles: workgroup slots, and in microseconds a step (one key tile of 64, fp32 32,
+// by the tile's rows, every slot busy), what a job costs beside its steps, and what a split costs: the join's launch, and each
+// part's rows written and joined. Fitted on MI355X (head_dim 128; 64 takes half a step).
+struct Kernel {
+  int64_t slots;
+  double step, job, join, part;
+};
+
+Kernel kernel_of(int32_t tile_rows, int32_t dtype, int32_t head_dim, int64_t n_cus) {
+  const double half = head_dim == 64 ? 0.6 : 1.0;
+  if (dtype == QVL_DTYPE_F32) return {2 * n_cus, 8.5 * half, 2.5, 5.0, 0.03 * half};
+  if (tile_rows == 256) return {n_cus, 1.35 * half, 5.0, 5.0, 0.06 * half};
+  return {(head_dim == 64 ? 3 : 2) * n_cus, 1.95 * half, 3.5, 5.0, 0.03 * half};
+}
+
 // Where the jobs do not fill the slots evenly (few rows over many keys, or a prompt of a few tiles whose last one is the
 // longest), long jobs are split along their keys. Candidates are part lengths of the mean load of a slot and fractions of
-// it; the one of least modelled time is taken, unsplit among them. The model's constants, in steps of one tile of 64
-// (fp32: 32) keys by 128 rows with two workgroups a CU: what a job costs beside its steps, a part's written and joined
-// rows, and the join's launch.
-void split_jobs(std::vector<Job>& jobs, std::vector<Job>& parts, int64_t total, int64_t slots, int32_t dtype) {
-  if (jobs.empty() || (int64_t)jobs.size() > 8 * slots) return;
-  const bool half = dtype == QVL_DTYPE_BF16;
-  const double fixed = half ? 1.5 : 0.3, join = half ? 2.5 : 0.6, each = half ? 0.015 : 0.004;
-  const int32_t least = 4;
+// it; the one of least modelled time is taken, unsplit among them. Returns that time and the part length (0: unsplit).
+double best_split(const std::vector<Job>& jobs, const Kernel& K, int32_t& length) {
+  length = 0;
   std::vector<double> cost;
-  for (const Job& j : jobs) cost.push_back(j.steps + fixed);
-  double best = makespan(cost, slots);
-  int32_t best_len = 0;
-  const double mean = (double)total / slots;
+  int64_t total = 0;
+  for (const Job& j : jobs) {
+    cost.push_back(j.steps * K.step + K.job);
+    total += j.steps;
+  }
+  double best = makespan(cost, K.slots);
+  if ((int64_t)jobs.size() > 8 * K.slots) return best;
+  const double mean = (double)total / K.slots;
   int32_t tried = 0;
   for (double f : {1.0, 0.75, 0.5, 0.334, 0.25, 0.167, 0.125}) {
-    const int32_t length = std::max((int32_t)std::ceil(mean * f), least);
-    if (length == tried) continue;
-    tried = length;
+    const int32_t len = std::max((int32_t)std::ceil(mean * f), 4);
+    if (len == tried) continue;
+    tried = len;
     cost.clear();
     int64_t n_parts = 0;
     for (const Job& j : jobs) {
-      const int32_t p = std::min<int32_t>((j.steps + length - 1) / length, 255);
-      if (p < 2) {
-        cost.push_back(j.steps + fixed);
-        continue;
-      }
-      for (int32_t k = 0; k < p; ++k) cost.push_back((double)j.steps / p + fixed);
-      n_parts += p;
+      const int32_t p = std::max<int32_t>(std::min<int32_t>((j.steps + len - 1) / len, 255), 1);
+      for (int32_t k = 0; k < p; ++k) cost.push_back((double)j.steps / p * K.step + K.job);
+      if (p > 1) n_parts += p;
     }
     if (n_parts == 0) continue;
-    const double t = makespan(cost, slots) + join + each * n_parts;
+    const double t = makespan(cost, K.slots) + K.join + K.part * n_parts;
     if (t < best) {
       best = t;
-      best_len = length;
+      length = len;
     }
   }
-  if (best_len == 0) return;
+  return best;
+}
+
+void split_jobs(std::vector<Job>& jobs, std::vector<Job>& parts, int32_t length) {
+  if (length == 0) return;
   std::vector<Job> whole;
   for (const Job& j : jobs) {
-    const int32_t p = std::min<int32_t>((j.steps + best_len - 1) / best_len, 255);
+    const int32_t p = std::min<int32_t>((j.steps + length - 1) / length, 255);
     if (p < 2) {
       whole.push_back(j);
       continue;
@@ -181,9 +195,9 @@ int qvl_text_rotary_table(int32_t head_dim, double theta, const int32_t* section
 }
 
 int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len, const int64_t* start, int32_t num_heads,
-                        int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus, int32_t* items,
-                        int64_t capacity, int64_t* n_items, int64_t* n_whole) {
-  if (!n_items || !n_whole) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_items / n_whole is NULL");
+                        int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus, int32_t* tile_rows,
+                        int32_t* items, int64_t capacity, int64_t* n_items, int64_t* n_whole) {
+  if (!n_items || !n_whole || !tile_rows) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_items / n_whole / tile_rows is NULL");
   if (n_seqs < 0 || (n_seqs > 0 && (!n_new || !len || !start)))
     return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: sequences are NULL");
   if (dtype != QVL_DTYPE_F32 && dtype != QVL_DTYPE_BF16) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: dtype %d", dtype);
@@ -192,11 +206,12 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
     return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: %d heads over %d key/value heads", num_heads, num_kv_heads);
   if (num_heads > kItemHeadMask) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: num_heads=%d", num_heads);
   if (n_cus <= 0) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_cus=%d", n_cus);
+  if (*tile_rows != 0 && *tile_rows != 128 && *tile_rows != 256) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: tile_rows=%d", *tile_rows);
+  if (*tile_rows == 256 && dtype == QVL_DTYPE_F32) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: tiles of 256 rows are bf16 only");
   const int64_t group = num_heads / num_kv_heads;
   const int64_t step_keys = dtype == QVL_DTYPE_BF16 ? 64 : 32;
-  std::vector<Job> jobs;
   std::vector<int64_t> q_first;
-  int64_t q0 = 0, total = 0;
+  int64_t q0 = 0;
   for (int64_t i = 0; i < n_seqs; ++i) {
     if (n_new[i] < 0 || len[i] < 0 || start[i] < 0 || start[i] > (int64_t)1 << 56)
       return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: sequence %lld: %lld new, %lld keys from row %lld", (long long)i,
@@ -204,17 +219,33 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
     if (len[i] > kItemMaxLen || q0 + n_new[i] > kItemMaxLen || n_new[i] * group > kItemMaxLen)
       return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: sequence %lld is too long", (long long)i);
     q_first.push_back(q0);
-    for (int64_t r = 0; r < n_new[i] * group; r += kItemRows) {
-      const int64_t last = (std::min(r + kItemRows, n_new[i] * group) - 1) / group;
-      const int64_t keys = std::max<int64_t>(std::min(len[i] - n_new[i] + 1 + last, len[i]), 0);
-      const int32_t steps = (int32_t)((keys + step_keys - 1) / step_keys);
-      for (int32_t h = 0; h < num_kv_heads; ++h) jobs.push_back({i, (int32_t)r, h, 0, 0, -1, steps});
-      total += steps * (int64_t)num_kv_heads;
-    }
     q0 += n_new[i];
   }
-  std::vector<Job> parts;
-  split_jobs(jobs, parts, total, (int64_t)n_cus * (head_dim == 64 ? 3 : 2), dtype);
+  // the tile height (where the caller leaves it open) and part length of least modelled time
+  std::vector<Job> jobs, parts;
+  int32_t length = 0, height = 0;
+  double best = 0;
+  for (int32_t rows : {128, 256}) {
+    if (*tile_rows ? rows != *tile_rows : rows == 256 && dtype == QVL_DTYPE_F32) continue;
+    std::vector<Job> mine;
+    for (int64_t i = 0; i < n_seqs; ++i)
+      for (int64_t r = 0; r < n_new[i] * group; r += rows) {
+        const int64_t last = (std::min(r + rows, n_new[i] * group) - 1) / group;
+        const int64_t keys = std::max<int64_t>(std::min(len[i] - n_new[i] + 1 + last, len[i]), 0);
+        const int32_t steps = (int32_t)((keys + step_keys - 1) / step_keys);
+        for (int32_t h = 0; h < num_kv_heads; ++h) mine.push_back({i, (int32_t)r, h, 0, 0, -1, steps});
+      }
+    int32_t l = 0;
+    const double t = best_split(mine, kernel_of(rows, dtype, head_dim, n_cus), l);
+    if (height == 0 || t < best) {
+      best = t;
+      height = rows;
+      length = l;
+      jobs.swap(mine);
+    }
+  }
+  *tile_rows = height;
+  split_jobs(jobs, parts, length);
   std::vector<Job> list = deal(jobs);
   const std::vector<Job> tail = deal(parts);
   *n_whole = (int64_t)list.size();

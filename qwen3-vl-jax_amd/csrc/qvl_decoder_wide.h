@@ -1,0 +1,218 @@
+// Attention tiles of 256 rows (bf16): 64 rows a wave, two sets of 32, so that each K and V fragment read from LDS serves two
+// products and each tile's bytes twice the rows of the 128-row units. One wave a SIMD with all 512 registers: matrix and
+// vector work overlap within the wave, by the order they are issued in.
+//
+// A tile of 64 keys is four units, (set A, keys 0..31), (B, 0..31), (A, 32..63), (B, 32..63), each with its scores' products
+// Q0..Q3, its weights and its products with V, P0..P3, D / 16 instructions a group. They are issued as
+//   Q0  Q1  Q2  P0  Q3  P1  P2  P3
+// and the 16 weights of each lane and unit, pair by pair, among Q1..P2: unit u's are complete when Pu begins, and while
+// they are formed the matrix cores work on another unit. LDS reads stand a group before their use; the next tile's
+// first K fragments are read during P3, from a third stage of the ring, so that no wait for LDS follows the barrier.
+//
+// No running maximum: a row's weights are 2^(s - m) with m the largest score of its first tile, whatever comes later, so that
+// the loop has no branch and no pass over the accumulators. fp32 sums lose nothing by that until they overflow, for which
+// some score has to exceed the first 64 by 2^127 in its weight. Then, and where V holds what is not finite, a row's sums are
+// not finite, and the workgroup runs once more: rows whose sum of weights passed 2^30 with their true maximum, and with
+// values that a row does not see kept from it.
+#pragma once
+#include <utility>
+
+#include "qvl_decoder_core.h"
+
+namespace qvl {
+
+// f(0), f(1), ... with constant arguments.
+template <typename F, int... I> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <int D> struct WideUnit {
+  using W = Wave<bf16, D>;
+  using C = Core<bf16, D>;
+  static constexpr int kRows = 256, kBN = 64, kG = D / 16, kDB = D / 32;
+  static constexpr int kTile = kBN * C::kRowBytes, kDmas = kTile / 1024 / 4, kLds = 3 * 2 * kTile;
+  static_assert(2 * kDmas == kG, "a DMA beside each product of one group");
+
+  static __device__ __forceinline__ float shift_of(const W& w) { return w.m == -INFINITY ? 0.f : -w.m; }
+  static __device__ __forceinline__ bf16x8 k_frag(const char* k, int b, int ks) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+    return *reinterpret_cast<const bf16x8*>(k + (b * 32 + l32) * C::kRowBytes + (((ks * 2 + hh) ^ C::k_swz(l32)) << 4));
+  }
+
+  // A tile that every row sees whole. k0: K's fragments of its first 32 keys; the next tile's on return.
+  template <typename F>
+  static __device__ __forceinline__ void tile(W& A, W& B, const char* k, const char* v, const char* knext, bf16x8 (&k0)[kG], float scale, F&& dma) {
+    f32x16 s[4];
+    u32x4 pw[4][2];
+    bf16x8 k1[kG], v0[2 * kDB], v1[2 * kDB];
+    const float sa = shift_of(A), sb = shift_of(B);
+    auto weights = [&](int p) {                 // pair p & 7 of unit p >> 3
+      const int u = p >> 3, i = p & 7;
+      const float sh = u & 1 ? sb : sa;
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * i], scale, sh));
+      const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * i + 1], scale, sh));
+      const uint32_t x = pack_bf16x2(a, c);
+      pw[u][i >> 2][i & 3] = x;
+      if (u & 1) B.core.add_pair(x);
+      else A.core.add_pair(x);
+    };
+    auto product = [&](W& w, int u, const bf16x8 (&vf)[2 * kDB], int i) {
+      const int e = i / kDB, db = i % kDB;
+      w.core.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i], __builtin_bit_cast(bf16x8, pw[u][e]), w.core.o[db], 0, 0, 0);
+    };
+    auto score = [&](W& w, int u, const bf16x8& kf, int i) {
+      s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, w.core.q[i], i ? s[u] : f32x16{}, 0, 0, 0);
+    };
+    each_of(std::make_integer_sequence<int, 8 * kG>{}, [&](auto at) {
+      constexpr int slot = decltype(at)::value, g = slot / kG, i = slot % kG;
+      if constexpr (g == 0) {
+        dma(i);
+        score(A, 0, k0[i], i);
+      } else if constexpr (g == 1) {
+        k1[i] = k_frag(k, 1, i);
+        score(B, 1, k0[i], i);
+      } else if constexpr (g == 2) {
+        v0[i] = A.core.v_frag(v, i % kDB, i / kDB);
+        score(A, 2, k1[i], i);
+      } else if constexpr (g == 3) {
+        product(A, 0, v0, i);
+      } else if constexpr (g == 4) {
+        score(B, 3, k1[i], i);
+      } else if constexpr (g == 5) {
+        v1[i] = A.core.v_frag(v, i % kDB, 2 + i / kDB);
+        product(B, 1, v0, i);
+      } else if constexpr (g == 6) {
+        product(A, 2, v1, i);
+      } else {
+        k0[i] = k_frag(knext, 0, i);
+        product(B, 3, v1, i);
+      }
+      // the pairs p whose turn it is: slots kG on, 32 of them over six groups
+      constexpr int in = slot - kG, first = in < 0 ? 0 : (in * 32 + 6 * kG - 1) / (6 * kG), last = in < 0 ? 0 : ((in + 1) * 32 + 6 * kG - 1) / (6 * kG);
+      each_of(std::make_integer_sequence<int, (last < 32 ? last : 32) - (first < 32 ? first : 32)>{}, [&](auto p) { weights(first + decltype(p)::value); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+  // 32 keys of a tile for one set of rows, of which some may not see them all.
+  template <bool SAFE>
+  static __device__ __forceinline__ void block(W& w, const char* k, const char* v, int b, int kb, float scale) {
+    if (kb >= w.lim_hi) return;
+    f32x16 s = w.core.scores(k, b);
+    const uint32_t seen = w.mask(s, kb);
+    const float shift = shift_of(w);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, shift));
+    if (SAFE && kb + 32 > w.lim_lo) w.core.pv_safe(v, b, s, seen);
+    else w.core.pv(v, b, s);
+  }
+  // The largest score of a tile, into m where it is larger.
+  static __device__ __forceinline__ void raise(W& w, const char* k, int kb, float scale) {
+    for (int b = 0; b < 2; ++b) {
+      if (kb + 32 * b >= w.lim_hi) return;
+      f32x16 s = w.core.scores(k, b);
+      w.mask(s, kb + 32 * b);
+      float mx = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      w.m = fmaxf(w.m, across_halves(mx) * scale);
+    }
+  }
+
+  struct Tiles {
+    Loader<bf16, D, false> lk;
+    Loader<bf16, D, true> lv;
+    const AttnParams& P;
+    const Unit& u;
+    uint32_t lds;
+    int wave, t1;
+    __device__ __forceinline__ Tiles(const AttnParams& P, const Unit& u, const char* smem, int t1)
+        : lk(P.k), lv(P.v), P(P), u(u), lds(lds_addr_of(smem)), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), t1(t1) {}
+    __device__ __forceinline__ void aim(int t) {
+      const int left = t < t1 ? u.len - t * kBN : 0;
+      lk.at(u.k + (int64_t)(t * kBN) * P.k.row, left);
+      lv.at(u.v + (int64_t)(t * kBN) * P.v.row, left);
+    }
+    // DMA i < 2 kDmas of this wave's share of the tile aimed at
+    __device__ __forceinline__ void load(int i, int stage) const {
+      if (i < kDmas) lk(wave * kDmas + i, lds + stage * 2 * kTile);
+      else lv(wave * kDmas + i - kDmas, lds + stage * 2 * kTile + kTile);
+    }
+    __device__ __forceinline__ void load_all(int t, int stage) {
+      aim(t);
+#pragma unroll
+      for (int i = 0; i < 2 * kDmas; ++i) load(i, stage);
+    }
+  };
+
+  // Tiles [t0, t1) of the unit: tile t in stage (t - t0) % 3, two tiles ahead.
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, W& A, W& B, char* smem, int t0, int t1) {
+    if (t0 >= t1) return;
+    Tiles T(P, u, smem, t1);
+    T.load_all(t0, 0);
+    T.load_all(t0 + 1, 1);
+    A.core.pin();
+    B.core.pin();
+    wait_dma();
+    __syncthreads();
+    raise(A, smem, t0 * kBN, P.scale);
+    raise(B, smem, t0 * kBN, P.scale);
+    const int whole = min(A.lim_lo, B.lim_lo) / kBN, some = max(A.lim_hi, B.lim_hi);
+    bf16x8 k0[kG];
+#pragma unroll
+    for (int i = 0; i < kG; ++i) k0[i] = k_frag(smem, 0, i);
+    // Two loops, so that the accumulators stay where they are in the first; a wave may pass a barrier of one while another
+    // does of the other.
+    int st = 0, t = t0;
+    const auto next = [&] {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      st = st == 2 ? 0 : st + 1;
+    };
+    const auto after = [](int s, int n) { return s + n >= 3 ? s + n - 3 : s + n; };
+    for (; t < min(whole, t1); ++t) {
+      const char* k = smem + st * 2 * kTile;
+      T.aim(t + 2);
+      tile(A, B, k, k + kTile, smem + after(st, 1) * 2 * kTile, k0, P.scale, [&](int i) { T.load(i, after(st, 2)); });
+      next();
+    }
+    for (; t < t1; ++t) {
+      const char* k = smem + st * 2 * kTile;
+      T.load_all(t + 2, after(st, 2));
+      if (t * kBN < some)
+        for (int b = 0; b < 2; ++b) {
+          block<false>(A, k, k + kTile, b, t * kBN + 32 * b, P.scale);
+          block<false>(B, k, k + kTile, b, t * kBN + 32 * b, P.scale);
+        }
+      next();
+    }
+  }
+  // Once more, a tile at a time, after a run that left sums that are not finite.
+  static __device__ __forceinline__ void run_safe(const AttnParams& P, const Unit& u, W& A, W& B, char* smem, int t0, int t1) {
+    Tiles T(P, u, smem, t1);
+    const float la = A.core.row_sum(), lb = B.core.row_sum();
+    const float ma = A.m, mb = B.m;
+    A.core.clear();
+    B.core.clear();
+    for (int t = t0; t < t1; ++t) {
+      T.load_all(t, 0);
+      wait_dma();
+      __syncthreads();
+      raise(A, smem, t * kBN, P.scale);
+      raise(B, smem, t * kBN, P.scale);
+      __syncthreads();
+    }
+    if (la < 0x1p30f) A.m = ma;
+    if (lb < 0x1p30f) B.m = mb;
+    for (int t = t0; t < t1; ++t) {
+      T.load_all(t, 0);
+      wait_dma();
+      __syncthreads();
+      for (int b = 0; b < 2; ++b) {
+        block<true>(A, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
+        block<true>(B, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
+      }
+      __syncthreads();
+    }
+  }
+};
+
+}  // namespace qvl

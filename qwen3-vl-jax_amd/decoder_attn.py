@@ -201,11 +201,11 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
 class CausalPlan:
     """The work list of `causal_attention` for one packed prefill: sequence i brings q_lens[i] new tokens and has k_lens[i]
     keys (default q_lens), the new ones among them, in cache rows from k_starts[i] (default: one sequence after the other).
-    Made on the host once and used by every layer."""
+    Made on the host once and used by every layer. tile_rows: 0, or the kernel's tile height (128, or 256 in bfloat16)."""
 
     def __init__(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None,
                  k_starts: Optional[Sequence[int]] = None, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype,
-                 device="cuda"):
+                 device="cuda", tile_rows: int = 0):
         torch = _torch()
         device = _device(device)
         new = np.ascontiguousarray(q_lens, np.int64).reshape(-1)
@@ -221,19 +221,19 @@ class CausalPlan:
         lib = capi.load()
         n_cus = torch.cuda.get_device_properties(device).multi_processor_count
         p64 = lambda a: a.ctypes.data_as(C.POINTER(C.c_int64))
-        n, whole = C.c_int64(), C.c_int64()
+        n, whole, rows = C.c_int64(), C.c_int64(), C.c_int32(int(tile_rows))
 
         def build(items, capacity):
             capi.check(lib.qvl_causal_worklist(len(new), p64(new), p64(keys), p64(first), self.num_heads, self.num_kv_heads,
-                                               self.head_dim, _qdtype(dtype), n_cus, items, capacity, C.byref(n),
+                                               self.head_dim, _qdtype(dtype), n_cus, C.byref(rows), items, capacity, C.byref(n),
                                                C.byref(whole)), "qvl_causal_worklist")
 
         build(None, 0)
         items = np.zeros((max(n.value, 1), 8), np.int32)
         build(items.ctypes.data_as(C.POINTER(C.c_int32)), n.value)
-        self.n_items, self.n_whole = n.value, whole.value
+        self.n_items, self.n_whole, self.tile_rows = n.value, whole.value, rows.value
         nb = C.c_size_t()
-        capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.n_items, self.n_whole, C.byref(nb)),
+        capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.tile_rows, self.n_items, self.n_whole, C.byref(nb)),
                    "qvl_causal_workspace_size")
         self.workspace_bytes = nb.value
         self.items = torch.from_numpy(items).to(device)
@@ -277,8 +277,8 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
     ws = _workspace(plan.workspace_bytes, q)
     with _On(like[1]) as st:
         capi.check(capi.load().qvl_causal_attention(
-            st, _qdtype(like[0]), *views, rows, plan.items.data_ptr(), plan.n_items, plan.n_whole, _scale(scale, D), *ov, N,
-            Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
+            st, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_whole,
+            _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
     return out
 
 

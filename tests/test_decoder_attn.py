@@ -46,28 +46,34 @@ def test_rotary_table_refusals(pkg):
     assert f(64, 1e4, sec(32, 0, 0), 0, None) == -1
 
 
-def worklist(pkg, new, length, start, hq, hkv, hd=128, dtype=1, n_cus=256):
+def worklist(pkg, new, length, start, hq, hkv, hd=128, dtype=1, n_cus=256, tile_rows=0):
     lib = pkg.capi.load()
     a = [np.array(v, np.int64) for v in (new, length, start)]
     p = [v.ctypes.data_as(C.POINTER(C.c_int64)) for v in a]
-    n, w = C.c_int64(), C.c_int64()
-    pkg.capi.check(lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, None, 0, C.byref(n), C.byref(w)))
+    n, w, rows = C.c_int64(), C.c_int64(), C.c_int32(tile_rows)
+    call = lambda items, cap: lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, C.byref(rows), items, cap, C.byref(n),
+                                                      C.byref(w))
+    pkg.capi.check(call(None, 0))
     items = np.zeros((n.value, 8), np.int32)
     ptr = items.ctypes.data_as(C.POINTER(C.c_int32))
-    pkg.capi.check(lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, ptr, n.value, C.byref(n), C.byref(w)))
+    pkg.capi.check(call(ptr, n.value))
     if n.value > 0:
-        assert lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, ptr, n.value - 1, C.byref(n), C.byref(w)) == -1
-    return items, w.value
+        assert call(ptr, n.value - 1) == -1
+    return items, w.value, rows.value
 
 
+@pytest.mark.parametrize("tile_rows", [0, 128, 256])
 @pytest.mark.parametrize("new,old,hq,hkv,hd,dtype", [
     ([1], [0], 16, 8, 128, 1), ([300, 0, 1, 129], [0, 5, 77, 4000], 16, 8, 128, 1), ([2048], [0], 32, 8, 128, 1),
     ([40], [24000], 32, 8, 128, 1), ([1181, 317, 5], [0, 64, 0], 14, 2, 64, 0), ([7] * 40, [0] * 40, 4, 1, 64, 1),
     ([513], [1000], 6, 2, 128, 0)])
-def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtype):
+def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtype, tile_rows):
+    if tile_rows == 256 and dtype == 0:
+        pytest.skip("bf16 only")
     length = [a + b for a, b in zip(new, old)]
     start = [(1 << 33) + 17 * i for i in range(len(new))]
-    items, n_whole = worklist(pkg, new, length, start, hq, hkv, hd, dtype)
+    items, n_whole, height = worklist(pkg, new, length, start, hq, hkv, hd, dtype, tile_rows=tile_rows)
+    assert height in ((128, 256) if dtype == 1 else (128,)) and tile_rows in (0, height)
     group = hq // hkv
     q0 = np.concatenate([[0], np.cumsum(new)])
     seen = {}
@@ -82,9 +88,9 @@ def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtyp
         assert (parts >= 2 and part < parts and k >= n_whole) if parts else k < n_whole
         if parts:
             slots.append(slot)
-        assert row0 % 128 == 0 and 0 <= row0 < n_new * group
+        assert row0 % height == 0 and 0 <= row0 < n_new * group
         seen.setdefault((i, row0, head & 0xfff), []).append((part, max(parts, 1)))
-    want = {(i, r, h) for i in range(len(new)) for r in range(0, new[i] * group, 128) for h in range(hkv)}
+    want = {(i, r, h) for i in range(len(new)) for r in range(0, new[i] * group, height) for h in range(hkv)}
     assert set(seen) == want
     for got in seen.values():
         assert sorted(p for p, _ in got) == list(range(got[0][1])) and len({n for _, n in got}) == 1
@@ -93,22 +99,24 @@ def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtyp
 
 def test_worklist_refusals(pkg):
     f = pkg.capi.load().qvl_causal_worklist
-    n, w = C.c_int64(), C.c_int64()
+    n, w, rows = C.c_int64(), C.c_int64(), C.c_int32()
     one = lambda v: (C.c_int64 * 1)(v)
-    ok = dict(new=4, length=9, start=0, hq=8, hkv=2, hd=128, dt=1, cus=256)
+    ok = dict(new=4, length=9, start=0, hq=8, hkv=2, hd=128, dt=1, cus=256, rows=0)
 
     def rc(**k):
         a = dict(ok, **k)
-        return f(1, one(a["new"]), one(a["length"]), one(a["start"]), a["hq"], a["hkv"], a["hd"], a["dt"], a["cus"], None, 0,
-                 C.byref(n), C.byref(w))
+        return f(1, one(a["new"]), one(a["length"]), one(a["start"]), a["hq"], a["hkv"], a["hd"], a["dt"], a["cus"],
+                 C.byref(C.c_int32(a["rows"])), None, 0, C.byref(n), C.byref(w))
 
     assert rc() == 0
-    for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57)):
+    for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57), dict(rows=64)):
         assert rc(**bad) == -1, bad
-    for bad in (dict(hd=96), dict(dt=2), dict(hq=8192, hkv=8192), dict(length=1 << 30), dict(new=1 << 29)):
+    for bad in (dict(hd=96), dict(dt=2), dict(hq=8192, hkv=8192), dict(length=1 << 30), dict(new=1 << 29),
+                dict(rows=256, dt=0)):
         assert rc(**bad) == -2, bad
-    assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, None, 0, C.byref(n), C.byref(w)) == -1
-    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, None, 0, None, C.byref(w)) == -1
+    assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), C.byref(w)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, None, C.byref(w)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, None, None, 0, C.byref(n), C.byref(w)) == -1
 
 
 def rotary_args(**change):
@@ -157,17 +165,18 @@ ATTN_BAD = [(-2, dict(dtype=3)), (-2, dict(hd=80)), (-1, dict(hq=12)), (-1, dict
 def test_causal_attention_refusals(pkg):
     f = pkg.capi.load().qvl_causal_attention
 
-    def rc(items=FAKE, n_items=3, n_whole=3, **k):
-        return f(*attn_common(**k), items, n_items, n_whole, *attn_tail(**k))
+    def rc(items=FAKE, n_items=3, n_whole=3, rows=128, **k):
+        return f(*attn_common(**k), rows, items, n_items, n_whole, *attn_tail(**k))
 
     for want, bad in ATTN_BAD + [(-1, dict(items=None)), (-3, dict(items=FAKE + 4)), (-1, dict(n_whole=4)), (-1, dict(n_whole=-1)),
-                                 (-1, dict(n_items=1 << 31))]:
+                                 (-1, dict(n_items=1 << 31)), (-1, dict(rows=64)), (-2, dict(rows=256, dtype=0))]:
         assert rc(**bad) == want, bad
     assert rc(n=0, q=None) == 0 and rc(items=None, n_items=0, n_whole=0) == 0
     nb = C.c_size_t()
     size = pkg.capi.load().qvl_causal_workspace_size
-    assert size(128, 4, 4, C.byref(nb)) == 0 and nb.value == 0
-    assert size(96, 4, 4, C.byref(nb)) == -2 and size(128, 3, 4, C.byref(nb)) == -1 and size(128, 4, 4, None) == -1
+    assert size(128, 128, 4, 4, C.byref(nb)) == 0 and nb.value == 0
+    assert size(96, 128, 4, 4, C.byref(nb)) == -2 and size(128, 128, 3, 4, C.byref(nb)) == -1
+    assert size(128, 128, 4, 4, None) == -1 and size(128, 64, 4, 4, C.byref(nb)) == -1
 
 
 def test_decode_attention_refusals(pkg):

@@ -202,9 +202,13 @@ def causal_case(hq, hkv, D, dtype, new, old, seed=0, kv=None):
     return q, k, v, seqs
 
 
-def plan_of(ops, seqs, hq, hkv, D, dtype):
+def plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows=0):
     return ops.CausalPlan([s[1] for s in seqs], [s[3] for s in seqs], [s[2] for s in seqs], num_heads=hq, num_kv_heads=hkv,
-                          head_dim=D, dtype=dtype, device=DEV)
+                          head_dim=D, dtype=dtype, device=DEV, tile_rows=tile_rows)
+
+
+# both tile heights of bf16, and fp32's
+KERNELS = [(BF, 128), (BF, 256), (F32, 128)]
 
 
 def check_causal(out, q, k, v, seqs, scale):
@@ -221,35 +225,35 @@ CAUSAL = [  # new tokens, keys before them (negative: fewer keys than new tokens
     ([300], [-40]), ([5], [-5]), ([257, 31], [129, 2049]), ([700], [0])]
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dtype,tile_rows", KERNELS)
 @pytest.mark.parametrize("hq,hkv,D", [(16, 8, 128), (32, 8, 128), (14, 2, 64), (4, 4, 64), (6, 2, 128), (5, 1, 128)])
 @pytest.mark.parametrize("new,old", CAUSAL)
-def test_causal(ops, dtype, hq, hkv, D, new, old):
+def test_causal(ops, dtype, tile_rows, hq, hkv, D, new, old):
     q, k, v, seqs = causal_case(hq, hkv, D, dtype, new, old, seed=sum(new) + hq)
-    plan = plan_of(ops, seqs, hq, hkv, D, dtype)
+    plan = plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows)
     out = torch.full_like(q, 7.0)
     assert ops.causal_attention(q, k, v, plan, out=out) is out
     check_causal(out, q, k, v, seqs, D ** -0.5)
     assert (out[sum(new):] == 7.0).all()            # rows behind the last sequence
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
-def test_causal_long_and_peaked(ops, dtype):
+@pytest.mark.parametrize("dtype,tile_rows", KERNELS)
+def test_causal_long_and_peaked(ops, dtype, tile_rows):
     """Scores whose maximum moves up along the keys, by far more than one power of two a tile, and a scale of its own."""
     hq, hkv, D = 4, 2, 128
     q, k, v, seqs = causal_case(hq, hkv, D, dtype, [900], [1500], seed=5)
     k = (k.float() * torch.linspace(0.1, 3.0, k.shape[0], device=DEV)[:, None, None]).to(dtype)
-    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype), scale=0.2)
+    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows), scale=0.2)
     check_causal(out, q, k, v, seqs, 0.2)
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
-def test_causal_large_scores(ops, dtype):
+@pytest.mark.parametrize("dtype,tile_rows", KERNELS)
+def test_causal_large_scores(ops, dtype, tile_rows):
     """Scores of hundreds, of both signs: the weights under- and overflow without the running maximum."""
     hq, hkv, D = 4, 2, 64
     q, k, v, seqs = causal_case(hq, hkv, D, dtype, [200], [77], seed=6)
     q = (q.float() * 40).to(dtype)
-    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype))
+    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows))
     for q0, n, row, length in seqs:
         visible = torch.arange(n, device=DEV) + length - n + 1
         want, A, ds = attention_ref(q[q0:q0 + n], k[row:row + length], v[row:row + length], visible, D ** -0.5)
@@ -261,9 +265,9 @@ def test_causal_large_scores(ops, dtype):
         assert ((out[q0:q0 + n].double() - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dtype,tile_rows", KERNELS)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_causal_masked_keys_hold_anything(ops, dtype, bad):
+def test_causal_masked_keys_hold_anything(ops, dtype, tile_rows, bad):
     """Rows of the caches outside the sequences, and a token's later keys, hold NaN or infinities; the tokens that do
     see a bad key may be anything, the others are exact."""
     hq, hkv, D, n, old = 8, 2, 128, 150, 70
@@ -276,19 +280,19 @@ def test_causal_masked_keys_hold_anything(ops, dtype, bad):
     at = seqs[0][2] + old + 100                     # key of new token 100 of the first sequence
     k[at], v[at + 1] = bad, bad                     # and the value of token 101
     v[at + 20, :, ::3] = bad
-    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype))
-    plan = plan_of(ops, seqs, hq, hkv, D, dtype)
+    out = ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows))
+    plan = plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows)
     want = ops.causal_attention(q, clean_k, clean_v, plan)
     assert torch.equal(bits(out[:100]), bits(want[:100])) and torch.equal(bits(out[n:n + 64]), bits(want[n:n + 64]))
     # token 101's value is seen by tokens 101 on, in every dim
     assert not out[101:n].isfinite().all(-1).any()
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
-def test_causal_strided_views(ops, dtype):
+@pytest.mark.parametrize("dtype,tile_rows", KERNELS)
+def test_causal_strided_views(ops, dtype, tile_rows):
     hq, hkv, D = 12, 4, 64
     q, k, v, seqs = causal_case(hq, hkv, D, dtype, [90, 45], [30, 0], seed=9)
-    plan = plan_of(ops, seqs, hq, hkv, D, dtype)
+    plan = plan_of(ops, seqs, hq, hkv, D, dtype, tile_rows)
     want = ops.causal_attention(q, k, v, plan)
     headmajor = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
     padded = lambda t: torch.cat([t, t, t], 2)[..., D:2 * D]
