@@ -44,7 +44,8 @@ __device__ __forceinline__ float across_halves(float x) {
 //
 // bf16: v_mfma_f32_32x32x16. K and V lie in LDS row by row as they come from memory. A lane's 8 keys of a 16-key group
 // are two runs of 4, so V^T is read by two transposing reads of 4 keys (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16
-// values, and each gets a column). The row sums add the rounded weights that multiply V, two to an instruction.
+// values, and each gets a column). The row sums are plain fp32 additions of the weights before their rounding: a dot
+// instruction that adds two rounded ones waits for the matrix cores (52 cycles beside a product of 32).
 // 16-byte chunks are XOR-swizzled by the row so that neither read meets a bank twice: 16 rows of one chunk for K, 4 rows
 // of 64 bytes for V.
 template <typename T, int D> struct Core;
@@ -106,20 +107,15 @@ template <int D> struct Core<bf16, D> {
     for (int e = 0; e < 2; ++e) {
       u32x4 pw;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pw[j] = pack_bf16x2(p[8 * e + 2 * j], p[8 * e + 2 * j + 1]);
-      add_weights(pw);
+      for (int j = 0; j < 4; ++j) {
+        pw[j] = pack_bf16x2(p[8 * e + 2 * j], p[8 * e + 2 * j + 1]);
+        l += p[8 * e + 2 * j];
+        l += p[8 * e + 2 * j + 1];
+      }
       const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
 #pragma unroll
       for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(lds, db, 2 * b + e), pf, o[db], 0, 0, 0);
     }
-  }
-  __device__ __forceinline__ void add_pair(uint32_t w) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);
-  }
-  __device__ __forceinline__ void add_weights(const u32x4& pw) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) add_pair(pw[j]);   // by value: __builtin_bit_cast of a vector's element takes element 0 here
   }
   // The scores of both blocks of a tile of 64 keys: a block's fragments are read ahead of its products.
   // `beside(i)`, i < 8, runs among the products.
@@ -150,13 +146,17 @@ template <int D> struct Core<bf16, D> {
 #pragma unroll
     for (int db = 0; db < kDB; ++db) v[db] = v_frag(lds, db, g);
   }
-  static __device__ __forceinline__ u32x4 pack8(const f32x16& s, int e, float scale, float shift) {
+  __device__ __forceinline__ u32x4 pack8(const f32x16& s, int e, float scale, float shift) {
     float p[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * e + r], scale, shift));
     u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) {
+      w[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
+      l += p[2 * j];
+      l += p[2 * j + 1];
+    }
     return w;
   }
   // Weights and their product with V, 16 keys at a time: a group's weights are formed and its V read beside the products of
@@ -170,7 +170,6 @@ template <int D> struct Core<bf16, D> {
       bf16x8 (&now)[kDB] = g & 1 ? v1 : v0;
       bf16x8 (&next)[kDB] = g & 1 ? v0 : v1;
       if (g < 3) v_group(lds, g + 1, next);
-      add_weights(pw);
       const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
 #pragma unroll
       for (int db = 0; db < kDB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now[db], pf, o[db], 0, 0, 0);
@@ -196,9 +195,10 @@ template <int D> struct Core<bf16, D> {
       for (int j = 0; j < 4; ++j) {
         const int r = 8 * e + 2 * j;
         pw[j] = pack_bf16x2(p[r], p[r + 1]);
+        l += p[r];
+        l += p[r + 1];
         sw[j] = ((seen >> r) & 1 ? 0x3f80u : 0u) | ((seen >> (r + 1)) & 1 ? 0x3f800000u : 0u);
       }
-      add_weights(pw);
       const bf16x8 pf = __builtin_bit_cast(bf16x8, pw), sf = __builtin_bit_cast(bf16x8, sw);
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {

@@ -53,8 +53,9 @@ template <int D> struct WideUnit {
       const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * i + 1], scale, sh));
       const uint32_t x = pack_bf16x2(a, c);
       pw[u][i >> 2][i & 3] = x;
-      if (u & 1) B.core.add_pair(x);
-      else A.core.add_pair(x);
+      float& l = u & 1 ? B.core.l : A.core.l;
+      l += a;
+      l += c;
     };
     auto product = [&](W& w, int u, const bf16x8 (&vf)[2 * kDB], int i) {
       const int e = i / kDB, db = i % kDB;
