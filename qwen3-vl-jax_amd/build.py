@@ -37,9 +37,9 @@ def common_flags() -> list:
 # MI355X it took fc1 / qkv 1.5-2 % and the config-2 / 3 / 4 forwards 0.5-0.8 % below the default
 # scheduler's (same-call A/B, no spills either way).
 # The 256-row attention tiles keep every product's result in vector registers and the operands in the accumulation ones; the
-# compiler's own choice copies the accumulators through each other in the loop.
+# compiler's own choices copy accumulators through each other in the loop (up to 250 moves a tile) or spill.
 FILE_FLAGS = {"qvl_gemm.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
-              "qvl_causal_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+              "qvl_causal_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-greedy-reverse-local-assignment=1"]}
 
 
 def build(verbose: bool = False, jobs: int = 8) -> Path:

@@ -5,9 +5,11 @@
 // A tile of 64 keys is four units, (set A, keys 0..31), (B, 0..31), (A, 32..63), (B, 32..63), each with its scores' products
 // Q0..Q3, its weights and its products with V, P0..P3, D / 16 instructions a group. They are issued as
 //   Q0  Q1  Q2  P0  Q3  P1  P2  P3
-// and the 16 weights of each lane and unit, pair by pair, among Q1..P2: unit u's are complete when Pu begins, and while
+// and the 16 weights of each lane and unit, one by one, among Q1..P2: unit u's are complete when Pu begins, and while
 // they are formed the matrix cores work on another unit. LDS reads stand a group before their use; the next tile's
-// first K fragments are read during P3, from a third stage of the ring, so that no wait for LDS follows the barrier.
+// first K fragments are read during P3, from a third stage of the ring, so that no wait for LDS follows the barrier. The
+// tile's DMAs stand apart, four products between two (one takes the CU's address unit long enough to hold the wave), and in
+// the tile's first half, so that they are there when it ends.
 //
 // No running maximum: a row's weights are 2^(s - m) with m the largest score of its first tile, whatever comes later, so that
 // the loop has no branch and no pass over the accumulators. fp32 sums lose nothing by that until they overflow, for which
@@ -46,16 +48,13 @@ template <int D> struct WideUnit {
     u32x4 pw[4][2];
     bf16x8 k1[kG], v0[2 * kDB], v1[2 * kDB];
     const float sa = shift_of(A), sb = shift_of(B);
-    auto weights = [&](int p) {                 // pair p & 7 of unit p >> 3
-      const int u = p >> 3, i = p & 7;
-      const float sh = u & 1 ? sb : sa;
-      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * i], scale, sh));
-      const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * i + 1], scale, sh));
-      const uint32_t x = pack_bf16x2(a, c);
-      pw[u][i >> 2][i & 3] = x;
-      float& l = u & 1 ? B.core.l : A.core.l;
-      l += a;
-      l += c;
+    float even;
+    auto weight = [&](int p) {                  // score p & 15 of unit p >> 4; packed by twos
+      const int u = p >> 4, i = p & 15;
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale, u & 1 ? sb : sa));
+      (u & 1 ? B.core.l : A.core.l) += a;
+      if (i & 1) pw[u][i >> 3][(i >> 1) & 3] = pack_bf16x2(even, a);
+      else even = a;
     };
     auto product = [&](W& w, int u, const bf16x8 (&vf)[2 * kDB], int i) {
       const int e = i / kDB, db = i % kDB;
@@ -67,7 +66,6 @@ template <int D> struct WideUnit {
     each_of(std::make_integer_sequence<int, 8 * kG>{}, [&](auto at) {
       constexpr int slot = decltype(at)::value, g = slot / kG, i = slot % kG;
       if constexpr (g == 0) {
-        dma(i);
         score(A, 0, k0[i], i);
       } else if constexpr (g == 1) {
         k1[i] = k_frag(k, 1, i);
@@ -88,9 +86,10 @@ template <int D> struct WideUnit {
         k0[i] = k_frag(knext, 0, i);
         product(B, 3, v1, i);
       }
-      // the pairs p whose turn it is: slots kG on, 32 of them over six groups
-      constexpr int in = slot - kG, first = in < 0 ? 0 : (in * 32 + 6 * kG - 1) / (6 * kG), last = in < 0 ? 0 : ((in + 1) * 32 + 6 * kG - 1) / (6 * kG);
-      each_of(std::make_integer_sequence<int, (last < 32 ? last : 32) - (first < 32 ? first : 32)>{}, [&](auto p) { weights(first + decltype(p)::value); });
+      if constexpr (slot % 4 == 1 && slot / 4 < kG) dma(slot / 4);
+      // the weights whose turn it is: 64 over the six groups from slot kG on
+      constexpr int in = slot - kG, first = in < 0 ? 0 : (in * 64 + 6 * kG - 1) / (6 * kG), last = in < 0 ? 0 : ((in + 1) * 64 + 6 * kG - 1) / (6 * kG);
+      each_of(std::make_integer_sequence<int, (last < 64 ? last : 64) - (first < 64 ? first : 64)>{}, [&](auto p) { weight(first + decltype(p)::value); });
       __builtin_amdgcn_sched_barrier(0);
     });
   }
