@@ -9,7 +9,7 @@ void launch_causal_wide(void* stream, int32_t head_dim, const AttnParams& P, con
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P, const int32_t* items, int n_whole) {
   using R = RowsUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[R::kLds];
+  __shared__ __attribute__((aligned(16))) char smem[std::max(R::kLds, 4 * kWriteLds)];
   const int32_t* it = items + 8 * (int64_t)blockIdx.x;
   const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4] & kItemHeadMask;
   const int part = (it[4] >> kItemPartShift) & 0xff, parts = (it[4] >> kItemPartsShift) & 0xff, slot = it[5];
@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(AttnParams P, const int3
   }
   const int r = wave * 32 + (threadIdx.x & 31);
   const int64_t at = (int64_t)slot * kItemRows + r;
-  write_rows<T, D>(P, u, w, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * R::kBN);
+  write_rows<T, D>(P, u, w, smem + wave * kWriteLds, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * R::kBN);
 }
 
 // The rows of split tiles: the workgroup of a part joins its share of the tile's 128 rows.

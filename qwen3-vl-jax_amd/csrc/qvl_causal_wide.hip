@@ -15,21 +15,17 @@ __global__ __launch_bounds__(256, 1) void causal_wide_kernel(AttnParams P, const
       start > P.kv_rows - len || row0 >= n_new * P.group || (parts && (part >= parts || slot < 0 || slot >= (int)gridDim.x - n_whole))) return;
   const Unit u{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
                n_new * P.group, row0, kvh};
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int last = min(row0 + U::kRows, u.rows) - 1;
   const int k_hi = max(min(u.lim0 + (int)((uint32_t)last / (uint32_t)P.group), len), 0);
   const int n_t = (k_hi + U::kBN - 1) / U::kBN;
   const int t0 = parts ? (int)((int64_t)n_t * part / parts) : 0, t1 = parts ? (int)((int64_t)n_t * (part + 1) / parts) : n_t;
   Wave<bf16, D> A, B;
-  A.init(P, u, row0 + wave * 64);
-  B.init(P, u, row0 + wave * 64 + 32);
-  U::run(P, u, A, B, smem, t0, t1);
-  const bool ok = A.finite() && B.finite() && A.core.l < INFINITY && B.core.l < INFINITY;
-  if (__builtin_expect(__syncthreads_or(!ok), 0)) U::run_safe(P, u, A, B, smem, t0, t1);
+  U::run_all(P, u, A, B, row0, smem, t0, t1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto write = [&](const Wave<bf16, D>& w, int first) {
     const int r = first + (threadIdx.x & 31);
     const int64_t at = (int64_t)slot * U::kRows + r;
-    write_rows<bf16, D>(P, u, w, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * U::kBN);
+    write_rows<bf16, D>(P, u, w, smem + wave * kWriteLds, row0 + r, parts ? P.part_o + at * D : nullptr, P.part_ml + at, w.lim > t0 * U::kBN);
   };
   write(A, wave * 64);
   write(B, wave * 64 + 32);

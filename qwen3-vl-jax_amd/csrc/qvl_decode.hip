@@ -356,7 +356,7 @@ template <typename T, int D, bool ROWS>
 __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeState& S) {
   using R = RowsUnit<T, D>;
   using K = KeysUnit<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[std::max({K::kLds, kJoinBytes<T, D>, ROWS ? R::kLds : 0})];
+  __shared__ __attribute__((aligned(16))) char smem[std::max({K::kLds, kJoinBytes<T, D>, ROWS ? std::max(R::kLds, 4 * kWriteLds) : 0})];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int prefix_units = P.hkv * S.prefix_parts * S.prefix_tiles * S.n_groups;
   const bool own = (int)blockIdx.x >= prefix_units;
@@ -376,8 +376,11 @@ __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeSta
   const int tokens = uniform(s1 > s0 ? (int)tokens_of(P, S, s0, s1, u.token0) : 0);
   u.rows = tokens * P.group;
   if (u.rows == 0) return;
-  const int64_t start = uniform(own ? S.k_start[who] : S.prefix_start[who]);
   u.token0 = uniform(u.token0);
+  // a sequence of no group has no prefix
+  if (own && p == 0 && (who < S.cu_groups[0] || who >= S.cu_groups[S.n_groups]))
+    for (int i = 0; i < S.prefix_parts; ++i) write_fixed(P, u, i, 0.f);
+  const int64_t start = uniform(own ? S.k_start[who] : S.prefix_start[who]);
   u.len = uniform(own ? S.k_len[who] : S.prefix_len[who]);
   if (bad_keys(P, start, u.len)) {
     write_fixed(P, u, part, NAN);
@@ -399,7 +402,8 @@ __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeSta
       R::run(P, u, w, smem, ka / R::kBN, (kb + R::kBN - 1) / R::kBN);
       const int row = row0 + wave * 32 + (threadIdx.x & 31);
       const int64_t at = part_row(P, u, part, min(row, u.rows - 1));
-      write_rows<T, D>(P, u, w, row, P.part_o + at * D, P.part_ml + at, true);
+      write_rows<T, D>(P, u, w, smem + wave * kWriteLds, row, P.part_o + at * D, P.part_ml + at, true);
+      __syncthreads();                         // the tiles may be written again
     }
   } else {
     const int step = own ? 32 : S.prefix_tiles * 32;

@@ -626,18 +626,51 @@ template <typename T, int D> struct KeysUnit {
 // (m, l) of a part as the combine reads it: no key seen (-inf, 0), only keys of score -inf (-inf, -0).
 __device__ __forceinline__ f32x2 part_state(float m, float l, bool sees) { return f32x2{m, l == 0.f && sees ? -0.f : l}; }
 
-// One wave writes its 32 rows: to the output, or as a part.
+// LDS of one wave that writes 32 rows.
+constexpr int kWriteLds = 32 * (256 + 16);
+
+// A wave's 32 rows of D values E, f(d, x) of the 4 that a lane holds from dim d on, lane by lane to where its row goes (nullptr: nowhere),
+// turned in LDS so that the stores cover whole rows: a lane's own 8 bytes of 32 rows at a time kept the CU's address unit for
+// 7900 cycles a tile of 256 rows, a sixth of a short one's time; so it takes 2500.
+template <typename E, int D, typename W, typename F>
+__device__ __forceinline__ void store_rows(const W& w, char* dst, char* lds, F&& f) {
+  constexpr int kBytes = D * (int)sizeof(E) < 256 ? D * (int)sizeof(E) : 256, kPieces = D * (int)sizeof(E) / kBytes, kDims = D / kPieces;
+  constexpr int kPitch = kBytes + 16, kChunks = kBytes / 16;      // the row's address stands behind its bytes
+  const int lane = threadIdx.x & 63, l32 = lane & 31;
+  char* mine = lds + l32 * kPitch;
+  if (lane < 32) *reinterpret_cast<char**>(mine + kBytes) = dst;
+#pragma unroll
+  for (int piece = 0; piece < kPieces; ++piece) {
+    w.core.each4([&](int d, const f32x4& x) {
+      if (d / kDims == piece) store4<E>(mine, d % kDims, f(x));
+    });
+    __builtin_amdgcn_wave_barrier();
+    char* to[kChunks / 2];
+    u32x4 x[kChunks / 2];
+#pragma unroll
+    for (int i = 0; i < kChunks / 2; ++i) {                       // 64 / kChunks rows each
+      const char* row = lds + (i * (64 / kChunks) + lane / kChunks) * kPitch;
+      to[i] = *reinterpret_cast<char* const*>(row + kBytes);
+      x[i] = *reinterpret_cast<const u32x4*>(row + lane % kChunks * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kChunks / 2; ++i)
+      if (to[i]) *reinterpret_cast<u32x4*>(to[i] + piece * kBytes + lane % kChunks * 16) = x[i];
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// One wave writes its 32 rows, through kWriteLds bytes of LDS that no other wave uses: to the output, or as a part.
 template <typename T, int D>
-__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, int row, float* po, f32x2* pml, bool sees) {
+__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, char* lds, int row, float* po, f32x2* pml, bool sees) {
   const float l = w.core.row_sum();
-  if (row >= u.rows) return;
   if (po) {
-    w.core.each4([&](int d, const f32x4& x) { *reinterpret_cast<f32x4*>(po + d) = x; });
-    if ((threadIdx.x & 63) < 32) *pml = part_state(w.m, l, sees);
+    store_rows<float, D>(w, row < u.rows ? (char*)po : nullptr, lds, [](const f32x4& x) { return x; });
+    if (row < u.rows && (threadIdx.x & 63) < 32) *pml = part_state(w.m, l, sees);
   } else {
     const float inv = 1.0f / l;
-    char* out = out_row<T, D>(P, u, row);
-    w.core.each4([&](int d, const f32x4& x) { store4<T>(out, d, sees ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f}); });
+    store_rows<T, D>(w, row < u.rows ? out_row<T, D>(P, u, row) : nullptr, lds,
+                     [&](const f32x4& x) { return sees ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f}; });
   }
 }
 

@@ -33,6 +33,7 @@ template <int D> struct WideUnit {
   using C = Core<bf16, D>;
   static constexpr int kRows = 256, kBN = 64, kG = D / 16, kDB = D / 32;
   static constexpr int kTile = kBN * C::kRowBytes, kDmas = kTile / 1024 / 4, kLds = 3 * 2 * kTile;
+  static_assert(kLds >= 4 * kWriteLds, "rows are written through the tiles' LDS");
   static_assert(2 * kDmas == kG, "a DMA beside each product of one group");
 
   static __device__ __forceinline__ float shift_of(const W& w) { return w.m == -INFINITY ? 0.f : -w.m; }
@@ -41,17 +42,21 @@ template <int D> struct WideUnit {
     return *reinterpret_cast<const bf16x8*>(k + (b * 32 + l32) * C::kRowBytes + (((ks * 2 + hh) ^ C::k_swz(l32)) << 4));
   }
 
-  // A tile that every row sees whole. k0: K's fragments of its first 32 keys; the next tile's on return.
-  template <typename F>
-  static __device__ __forceinline__ void tile(W& A, W& B, const char* k, const char* v, const char* knext, bf16x8 (&k0)[kG], float scale, F&& dma) {
+  // A tile; EDGE: some row may not see it whole, and its keys start at kb. k0: K's fragments of its first 32 keys; the next
+  // tile's on return.
+  template <bool EDGE, typename F>
+  static __device__ __forceinline__ void tile(W& A, W& B, const char* k, const char* v, const char* knext, bf16x8 (&k0)[kG], int kb, float scale, F&& dma) {
     f32x16 s[4];
     u32x4 pw[4][2];
     bf16x8 k1[kG], v0[2 * kDB], v1[2 * kDB];
     const float sa = shift_of(A), sb = shift_of(B);
+    const int first = kb + 4 * (int)((threadIdx.x & 63) >> 5), la = A.lim - first, lb = B.lim - first;
     float even;
     auto weight = [&](int p) {                  // score p & 15 of unit p >> 4; packed by twos
       const int u = p >> 4, i = p & 15;
-      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale, u & 1 ? sb : sa));
+      float x = s[u][i];
+      if (EDGE) x = 32 * (u >> 1) + 8 * (i >> 2) + (i & 3) < (u & 1 ? lb : la) ? x : -INFINITY;
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, u & 1 ? sb : sa));
       (u & 1 ? B.core.l : A.core.l) += a;
       if (i & 1) pw[u][i >> 3][(i >> 1) & 3] = pack_bf16x2(even, a);
       else even = a;
@@ -93,29 +98,42 @@ template <int D> struct WideUnit {
       __builtin_amdgcn_sched_barrier(0);
     });
   }
-  // 32 keys of a tile for one set of rows, of which some may not see them all.
-  template <bool SAFE>
-  static __device__ __forceinline__ void block(W& w, const char* k, const char* v, int b, int kb, float scale) {
+  // 32 keys of a tile for one set of rows, with values that a row does not see kept from it.
+  static __device__ __forceinline__ void block_safe(W& w, const char* k, const char* v, int b, int kb, float scale) {
     if (kb >= w.lim_hi) return;
     f32x16 s = w.core.scores(k, b);
     const uint32_t seen = w.mask(s, kb);
     const float shift = shift_of(w);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, shift));
-    if (SAFE && kb + 32 > w.lim_lo) w.core.pv_safe(v, b, s, seen);
+    if (kb + 32 > w.lim_lo) w.core.pv_safe(v, b, s, seen);
     else w.core.pv(v, b, s);
   }
-  // The largest score of a tile, into m where it is larger.
-  static __device__ __forceinline__ void raise(W& w, const char* k, int kb, float scale) {
-    for (int b = 0; b < 2; ++b) {
-      if (kb + 32 * b >= w.lim_hi) return;
-      f32x16 s = w.core.scores(k, b);
-      w.mask(s, kb + 32 * b);
-      float mx = s[0];
+  // The largest score of a tile, into m where it is larger. k0: K's fragments of its first 32 keys.
+  static __device__ __forceinline__ void raise(W& A, W& B, const char* k, const bf16x8 (&k0)[kG], int kb, float scale) {
+    f32x16 s[4] = {};                           // four chains of products, so that one hides another's latency
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-      w.m = fmaxf(w.m, across_halves(mx) * scale);
+    for (int i = 0; i < kG; ++i) {
+      const bf16x8 k1 = k_frag(k, 1, i);
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0[i], A.core.q[i], s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0[i], B.core.q[i], s[1], 0, 0, 0);
+      s[2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, A.core.q[i], s[2], 0, 0, 0);
+      s[3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, B.core.q[i], s[3], 0, 0, 0);
     }
+    if (kb + kBN > min(A.lim_lo, B.lim_lo)) {
+      A.mask(s[0], kb);
+      B.mask(s[1], kb);
+      A.mask(s[2], kb + 32);
+      B.mask(s[3], kb + 32);
+    }
+    float ma = fmaxf(s[0][0], s[2][0]), mb = fmaxf(s[1][0], s[3][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) {
+      ma = fmaxf(fmaxf(ma, s[0][r]), s[2][r]);
+      mb = fmaxf(fmaxf(mb, s[1][r]), s[3][r]);
+    }
+    A.m = fmaxf(A.m, across_halves(ma) * scale);
+    B.m = fmaxf(B.m, across_halves(mb) * scale);
   }
 
   struct Tiles {
@@ -144,46 +162,40 @@ template <int D> struct WideUnit {
     }
   };
 
-  // Tiles [t0, t1) of the unit: tile t in stage (t - t0) % 3, two tiles ahead.
-  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, W& A, W& B, char* smem, int t0, int t1) {
-    if (t0 >= t1) return;
+  // Rows [row0, row0 + 256) of the unit over tiles [t0, t1): tile t in stage (t - t0) % 3, two tiles ahead.
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, W& A, W& B, int row0, char* smem, int t0, int t1) {
     Tiles T(P, u, smem, t1);
     T.load_all(t0, 0);
+    A.init(P, u, row0 + T.wave * 64);
+    B.init(P, u, row0 + T.wave * 64 + 32);
     T.load_all(t0 + 1, 1);
     A.core.pin();
     B.core.pin();
     wait_dma();
     __syncthreads();
-    raise(A, smem, t0 * kBN, P.scale);
-    raise(B, smem, t0 * kBN, P.scale);
-    const int whole = min(A.lim_lo, B.lim_lo) / kBN, some = max(A.lim_hi, B.lim_hi);
+    if (t0 >= t1) return;
     bf16x8 k0[kG];
 #pragma unroll
     for (int i = 0; i < kG; ++i) k0[i] = k_frag(smem, 0, i);
-    // Two loops, so that the accumulators stay where they are in the first; a wave may pass a barrier of one while another
-    // does of the other.
+    raise(A, B, smem, k0, t0 * kBN, P.scale);
+    // Two loops, so that the accumulators stay where they are in the first and its weights need no comparisons; a wave may
+    // pass a barrier of one while another does of the other.
+    const int whole = min(A.lim_lo, B.lim_lo) / kBN, some = max(A.lim_hi, B.lim_hi);
     int st = 0, t = t0;
-    const auto next = [&] {
+    const auto after = [&](int n) { return smem + (st + n >= 3 ? st + n - 3 : st + n) * 2 * kTile; };
+    const auto step = [&](auto edge) {
+      const int to = st == 0 ? 2 : st - 1;      // of tile t + 2
+      T.aim(t + 2);
+      if (!decltype(edge)::value || t * kBN < some)
+        tile<decltype(edge)::value>(A, B, after(0), after(0) + kTile, after(1), k0, t * kBN, P.scale, [&](int i) { T.load(i, to); });
+      else
+        for (int i = 0; i < 2 * kDmas; ++i) T.load(i, to);
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
       st = st == 2 ? 0 : st + 1;
+      ++t;
     };
-    const auto after = [](int s, int n) { return s + n >= 3 ? s + n - 3 : s + n; };
-    for (; t < min(whole, t1); ++t) {
-      const char* k = smem + st * 2 * kTile;
-      T.aim(t + 2);
-      tile(A, B, k, k + kTile, smem + after(st, 1) * 2 * kTile, k0, P.scale, [&](int i) { T.load(i, after(st, 2)); });
-      next();
-    }
-    for (; t < t1; ++t) {
-      const char* k = smem + st * 2 * kTile;
-      T.load_all(t + 2, after(st, 2));
-      if (t * kBN < some)
-        for (int b = 0; b < 2; ++b) {
-          block<false>(A, k, k + kTile, b, t * kBN + 32 * b, P.scale);
-          block<false>(B, k, k + kTile, b, t * kBN + 32 * b, P.scale);
-        }
-      next();
-    }
+    while (t < min(whole, t1)) step(std::false_type{});
+    while (t < t1) step(std::true_type{});
   }
   // Once more, a tile at a time, after a run that left sums that are not finite.
   static __device__ __forceinline__ void run_safe(const AttnParams& P, const Unit& u, W& A, W& B, char* smem, int t0, int t1) {
@@ -196,8 +208,10 @@ template <int D> struct WideUnit {
       T.load_all(t, 0);
       wait_dma();
       __syncthreads();
-      raise(A, smem, t * kBN, P.scale);
-      raise(B, smem, t * kBN, P.scale);
+      bf16x8 k0[kG];
+#pragma unroll
+      for (int i = 0; i < kG; ++i) k0[i] = k_frag(smem, 0, i);
+      raise(A, B, smem, k0, t * kBN, P.scale);
       __syncthreads();
     }
     if (la < 0x1p30f) A.m = ma;
@@ -207,11 +221,16 @@ template <int D> struct WideUnit {
       wait_dma();
       __syncthreads();
       for (int b = 0; b < 2; ++b) {
-        block<true>(A, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
-        block<true>(B, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
+        block_safe(A, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
+        block_safe(B, smem, smem + kTile, b, t * kBN + 32 * b, P.scale);
       }
       __syncthreads();
     }
+  }
+  static __device__ __forceinline__ void run_all(const AttnParams& P, const Unit& u, W& A, W& B, int row0, char* smem, int t0, int t1) {
+    run(P, u, A, B, row0, smem, t0, t1);
+    const bool ok = A.finite() && B.finite() && A.core.l < INFINITY && B.core.l < INFINITY;
+    if (__builtin_expect(__syncthreads_or(!ok), 0)) run_safe(P, u, A, B, smem, t0, t1);
   }
 };
 
