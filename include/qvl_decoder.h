@@ -58,26 +58,29 @@ int qvl_qk_norm_rotary(void* stream, int32_t dtype,
 
 /* Work list of qvl_causal_attention (host): sequence i brings h_new[i] query tokens (packed one sequence after the other)
  * and has h_len[i] keys, the new tokens' own among them, in cache rows [h_start[i], h_start[i] + h_len[i]). Query token t
- * sees keys j <= h_len - h_new + t; where h_len < h_new the first tokens see none. Items of 8 int32, dealt to 8 queues
- * (one per XCD) and ordered by work; where they would leave compute units idle, long ones are split along their keys
- * into parts, items [n_whole, n_items). *tile_rows: the rows (token, head) of a tile, 128 or 256 (bf16 only); 0 on entry
- * lets a model of the kernels' times choose, and the choice is written. h_items NULL: only the counts and the tile height
- * are written. */
+ * sees keys j <= h_len - h_new + t; where h_len < h_new the first tokens see none. Items of QVL_CAUSAL_ITEM_WORDS int32,
+ * dealt to 8 queues (one per XCD) and ordered by work; where tiles would leave compute units idle, they are cut along their
+ * keys. The list holds n_items items, n_parts of which are parts of a tile, and after them n_joins entries for the tiles
+ * that are in parts. *tile_rows: the rows (token, head) of a tile, 128 or 256 (bf16 only); 0 on entry lets a model of the
+ * kernels' times choose, and the choice is written. h_items NULL: only the counts and the tile height are written;
+ * capacity: the entries there is room for, n_items + n_joins at least. */
+#define QVL_CAUSAL_ITEM_WORDS 10
 int qvl_causal_worklist(int64_t n_seqs, const int64_t* h_new, const int64_t* h_len, const int64_t* h_start,
                         int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus,
-                        int32_t* tile_rows, int32_t* h_items, int64_t capacity, int64_t* n_items, int64_t* n_whole);
+                        int32_t* tile_rows, int32_t* h_items, int64_t capacity, int64_t* n_items, int64_t* n_parts,
+                        int64_t* n_joins);
 
 /* out = softmax(scale * q k^T, keys the token does not see left out) v, for every token of the sequences of a
  * qvl_causal_worklist list (device copy, 16-byte aligned; made for the same heads, head_dim, dtype and tile_rows). A token that sees
  * no key gets zeros; rows of no sequence are left as they are. Keys a token does not see never enter its output, whatever
  * they hold. An item whose rows leave [0, n_tokens) or [0, kv_rows) is not run. scale: finite, > 0. The workspace
  * (qvl_causal_workspace_size; 16-byte aligned) holds the parts' partial outputs: calls that overlap need one each. */
-int qvl_causal_workspace_size(int32_t head_dim, int32_t tile_rows, int64_t n_items, int64_t n_whole, size_t* bytes);
+int qvl_causal_workspace_size(int32_t head_dim, int32_t tile_rows, int64_t n_parts, size_t* bytes);
 int qvl_causal_attention(void* stream, int32_t dtype,
                          const void* d_q, int64_t q_row_stride, int64_t q_head_stride,
                          const void* d_k, int64_t k_row_stride, int64_t k_head_stride,
                          const void* d_v, int64_t v_row_stride, int64_t v_head_stride, int64_t kv_rows,
-                         int32_t tile_rows, const int32_t* d_items, int64_t n_items, int64_t n_whole, float scale,
+                         int32_t tile_rows, const int32_t* d_items, int64_t n_items, int64_t n_parts, int64_t n_joins, float scale,
                          void* d_out, int64_t out_row_stride, int64_t out_head_stride,
                          int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                          void* d_workspace, size_t workspace_bytes);

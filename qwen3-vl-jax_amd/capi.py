@@ -17,6 +17,7 @@ QVL_EPI_BIAS = 0
 QVL_EPI_BIAS_GELU = 1
 QVL_EPI_BIAS_RESIDUAL = 2
 QVL_FLAGGED_MAX_SEQ = 32768
+QVL_CAUSAL_ITEM_WORDS = 10
 QVL_SCATTER_SET = 0
 QVL_SCATTER_ADD = 1
 
@@ -154,10 +155,10 @@ SIGNATURES = {
     "qvl_qk_norm_rotary": (C.c_int, [_p, _i32, *_view, *_view, *_view, _p, _p, _f32, _p, _i64, _p, _p, _i64, *_view,
                                      *_view, *_view, _i64, _i32, _i32, _i32]),
     "qvl_causal_worklist": (C.c_int, [_i64, _pi64, _pi64, _pi64, _i32, _i32, _i32, _i32, _i32, _pi32, _pi32, _i64, _pi64,
-                                      _pi64]),
-    "qvl_causal_workspace_size": (C.c_int, [_i32, _i32, _i64, _i64, C.POINTER(_sz)]),
-    "qvl_causal_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _i32, _p, _i64, _i64, _f32, *_view, _i64,
-                                       _i32, _i32, _i32, _p, _sz]),
+                                      _pi64, _pi64]),
+    "qvl_causal_workspace_size": (C.c_int, [_i32, _i32, _i64, C.POINTER(_sz)]),
+    "qvl_causal_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _i32, _p, _i64, _i64, _i64, _f32, *_view,
+                                       _i64, _i32, _i32, _i32, _p, _sz]),
     "qvl_decode_workspace_size": (C.c_int, [_i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
     "qvl_decode_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
                                        _i64, _f32, *_view, _i64, _i32, _i32, _i32, _p, _sz]),

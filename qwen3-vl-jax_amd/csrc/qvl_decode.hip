@@ -464,7 +464,7 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
     return set_error(QVL_ERR_INVALID_ARG, "%s: %d heads over %d key/value heads", what, num_heads, num_kv_heads);
   const int64_t rows = n_tokens * (num_heads / num_kv_heads);
-  if (num_heads > kItemHeadMask || n_tokens > kItemMaxLen || rows > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  if (num_heads > kItemMaxHeads || n_tokens > kItemMaxLen || rows > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   // workgroups a GPU holds: two a CU, one where the tiles take 128 KB (fp32, head_dim 128)
   const int64_t slots = (int64_t)gemm_device_cus() * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
   D = DecodePlan{};

@@ -750,6 +750,27 @@ __device__ __forceinline__ void join_parts(const AttnParams& P, int row0, int ro
   }
 }
 
+// The item of a work list (qvl_decoder_items.h) that this workgroup computes; false if it is none or leaves its bounds.
+struct Item {
+  Unit u;
+  int slot, t0, t1;   // slot < 0: whole
+};
+__device__ __forceinline__ bool item_of(const AttnParams& P, const int32_t* items, int n_parts, int rows, int keys, Item& x) {
+  const int32_t* it = items + kItemWords * (int64_t)blockIdx.x;
+  const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4], slot = it[5];
+  const int64_t start = (int64_t)(((uint64_t)(uint32_t)it[7] << 32) | (uint32_t)it[6]);
+  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 || len > kItemMaxLen || start < 0 ||
+      start > P.kv_rows - len || row0 >= n_new * P.group || slot >= n_parts) return false;
+  x.u = Unit{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
+             n_new * P.group, row0, kvh};
+  x.slot = slot;
+  const int last = min(row0 + rows, x.u.rows) - 1;
+  const int k_hi = max(min(x.u.lim0 + (int)((uint32_t)last / (uint32_t)P.group), len), 0);
+  x.t0 = max(it[8], 0);
+  x.t1 = min(it[9], (k_hi + keys - 1) / keys);
+  return true;
+}
+
 // Checks shared by the entries, and the views (qvl_causal.hip).
 int attn_params(const char* what, int32_t dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                 int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int64_t kv_rows, const void* out,

@@ -221,19 +221,19 @@ class CausalPlan:
         lib = capi.load()
         n_cus = torch.cuda.get_device_properties(device).multi_processor_count
         p64 = lambda a: a.ctypes.data_as(C.POINTER(C.c_int64))
-        n, whole, rows = C.c_int64(), C.c_int64(), C.c_int32(int(tile_rows))
+        n, parts, joins, rows = C.c_int64(), C.c_int64(), C.c_int64(), C.c_int32(int(tile_rows))
 
         def build(items, capacity):
             capi.check(lib.qvl_causal_worklist(len(new), p64(new), p64(keys), p64(first), self.num_heads, self.num_kv_heads,
                                                self.head_dim, _qdtype(dtype), n_cus, C.byref(rows), items, capacity, C.byref(n),
-                                               C.byref(whole)), "qvl_causal_worklist")
+                                               C.byref(parts), C.byref(joins)), "qvl_causal_worklist")
 
         build(None, 0)
-        items = np.zeros((max(n.value, 1), 8), np.int32)
-        build(items.ctypes.data_as(C.POINTER(C.c_int32)), n.value)
-        self.n_items, self.n_whole, self.tile_rows = n.value, whole.value, rows.value
+        items = np.zeros((max(n.value + joins.value, 1), capi.QVL_CAUSAL_ITEM_WORDS), np.int32)
+        build(items.ctypes.data_as(C.POINTER(C.c_int32)), n.value + joins.value)
+        self.n_items, self.n_parts, self.n_joins, self.tile_rows = n.value, parts.value, joins.value, rows.value
         nb = C.c_size_t()
-        capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.tile_rows, self.n_items, self.n_whole, C.byref(nb)),
+        capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.tile_rows, self.n_parts, C.byref(nb)),
                    "qvl_causal_workspace_size")
         self.workspace_bytes = nb.value
         self.items = torch.from_numpy(items).to(device)
@@ -277,8 +277,8 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
     ws = _workspace(plan.workspace_bytes, q)
     with _On(like[1]) as st:
         capi.check(capi.load().qvl_causal_attention(
-            st, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_whole,
-            _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
+            st, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
+            plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
     return out
 
 

@@ -50,16 +50,16 @@ def worklist(pkg, new, length, start, hq, hkv, hd=128, dtype=1, n_cus=256, tile_
     lib = pkg.capi.load()
     a = [np.array(v, np.int64) for v in (new, length, start)]
     p = [v.ctypes.data_as(C.POINTER(C.c_int64)) for v in a]
-    n, w, rows = C.c_int64(), C.c_int64(), C.c_int32(tile_rows)
+    n, parts, joins, rows = C.c_int64(), C.c_int64(), C.c_int64(), C.c_int32(tile_rows)
     call = lambda items, cap: lib.qvl_causal_worklist(len(new), *p, hq, hkv, hd, dtype, n_cus, C.byref(rows), items, cap, C.byref(n),
-                                                      C.byref(w))
+                                                      C.byref(parts), C.byref(joins))
     pkg.capi.check(call(None, 0))
-    items = np.zeros((n.value, 8), np.int32)
+    items = np.zeros((n.value + joins.value, pkg.capi.QVL_CAUSAL_ITEM_WORDS), np.int32)
     ptr = items.ctypes.data_as(C.POINTER(C.c_int32))
-    pkg.capi.check(call(ptr, n.value))
-    if n.value > 0:
-        assert call(ptr, n.value - 1) == -1
-    return items, w.value, rows.value
+    pkg.capi.check(call(ptr, len(items)))
+    if len(items):
+        assert call(ptr, len(items) - 1) == -1
+    return items[:n.value].tolist(), items[n.value:].tolist(), parts.value, rows.value
 
 
 @pytest.mark.parametrize("tile_rows", [0, 128, 256])
@@ -72,41 +72,63 @@ def test_worklist_covers_every_row_and_key_once(pkg, new, old, hq, hkv, hd, dtyp
         pytest.skip("bf16 only")
     length = [a + b for a, b in zip(new, old)]
     start = [(1 << 33) + 17 * i for i in range(len(new))]
-    items, n_whole, height = worklist(pkg, new, length, start, hq, hkv, hd, dtype, tile_rows=tile_rows)
+    items, joins, n_parts, height = worklist(pkg, new, length, start, hq, hkv, hd, dtype, tile_rows=tile_rows)
     assert height in ((128, 256) if dtype == 1 else (128,)) and tile_rows in (0, height)
     group = hq // hkv
     q0 = np.concatenate([[0], np.cumsum(new)])
-    seen = {}
-    slots = []
-    for k, it in enumerate(items.tolist()):
-        first, n_new, n_keys, row0, head, slot, lo, hi = it
+    seq_of = lambda first, n_new: [j for j in range(len(new)) if q0[j] == first and new[j] == n_new][0]
+    tiles = {}
+    for first, n_new, n_keys, row0, head, slot, lo, hi, t0, t1 in items:
         if n_new == 0:          # padding of a short queue
             continue
-        i = [j for j in range(len(new)) if q0[j] == first and new[j] == n_new][0]
+        i = seq_of(first, n_new)
         assert n_keys == length[i] and (hi << 32 | lo & 0xffffffff) == start[i]
-        part, parts = head >> 12 & 0xff, head >> 20 & 0xff
-        assert (parts >= 2 and part < parts and k >= n_whole) if parts else k < n_whole
-        if parts:
-            slots.append(slot)
-        assert row0 % height == 0 and 0 <= row0 < n_new * group
-        seen.setdefault((i, row0, head & 0xfff), []).append((part, max(parts, 1)))
-    want = {(i, r, h) for i in range(len(new)) for r in range(0, new[i] * group, height) for h in range(hkv)}
-    assert set(seen) == want
-    for got in seen.values():
-        assert sorted(p for p, _ in got) == list(range(got[0][1])) and len({n for _, n in got}) == 1
-    assert sorted(slots) == list(range(len(items) - n_whole))
+        assert row0 % height == 0 and 0 <= row0 < n_new * group and -1 <= slot < n_parts
+        tiles.setdefault((i, row0, head), []).append((t0, t1, slot))
+    assert set(tiles) == {(i, r, h) for i in range(len(new)) for r in range(0, new[i] * group, height) for h in range(hkv)}
+    cut = {}
+    for (i, row0, head), got in tiles.items():
+        got.sort()
+        last = (min(row0 + height, new[i] * group) - 1) // group         # the tile's last token
+        keys = max(min(old[i] + last + 1, length[i]), 0)
+        assert got[0][0] == 0 and got[-1][1] == -(-keys // (64 if dtype == 1 else 32))
+        assert all(a[1] == b[0] and a[1] > a[0] for a, b in zip(got, got[1:]))
+        if len(got) > 1:                                                # consecutive slots, in the order of the keys
+            assert [s for _, _, s in got] == list(range(got[0][2], got[0][2] + len(got)))
+            cut[i, row0, head] = got[0][2], len(got)
+        else:
+            assert got[0][2] == -1
+    assert sum(n for _, n in cut.values()) == n_parts
+    slots = sorted(s for got in tiles.values() for _, _, s in got if s >= 0)
+    assert slots == list(range(n_parts))
+    assert {(seq_of(j[0], j[1]), j[3], j[4]): (j[5], j[9]) for j in joins} == cut and len(joins) == len(cut)
+
+
+def test_worklist_cuts_all_tiles_of_a_sequence_at_the_same_keys(pkg):
+    """Tiles of about 120 and 380 key steps on 256 slots: the long ones are cut, so that they end with the short ones."""
+    items, joins, n_parts, height = worklist(pkg, [811, 300], [7824, 24301], [0, 7824], 32, 8, tile_rows=256)
+    assert n_parts > 0 and joins
+    steps = sorted((it[9] - it[8] for it in items if it[1]), reverse=True)
+    slots = [0] * 256
+    for s in steps:                                                     # as the dispatcher does: next job to the first slot free
+        slots[slots.index(min(slots))] += s
+    assert max(slots) <= 1.25 * sum(steps) / 256
+    for i in (0, 811):
+        ends = [{it[9] for it in items if it[1] and it[0] == i and it[3] == r and it[5] >= 0} for r in {it[3] for it in items if it[0] == i}]
+        common = min(ends, key=len)
+        assert all(len(common - e) <= 1 for e in ends)                  # but for the last, where the tile's keys end
 
 
 def test_worklist_refusals(pkg):
     f = pkg.capi.load().qvl_causal_worklist
-    n, w, rows = C.c_int64(), C.c_int64(), C.c_int32()
+    n, w, g, rows = C.c_int64(), C.c_int64(), C.c_int64(), C.c_int32()
     one = lambda v: (C.c_int64 * 1)(v)
     ok = dict(new=4, length=9, start=0, hq=8, hkv=2, hd=128, dt=1, cus=256, rows=0)
 
     def rc(**k):
         a = dict(ok, **k)
         return f(1, one(a["new"]), one(a["length"]), one(a["start"]), a["hq"], a["hkv"], a["hd"], a["dt"], a["cus"],
-                 C.byref(C.c_int32(a["rows"])), None, 0, C.byref(n), C.byref(w))
+                 C.byref(C.c_int32(a["rows"])), None, 0, C.byref(n), C.byref(w), C.byref(g))
 
     assert rc() == 0
     for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57), dict(rows=64)):
@@ -114,9 +136,11 @@ def test_worklist_refusals(pkg):
     for bad in (dict(hd=96), dict(dt=2), dict(hq=8192, hkv=8192), dict(length=1 << 30), dict(new=1 << 29),
                 dict(rows=256, dt=0)):
         assert rc(**bad) == -2, bad
-    assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), C.byref(w)) == -1
-    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, None, C.byref(w)) == -1
-    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, None, None, 0, C.byref(n), C.byref(w)) == -1
+    assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), C.byref(w), C.byref(g)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, None, C.byref(w), C.byref(g)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), None, C.byref(g)) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), C.byref(w), None) == -1
+    assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, None, None, 0, C.byref(n), C.byref(w), C.byref(g)) == -1
 
 
 def rotary_args(**change):
@@ -165,18 +189,23 @@ ATTN_BAD = [(-2, dict(dtype=3)), (-2, dict(hd=80)), (-1, dict(hq=12)), (-1, dict
 def test_causal_attention_refusals(pkg):
     f = pkg.capi.load().qvl_causal_attention
 
-    def rc(items=FAKE, n_items=3, n_whole=3, rows=128, **k):
-        return f(*attn_common(**k), rows, items, n_items, n_whole, *attn_tail(**k))
+    def rc(items=FAKE, n_items=3, n_parts=0, n_joins=0, rows=128, **k):
+        return f(*attn_common(**k), rows, items, n_items, n_parts, n_joins, *attn_tail(**k))
 
-    for want, bad in ATTN_BAD + [(-1, dict(items=None)), (-3, dict(items=FAKE + 4)), (-1, dict(n_whole=4)), (-1, dict(n_whole=-1)),
-                                 (-1, dict(n_items=1 << 31)), (-1, dict(rows=64)), (-2, dict(rows=256, dtype=0))]:
+    for want, bad in ATTN_BAD + [(-1, dict(items=None)), (-3, dict(items=FAKE + 4)), (-1, dict(n_parts=4, n_joins=1)),
+                                 (-1, dict(n_parts=-1)), (-1, dict(n_items=1 << 31)), (-1, dict(n_items=-1)), (-1, dict(rows=64)),
+                                 (-1, dict(n_parts=2)), (-1, dict(n_joins=1)), (-1, dict(n_parts=2, n_joins=2)),
+                                 (-1, dict(n_parts=2, n_joins=-1)), (-2, dict(rows=256, dtype=0)),
+                                 (-4, dict(n_parts=2, n_joins=1, ws=None)), (-4, dict(n_parts=2, n_joins=1, ws_bytes=2 * 128 * 130 * 4 - 1)),
+                                 (-3, dict(n_parts=2, n_joins=1, ws=FAKE + 8))]:
         assert rc(**bad) == want, bad
-    assert rc(n=0, q=None) == 0 and rc(items=None, n_items=0, n_whole=0) == 0
+    assert rc(n=0, q=None) == 0 and rc(items=None, n_items=0) == 0
     nb = C.c_size_t()
     size = pkg.capi.load().qvl_causal_workspace_size
-    assert size(128, 128, 4, 4, C.byref(nb)) == 0 and nb.value == 0
-    assert size(96, 128, 4, 4, C.byref(nb)) == -2 and size(128, 128, 3, 4, C.byref(nb)) == -1
-    assert size(128, 128, 4, 4, None) == -1 and size(128, 64, 4, 4, C.byref(nb)) == -1
+    assert size(128, 128, 0, C.byref(nb)) == 0 and nb.value == 0
+    assert size(128, 256, 3, C.byref(nb)) == 0 and nb.value == 3 * 256 * 130 * 4
+    assert size(96, 128, 4, C.byref(nb)) == -2 and size(128, 128, -1, C.byref(nb)) == -1
+    assert size(128, 128, 4, None) == -1 and size(128, 64, 4, C.byref(nb)) == -1
 
 
 def test_decode_attention_refusals(pkg):
