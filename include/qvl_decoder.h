@@ -13,11 +13,14 @@
  *   - q, k, v, out and the caches are views [rows, heads, head_dim] of one dtype: element (r, h, d) lies at
  *     p[r * row_stride + h * head_stride + d], strides in elements, 0 <= stride < 2^31, both multiples of 16 bytes
  *     like the pointers (QVL_ERR_MISALIGNED). So the column blocks of a qkv Dense output, a cache [rows, heads, dim]
- *     and one [heads, rows, dim] all serve as they are.
+ *     and one [heads, rows, dim] all serve as they are. Rows of k and v of the attention lie at most 64 MiB apart
+ *     (QVL_ERR_UNSUPPORTED). Rows and heads of an output do not lie over one another, nor over an input.
  *   - num_heads is a multiple of num_kv_heads; query head h reads key/value head h / (num_heads / num_kv_heads).
  *   - head_dim 64 or 128, bf16 or fp32. Sums, softmax statistics and norms are held in fp32 in both; outputs are
  *     rounded once.
- *   - Offsets are 64-bit: a cache may be larger than 4 GiB.
+ *   - Offsets are 64-bit: a cache may be larger than 4 GiB. Counts of tokens, tokens x (num_heads / num_kv_heads) and keys
+ *     of a sequence stay below 2^30, heads below 4096 (QVL_ERR_UNSUPPORTED; lengths that lie on the device: NaN).
+ *   - What a call computes depends on its inputs alone, bit for bit: no atomics, and parts are joined in a fixed order.
  */
 #ifndef QVL_DECODER_H
 #define QVL_DECODER_H
@@ -41,9 +44,9 @@ int qvl_text_rotary_table(int32_t head_dim, double theta, const int32_t* h_secti
  * d_positions[axis * pos_stride + n] (int32; pos_stride 0: one position for the three axes), all in fp32 and rounded
  * once. The angle is reduced in 64-bit fixed point, so positions of any int32 keep full precision.
  * q goes to q_out row n; k to k_out and v (copied as it is) to v_out at row d_rows[n] (int64; NULL: row n), and a token
- * whose row lies outside [0, out_rows) writes neither. v and v_out may be NULL together. Rows should differ: of two
- * tokens with one row, either's values may stay. Outputs may be their inputs (same pointer and strides, d_rows NULL);
- * other overlaps are not allowed. */
+ * whose row lies outside [0, out_rows) writes neither. v and v_out may be NULL together. Rows should differ: the row of
+ * two tokens holds values of either. Outputs may be their inputs (same pointer and strides, d_rows NULL); other overlaps
+ * are not allowed. */
 int qvl_qk_norm_rotary(void* stream, int32_t dtype,
                        const void* d_q, int64_t q_row_stride, int64_t q_head_stride,
                        const void* d_k, int64_t k_row_stride, int64_t k_head_stride,
@@ -89,9 +92,9 @@ int qvl_causal_attention(void* stream, int32_t dtype,
  * of the moment. Sequence i brings query tokens [d_cu_q[i], d_cu_q[i+1]) (NULL: token i, n_tokens == n_seqs) and has
  * d_k_len[i] keys in cache rows from d_k_start[i], the new tokens' own among them, seen as in qvl_causal_attention.
  * With n_groups > 0, sequences [d_cu_groups[g], d_cu_groups[g+1]) also see, before their own keys, all of the
- * d_prefix_len[g] cache rows from d_prefix_start[g]; one softmax covers both. d_cu_groups runs from 0 to n_seqs and
- * d_cu_q from 0 to at most n_tokens, neither ever falling; rows from d_cu_q[n_seqs] on are left as they are. A token that sees
- * no key gets zeros. The tokens of a sequence whose keys (or prefix) leave [0, kv_rows) come out NaN; nothing outside is read.
+ * d_prefix_len[g] cache rows from d_prefix_start[g]; one softmax covers both; sequences of no group have no prefix.
+ * d_cu_groups stays in [0, n_seqs] and d_cu_q in [0, n_tokens], neither ever falling; rows before d_cu_q[0] and from
+ * d_cu_q[n_seqs] on are left as they are. A token that sees no key gets zeros. The tokens of a sequence whose keys (or prefix) leave [0, kv_rows) come out NaN; nothing outside is read.
  * max_len and max_prefix are the lengths the launch is laid out for (a captured call's largest); longer ones are still
  * right. The workspace (qvl_decode_workspace_size of the same sizes; 16-byte aligned) holds partial outputs: calls that
  * overlap need one each. */

@@ -486,7 +486,7 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
   D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, slots, D.prefix_chunk);
   D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
-  if (D.units > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
+  if (D.units > 0x7fffffffLL || n_tokens * num_heads > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   D.part_rows = (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads;
   return QVL_OK;
 }

@@ -8,6 +8,7 @@
 #include <cmath>
 #include <functional>
 #include <map>
+#include <new>
 #include <queue>
 #include <vector>
 
@@ -23,6 +24,8 @@ struct Job {
   int32_t t0, t1;   // key tiles
   int32_t steps() const { return t1 - t0; }
 };
+
+constexpr int64_t kMaxJobs = 1 << 22;   // 5 10^8 rows
 
 // Greedy time of jobs, longest first, on `slots` workgroup slots.
 double makespan(std::vector<double> cost, int64_t slots) {
@@ -182,34 +185,9 @@ std::vector<Job> deal(const std::vector<Job>& jobs, int32_t beside) {
   return out;
 }
 
-}  // namespace
-
-extern "C" {
-
-int qvl_text_rotary_table(int32_t head_dim, double theta, const int32_t* section, int32_t interleaved, uint64_t* table) {
-  if (head_dim <= 0 || head_dim % 4 || head_dim > 256) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: head_dim=%d", head_dim);
-  if (!(theta > 1.0) || !isfinite(theta)) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: theta=%g", theta);
-  if (!section || !table) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: NULL pointer");
-  const int half = head_dim / 2;
-  for (int a = 0; a < 3; ++a)
-    if (section[a] < 0 || section[a] > half) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: section[%d]=%d", a, section[a]);
-  if (!interleaved && section[0] + section[1] + section[2] != half)
-    return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: section sums to %d, not head_dim / 2 = %d",
-                     section[0] + section[1] + section[2], half);
-  for (int j = 0; j < half; ++j) {
-    // Turns per position, below 1/2pi: 64 fraction bits hold it to 2^-64 turns, 2^31 positions of it to 2^-33.
-    const long double turns = powl((long double)theta, -2.0L * j / head_dim) / 6.283185307179586476925286766559L;
-    table[2 * j] = (uint64_t)roundl(ldexpl(turns, 64));
-    const int a = j % 3;
-    table[2 * j + 1] = interleaved ? (j < 3 * section[a] ? a : 0)
-                                   : (j < section[0] ? 0 : j < section[0] + section[1] ? 1 : 2);
-  }
-  return QVL_OK;
-}
-
-int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len, const int64_t* start, int32_t num_heads,
-                        int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus, int32_t* tile_rows,
-                        int32_t* items, int64_t capacity, int64_t* n_items, int64_t* n_parts, int64_t* n_joins) {
+int causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len, const int64_t* start, int32_t num_heads,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus, int32_t* tile_rows,
+                    int32_t* items, int64_t capacity, int64_t* n_items, int64_t* n_parts, int64_t* n_joins) {
   if (!n_items || !n_parts || !n_joins || !tile_rows)
     return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_items / n_parts / n_joins / tile_rows is NULL");
   if (n_seqs < 0 || (n_seqs > 0 && (!n_new || !len || !start)))
@@ -219,13 +197,13 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
     return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: %d heads over %d key/value heads", num_heads, num_kv_heads);
   if (num_heads > kItemMaxHeads) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: num_heads=%d", num_heads);
-  if (n_cus <= 0) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_cus=%d", n_cus);
+  if (n_cus <= 0 || n_cus > 65536) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: n_cus=%d", n_cus);
   if (*tile_rows != 0 && *tile_rows != 128 && *tile_rows != 256) return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: tile_rows=%d", *tile_rows);
   if (*tile_rows == 256 && dtype == QVL_DTYPE_F32) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: tiles of 256 rows are bf16 only");
   const int64_t group = num_heads / num_kv_heads;
   const int64_t step_keys = dtype == QVL_DTYPE_BF16 ? 64 : 32;
   std::vector<int64_t> q_first;
-  int64_t q0 = 0;
+  int64_t q0 = 0, n_jobs = 0;
   for (int64_t i = 0; i < n_seqs; ++i) {
     if (n_new[i] < 0 || len[i] < 0 || start[i] < 0 || start[i] > (int64_t)1 << 56)
       return set_error(QVL_ERR_INVALID_ARG, "causal_worklist: sequence %lld: %lld new, %lld keys from row %lld", (long long)i,
@@ -234,6 +212,8 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
       return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: sequence %lld is too long", (long long)i);
     q_first.push_back(q0);
     q0 += n_new[i];
+    n_jobs += (n_new[i] * group + kItemRows - 1) / kItemRows * num_kv_heads;
+    if (n_jobs > kMaxJobs) return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: more than %lld tiles", (long long)kMaxJobs);
   }
   // the tile height (where the caller leaves it open) and the cut of least modelled time
   std::vector<Job> jobs;
@@ -295,6 +275,43 @@ int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len
     it[9] = j.t1;
   }
   return QVL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qvl_text_rotary_table(int32_t head_dim, double theta, const int32_t* section, int32_t interleaved, uint64_t* table) {
+  if (head_dim <= 0 || head_dim % 4 || head_dim > 256) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: head_dim=%d", head_dim);
+  if (!(theta > 1.0) || !isfinite(theta)) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: theta=%g", theta);
+  if (!section || !table) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: NULL pointer");
+  const int half = head_dim / 2;
+  for (int a = 0; a < 3; ++a)
+    if (section[a] < 0 || section[a] > half) return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: section[%d]=%d", a, section[a]);
+  if (!interleaved && section[0] + section[1] + section[2] != half)
+    return set_error(QVL_ERR_INVALID_ARG, "text_rotary_table: section sums to %d, not head_dim / 2 = %d",
+                     section[0] + section[1] + section[2], half);
+  for (int j = 0; j < half; ++j) {
+    // Turns per position, below 1/2pi: 64 fraction bits hold it to 2^-64 turns, 2^31 positions of it to 2^-33.
+    const long double turns = powl((long double)theta, -2.0L * j / head_dim) / 6.283185307179586476925286766559L;
+    table[2 * j] = (uint64_t)roundl(ldexpl(turns, 64));
+    const int a = j % 3;
+    table[2 * j + 1] = interleaved ? (j < 3 * section[a] ? a : 0)
+                                   : (j < section[0] ? 0 : j < section[0] + section[1] ? 1 : 2);
+  }
+  return QVL_OK;
+}
+
+int qvl_causal_worklist(int64_t n_seqs, const int64_t* n_new, const int64_t* len, const int64_t* start, int32_t num_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int32_t n_cus, int32_t* tile_rows,
+                        int32_t* items, int64_t capacity, int64_t* n_items, int64_t* n_parts, int64_t* n_joins) {
+  // (a list too long for the host's memory is an error like any other, not an exception through a C call)
+  try {
+    return causal_worklist(n_seqs, n_new, len, start, num_heads, num_kv_heads, head_dim, dtype, n_cus, tile_rows, items, capacity,
+                           n_items, n_parts, n_joins);
+  } catch (const std::bad_alloc&) {
+    return set_error(QVL_ERR_UNSUPPORTED, "causal_worklist: out of host memory");
+  }
 }
 
 }  // extern "C"

@@ -13,7 +13,8 @@ tensors [rows, heads, head_dim] (any row and head strides of whole 16 bytes), fl
                            max_prefix=...)                               # where sequences share an image's tokens
 
 Everything runs on the tensors' device and its current stream; nothing synchronises. Workspaces come from torch's
-allocator with every call, so calls on several streams and captured graphs share none.
+allocator with every call, so calls on several streams and captured graphs share none. No operator has a gradient: a tensor
+that requires one is refused while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -151,7 +152,7 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
     `positions` (int32 [3, N] for t, h, w, or [N] for text), one pass. Returns (q, k, v): without a cache new tensors q
     and k and v itself; with k_cache, v_cache [R, Hkv, D] and rows (int64 [N]), token n's key and value go to row
     rows[n] of the caches, which are returned (a row outside [0, R) is dropped; rows should differ). q_out, if given,
-    takes q (it may be q itself)."""
+    takes q (it may be q itself). Outputs lie over no other input."""
     torch = _torch()
     like = _like(q)
     N, Hq, D = q.shape
@@ -296,7 +297,7 @@ def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
     views, ov, out = _attention_views(q, k, v, out, like)
     N, Hq, D = q.shape
     rows, Hkv = k.shape[0], k.shape[1]
-    n_seqs = k_start.shape[0]
+    n_seqs = k_start.numel()
     ks = _word(k_start, "k_start", like, torch.int64, (n_seqs,))
     kl = _word(k_len, "k_len", like, torch.int32, (n_seqs,))
     cq = None if cu_q is None else _word(cu_q, "cu_q", like, torch.int32, (n_seqs + 1,))
@@ -304,7 +305,7 @@ def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
     n_groups = max_prefix = 0
     if groups is not None:
         prefix_start, prefix_len, cu_groups, max_prefix = groups
-        n_groups = prefix_start.shape[0]
+        n_groups = prefix_start.numel()
         ps = _word(prefix_start, "prefix_start", like, torch.int64, (n_groups,))
         pl = _word(prefix_len, "prefix_len", like, torch.int32, (n_groups,))
         cg = _word(cu_groups, "cu_groups", like, torch.int32, (n_groups + 1,))
@@ -329,6 +330,6 @@ def decode_attention(q, k, v, k_start, k_len, *, max_len: int, cu_q=None, scale:
 def prefix_attention(q, k, v, k_start, k_len, prefix_start, prefix_len, cu_groups, *, max_len: int, max_prefix: int,
                      cu_q=None, scale: Optional[float] = None, out=None):
     """`decode_attention` of sequences that share prefixes: every token of sequences cu_groups[g]..cu_groups[g+1] (int32
-    [G + 1], from 0 to the number of sequences) also sees the prefix_len[g] (int32) cache rows from prefix_start[g]
-    (int64), which lie in the cache once and are read once for the group."""
+    [G + 1], never falling) also sees the prefix_len[g] (int32) cache rows from prefix_start[g]
+    (int64), which lie in the cache once and are read once for the group. Sequences of no group have no prefix."""
     return _decode(q, k, v, k_start, k_len, max_len, cu_q, (prefix_start, prefix_len, cu_groups, max_prefix), scale, out)

@@ -131,10 +131,10 @@ def test_worklist_refusals(pkg):
                  C.byref(C.c_int32(a["rows"])), None, 0, C.byref(n), C.byref(w), C.byref(g))
 
     assert rc() == 0
-    for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57), dict(rows=64)):
+    for bad in (dict(new=-1), dict(length=-1), dict(start=-1), dict(hq=7), dict(hq=0), dict(hkv=0), dict(cus=0), dict(start=1 << 57), dict(rows=64), dict(cus=1 << 17)):
         assert rc(**bad) == -1, bad
     for bad in (dict(hd=96), dict(dt=2), dict(hq=8192, hkv=8192), dict(length=1 << 30), dict(new=1 << 29),
-                dict(rows=256, dt=0)):
+                dict(rows=256, dt=0), dict(new=1 << 26, hq=64, hkv=64)):
         assert rc(**bad) == -2, bad
     assert f(1, None, one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, C.byref(n), C.byref(w), C.byref(g)) == -1
     assert f(1, one(1), one(1), one(0), 8, 2, 128, 1, 256, C.byref(rows), None, 0, None, C.byref(w), C.byref(g)) == -1

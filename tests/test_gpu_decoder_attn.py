@@ -108,6 +108,24 @@ def test_rotary_far_and_negative_positions(ops, dtype):
     assert_rotary(ko, k, w, pos[None].repeat(3, 1), rot)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rotary_two_tokens_of_one_row(ops, dtype):
+    """The row holds values of the one or the other, and no other row changes."""
+    n, hq, hkv, D = 64, 4, 2, 64
+    rot = ops.TextRotary(D, 1e4, (12, 10, 10), True, DEV)
+    w = 1 + 0.1 * rand((D,), F32, 3)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    q, k, v = rand((n, hq, D), dtype, 1), rand((n, hkv, D), dtype, 2), rand((n, hkv, D), dtype, 4)
+    _, alone, _ = ops.qk_norm_rotary(q, k, v, w, w, pos, rot)
+    kc, vc = rand((40, hkv, D), dtype, 5), rand((40, hkv, D), dtype, 6)
+    kc0, vc0 = kc.clone(), vc.clone()
+    rows = (torch.arange(n, device=DEV) // 2) + 4                            # tokens 2 i and 2 i + 1 both to row i + 4
+    ops.qk_norm_rotary(q, k, v, w, w, pos, rot, k_cache=kc, v_cache=vc, rows=rows)
+    for got, a in ((kc, alone), (vc, v)):
+        assert ((got[4:36] == a[0::2]) | (got[4:36] == a[1::2])).all()
+    assert torch.equal(kc[36:], kc0[36:]) and torch.equal(vc[:4], vc0[:4]) and torch.equal(kc[:4], kc0[:4])
+
+
 def test_rotary_strides_in_place_and_dropped_rows(ops):
     n, hq, hkv, D = 70, 6, 2, 64
     rot = ops.TextRotary(D, 1e4, (12, 10, 10), True, DEV)
@@ -265,6 +283,64 @@ def test_causal_large_scores(ops, dtype, tile_rows):
         assert ((out[q0:q0 + n].double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_causal_scores_far_above_the_first_tile(ops, D):
+    """Some rows' scores from key 64 on exceed the first 64 by 2^400 in the weight, others stay far below: sums held against
+    the first tile's maximum overflow, and those rows alone are formed again. Every row is exact to the usual bound."""
+    hq, hkv, n, old = 4, 2, 130, 200
+    q, k, v, seqs = causal_case(hq, hkv, D, BF, [n], [old], seed=31)
+    row = seqs[0][2]
+    u = rand((D,), F32, 32)
+    u = u / u.norm()
+    away = lambda x: x.float() - (x.float() @ u)[..., None] * u           # nothing of direction u in it
+    kf, qf = away(k), away(q)
+    kf[row + 64:row + old + n] += 20.0 * u                                  # keys 64 and later
+    side = torch.where(torch.arange(n, device=DEV) % 3 == 0, 1.0, -1.0)     # every third token looks there, the others away
+    qf[:n] += (side * 14.0 * math.sqrt(D))[:, None, None] * u               # +-280 of a score, +-404 in powers of two
+    q, k = qf.to(BF), kf.to(BF)
+    for rows in (128, 256):
+        check_causal(ops.causal_attention(q, k, v, plan_of(ops, seqs, hq, hkv, D, BF, rows)), q, k, v, seqs, D ** -0.5)
+
+
+def test_captured_causal_attention(ops):
+    """A captured prefill of cut and joined tiles, replayed with other inputs in the same buffers and eager work between."""
+    hq, hkv, D = 32, 8, 128
+    q, k, v, seqs = causal_case(hq, hkv, D, BF, [300, 20], [3000, 5], seed=33)
+    plan = plan_of(ops, seqs, hq, hkv, D, BF)
+    assert plan.n_joins > 0
+    n = sum(s[1] for s in seqs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.causal_attention(q, k, v, plan)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.causal_attention(q, k, v, plan)
+    for i in range(4):
+        q.copy_(rand(tuple(q.shape), BF, 70 + i))
+        v.copy_(rand(tuple(v.shape), BF, 80 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bits(got[:n]), bits(ops.causal_attention(q, k, v, plan)[:n])), i
+
+
+def test_nothing_to_do(ops):
+    """Plans without sequences or without tokens, caches without rows, decode steps without sequences."""
+    q, k = rand((3, 8, 64), BF, 1), rand((5, 2, 64), BF, 2)
+    for new, keys in ([], []), ([0, 0], [0, 4]):
+        plan = ops.CausalPlan(new, keys, [0] * len(new), num_heads=8, num_kv_heads=2, head_dim=64, dtype=BF, device=DEV)
+        out = torch.full_like(q, 7.0)
+        assert (ops.causal_attention(q, k, k, plan, out=out) == 7.0).all()
+        assert ops.causal_attention(q[:0], k, k, plan).shape == (0, 8, 64)
+    plan = ops.CausalPlan([3], [0], [0], num_heads=8, num_kv_heads=2, head_dim=64, dtype=BF, device=DEV)
+    assert (ops.causal_attention(q, k[:0], k[:0], plan) == 0).all()          # no keys at all: zeros
+    none = lambda dt: torch.zeros(0, dtype=dt, device=DEV)
+    assert ops.decode_attention(q[:0], k, k, none(torch.int64), none(torch.int32), max_len=9).shape == (0, 8, 64)
+    zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+    assert (ops.decode_attention(q, k[:0], k[:0], zero.long(), zero, max_len=0) == 0).all()
+
+
 @pytest.mark.parametrize("dtype,tile_rows", KERNELS)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_causal_masked_keys_hold_anything(ops, dtype, tile_rows, bad):
@@ -383,6 +459,51 @@ def test_decode_and_prefix(ops, dtype, hq, hkv, D, lengths, new, prefixes, group
     assert decode_call(ops, st, q, k, v, lengths, prefixes, out=out) is out
     check_decode(out, st, q, k, v, lengths, prefixes, groups, D ** -0.5)
     assert (out[n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (F32, 64)])
+@pytest.mark.parametrize("n", [65, 256, 257, 300, 1100])
+def test_decode_of_many_sequences(ops, dtype, D, n):
+    """More sequences than a wave's lanes, and than a workgroup's threads; some empty, one much longer than the rest."""
+    g = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 90, (n,), generator=g).tolist()
+    lengths[n // 3], lengths[n - 1] = 5000, 0
+    new = None if n % 2 else torch.randint(0, 3, (n,), generator=g).tolist()
+    st = decode_state(lengths, new=new)
+    m = sum(st["new"])
+    k, v, q = rand((st["rows"], 2, D), dtype, 1, 1.4), rand((st["rows"], 2, D), dtype, 2), rand((m, 8, D), dtype, 3, 1.4)
+    out = decode_call(ops, st, q, k, v, lengths, [])
+    check_decode(out, st, q, k, v, lengths, [], [], D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_sequences_of_no_group_have_no_prefix(ops, dtype):
+    """cu_groups that covers sequences 2 to 4 of 7: the others (a padded batch's tail, say) see their own keys alone."""
+    lengths, prefixes, groups = [40, 3, 17, 60, 9, 0, 33], [700, 129], [2, 1]
+    st = decode_state(lengths, prefixes, groups)
+    k, v, q = rand((st["rows"], 2, 64), dtype, 1), rand((st["rows"], 2, 64), dtype, 2), rand((7, 8, 64), dtype, 3)
+    st["cu_groups"] = torch.tensor([2, 4, 5], dtype=torch.int32, device=DEV)
+    want = torch.empty_like(q)
+    for i, g in enumerate([None, None, 0, 0, 1, None, None]):
+        one = decode_state(lengths, prefixes, groups)
+        pick = lambda t: t[i:i + 1].contiguous()
+        if g is None:
+            want[i] = ops.decode_attention(q[i:i + 1], k, v, pick(one["k_start"]), pick(one["k_len"]), max_len=lengths[i])[0]
+        else:
+            want[i] = ops.prefix_attention(q[i:i + 1], k, v, pick(one["k_start"]), pick(one["k_len"]), one["prefix_start"][g:g + 1],
+                                           one["prefix_len"][g:g + 1], torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                                           max_len=lengths[i], max_prefix=prefixes[g])[0]
+    for _ in range(3):                                                      # with whatever an earlier call left in the workspace
+        junk = torch.full((1 << 22,), float("nan"), device=DEV)
+        del junk
+        out = decode_call(ops, st, q, k, v, lengths, prefixes)
+        check_rows = [attention_ref(q[i:i + 1], k[s:s + n], v[s:s + n], torch.tensor([n], device=DEV), 64 ** -0.5)
+                      for i, (s, n) in enumerate(zip(st["starts"], lengths))]
+        for i in (0, 1, 5, 6):
+            assert_attention(out[i:i + 1], check_rows[i], max(lengths[i], 1))
+        # the two orders of joining differ by their fp32 sums and each output's rounding
+        err = (out.double() - want.double()).abs()
+        assert (err <= (2 * HALF_STEP[dtype] + 8192 * 2.0 ** -24 + (4 * 2.0 ** -8 if dtype == BF else 0)) * float(v.double().abs().max())).all()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
