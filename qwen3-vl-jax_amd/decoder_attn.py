@@ -223,15 +223,16 @@ class CausalPlan:
         n_cus = torch.cuda.get_device_properties(device).multi_processor_count
         p64 = lambda a: a.ctypes.data_as(C.POINTER(C.c_int64))
         n, parts, joins, rows = C.c_int64(), C.c_int64(), C.c_int64(), C.c_int32(int(tile_rows))
-
-        def build(items, capacity):
-            capi.check(lib.qvl_causal_worklist(len(new), p64(new), p64(keys), p64(first), self.num_heads, self.num_kv_heads,
-                                               self.head_dim, _qdtype(dtype), n_cus, C.byref(rows), items, capacity, C.byref(n),
-                                               C.byref(parts), C.byref(joins)), "qvl_causal_worklist")
-
-        build(None, 0)
-        items = np.zeros((max(n.value + joins.value, 1), capi.QVL_CAUSAL_ITEM_WORDS), np.int32)
-        build(items.ctypes.data_as(C.POINTER(C.c_int32)), n.value + joins.value)
+        for entries in (4096, None):                # room for most lists; the call says how much one needs
+            entries = entries or n.value + joins.value
+            items = np.zeros((entries, capi.QVL_CAUSAL_ITEM_WORDS), np.int32)
+            rc = lib.qvl_causal_worklist(len(new), p64(new), p64(keys), p64(first), self.num_heads, self.num_kv_heads,
+                                         self.head_dim, _qdtype(dtype), n_cus, C.byref(rows),
+                                         items.ctypes.data_as(C.POINTER(C.c_int32)), entries, C.byref(n), C.byref(parts), C.byref(joins))
+            if rc == capi.QVL_OK or n.value + joins.value <= entries:
+                break
+        capi.check(rc, "qvl_causal_worklist")
+        items = items[:max(n.value + joins.value, 1)]
         self.n_items, self.n_parts, self.n_joins, self.tile_rows = n.value, parts.value, joins.value, rows.value
         nb = C.c_size_t()
         capi.check(lib.qvl_causal_workspace_size(self.head_dim, self.tile_rows, self.n_parts, C.byref(nb)),
