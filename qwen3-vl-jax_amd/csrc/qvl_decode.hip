@@ -447,7 +447,7 @@ struct DecodePlan {
   size_t part_rows, split_bytes;
 };
 
-// Parts of at least 128 keys (a block of 32 a wave), as many as fill the workgroup slots once.
+// Parts of at least 128 keys (a block of 32 a wave), as many as fill `slots` workgroups once.
 static int split_parts(int64_t keys, int64_t units, int64_t slots, int& chunk) {
   int64_t parts = std::min({slots / std::max<int64_t>(units, 1), (keys + 127) / 128, (int64_t)64});
   parts = std::max<int64_t>(parts, 1);
@@ -466,13 +466,16 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   const int64_t rows = n_tokens * (num_heads / num_kv_heads);
   if (num_heads > kItemMaxHeads || n_tokens > kItemMaxLen || rows > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   // workgroups a GPU holds: two a CU, one where the tiles take 128 KB (fp32, head_dim 128)
-  const int64_t slots = (int64_t)gemm_device_cus() * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
+  const int64_t cus = gemm_device_cus(), slots = cus * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
   D = DecodePlan{};
   if (n_groups == 0) {
-    // a run for each slot, but no more than give each wave a block, nor fewer than there are jobs
+    // A run for each compute unit where that leaves it at most 40 blocks, else for each slot (8 heads: one sequence of 9001 keys
+    // 19 us and not 24, of 31000 32.5 and not 34.5; 16 of up to 8000 61.6 and not 69); no more than give each wave a block,
+    // nor fewer than there are jobs.
     const int64_t tiles = std::max<int64_t>((rows + 32 * n_seqs - 1) / (32 * std::max<int64_t>(n_seqs, 1)), 1);
     const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + 31) / 32);
-    D.runs = (int)std::max<int64_t>(std::min(slots / num_kv_heads, std::max((blocks + 3) / 4, jobs)), 1);
+    const int64_t one = cus / num_kv_heads, most = jobs <= one && blocks <= 40 * one ? one : slots / num_kv_heads;
+    D.runs = (int)std::max<int64_t>(std::min(most, std::max((blocks + 3) / 4, jobs)), 1);
     D.units = (int64_t)D.runs * num_kv_heads;
     D.slot_rows = (int)std::min<int64_t>(32, std::max<int64_t>(rows, 1));
     D.part_rows = (size_t)D.units * 2 * D.slot_rows;
@@ -484,7 +487,9 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   const int64_t tile = D.prefix_rows ? kItemRows : 32;
   D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
   D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
-  D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, slots, D.prefix_chunk);
+  // one unit on the prefixes for each compute unit, beside units on the sequences' own keys (one for each slot: 192 rows
+  // on 9216 keys 36 us, not 30; 1024 on 24007 145, not 140)
+  D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, cus, D.prefix_chunk);
   D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
   if (D.units > 0x7fffffffLL || n_tokens * num_heads > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   D.part_rows = (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads;
@@ -547,7 +552,7 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
     QVL_TRY_RC(check_launch("decode_stream"));
     if (plan.runs == 1) return QVL_OK;
     // a split job's rows over a few workgroups: they are few, and each reads every part
-    QVL_ATTN_LAUNCH(decode_stream_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)std::min(plan.slot_rows, 8)), P, S);
+    QVL_ATTN_LAUNCH(decode_stream_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)std::min(plan.slot_rows, 16)), P, S);
     return check_launch("decode_stream_join");
   }
   if (plan.prefix_rows) QVL_ATTN_LAUNCH(prefix_rows_kernel, units, P, S);
