@@ -9,8 +9,13 @@
 // there. (One line over heads too, its runs at unlike places: 438 us.) A job, a tile of a sequence's rows, that lies in one
 // run is finished there; one that crosses runs leaves parts, which a second launch joins.
 //
+// 96 sequences of up to 7900 keys, 32/8 heads of 128, bf16: 320 us, 4.9 TB/s; one of 9001 keys: 14 us and 5.5 for the join.
+//
 // With prefixes the tokens of a group are the rows of one more problem, the prefix's keys for all of them at once, 128 (32)
-// rows a workgroup and the keys in parts; the sequences' own keys are parts beside them, and one join covers both.
+// rows a workgroup and the keys in parts; the sequences' own keys are parts beside them, and one join covers both. (Tiles of
+// 256 rows for the prefix, then the own keys and the join in a second launch: 160 us, not 147, for 256 sequences on 24007
+// keys: the own keys, bound by memory, no longer run beside the prefix, bound by the matrix cores.)
+// 48 sequences after 9216 shared keys 28.5 us, 256 after 24007 146 us.
 #include "qvl_decoder_core.h"
 
 namespace qvl {

@@ -629,9 +629,9 @@ __device__ __forceinline__ f32x2 part_state(float m, float l, bool sees) { retur
 // LDS of one wave that writes 32 rows.
 constexpr int kWriteLds = 32 * (256 + 16);
 
-// A wave's 32 rows of D values E, f(d, x) of the 4 that a lane holds from dim d on, lane by lane to where its row goes (nullptr: nowhere),
-// turned in LDS so that the stores cover whole rows: a lane's own 8 bytes of 32 rows at a time kept the CU's address unit for
-// 7900 cycles a tile of 256 rows, a sixth of a short one's time; so it takes 2500.
+// A wave's 32 rows of D values E, f of the 4 that a lane holds at a time, to where each lane's row goes (dst; nullptr:
+// nowhere). They are turned in LDS so that the stores cover whole rows: a lane's own 8 bytes of 32 rows at a time kept the
+// CU's address unit for 7900 cycles a tile of 256 rows, so it takes 5500.
 template <typename E, int D, typename W, typename F>
 __device__ __forceinline__ void store_rows(const W& w, char* dst, char* lds, F&& f) {
   constexpr int kBytes = D * (int)sizeof(E) < 256 ? D * (int)sizeof(E) : 256, kPieces = D * (int)sizeof(E) / kBytes, kDims = D / kPieces;
@@ -662,7 +662,8 @@ __device__ __forceinline__ void store_rows(const W& w, char* dst, char* lds, F&&
 
 // One wave writes its 32 rows, through kWriteLds bytes of LDS that no other wave uses: to the output, or as a part.
 template <typename T, int D>
-__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, char* lds, int row, float* po, f32x2* pml, bool sees) {
+__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, char* lds, int row, float* po,
+                                           f32x2* pml, bool sees) {
   const float l = w.core.row_sum();
   if (po) {
     store_rows<float, D>(w, row < u.rows ? (char*)po : nullptr, lds, [](const f32x4& x) { return x; });
@@ -759,8 +760,8 @@ __device__ __forceinline__ bool item_of(const AttnParams& P, const int32_t* item
   const int32_t* it = items + kItemWords * (int64_t)blockIdx.x;
   const int q0 = it[0], n_new = it[1], len = it[2], row0 = it[3], kvh = it[4], slot = it[5];
   const int64_t start = (int64_t)(((uint64_t)(uint32_t)it[7] << 32) | (uint32_t)it[6]);
-  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 || len > kItemMaxLen || start < 0 ||
-      start > P.kv_rows - len || row0 >= n_new * P.group || slot >= n_parts) return false;
+  if (q0 < 0 || n_new <= 0 || row0 < 0 || kvh < 0 || kvh >= P.hkv || q0 + (int64_t)n_new > P.n_tokens || len < 0 ||
+      len > kItemMaxLen || start < 0 || start > P.kv_rows - len || row0 >= n_new * P.group || slot >= n_parts) return false;
   x.u = Unit{P.k.p + start * P.k.row + kvh * P.k.head, P.v.p + start * P.v.row + kvh * P.v.head, len, len - n_new + 1, q0,
              n_new * P.group, row0, kvh};
   x.slot = slot;
