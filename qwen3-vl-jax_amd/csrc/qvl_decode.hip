@@ -37,6 +37,7 @@ struct DecodeState {
   int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // with prefixes: parts of so many keys each
   SplitJob* split;                                                      // streaming: [runs]
   int slot_rows;                                                        // streaming: rows a part's slot has
+  int tile;                                                             // rows of a tile: 32, or 16 (FewWave)
 };
 
 // A barrier for what lies in LDS alone: __syncthreads also waits until stores to memory are through (3 us of a launch of 20).
@@ -47,25 +48,25 @@ template <typename T, int D> constexpr int kJoinBytes = 4 * 32 * (D * 4 + 16);
 
 // The four waves' results of the same rows joined in LDS and written: to the output, or as
 // a part, row r of which is row at(r) of the part buffers. `ka`: the first key of the range the waves covered.
-template <typename T, int D, typename F>
-__device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int first_row, int ka,
-                                           bool part, F&& at) {
+template <typename T, int D, typename W, typename F>
+__device__ __forceinline__ void join_waves(const AttnParams& P, const Unit& u, W& w, char* smem, int first_row, int ka, bool part,
+                                           F&& at) {
   // Rows of kPitch bytes: 16 more than a row, so that neither rows nor chunks meet in a bank and every address is one lane's
   // base and a constant (each line of code that runs once costs a workgroup some 800 cycles of fetching it).
   constexpr int kC = D / 4, kPitch = D * 4 + 16, kWave = kJoinBytes<T, D> / 4;
   __shared__ float sm[4][32], sl[4][32];
   __shared__ int slim[32];
-  const int lane = threadIdx.x & 63, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = min(32, u.rows - first_row);
+  const int lane = threadIdx.x & 63, lr = lane & (W::kRows - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = min(W::kRows, u.rows - first_row);
   const float lw = w.core.row_sum();
-  if (lane < 32) {
-    sm[wave][l32] = w.m;
-    sl[wave][l32] = lw;
-    slim[l32] = w.lim;
+  if (lane < W::kRows) {
+    sm[wave][lr] = w.m;
+    sl[wave][lr] = lw;
+    slim[lr] = w.lim;
   }
   lds_barrier();                               // every wave is past its tiles
-  if (l32 < n) {
-    char* row = smem + wave * kWave + l32 * kPitch;
+  if (lr < n) {
+    char* row = smem + wave * kWave + lr * kPitch;
     w.core.each4([&](int d, const f32x4& x) { *reinterpret_cast<f32x4*>(row + d * 4) = x; });
   }
   lds_barrier();
@@ -112,7 +113,7 @@ __device__ __forceinline__ bool bad_keys(const AttnParams& P, int64_t start, int
 // ---------------------------------------------------------------------------------------------
 // streaming
 // ---------------------------------------------------------------------------------------------
-// What the line holds of a sequence: its jobs (tiles of 32 rows), and the blocks of 32 keys of each, one where there is
+// What the line holds of a sequence: its jobs (tiles of S.tile rows), and the blocks of 32 keys of each, one where there is
 // nothing to read, for the rows' zeros (or NaN).
 struct Sequence {
   int64_t token0, start;
@@ -124,7 +125,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttnParams& P, const Decod
   q.tokens = (int)tokens_of(P, S, seq, seq + 1, q.token0);
   q.start = S.k_start[seq];
   q.len = S.k_len[seq];
-  q.jobs = (int)(((int64_t)q.tokens * P.group + 31) / 32);
+  q.jobs = (int)(((int64_t)q.tokens * P.group + S.tile - 1) / S.tile);
   q.blocks = bad_keys(P, q.start, q.len) ? 1 : max((q.len + 31) >> 5, 1);
   return q;
 }
@@ -266,8 +267,8 @@ __device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState&
   q = uniform(sequence_of(P, S, seq));
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, DecodeState S) {
+template <typename T, int D, typename W>
+__device__ __forceinline__ void decode_stream(const AttnParams& P, const DecodeState& S) {
   using K = KeysUnit<T, D>;
   __shared__ __attribute__((aligned(16))) char smem[std::max(K::kLds, kJoinBytes<T, D>)];
   __shared__ Line L;
@@ -297,10 +298,10 @@ __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, Dec
     }
     const int b1 = (int)min((int64_t)blocks, b0 + (end - pos));
     u.kvh = kvh;
-    u.row0 = job * 32;
+    u.row0 = job * W::kRows;
     u.rows = q.tokens * P.group;
     u.lim0 = u.len - q.tokens + 1;
-    const int n_rows = min(32, u.rows - u.row0);
+    const int n_rows = min(W::kRows, u.rows - u.row0);
     const bool whole = b0 == 0 && b1 == blocks, bad = bad_keys(P, start, u.len);
     if (bad) {
       for (int i = threadIdx.x; i < n_rows * (D / 4); i += 256)
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, Dec
     } else {
       u.k = P.k.p + start * P.k.row + u.kvh * P.k.head;
       u.v = P.v.p + start * P.v.row + u.kvh * P.v.head;
-      Wave<T, D> w;
+      W w;
       w.init(P, u, u.row0);
       K::run(P, u, w, smem, b0, min(b1, (u.len + 31) >> 5));
       const int64_t slot = ((int64_t)(2 * run + (b0 == 0)) * P.hkv + kvh) * S.slot_rows;
@@ -326,6 +327,10 @@ __global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, Dec
   }
   if (threadIdx.x == 0 && kvh == 0) S.split[run] = joined;
 }
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void decode_stream_kernel(AttnParams P, DecodeState S) { decode_stream<T, D, Wave<T, D>>(P, S); }
+template <int D>
+__global__ __launch_bounds__(256, 2) void decode_stream_few_kernel(AttnParams P, DecodeState S) { decode_stream<float, D, FewWave<D>>(P, S); }
 
 // Part p of a split job: the second slot of its first run (the job begins inside it), the first slot of each later one.
 template <typename T, int D>
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(256) void decode_stream_join_kernel(AttnParams P, D
   if (j.parts == 0) return;
   const int kvh = blockIdx.y;
   const Unit u{nullptr, nullptr, 0, 0, j.token0, j.rows, j.row0, kvh};
-  const int n = min(32, j.rows - j.row0), per = (n + gridDim.z - 1) / gridDim.z, r0 = blockIdx.z * per;
+  const int n = min(S.tile, j.rows - j.row0), per = (n + gridDim.z - 1) / gridDim.z, r0 = blockIdx.z * per;
   join_parts<T, D>(P, r0, min(r0 + per, n), j.parts,
                    [&](int r, int p) { return ((int64_t)(2 * (j.first + p) + (p == 0)) * P.hkv + kvh) * S.slot_rows + r; },
                    [&](int r) { return out_row<T, D>(P, u, j.row0 + r); });
@@ -354,10 +359,10 @@ __device__ __forceinline__ void write_fixed(const AttnParams& P, const Unit& u, 
   for (int r = threadIdx.x; r < u.rows; r += 256) P.part_ml[part_row(P, u, part, r)] = f32x2{value == 0.f ? -INFINITY : value, value};
 }
 
-// Workgroups [0, prefix units): a part of a group's prefix for a tile of the group's rows (ROWS: tiles of 128, else of 32);
+// Workgroups [0, prefix units): a part of a group's prefix for a tile of the group's rows (ROWS: tiles of 128, else of W's);
 // the others: a part of a sequence's own keys for its rows. The key/value head runs fastest, then the part, so that the
 // tiles of one part of the prefix meet in one L2 where heads x parts fill the 8 XCDs evenly.
-template <typename T, int D, bool ROWS>
+template <typename T, int D, typename W, bool ROWS>
 __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeState& S) {
   using R = RowsUnit<T, D>;
   using K = KeysUnit<T, D>;
@@ -411,9 +416,9 @@ __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeSta
       __syncthreads();                         // the tiles may be written again
     }
   } else {
-    const int step = own ? 32 : S.prefix_tiles * 32;
-    for (int row0 = tile0 * 32; row0 < u.rows; row0 += step) {
-      Wave<T, D> w;
+    const int step = own ? W::kRows : S.prefix_tiles * W::kRows;
+    for (int row0 = tile0 * W::kRows; row0 < u.rows; row0 += step) {
+      W w;
       w.init(P, u, row0);
       K::run(P, u, w, smem, ka / 32, (kb + 31) / 32);
       join_waves<T, D>(P, u, w, smem, row0, ka, true, [&](int r) { return part_row(P, u, part, row0 + r); });
@@ -422,9 +427,11 @@ __device__ __forceinline__ void prefix_unit(const AttnParams& P, const DecodeSta
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void prefix_rows_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, true>(P, S); }
+__global__ __launch_bounds__(256, 2) void prefix_rows_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, Wave<T, D>, true>(P, S); }
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void prefix_keys_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, false>(P, S); }
+__global__ __launch_bounds__(256, 2) void prefix_keys_kernel(AttnParams P, DecodeState S) { prefix_unit<T, D, Wave<T, D>, false>(P, S); }
+template <int D>
+__global__ __launch_bounds__(256, 2) void prefix_few_kernel(AttnParams P, DecodeState S) { prefix_unit<float, D, FewWave<D>, false>(P, S); }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_join_kernel(AttnParams P, DecodeState S) {
@@ -447,7 +454,8 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(AttnParams P, DecodeSt
 struct DecodePlan {
   int runs, slot_rows;                                                  // streaming
   int own_parts, own_chunk, prefix_parts, prefix_chunk, prefix_tiles;   // with prefixes
-  bool prefix_rows;
+  bool prefix_rows, few;   // with prefixes: tiles of 128 rows; fp32: tiles of 16 rows
+  int tile;
   int64_t units;
   size_t part_rows, split_bytes;
 };
@@ -473,23 +481,29 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   // workgroups a GPU holds: two a CU, one where the tiles take 128 KB (fp32, head_dim 128)
   const int64_t cus = gemm_device_cus(), slots = cus * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
   D = DecodePlan{};
+  // fp32 is bound by its matrix products (32 rows: 8192 cycles a block of 32 keys), so few rows take tiles of 16: 16/8 heads of
+  // 128, 96 sequences of up to 5700 keys 396 us, not 473 (2.2 GB: 5.7 TB/s), one of 9000 25, not 31; 18 sequences after
+  // prefixes of 2000 to 4000 keys, 3 tokens each, 31, not 45
+  const int64_t own_rows = (rows + std::max<int64_t>(n_seqs, 1) - 1) / std::max<int64_t>(n_seqs, 1);   // a sequence's, in the mean
+  D.few = dtype == QVL_DTYPE_F32 && own_rows <= 16 && (n_groups == 0 || rows <= 16 * n_groups);
+  D.tile = D.few ? 16 : 32;
   if (n_groups == 0) {
     // A run for each compute unit where that leaves it at most 40 blocks, else for each slot (8 heads: one sequence of 9001 keys
     // 19 us and not 24, of 31000 32.5 and not 34.5; 16 of up to 8000 61.6 and not 69); no more than give each wave a block,
     // nor fewer than there are jobs.
-    const int64_t tiles = std::max<int64_t>((rows + 32 * n_seqs - 1) / (32 * std::max<int64_t>(n_seqs, 1)), 1);
+    const int64_t tiles = std::max<int64_t>((own_rows + D.tile - 1) / D.tile, 1);
     const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + 31) / 32);
     const int64_t one = cus / num_kv_heads, most = jobs <= one && blocks <= 40 * one ? one : slots / num_kv_heads;
     D.runs = (int)std::max<int64_t>(std::min(most, std::max((blocks + 3) / 4, jobs)), 1);
     D.units = (int64_t)D.runs * num_kv_heads;
-    D.slot_rows = (int)std::min<int64_t>(32, std::max<int64_t>(rows, 1));
+    D.slot_rows = (int)std::min<int64_t>(D.tile, std::max<int64_t>(rows, 1));
     D.part_rows = (size_t)D.units * 2 * D.slot_rows;
     D.split_bytes = round_up(D.runs * sizeof(SplitJob), 16);
     return QVL_OK;
   }
   const int64_t mean = (rows + n_groups - 1) / n_groups;
   D.prefix_rows = mean > 32;
-  const int64_t tile = D.prefix_rows ? kItemRows : 32;
+  const int64_t tile = D.prefix_rows ? kItemRows : D.tile;
   D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
   D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
   // one unit on the prefixes for each compute unit, beside units on the sequences' own keys (one for each slot: 192 rows
@@ -500,6 +514,12 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   D.part_rows = (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads;
   return QVL_OK;
 }
+
+#define QVL_FEW_LAUNCH(KERNEL, GRID, ...)                                                                        \
+  do {                                                                                                           \
+    if (head_dim == 128) hipLaunchKernelGGL((KERNEL<128>), GRID, dim3(256), 0, (hipStream_t)stream, __VA_ARGS__); \
+    else hipLaunchKernelGGL((KERNEL<64>), GRID, dim3(256), 0, (hipStream_t)stream, __VA_ARGS__);                 \
+  } while (0)
 
 static size_t workspace_bytes_of(const DecodePlan& D, int32_t head_dim) {
   return D.split_bytes + D.part_rows * ((size_t)head_dim + 2) * sizeof(float);
@@ -550,10 +570,11 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
   P.part_o = (float*)((char*)workspace + plan.split_bytes);
   P.part_ml = (f32x2*)(P.part_o + plan.part_rows * head_dim);
   const DecodeState S{cu_q, k_start, k_len, cu_groups, prefix_start, prefix_len, (int)n_seqs, (int)n_groups, plan.own_parts,
-                      plan.own_chunk, plan.prefix_parts, plan.prefix_chunk, plan.prefix_tiles, (SplitJob*)workspace, plan.slot_rows};
+                      plan.own_chunk, plan.prefix_parts, plan.prefix_chunk, plan.prefix_tiles, (SplitJob*)workspace, plan.slot_rows, plan.tile};
   const dim3 units((unsigned)plan.units);
   if (n_groups == 0) {
-    QVL_ATTN_LAUNCH(decode_stream_kernel, units, P, S);
+    if (plan.few) QVL_FEW_LAUNCH(decode_stream_few_kernel, units, P, S);
+    else QVL_ATTN_LAUNCH(decode_stream_kernel, units, P, S);
     QVL_TRY_RC(check_launch("decode_stream"));
     if (plan.runs == 1) return QVL_OK;
     // a split job's rows over a few workgroups: they are few, and each reads every part
@@ -561,6 +582,7 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
     return check_launch("decode_stream_join");
   }
   if (plan.prefix_rows) QVL_ATTN_LAUNCH(prefix_rows_kernel, units, P, S);
+  else if (plan.few) QVL_FEW_LAUNCH(prefix_few_kernel, units, P, S);
   else QVL_ATTN_LAUNCH(prefix_keys_kernel, units, P, S);
   QVL_TRY_RC(check_launch("prefix_attention"));
   const int64_t per = 256 / (head_dim / 4) / join_split(plan.prefix_parts + plan.own_parts);

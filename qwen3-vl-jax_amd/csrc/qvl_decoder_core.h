@@ -51,7 +51,7 @@ __device__ __forceinline__ float across_halves(float x) {
 template <typename T, int D> struct Core;
 
 template <int D> struct Core<bf16, D> {
-  static constexpr int kRowBytes = D * 2, kDB = D / 32;
+  static constexpr int kRows = 32, kRowBytes = D * 2, kDB = D / 32;
   static constexpr int kChunks = kRowBytes / 16;
   bf16x8 q[D / 16];
   f32x16 o[kDB];
@@ -251,7 +251,7 @@ template <int D> struct Core<bf16, D> {
 // is read 16 bytes at a time; a lane of V^T takes the dims kDB i + db of its row i, which lie together in V's row: one
 // read serves all of a key's output blocks. P needs no packing.
 template <int D> struct Core<float, D> {
-  static constexpr int kRowBytes = D * 4, kDB = D / 32;
+  static constexpr int kRows = 32, kRowBytes = D * 4, kDB = D / 32;
   static constexpr int kChunks = kRowBytes / 16;
   f32x4 q[D / 8];
   f32x16 o[kDB];
@@ -369,24 +369,46 @@ struct Unit {
   int rows, row0, kvh;
 };
 
-// The online softmax of one wave: 32 rows over the keys it is given.
-template <typename T, int D> struct Wave {
-  Core<T, D> core;
+// The rows of one wave, one a lane (and more lanes of the same row), and what they see.
+template <typename C> struct RowState {
+  static constexpr int kRows = C::kRows;
+  C core;
   float m;             // running maximum of the lane's row, in powers of two; -inf before the first key it sees
   int lim, lim_lo;     // keys the lane's row sees; the fewest any row of the wave does
   int lim_hi;          // the most
 
   __device__ __forceinline__ void init(const AttnParams& P, const Unit& u, int first_row) {
-    const int row = min(first_row + (int)(threadIdx.x & 31), u.rows - 1);
+    const int row = min(first_row + (int)(threadIdx.x & (kRows - 1)), u.rows - 1);
     const int t = (int)((uint32_t)row / (uint32_t)P.group), g = row - t * P.group;
     const char* q = P.q.p + (u.token0 + t) * P.q.row + (int64_t)(u.kvh * P.group + g) * P.q.head;
     lim = max(min(u.lim0 + t, u.len), 0);
-    const int lo = min(first_row, u.rows - 1), hi = min(first_row + 31, u.rows - 1);
+    const int lo = min(first_row, u.rows - 1), hi = min(first_row + kRows - 1, u.rows - 1);
     lim_lo = max(min(u.lim0 + (int)((uint32_t)lo / (uint32_t)P.group), u.len), 0);
     lim_hi = max(min(u.lim0 + (int)((uint32_t)hi / (uint32_t)P.group), u.len), 0);
     m = -INFINITY;
     core.init(q);
   }
+  // The maximum moved to cover mx, the largest score of a step (times the scale). It moves only where it grew by more than
+  // 2^8: until then weights of up to 2^8 lose nothing (fp32 sums, and bf16 weights of the same relative rounding), and the
+  // accumulators need no pass. Row by row, so that a row's result does not depend on the others of its wave.
+  __device__ __forceinline__ void cover(float mx) {
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+      const float mn = mx > m + 8.f ? mx : m;
+      // (nothing to rescale before a row's first key)
+      if (__builtin_amdgcn_ballot_w64(m != -INFINITY) != 0) core.rescale(__builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn)));
+      m = mn;
+    }
+  }
+  __device__ __forceinline__ float shift() const { return m == -INFINITY ? 0.f : -m; }
+};
+
+// The online softmax of one wave: 32 rows over the keys it is given.
+template <typename T, int D> struct Wave : RowState<Core<T, D>> {
+  using RowState<Core<T, D>>::core;
+  using RowState<Core<T, D>>::m;
+  using RowState<Core<T, D>>::lim;
+  using RowState<Core<T, D>>::lim_lo;
+
   // Scores of 32 keys from kb on that the lane's row does not see become -inf; returns which it sees, a bit per register.
   __device__ __forceinline__ uint32_t mask(f32x16& s, int kb) const {
     const int base = lim - kb - 4 * (int)((threadIdx.x & 63) >> 5);
@@ -432,16 +454,8 @@ template <typename T, int D> struct Wave {
         for (int r = b ? 0 : 4; r < 16; r += 4) m4[c] = fmaxf(m4[c], s[b][r + c]);
     }
     const float mx = across_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * scale;
-    // A row's maximum moves only where it grew by more than 2^8: until then weights of up to 2^8 lose nothing (fp32 sums,
-    // and bf16 weights of the same relative rounding), and the accumulators need no pass. Row by row, so that a row's result
-    // does not depend on the others of its wave.
-    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-      const float mn = mx > m + 8.f ? mx : m;
-      // (nothing to rescale before a row's first key)
-      if (__builtin_amdgcn_ballot_w64(m != -INFINITY) != 0) core.rescale(__builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn)));
-      m = mn;
-    }
-    const float shift = m == -INFINITY ? 0.f : -m;
+    this->cover(mx);
+    const float shift = this->shift();
     if constexpr (kAhead) {
       core.pv2(vlds, v0, s, scale, shift);
       return;
@@ -466,6 +480,141 @@ template <typename T, int D> struct Wave {
       for (int e = 0; e < 4; ++e) ok = ok & (fabsf(x[e]) < INFINITY);
     });
     return ok;
+  }
+};
+
+// fp32 and at most 16 rows, on v_mfma_f32_16x16x4_f32: half the products of a tile of 32 rows, 4096 cycles a block of 32 keys
+// at head_dim 128. A row has four lanes (column lane % 16 of S^T = K Q^T); of half b of the block, register r of a lane is
+// key 16 b + 4 (lane / 16) + r. Its lanes take dims 16 j + 4 (lane / 16) + e of K and Q; a lane of V^T takes dims
+// 64 h + 4 (lane % 16) + e. K and V lie in LDS as for Core<float, D>.
+template <int D> struct FewCore {
+  using C = Core<float, D>;
+  static constexpr int kRows = 16, kDB = D / 16;
+  f32x4 q[D / 16], o[kDB];
+  float l;
+
+  static __device__ __forceinline__ int quad() { return (threadIdx.x & 63) >> 4; }
+  static __device__ __forceinline__ int l16() { return threadIdx.x & 15; }
+  __device__ __forceinline__ void init(const char* qrow) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) q[j] = *reinterpret_cast<const f32x4*>(qrow + (j * 16 + quad() * 4) * 4);
+#pragma unroll
+    for (auto& x : o) x = f32x4{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+  }
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (auto& x : q) asm volatile("" : "+v"(x));
+  }
+  __device__ __forceinline__ void scores(const char* lds, f32x4 (&s)[2]) const {
+    s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      f32x4 k[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int row = 16 * b + l16();
+        k[b] = *reinterpret_cast<const f32x4*>(lds + row * C::kRowBytes + (((j * 4 + quad()) ^ C::k_swz(row)) << 4));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][e], q[j][e], s[b], 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ f32x4 v_frag(const char* lds, int b, int r, int h) {
+    return *reinterpret_cast<const f32x4*>(lds + (16 * b + 4 * quad() + r) * C::kRowBytes + (16 * h + l16()) * 16);
+  }
+  __device__ __forceinline__ void pv(const char* lds, const f32x4 (&p)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = p[i >> 2][i & 3];
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        const f32x4 v = v_frag(lds, i >> 2, i & 3, h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], w, o[4 * h + e], 0, 0, 0);
+      }
+      l += w;
+    }
+  }
+  __device__ __forceinline__ void pv_safe(const char* lds, const f32x4 (&p)[2], uint32_t seen) {
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      f32x4 n = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = v_frag(lds, i >> 2, i & 3, db >> 2)[db & 3];
+        const bool ok = fabsf(v) < INFINITY;
+        const float mark = ok ? 0.f : v == INFINITY ? 1.f : v == -INFINITY ? 256.f : 65536.f;
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? v : 0.f, p[i >> 2][i & 3], o[db], 0, 0, 0);
+        n = __builtin_amdgcn_mfma_f32_16x16x4f32(mark, (seen >> i) & 1 ? 1.f : 0.f, n, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t c = (uint32_t)n[r];
+        if (c & 0xffu) o[db][r] += INFINITY;
+        if (c & 0xff00u) o[db][r] -= INFINITY;
+        if (c >> 16) o[db][r] = NAN;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l += p[i >> 2][i & 3];
+  }
+  __device__ __forceinline__ void rescale(float a) {
+#pragma unroll
+    for (auto& x : o) x *= a;
+    l *= a;
+  }
+  __device__ __forceinline__ float row_sum() const {
+    const float two = l + __shfl_xor(l, 16);
+    return two + __shfl_xor(two, 32);
+  }
+  template <typename F> __device__ __forceinline__ void each4(F&& f) const {
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        f(64 * h + 4 * (4 * quad() + r), f32x4{o[4 * h][r], o[4 * h + 1][r], o[4 * h + 2][r], o[4 * h + 3][r]});
+  }
+};
+
+template <int D> struct FewWave : RowState<FewCore<D>> {
+  using RowState<FewCore<D>>::core;
+  using RowState<FewCore<D>>::lim;
+  using RowState<FewCore<D>>::lim_lo;
+
+  // Wave::step for a block of 32 keys
+  template <int NB, bool SAFE, typename F, typename G>
+  __device__ __forceinline__ void step(const char* klds, const char* vlds, int kb, float scale, F&& between, G&& before_v) {
+    static_assert(NB == 1, "a block at a time");
+    f32x4 s[2];
+    core.scores(klds, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) between(i);
+    const bool edge = kb + 32 > lim_lo;
+    uint32_t seen = 0;
+    if (edge) {
+      const int base = lim - kb - 4 * core.quad();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = 16 * (i >> 2) + (i & 3) < base;
+        seen |= (in ? 1u : 0u) << i;
+        s[i >> 2][i & 3] = in ? s[i >> 2][i & 3] : -INFINITY;
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+    mx = across_halves(mx);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    this->cover(mx * scale);
+    const float shift = this->shift();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], scale, shift));
+    before_v();
+    if (SAFE && edge) core.pv_safe(vlds, s, seen);
+    else core.pv(vlds, s);
   }
 };
 
@@ -569,13 +718,14 @@ template <typename T, int D> struct RowsUnit {
   }
 };
 
-// Up to 32 rows a workgroup; the four waves take every fourth block of 32 keys, each through LDS of its own: while a block's
+// Up to 32 rows a workgroup (W: Wave, or FewWave of 16); the four waves take every fourth block of 32 keys, each through LDS of its own: while a block's
 // weights are formed the next block's keys arrive, while its scores are formed the next values do. Joined in LDS at the end.
 template <typename T, int D> struct KeysUnit {
   static constexpr int kTile = 32 * Core<T, D>::kRowBytes, kLds = 4 * 2 * kTile;
   static constexpr int kDmas = kTile / 1024;
 
-  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
+  template <typename W>
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, W& w, char* smem, int t0, int t1) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const char* k = smem + wave * 2 * kTile;
     const uint32_t kl = lds_addr_of(k), vl = kl + kTile;
