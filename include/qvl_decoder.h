@@ -96,8 +96,8 @@ int qvl_causal_attention(void* stream, int32_t dtype,
  * d_cu_groups stays in [0, n_seqs] and d_cu_q in [0, n_tokens], neither ever falling; rows before d_cu_q[0] and from
  * d_cu_q[n_seqs] on are left as they are. A token that sees no key gets zeros. The tokens of a sequence whose keys (or prefix) leave [0, kv_rows) come out NaN; nothing outside is read.
  * max_len and max_prefix are the lengths the launch is laid out for (a captured call's largest); longer ones are still
- * right. The workspace (qvl_decode_workspace_size of the same sizes; 16-byte aligned) holds partial outputs: calls that
- * overlap need one each. */
+ * right. The workspace (qvl_decode_workspace_size of the same sizes, with the same device current; 16-byte aligned) holds
+ * partial outputs: calls that overlap need one each. */
 int qvl_decode_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t max_len, int64_t n_groups, int64_t max_prefix,
                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, size_t* bytes);
 int qvl_decode_attention(void* stream, int32_t dtype,
