@@ -102,24 +102,16 @@ def _word(t, what: str, like, dtype, shape):
     return t.data_ptr()
 
 
-class _On:
-    """The tensors' device made current for a launch (a kernel goes to the current device's stream)."""
+def _elsewhere(device) -> bool:
+    """Whether the tensors lie on another device than the current one: the operator then calls itself with theirs current
+    (a kernel goes to the current device)."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: the decoder operators run on the GPU")
+    return device.index != _torch()._C._cuda_getDevice()
 
-    def __init__(self, device):
-        torch = _torch()
-        if device.type != "cuda":
-            raise ValueError(f"tensors on {device}: the decoder operators run on the GPU")
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-        self.index = device.index
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _torch()._C._cuda_getCurrentRawStream(self.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _stream(device) -> int:
+    return _torch()._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
 
 
 class TextRotary:
@@ -192,10 +184,13 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
         if out_rows == 0:
             raise ValueError("the caches have no rows")
     ko = _heads_view(k_cache, "k_cache", like, Hkv, True)
-    with _On(like[1]) as st:
-        capi.check(capi.load().qvl_qk_norm_rotary(
-            st, _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
-            *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
+    if _elsewhere(like[1]):
+        with torch.cuda.device(like[1]):
+            return qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary, eps=eps, k_cache=None if rows is None else k_cache,
+                                  v_cache=v_cache, rows=rows, q_out=q_out)
+    capi.check(capi.load().qvl_qk_norm_rotary(
+        _stream(like[1]), _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
+        *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
     return q_out, k_cache, v if v_cache is None else v_cache
 
 
@@ -276,11 +271,14 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
     rows = k.shape[0]
     if N < plan.n_tokens or rows < plan.kv_rows:
         raise ValueError(f"{N} tokens and {rows} cache rows; the plan needs {plan.n_tokens} and {plan.kv_rows}")
+    if _elsewhere(like[1]):
+        with _torch().cuda.device(like[1]):
+            return causal_attention(q, k, v, plan, scale=scale, out=out)
     ws = _workspace(plan.workspace_bytes, q)
-    with _On(like[1]) as st:
-        capi.check(capi.load().qvl_causal_attention(
-            st, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
-            plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(), plan.workspace_bytes), "qvl_causal_attention")
+    capi.check(capi.load().qvl_causal_attention(
+        _stream(like[1]), _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
+        plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
+        plan.workspace_bytes), "qvl_causal_attention")
     return out
 
 
@@ -311,12 +309,14 @@ def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
         pl = _word(prefix_len, "prefix_len", like, torch.int32, (n_groups,))
         cg = _word(cu_groups, "cu_groups", like, torch.int32, (n_groups + 1,))
     dt, max_len, max_prefix = _qdtype(like[0]), int(max_len), int(max_prefix)
-    with _On(like[1]) as st:
-        nb = _decode_bytes(like[1].index, N, n_seqs, max_len, n_groups, max_prefix, Hq, Hkv, D, dt)
-        ws = _workspace(nb, q)
-        capi.check(capi.load().qvl_decode_attention(
-            st, dt, *views, rows, cq, n_seqs, ks, kl, max_len, cg, n_groups, ps, pl, max_prefix, _scale(scale, D), *ov, N,
-            Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb), "qvl_decode_attention")
+    if _elsewhere(like[1]):
+        with torch.cuda.device(like[1]):
+            return _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out)
+    nb = _decode_bytes(like[1].index, N, n_seqs, max_len, n_groups, max_prefix, Hq, Hkv, D, dt)
+    ws = _workspace(nb, q)
+    capi.check(capi.load().qvl_decode_attention(
+        _stream(like[1]), dt, *views, rows, cq, n_seqs, ks, kl, max_len, cg, n_groups, ps, pl, max_prefix, _scale(scale, D), *ov, N,
+        Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb), "qvl_decode_attention")
     return out
 
 

@@ -602,6 +602,30 @@ def test_captured_steps_follow_the_lengths(ops, dtype):
         rows += 1
 
 
+def test_called_from_another_device(ops, monkeypatch):
+    """The path that makes the tensors' device current first (taken here by saying so once a call)."""
+    hq, hkv, D = 8, 2, 64
+    q, k, v, seqs = causal_case(hq, hkv, D, BF, [70], [30], seed=41)
+    plan, rot = plan_of(ops, seqs, hq, hkv, D, BF), ops.TextRotary(D, 1e4, (12, 10, 10), True, DEV)
+    w, pos, rows = torch.ones(D, device=DEV), torch.arange(100, dtype=torch.int32, device=DEV), torch.arange(100, device=DEV)
+    start, lens = torch.tensor([seqs[0][2]], device=DEV), torch.tensor([100], dtype=torch.int32, device=DEV)
+
+    def calls():
+        kc, vc = torch.zeros(100, hkv, D, dtype=BF, device=DEV), torch.zeros(100, hkv, D, dtype=BF, device=DEV)
+        n, alone = q.shape[0], ops.qk_norm_rotary(q, k[:q.shape[0]], None, w, w, pos[:q.shape[0]], rot)
+        cached = ops.qk_norm_rotary(q, k[:n], v[:n], w, w, pos[:n], rot, k_cache=kc, v_cache=vc, rows=rows[:n])
+        return [alone[0], alone[1], *cached, ops.causal_attention(q, k, v, plan)[:70],
+                ops.decode_attention(q[:1], k, v, start, lens, max_len=100)]
+
+    want = calls()
+    real, said = ops._elsewhere, []
+    monkeypatch.setattr(ops, "_elsewhere", lambda device: (said.append(1), len(said) % 2 == 1 or real(device))[1])
+    got = calls()
+    assert len(said) == 8
+    for a, b in zip(got, want):
+        assert torch.equal(bits(a), bits(b))
+
+
 def test_two_streams_at_once(ops):
     """The same plan and caches used from two streams that overlap: each call's workspace is its own."""
     hq, hkv, D = 32, 8, 128
