@@ -506,9 +506,11 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   const int64_t tile = D.prefix_rows ? kItemRows : D.tile;
   D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
   D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
-  // one unit on the prefixes for each compute unit, beside units on the sequences' own keys (one for each slot: 192 rows
-  // on 9216 keys 36 us, not 30; 1024 on 24007 145, not 140)
-  D.prefix_parts = split_parts(max_prefix, n_groups * num_kv_heads * D.prefix_tiles, cus, D.prefix_chunk);
+  // About one unit on the prefixes for each compute unit, beside units on the sequences' own keys (one for each slot: 192
+  // rows on 9216 keys 36 us, not 30; 1024 on 24007 145, not 140). Tiles that groups of unlike size may leave empty
+  // count half: twice 1024 rows 231 us, not 328.
+  const int64_t busy = std::min(n_groups * D.prefix_tiles, (rows + tile - 1) / tile + n_groups / 2) * num_kv_heads;
+  D.prefix_parts = split_parts(max_prefix, busy, cus + busy / 8, D.prefix_chunk);
   D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);
   if (D.units > 0x7fffffffLL || n_tokens * num_heads > 0x7fffffffLL) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   D.part_rows = (size_t)(D.prefix_parts + D.own_parts) * n_tokens * num_heads;
