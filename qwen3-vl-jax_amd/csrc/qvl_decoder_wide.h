@@ -13,10 +13,12 @@
 // the tile's first half, so that they are there when it ends.
 //
 // No running maximum: a row's weights are 2^(s - m) with m the largest score of its first tile, whatever comes later, so that
-// the loop has no branch and no pass over the accumulators. fp32 sums lose nothing by that until they overflow, for which
-// some score has to exceed the first 64 by 2^127 in its weight. Then, and where V holds what is not finite, a row's sums are
-// not finite, and the workgroup runs once more: rows whose sum of weights passed 2^30 with their true maximum, and with
-// values that a row does not see kept from it.
+// the loop has no branch and no pass over the accumulators. fp32 sums lose nothing by that until they overflow. A part of a
+// cut tile has to be joined besides: by 2^(m - M), which the exponential makes 0 below 2^-126, so that a sum held against an m
+// so far below the others' M may not be large. Where a row's sum of weights, both its lanes', reaches 2^60 (a later score 41
+// nats above the first 64), or where V holds what is not finite, the workgroup runs once more: rows whose sum passed 2^30
+// with their true maximum, and with values that a row does not see kept from it. What a join then drops is below 2^-66 of the
+// row.
 #pragma once
 #include <algorithm>
 #include <utility>
@@ -37,6 +39,7 @@ template <int D> struct WideUnit {
   static constexpr int kTile = kBN * C::kRowBytes, kDmas = kTile / 1024 / 4, kLds = 3 * 2 * kTile;
   static_assert(kLds >= 4 * kWriteLds, "rows are written through the tiles' LDS");
   static_assert(2 * kDmas == kG, "a DMA beside each product of one group");
+  static constexpr float kMostSum = 0x1p60f;
 
   static __device__ __forceinline__ float shift_of(const W& w) { return w.m == -INFINITY ? 0.f : -w.m; }
   static __device__ __forceinline__ bf16x8 k_frag(const char* k, int b, int ks) {
@@ -233,7 +236,7 @@ template <int D> struct WideUnit {
   }
   static __device__ __forceinline__ void run_all(const AttnParams& P, const Unit& u, W& A, W& B, int row0, char* smem, int t0, int t1) {
     run(P, u, A, B, row0, smem, t0, t1);
-    const bool ok = A.finite() && B.finite() && A.core.l < INFINITY && B.core.l < INFINITY;
+    const bool ok = A.finite() && B.finite() && A.core.row_sum() < kMostSum && B.core.row_sum() < kMostSum;
     if (__builtin_expect(__syncthreads_or(!ok), 0)) run_safe(P, u, A, B, smem, t0, t1);
   }
 };
