@@ -16,9 +16,10 @@
 // the loop has no branch and no pass over the accumulators. fp32 sums lose nothing by that until they overflow. A part of a
 // cut tile has to be joined besides: by 2^(m - M), which the exponential makes 0 below 2^-126, so that a sum held against an m
 // so far below the others' M may not be large. Where a row's sum of weights, both its lanes', reaches 2^60 (a later score 41
-// nats above the first 64), or where V holds what is not finite, the workgroup runs once more: rows whose sum passed 2^30
-// with their true maximum, and with values that a row does not see kept from it. What a join then drops is below 2^-66 of the
-// row.
+// nats above the first 64), where a row's first scores are all -inf (weights without a shift, and a part that counts as empty
+// in a join), or where V holds what is not finite, the workgroup runs once more: rows of the first two kinds, from a sum of
+// 2^30 on, with their true maximum, and with values that a row does not see kept from it. What a join then drops is below
+// 2^-66 of the row.
 #pragma once
 #include <algorithm>
 #include <utility>
@@ -221,8 +222,8 @@ template <int D> struct WideUnit {
       raise(A, B, smem, k0, t * kBN, P.scale);
       __syncthreads();
     }
-    if (la < 0x1p30f) A.m = ma;
-    if (lb < 0x1p30f) B.m = mb;
+    if (la < 0x1p30f && ma != -INFINITY) A.m = ma;
+    if (lb < 0x1p30f && mb != -INFINITY) B.m = mb;
     for (int t = t0; t < t1; ++t) {
       T.load_all(t, 0);
       wait_dma();
@@ -236,7 +237,8 @@ template <int D> struct WideUnit {
   }
   static __device__ __forceinline__ void run_all(const AttnParams& P, const Unit& u, W& A, W& B, int row0, char* smem, int t0, int t1) {
     run(P, u, A, B, row0, smem, t0, t1);
-    const bool ok = A.finite() && B.finite() && A.core.row_sum() < kMostSum && B.core.row_sum() < kMostSum;
+    const auto good = [&](const W& w) { return w.finite() && w.core.row_sum() < kMostSum && (w.m != -INFINITY || w.lim <= t0 * kBN); };
+    const bool ok = good(A) & good(B);
     if (__builtin_expect(__syncthreads_or(!ok), 0)) run_safe(P, u, A, B, smem, t0, t1);
   }
 };

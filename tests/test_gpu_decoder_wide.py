@@ -106,3 +106,22 @@ def test_parts_whose_sums_are_large_together(ops, D, tile_rows):
             k[at, :, 0], k[at, :, 1:] = level, 0.0
             v[at] = 0.25 + 0.125 * p
         check(ops, q, k, v, n, length, tile_rows, joins=True)
+
+
+@pytest.mark.parametrize("tile_rows", [128, 256])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cut", [False, True])
+@pytest.mark.parametrize("level", [0.0, 100.0, -100.0, -126.0, -200.0])
+def test_first_tile_of_scores_of_minus_infinity(ops, D, tile_rows, cut, level):
+    """The first 64 keys hold -inf (a way to take keys out): their scores are -inf, and the later keys lie at any level."""
+    n, length = 130, 1630 if cut else 330
+    q, k, v = inputs(n, length, D, 4)
+    k[:, :, 0] = level
+    k[:64, :, 0] = -math.inf
+    check(ops, q, k, v, n, length, tile_rows, joins=cut, skip=64)
+    # a row that sees keys of score -inf alone has no answer, and touches no other row
+    k[:, :, 0], k[:200, :, 0] = 0.0, -math.inf
+    q, k, v = (x.to(BF).to(DEV) for x in (q, k, v))
+    plan = ops.CausalPlan([n], [230], [0], num_heads=HQ, num_kv_heads=HKV, head_dim=D, dtype=BF, device=DEV, tile_rows=tile_rows)
+    out = ops.causal_attention(q, k, v, plan, scale=math.log(2.0))
+    assert out[:100].isnan().all() and out[100:].isfinite().all()
