@@ -50,6 +50,11 @@ def _device(device):
     return torch.device("cuda", torch.cuda.current_device()) if d.index is None else d
 
 
+def _no_gradient(t, what: str):
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
+
+
 def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool = False):
     """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor, checked against `like`: q's (dtype, device,
     head_dim)."""
@@ -68,8 +73,7 @@ def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool =
         raise ValueError(f"{what}: head_dim {dim}, q has {like[2]}")
     if heads is not None and n != heads:
         raise ValueError(f"{what}: {n} heads, expected {heads}")
-    if t.requires_grad and _torch().is_grad_enabled():
-        raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
+    _no_gradient(t, what)
     # the stride of an axis of one entry is never used: torch may hold any value there
     if rows < 2:
         row = 0
@@ -92,13 +96,14 @@ def _like(q):
 
 
 def _word(t, what: str, like, dtype, shape):
-    """Pointer of a contiguous device tensor of whole numbers beside q."""
+    """Pointer of a contiguous device tensor beside q: whole numbers, or a norm's weights."""
     if t.dtype != dtype:
         raise TypeError(f"{what} is {t.dtype}, expected {dtype}")
     if t.device != like[1]:
         raise ValueError(f"{what} on {t.device}, q on {like[1]}")
     if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
+    _no_gradient(t, what)
     return t.data_ptr()
 
 

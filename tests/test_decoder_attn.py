@@ -268,3 +268,29 @@ def test_python_refusals_on_the_cpu(pkg):
                                                                   "factor": 2.0}}})
     with pytest.raises(ValueError, match="factor"):
         ops.TextRotary.from_spec(spec.text, device="cpu")
+
+
+def rotary_call(pkg, torch, **a):
+    """qk_norm_rotary on CPU tensors: past its own checks it ends at the refusal of the device."""
+    ops = pkg.decoder_attn
+    rot = ops.TextRotary.__new__(ops.TextRotary)
+    rot.head_dim, rot.table = 64, torch.zeros(32, 2, dtype=torch.int64)
+    z = lambda *shape: torch.zeros(*shape)
+    t = dict(q=z(3, 8, 64), k=z(3, 2, 64), v=z(3, 2, 64), q_norm=z(64), k_norm=z(64), k_cache=z(9, 2, 64), v_cache=z(9, 2, 64))
+    t.update(a)
+    return ops.qk_norm_rotary(t["q"], t["k"], t["v"], t["q_norm"], t["k_norm"], torch.zeros(3, dtype=torch.int32), rot,
+                              k_cache=t["k_cache"], v_cache=t["v_cache"], rows=torch.arange(3), q_out=t.get("q_out"))
+
+
+@pytest.mark.parametrize("name,shape", [("q", (3, 8, 64)), ("k", (3, 2, 64)), ("v", (3, 2, 64)), ("q_norm", (64,)), ("k_norm", (64,)),
+                                        ("k_cache", (9, 2, 64)), ("v_cache", (9, 2, 64)), ("q_out", (3, 8, 64))])
+def test_gradients_of_every_input_are_refused(pkg, name, shape):
+    """The norms' weights above all: they are a model's parameters, and would get no gradient without a word."""
+    torch = pytest.importorskip("torch")
+    learned = torch.nn.Parameter(torch.zeros(shape))
+    with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+        rotary_call(pkg, torch, **{name: learned})
+    with torch.no_grad(), pytest.raises(ValueError, match="run on the GPU"):
+        rotary_call(pkg, torch, **{name: learned})
+    with pytest.raises(ValueError, match="run on the GPU"):
+        rotary_call(pkg, torch, **{name: learned.detach()})
