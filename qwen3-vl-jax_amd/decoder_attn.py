@@ -14,7 +14,7 @@ tensors [rows, heads, head_dim] (any row and head strides of whole 16 bytes), fl
 
 Everything runs on the tensors' device and its current stream; nothing synchronises. Workspaces come from torch's
 allocator with every call, so calls on several streams and captured graphs share none. No operator has a gradient: a tensor
-that requires one is refused while gradients are recorded.
+that requires one is refused while gradients are recorded, and one that carries a forward-mode tangent always.
 """
 from __future__ import annotations
 
@@ -31,6 +31,12 @@ from . import capi
 def _torch():
     import torch
     return torch
+
+
+@functools.lru_cache(maxsize=None)
+def _forward_ad():
+    import torch.autograd.forward_ad
+    return torch.autograd.forward_ad
 
 
 def _qdtype(dtype):
@@ -53,6 +59,9 @@ def _device(device):
 def _no_gradient(t, what: str):
     if t.requires_grad and _torch().is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
+    fa = _forward_ad()
+    if fa._current_level >= 0 and fa.unpack_dual(t).tangent is not None:      # (-1: no dual_level is entered)
+        raise ValueError(f"{what} carries a tangent: the decoder operators have no forward-mode gradient")
 
 
 def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool = False):

@@ -294,3 +294,18 @@ def test_gradients_of_every_input_are_refused(pkg, name, shape):
         rotary_call(pkg, torch, **{name: learned})
     with pytest.raises(ValueError, match="run on the GPU"):
         rotary_call(pkg, torch, **{name: learned.detach()})
+
+
+@pytest.mark.parametrize("name,shape", [("q", (3, 8, 64)), ("v", (3, 2, 64)), ("k_norm", (64,)), ("k_cache", (9, 2, 64))])
+def test_forward_gradients_are_refused(pkg, name, shape):
+    """A tangent of forward-mode differentiation would be dropped; its tensor does not say that it requires a gradient."""
+    torch = pytest.importorskip("torch")
+    import torch.autograd.forward_ad as fa
+    with fa.dual_level():
+        dual = fa.make_dual(torch.zeros(shape), torch.ones(shape))
+        with pytest.raises(ValueError, match=f"{name} carries a tangent"):
+            rotary_call(pkg, torch, **{name: dual})
+        with pytest.raises(ValueError, match="run on the GPU"):                  # others beside it are no matter
+            rotary_call(pkg, torch, **{name: fa.unpack_dual(dual).primal})
+    with pytest.raises(ValueError, match="run on the GPU"):
+        rotary_call(pkg, torch)
