@@ -128,9 +128,23 @@ def _stream(device) -> int:
     return _torch()._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
 
 
+def _streams_of(device) -> set:
+    """The streams that torch's allocator knows a tensor made now to be used on: the current one."""
+    return {_stream(device)}
+
+
+def _read_on(t, streams: set, stream: int):
+    """t, of an object that may go before the kernel that reads it has run, is read on `stream`: its memory is not handed out
+    again before that work is through."""
+    if stream not in streams:
+        t.record_stream(_torch().cuda.current_stream(t.device))
+        streams.add(stream)
+
+
 class TextRotary:
     """The rotation of `qk_norm_rotary`: frequencies theta^(-2j/head_dim), j < head_dim/2, each following the t, h or w
-    position (`section`: how many follow which, one axis after the other or interleaved)."""
+    position (`section`: how many follow which, one axis after the other or interleaved). Like a CausalPlan, it has to
+    outlive the graphs that captured a call with it."""
 
     def __init__(self, head_dim: int, theta: float, section: Sequence[int], interleaved: bool = True, device="cuda"):
         torch = _torch()
@@ -143,6 +157,7 @@ class TextRotary:
         capi.check(capi.load().qvl_text_rotary_table(self.head_dim, self.theta, sec, int(self.interleaved),
                                                      table.ctypes.data), "qvl_text_rotary_table")
         self.table = torch.from_numpy(table.view(np.int64)).to(_device(device))
+        self._streams = _streams_of(self.table.device)
 
     @classmethod
     def from_spec(cls, text, device="cuda"):
@@ -202,8 +217,10 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
         with torch.cuda.device(like[1]):
             return qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary, eps=eps, k_cache=None if rows is None else k_cache,
                                   v_cache=v_cache, rows=rows, q_out=q_out)
+    stream = _stream(like[1])
+    _read_on(table, rotary._streams, stream)
     capi.check(capi.load().qvl_qk_norm_rotary(
-        _stream(like[1]), _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
+        stream, _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
         *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
     return q_out, k_cache, v if v_cache is None else v_cache
 
@@ -211,7 +228,8 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
 class CausalPlan:
     """The work list of `causal_attention` for one packed prefill: sequence i brings q_lens[i] new tokens and has k_lens[i]
     keys (default q_lens), the new ones among them, in cache rows from k_starts[i] (default: one sequence after the other).
-    Made on the host once and used by every layer. tile_rows: 0, or the kernel's tile height (128, or 256 in bfloat16)."""
+    Made on the host once and used by every layer, on any stream. A graph that captured a call reads the list at every
+    replay: the plan has to outlive it. tile_rows: 0, or the kernel's tile height (128, or 256 in bfloat16)."""
 
     def __init__(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None,
                  k_starts: Optional[Sequence[int]] = None, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype,
@@ -248,6 +266,7 @@ class CausalPlan:
                    "qvl_causal_workspace_size")
         self.workspace_bytes = nb.value
         self.items = torch.from_numpy(items).to(device)
+        self._streams = _streams_of(device)
 
 
 def _attention_views(q, k, v, out, like):
@@ -289,8 +308,10 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
         with _torch().cuda.device(like[1]):
             return causal_attention(q, k, v, plan, scale=scale, out=out)
     ws = _workspace(plan.workspace_bytes, q)
+    stream = _stream(like[1])
+    _read_on(plan.items, plan._streams, stream)
     capi.check(capi.load().qvl_causal_attention(
-        _stream(like[1]), _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
+        stream, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
         plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
         plan.workspace_bytes), "qvl_causal_attention")
     return out

@@ -309,3 +309,40 @@ def test_forward_gradients_are_refused(pkg, name, shape):
             rotary_call(pkg, torch, **{name: fa.unpack_dual(dual).primal})
     with pytest.raises(ValueError, match="run on the GPU"):
         rotary_call(pkg, torch)
+
+
+class Recorded:
+    """Stands for a device tensor that an object of the package owns."""
+    def __init__(self, device):
+        self.device, self.streams = device, []
+
+    def data_ptr(self):
+        return FAKE
+
+    def record_stream(self, stream):
+        self.streams.append(stream)
+
+
+def test_lists_and_tables_outlive_the_streams_they_are_used_on(pkg, monkeypatch):
+    """The memory of a plan's list and of a rotation's table belongs to the stream that they were made on: torch's allocator has
+    to hear of every other stream that reads them, or hands it out again while a kernel there still waits. (Nothing is launched.)"""
+    torch = pytest.importorskip("torch")
+    ops = pkg.decoder_attn
+    now, cpu = [7], torch.device("cpu")
+    monkeypatch.setattr(ops, "_elsewhere", lambda device: False)
+    monkeypatch.setattr(ops, "_stream", lambda device: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: ("stream", now[0]))
+    monkeypatch.setattr(pkg.capi, "load", lambda: type("Lib", (), {"__getattr__": lambda self, name: lambda *a: 0})())
+    plan = ops.CausalPlan.__new__(ops.CausalPlan)
+    plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype, plan.device = 8, 2, 64, torch.float32, cpu
+    plan.n_tokens, plan.kv_rows, plan.tile_rows, plan.n_items, plan.n_parts, plan.n_joins = 3, 3, 128, 2, 0, 0
+    plan.workspace_bytes, plan.items = 0, Recorded(cpu)
+    plan._streams = {7}
+    rot = ops.TextRotary.__new__(ops.TextRotary)
+    rot.head_dim, rot.table, rot._streams = 64, Recorded(cpu), {7}
+    q, k, w = torch.zeros(3, 8, 64), torch.zeros(3, 2, 64), torch.zeros(64)
+    for step, want in [(7, []), (9, [9]), (7, [9]), (9, [9]), (11, [9, 11])]:
+        now[0] = step
+        ops.causal_attention(q, k, k, plan)
+        ops.qk_norm_rotary(q, k, None, w, w, torch.zeros(3, dtype=torch.int32), rot)
+        assert plan.items.streams == rot.table.streams == [("stream", s) for s in want], step
