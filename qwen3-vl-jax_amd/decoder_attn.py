@@ -128,6 +128,11 @@ def _stream(device) -> int:
     return _torch()._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
 
 
+def _written(*tensors):
+    """The kernels write through pointers: autograd's check of what other operations saved looks at the tensors' versions."""
+    _torch()._C._increment_version(tensors)                       # torch.autograd.graph.increment_version, of a tuple
+
+
 def _streams_of(device) -> set:
     """The streams that torch's allocator knows a tensor made now to be used on: the current one."""
     return {_stream(device)}
@@ -222,6 +227,7 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
     capi.check(capi.load().qvl_qk_norm_rotary(
         stream, _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
         *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
+    _written(q_out, k_cache) if v_cache is None else _written(q_out, k_cache, v_cache)
     return q_out, k_cache, v if v_cache is None else v_cache
 
 
@@ -314,6 +320,7 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
         stream, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
         plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
         plan.workspace_bytes), "qvl_causal_attention")
+    _written(out)
     return out
 
 
@@ -352,6 +359,7 @@ def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
     capi.check(capi.load().qvl_decode_attention(
         _stream(like[1]), dt, *views, rows, cq, n_seqs, ks, kl, max_len, cg, n_groups, ps, pl, max_prefix, _scale(scale, D), *ov, N,
         Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb), "qvl_decode_attention")
+    _written(out)
     return out
 
 

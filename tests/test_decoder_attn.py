@@ -346,3 +346,41 @@ def test_lists_and_tables_outlive_the_streams_they_are_used_on(pkg, monkeypatch)
         ops.causal_attention(q, k, k, plan)
         ops.qk_norm_rotary(q, k, None, w, w, torch.zeros(3, dtype=torch.int32), rot)
         assert plan.items.streams == rot.table.streams == [("stream", s) for s in want], step
+
+
+def test_written_tensors_count_as_changed(pkg, monkeypatch):
+    """Autograd keeps what another operation saved for its backward pass, and looks at the version of it: a cache that a decoder
+    operator wrote to in between must not pass as unchanged. (Nothing is launched.)"""
+    torch = pytest.importorskip("torch")
+    ops = pkg.decoder_attn
+    monkeypatch.setattr(ops, "_elsewhere", lambda device: False)
+    monkeypatch.setattr(ops, "_stream", lambda device: 7)
+    monkeypatch.setattr(pkg.capi, "load", lambda: type("Lib", (), {"__getattr__": lambda self, name: lambda *a: 0})())
+    rot = ops.TextRotary.__new__(ops.TextRotary)
+    rot.head_dim, rot.table, rot._streams = 64, Recorded(torch.device("cpu")), {7}
+    plan = ops.CausalPlan.__new__(ops.CausalPlan)
+    plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype, plan.device = 8, 2, 64, torch.float32, torch.device("cpu")
+    plan.n_tokens, plan.kv_rows, plan.tile_rows, plan.n_items, plan.n_parts, plan.n_joins = 3, 3, 128, 2, 0, 0
+    plan.workspace_bytes, plan.items, plan._streams = 0, Recorded(torch.device("cpu")), {7}
+    q, k, v, w = torch.zeros(3, 8, 64), torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), torch.zeros(64)
+    kc, vc, out = torch.zeros(9, 2, 64), torch.zeros(9, 2, 64), torch.zeros(3, 8, 64)
+    pos, start, n = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.int32)
+
+    learned = torch.zeros(9, 2, 64, requires_grad=True)
+    loss = (learned * kc).sum()                                      # saves kc
+    ops.qk_norm_rotary(q, k, v, w, w, pos, rot, k_cache=kc, v_cache=vc, rows=start, q_out=out)
+    assert (kc._version, vc._version, out._version) == (1, 1, 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    ops.qk_norm_rotary(q, k, None, w, w, pos, rot, q_out=q)
+    assert (q._version, k._version) == (1, 0)
+    ops.causal_attention(q, k, v, plan, out=out)
+    assert out._version == 2
+    ops.decode_attention(q, kc, vc, start, n, max_len=9, out=out)
+    assert out._version == 3
+    ops.prefix_attention(q, kc, vc, start, n, start[:1], n[:1], n[:2], max_len=9, max_prefix=9, out=out)
+    assert out._version == 4
+    assert (k._version, v._version, kc._version, vc._version, w._version) == (0, 0, 1, 1, 0)
+    with torch.inference_mode():                                     # tensors without a version
+        made = torch.zeros(3, 8, 64)
+        ops.decode_attention(q, kc, vc, start, n, max_len=9, out=made)
