@@ -583,7 +583,9 @@ int qvl_decode_attention(void* stream, int32_t dtype, const void* q, int64_t q_r
     QVL_ATTN_LAUNCH(decode_stream_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)std::min(plan.slot_rows, 16)), P, S);
     return check_launch("decode_stream_join");
   }
-  if (plan.prefix_rows) QVL_ATTN_LAUNCH(prefix_rows_kernel, units, P, S);
+  // (tiles of 128 rows take what lies behind a prefix's last key for zeros; where V's rows lie closer than a row is long it is
+  // not, and the tiles of 32 tell it apart)
+  if (plan.prefix_rows && v_row >= head_dim) QVL_ATTN_LAUNCH(prefix_rows_kernel, units, P, S);
   else if (plan.few) QVL_FEW_LAUNCH(prefix_few_kernel, units, P, S);
   else QVL_ATTN_LAUNCH(prefix_keys_kernel, units, P, S);
   QVL_TRY_RC(check_launch("prefix_attention"));

@@ -633,7 +633,7 @@ template <typename T, int D, bool V> struct Loader {
     chunk = (uint32_t)((lane % C::kChunks) ^ swz(lane / C::kChunks)) << 4;
   }
   static __device__ __forceinline__ int swz(int row) { return V ? C::v_swz(row) : C::k_swz(row); }
-  // `left` rows from `base` on; past them zeros arrive
+  // `left` rows from `base` on; past them zeros arrive (copies, where rows lie closer than a row is long)
   __device__ __forceinline__ void at(const char* base, int left) {
     rsrc = rsrc_words((const char*)uniform((int64_t)base),
                       (uint32_t)uniform((int)(left > 0 ? (uint32_t)((int64_t)(min(left, 64) - 1) * stride + C::kRowBytes) : 0u)));
@@ -765,8 +765,9 @@ template <typename T, int D> struct KeysUnit {
       if (more) load_v(t + 4);
       t += 4;
     };
-    // blocks that every row sees whole, or that only end inside (what lies behind the keys reads as zeros); then the rest
-    const int whole = w.lim_lo < u.len ? min(w.lim_lo / 32, t1) : t1;
+    // blocks that every row sees whole, or that only end inside (what lies behind the keys reads as zeros, unless V's rows lie
+    // closer than a row is long: then it is a copy of keys before); then the rest
+    const int whole = w.lim_lo < u.len || P.v.row < Core<T, D>::kRowBytes ? min(w.lim_lo / 32, t1) : t1;
     while (t < whole) each(std::false_type{});
     while (t < t1) each(std::true_type{});
   }

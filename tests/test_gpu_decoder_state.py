@@ -46,3 +46,66 @@ def test_plan_dropped_before_its_kernel_has_run(ops):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def short_rows(name, rows, hkv, D, dtype):
+    """Caches whose rows lie closer than a row is long, with a value that only seen rows hold: (k, v)."""
+    inf = float("inf")
+    if name == "one row":
+        k, v = rand((1, hkv, D), dtype, 1), rand((1, hkv, D), dtype, 2)
+        v[0, :, 3], v[0, :, D - 1] = inf, -inf
+        return k, v
+    if name == "expanded":
+        k, v = short_rows("one row", 1, hkv, D, dtype)
+        return k.expand(rows, hkv, D), v.expand(rows, hkv, D)
+    flat = rand((2, hkv, rows * 16 + D), dtype, 3)
+    k, v = (x.as_strided((rows, hkv, D), (16, rows * 16 + D, 1), x.storage_offset()) for x in flat)
+    return k, v
+
+
+def assert_sees_all(got, q, k, v):
+    """Tokens that see every key, against float64: infinite where a value is, else within the bound of the attention tests (scores
+    of D products off by (D + 8) 2^-24 sum|q_i k_i| scale + 4 2^-24 max|s|, sums of n terms by n 2^-24, bf16 weights and the
+    output by half a step)."""
+    D, g, u = q.shape[-1], q.shape[1] // k.shape[1], 2.0 ** -8 if got.dtype == BF else 2.0 ** -24
+    for h in range(q.shape[1]):
+        qh, kh, vh = q[:, h].double(), k[:, h // g].double(), v[:, h // g].double()
+        s, mass = qh @ kh.t() * D ** -0.5, qh.abs() @ kh.abs().t() * D ** -0.5
+        w, bad = torch.softmax(s, 1), ~vh.isfinite().all(0)
+        vh = torch.where(bad[None], 0.0, vh)
+        ds = (D + 8) * 2.0 ** -24 * mass.amax(1, keepdim=True) + 4 * 2.0 ** -24 * s.abs().amax(1, keepdim=True)
+        A, want = w @ vh.abs(), w @ vh
+        tol = (2 * ds + 2 * k.shape[0] * 2.0 ** -24 + (2 * u if got.dtype == BF else 0.0)) * A + u * want.abs()
+        assert ((got[:, h].double() - want).abs() <= tol)[:, ~bad].all() and got[:, h][:, bad].isinf().all()
+
+
+@pytest.mark.parametrize("dtype,hq", [(BF, 8), (BF, 80), (F32, 8), (F32, 80)])     # fp32: tiles of 16 rows, and of 32
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("name", ["one row", "expanded", "overlapping"])
+@pytest.mark.parametrize("n", [1, 40])                                          # 40: prefixes in tiles of 128 rows
+def test_rows_closer_than_a_row_is_long(ops, dtype, hq, D, name, n):
+    """What lies behind a sequence's last key is then a copy of keys before it, not outside: infinite values there must not
+    meet the weight 0 of a key that is not seen. Against float64, and bit for bit against the same rows in a cache of their own
+    but for prefixes, which take tiles of 32 rows here and may take 128 there."""
+    length = 1 if name == "one row" else 70
+    k, v = short_rows(name, 200, 2, D, dtype)
+    if name == "overlapping":
+        v[length - 1, :, D - 5] = float("inf")
+    kc, vc = torch.zeros(400, 2, D, dtype=dtype, device=DEV), torch.zeros(400, 2, D, dtype=dtype, device=DEV)
+    kc[:length], vc[:length] = k[:length], v[:length]
+    q = rand((n, hq, D), dtype, 5)
+    t = lambda x, dt: torch.tensor(x, dtype=dt, device=DEV)
+    start, lens, none = t([0] * n, torch.int64), t([length] * n, torch.int32), t([0] * n, torch.int32)
+    calls = {"decode": lambda k, v: ops.decode_attention(q, k, v, start, lens, max_len=length),
+             "own": lambda k, v: ops.prefix_attention(q, k, v, start, lens, start[:1], none[:1], t([0, n], torch.int32), max_len=length,
+                                                      max_prefix=0),
+             "prefix": lambda k, v: ops.prefix_attention(q, k, v, start, none, start[:1], lens[:1], t([0, n], torch.int32), max_len=0,
+                                                         max_prefix=length),
+             "causal": lambda k, v: ops.causal_attention(q, k, v, ops.CausalPlan([n], [length], [0], num_heads=hq, num_kv_heads=2,
+                                                                                 head_dim=D, dtype=dtype, device=DEV))}
+    for what, call in calls.items():
+        got, want = call(k, v), call(kc, vc)
+        if what != "prefix":
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(1e3), want.nan_to_num(1e3)), what
+        last = got if what != "causal" else got[-1:]                 # (a prompt's last token sees every key)
+        assert_sees_all(last, q[-last.shape[0]:], k[:length], v[:length])
