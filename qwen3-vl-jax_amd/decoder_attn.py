@@ -57,16 +57,16 @@ def _device(device):
 
 
 def _no_gradient(t, what: str):
+    """For a tensor that requires a gradient, or inside a forward-mode dual_level."""
     if t.requires_grad and _torch().is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: the decoder operators have none (call them under torch.no_grad())")
-    fa = _forward_ad()
-    if fa._current_level >= 0 and fa.unpack_dual(t).tangent is not None:      # (-1: no dual_level is entered)
+    if _forward_ad().unpack_dual(t).tangent is not None:
         raise ValueError(f"{what} carries a tangent: the decoder operators have no forward-mode gradient")
 
 
 def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool = False):
     """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor, checked against `like`: q's (dtype, device,
-    head_dim)."""
+    head_dim), and whether a forward-mode dual_level is entered."""
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{what} must be [rows, heads, head_dim], not {tuple(shape)}")
@@ -82,7 +82,8 @@ def _heads_view(t, what: str, like, heads: Optional[int] = None, written: bool =
         raise ValueError(f"{what}: head_dim {dim}, q has {like[2]}")
     if heads is not None and n != heads:
         raise ValueError(f"{what}: {n} heads, expected {heads}")
-    _no_gradient(t, what)
+    if t.requires_grad or like[3]:
+        _no_gradient(t, what)
     # the stride of an axis of one entry is never used: torch may hold any value there
     if rows < 2:
         row = 0
@@ -101,18 +102,17 @@ def _like(q):
     shape = q.shape
     if len(shape) != 3:
         raise ValueError(f"q must be [rows, heads, head_dim], not {tuple(shape)}")
-    return q.dtype, q.device, shape[2]
+    return q.dtype, q.device, shape[2], _forward_ad()._current_level >= 0
 
 
 def _word(t, what: str, like, dtype, shape):
-    """Pointer of a contiguous device tensor beside q: whole numbers, or a norm's weights."""
+    """Pointer of a contiguous device tensor beside q."""
     if t.dtype != dtype:
         raise TypeError(f"{what} is {t.dtype}, expected {dtype}")
     if t.device != like[1]:
         raise ValueError(f"{what} on {t.device}, q on {like[1]}")
     if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
-    _no_gradient(t, what)
     return t.data_ptr()
 
 
@@ -128,9 +128,11 @@ def _stream(device) -> int:
     return _torch()._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, 1.5 us cheaper
 
 
-def _written(*tensors):
-    """The kernels write through pointers: autograd's check of what other operations saved looks at the tensors' versions."""
-    _torch()._C._increment_version(tensors)                       # torch.autograd.graph.increment_version, of a tuple
+@functools.lru_cache(maxsize=None)
+def _written():
+    """Called with the tensors that a kernel wrote through pointers: autograd's check of what other operations saved looks at
+    their versions."""
+    return _torch()._C._increment_version                          # torch.autograd.graph.increment_version, for a tuple
 
 
 def _streams_of(device) -> set:
@@ -139,11 +141,10 @@ def _streams_of(device) -> set:
 
 
 def _read_on(t, streams: set, stream: int):
-    """t, of an object that may go before the kernel that reads it has run, is read on `stream`: its memory is not handed out
-    again before that work is through."""
-    if stream not in streams:
-        t.record_stream(_torch().cuda.current_stream(t.device))
-        streams.add(stream)
+    """t, of an object that may go before the kernel that reads it has run, is read on `stream`, none of `streams`: its memory is
+    not handed out again before that work is through."""
+    t.record_stream(_torch().cuda.current_stream(t.device))
+    streams.add(stream)
 
 
 class TextRotary:
@@ -193,6 +194,9 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
     if table.device != like[1]:
         raise ValueError(f"the rotation on {table.device}, q on {q.device}")
     qw, kw = _word(q_norm, "q_norm", like, torch.float32, (D,)), _word(k_norm, "k_norm", like, torch.float32, (D,))
+    if q_norm.requires_grad or k_norm.requires_grad or like[3]:
+        _no_gradient(q_norm, "q_norm")
+        _no_gradient(k_norm, "k_norm")
     if positions.dim() == 1:
         pos, pos_stride = _word(positions, "positions", like, torch.int32, (N,)), 0
     else:
@@ -223,11 +227,12 @@ def qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary: TextRotary, *, ep
             return qk_norm_rotary(q, k, v, q_norm, k_norm, positions, rotary, eps=eps, k_cache=None if rows is None else k_cache,
                                   v_cache=v_cache, rows=rows, q_out=q_out)
     stream = _stream(like[1])
-    _read_on(table, rotary._streams, stream)
+    if stream not in rotary._streams:
+        _read_on(table, rotary._streams, stream)
     capi.check(capi.load().qvl_qk_norm_rotary(
         stream, _qdtype(like[0]), *qv, *kv, *vv, qw, kw, float(eps), pos, pos_stride, table.data_ptr(), prow, out_rows,
         *qo, *ko, *vo, N, Hq, Hkv, D), "qvl_qk_norm_rotary")
-    _written(q_out, k_cache) if v_cache is None else _written(q_out, k_cache, v_cache)
+    _written()((q_out, k_cache) if v_cache is None else (q_out, k_cache, v_cache))
     return q_out, k_cache, v if v_cache is None else v_cache
 
 
@@ -315,12 +320,13 @@ def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None
             return causal_attention(q, k, v, plan, scale=scale, out=out)
     ws = _workspace(plan.workspace_bytes, q)
     stream = _stream(like[1])
-    _read_on(plan.items, plan._streams, stream)
+    if stream not in plan._streams:
+        _read_on(plan.items, plan._streams, stream)
     capi.check(capi.load().qvl_causal_attention(
         stream, _qdtype(like[0]), *views, rows, plan.tile_rows, plan.items.data_ptr(), plan.n_items, plan.n_parts,
         plan.n_joins, _scale(scale, D), *ov, N, Hq, plan.num_kv_heads, D, None if ws is None else ws.data_ptr(),
         plan.workspace_bytes), "qvl_causal_attention")
-    _written(out)
+    _written()((out,))
     return out
 
 
@@ -359,7 +365,7 @@ def _decode(q, k, v, k_start, k_len, max_len, cu_q, groups, scale, out):
     capi.check(capi.load().qvl_decode_attention(
         _stream(like[1]), dt, *views, rows, cq, n_seqs, ks, kl, max_len, cg, n_groups, ps, pl, max_prefix, _scale(scale, D), *ov, N,
         Hq, Hkv, D, None if ws is None else ws.data_ptr(), nb), "qvl_decode_attention")
-    _written(out)
+    _written()((out,))
     return out
 
 
