@@ -77,8 +77,8 @@ template <int D> struct Core<bf16, D> {
     for (int db = 0; db < kDB; ++db) o[db] = f32x16{};
     l = 0.f;
   }
-  // keys block b of the tile at `lds`
-  __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
+  // keys block b of the tile at `lds` (one sum: D / 16 additions, each of 16 exact products)
+  template <int SUMS = 1> __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
     const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
     f32x16 s = f32x16{};
     const char* row = lds + (b * 32 + l32) * kRowBytes;
@@ -275,17 +275,22 @@ template <int D> struct Core<float, D> {
     for (int db = 0; db < kDB; ++db) o[db] = f32x16{};
     l = 0.f;
   }
-  __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
+  // SUMS sums of D / SUMS products each, added in pairs: of a score of 128 products one sum is off by 3.4 2^-24 in the root
+  // mean square, two by 2.5, four by 1.9.
+  template <int SUMS> __device__ __forceinline__ f32x16 scores(const char* lds, int b) const {
+    static_assert(SUMS == 1 || SUMS == 2 || SUMS == 4, "sums of a score");
     const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
-    f32x16 s = f32x16{};
+    f32x16 s[SUMS] = {};
     const char* row = lds + (b * 32 + l32) * kRowBytes;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
       const f32x4 k = *reinterpret_cast<const f32x4*>(row + (((j * 2 + hh) ^ k_swz(l32)) << 4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[j][e], s, 0, 0, 0);
+      for (int e = 0; e < 4; ++e) s[e % SUMS] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[j][e], s[e % SUMS], 0, 0, 0);
     }
-    return s;
+    if constexpr (SUMS == 4) return (s[0] + s[1]) + (s[2] + s[3]);
+    else if constexpr (SUMS == 2) return s[0] + s[1];
+    else return s[0];
   }
   // dims kDB (lane % 32) + db of the lane's key in register r of block b
   __device__ __forceinline__ void v_frag(const char* lds, int b, int r, float (&v)[kDB]) const {
@@ -402,8 +407,9 @@ template <typename C> struct RowState {
   __device__ __forceinline__ float shift() const { return m == -INFINITY ? 0.f : -m; }
 };
 
-// The online softmax of one wave: 32 rows over the keys it is given.
-template <typename T, int D> struct Wave : RowState<Core<T, D>> {
+// The online softmax of one wave: 32 rows over the keys it is given. SUMS: Core's, fp32 (4000 keys, head_dim 128: 1.12e-6 off
+// with one, 6.5e-7 with two, 4.6e-7 with four, no slower; head_dim 64 has no registers for four).
+template <typename T, int D, int SUMS = D == 128 ? 4 : 2> struct Wave : RowState<Core<T, D>> {
   using RowState<Core<T, D>>::core;
   using RowState<Core<T, D>>::m;
   using RowState<Core<T, D>>::lim;
@@ -434,7 +440,7 @@ template <typename T, int D> struct Wave : RowState<Core<T, D>> {
       core.v_group(vlds, 0, v0);
     } else {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) s[b] = core.scores(klds, b);
+      for (int b = 0; b < NB; ++b) s[b] = core.template scores<SUMS>(klds, b);
 #pragma unroll
       for (int i = 0; i < 8; ++i) between(i);
     }
@@ -506,8 +512,9 @@ template <int D> struct FewCore {
 #pragma unroll
     for (auto& x : q) asm volatile("" : "+v"(x));
   }
+  // Four sums of a quarter of the products each, as in Core<float, D>: 2310 keys and one sum 1.15e-6 off, four 4.0e-7.
   __device__ __forceinline__ void scores(const char* lds, f32x4 (&s)[2]) const {
-    s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 t[2][4] = {};
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       f32x4 k[2];
@@ -519,8 +526,10 @@ template <int D> struct FewCore {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][e], q[j][e], s[b], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) t[b][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][e], q[j][e], t[b][e], 0, 0, 0);
     }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) s[b] = (t[b][0] + t[b][1]) + (t[b][2] + t[b][3]);
   }
   static __device__ __forceinline__ f32x4 v_frag(const char* lds, int b, int r, int h) {
     return *reinterpret_cast<const f32x4*>(lds + (16 * b + 4 * quad() + r) * C::kRowBytes + (16 * h + l16()) * 16);
@@ -663,7 +672,8 @@ template <typename T, int D> struct RowsUnit {
 
   // Tiles [t0, t1) of the unit. The next tile's DMAs stand among this one's products: issued together they would hold the
   // wave for as long as they take to address (8 of them: 900 cycles of 3850 a tile).
-  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
+  template <typename W>
+  static __device__ __forceinline__ void run(const AttnParams& P, const Unit& u, W& w, char* smem, int t0, int t1) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds0 = lds_addr_of(smem);
     Loader<T, D, false> lk(P.k);
@@ -698,7 +708,8 @@ template <typename T, int D> struct RowsUnit {
     }
   }
   // The same, telling apart what a row sees where V is not finite; a tile at a time.
-  static __device__ __forceinline__ void run_safe(const AttnParams& P, const Unit& u, Wave<T, D>& w, char* smem, int t0, int t1) {
+  template <typename W>
+  static __device__ __forceinline__ void run_safe(const AttnParams& P, const Unit& u, W& w, char* smem, int t0, int t1) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds0 = lds_addr_of(smem);
     Loader<T, D, false> lk(P.k);
@@ -812,8 +823,8 @@ __device__ __forceinline__ void store_rows(const W& w, char* dst, char* lds, F&&
 }
 
 // One wave writes its 32 rows, through kWriteLds bytes of LDS that no other wave uses: to the output, or as a part.
-template <typename T, int D>
-__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const Wave<T, D>& w, char* lds, int row, float* po,
+template <typename T, int D, typename W>
+__device__ __forceinline__ void write_rows(const AttnParams& P, const Unit& u, const W& w, char* lds, int row, float* po,
                                            f32x2* pml, bool sees) {
   const float l = w.core.row_sum();
   if (po) {
