@@ -109,3 +109,41 @@ def test_rows_closer_than_a_row_is_long(ops, dtype, hq, D, name, n):
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(1e3), want.nan_to_num(1e3)), what
         last = got if what != "causal" else got[-1:]                 # (a prompt's last token sees every key)
         assert_sees_all(last, q[-last.shape[0]:], k[:length], v[:length])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_nothing_is_taken_from_what_a_workspace_held(ops, monkeypatch, dtype, D):
+    """Workspaces full of NaN: what a join reads of them has to be written first, the parts of sequences without a prefix, without
+    keys and of bad keys too."""
+    hkv, hq = 2, 8
+    t = lambda x, dt: torch.tensor(x, dtype=dt, device=DEV)
+    lengths = [40, 3, 17, 900, 9, 0, 33]
+    start = [3 + sum(lengths[:i]) for i in range(7)]
+    k, v = rand((3000, hkv, D), dtype, 1), rand((3000, hkv, D), dtype, 2)
+    one, few, many = rand((7, hq, D), dtype, 3), rand((21, hq, D), dtype, 4), rand((200, hq, D), dtype, 5)
+    ks, kl = t(start, torch.int64), t(lengths, torch.int32)
+    bad = t([-1] + start[1:], torch.int64)
+    cu = t([0, 3, 6, 9, 12, 15, 18, 21], torch.int32)
+    pre = (t([1100, 2000], torch.int64), t([700, 129], torch.int32))
+    cut = ops.CausalPlan([200], [2900], [0], num_heads=hq, num_kv_heads=hkv, head_dim=D, dtype=dtype, device=DEV)
+    assert cut.n_joins > 0
+    prefix = lambda q, start, cu_g, **kw: ops.prefix_attention(q, k, v, start, kl, *pre, t(cu_g, torch.int32), max_len=900, max_prefix=700, **kw)
+    calls = [lambda: ops.decode_attention(one, k, v, ks, kl, max_len=900), lambda: ops.decode_attention(few, k, v, ks, kl, max_len=900, cu_q=cu),
+             lambda: ops.decode_attention(one, k, v, bad, kl, max_len=900), lambda: prefix(one, ks, [2, 4, 5]),
+             lambda: prefix(one, bad, [0, 4, 4]), lambda: prefix(few, ks, [2, 4, 5], cu_q=cu), lambda: prefix(few, ks, [0, 0, 7], cu_q=cu),
+             lambda: ops.causal_attention(many, k, v, cut)]
+    want = [c() for c in calls]
+    held = []
+
+    def poisoned(nbytes, q):
+        if nbytes:
+            held.append(torch.full((nbytes,), 255, dtype=torch.uint8, device=DEV))      # of every float: NaN
+        return held[-1] if nbytes else None
+
+    monkeypatch.setattr(ops, "_workspace", poisoned)
+    for i, (c, w) in enumerate(zip(calls, want)):
+        got = c()
+        assert len(held) == i + 1 and torch.equal(got.isnan(), w.isnan()) and torch.equal(got.nan_to_num(7.0), w.nan_to_num(7.0)), i
+    for i, w in enumerate(want):
+        assert w.isnan().any() == (i in (2, 4)), i
