@@ -56,40 +56,42 @@ __device__ __forceinline__ void sincos_turns(uint64_t f, float& c, float& s) {
   c = ((quarter + 1) & 2) ? -b : b;
 }
 
-// E consecutive values as fp32, and back (bf16 rounds to nearest even).
-template <typename T, int E>
-__device__ __forceinline__ void load_vals(const char* p, float (&x)[E]) {
-  if constexpr (std::is_same<T, float>::value) {
+// N words at p, 16 bytes at a time (8 where there are no more).
+template <int N> __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[N]) {
+  if constexpr (N == 2) *reinterpret_cast<u32x2*>(w) = *reinterpret_cast<const u32x2*>(p);
+  else
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4 * i);
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<u32x4*>(w + i) = *reinterpret_cast<const u32x4*>(p + 4 * i);
+}
+template <int N> __device__ __forceinline__ void store_words(char* p, const uint32_t (&w)[N]) {
+  if constexpr (N == 2) *reinterpret_cast<u32x2*>(p) = *reinterpret_cast<const u32x2*>(w);
+  else
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i + e] = v[e];
-    }
-  } else {
-    uint32_t w[E / 2];
-    if constexpr (E == 8) *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(p);
-    else *reinterpret_cast<u32x2*>(w) = *reinterpret_cast<const u32x2*>(p);
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<u32x4*>(p + 4 * i) = *reinterpret_cast<const u32x4*>(w + i);
+}
+
+// E values of T in words as fp32, and back to memory (bf16 rounds to nearest even).
+template <typename T, int E, int N> __device__ __forceinline__ void values_of(const uint32_t (&w)[N], float (&x)[E]) {
+  static_assert(N * 4 == E * (int)sizeof(T), "E values");
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
+  for (int i = 0; i < N; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
       x[2 * i] = bf16_lo(w[i]);
       x[2 * i + 1] = bf16_hi(w[i]);
     }
   }
 }
 
-template <typename T, int E>
-__device__ __forceinline__ void store_vals(char* p, const float (&x)[E]) {
-  if constexpr (std::is_same<T, float>::value) {
+template <typename T, int E> __device__ __forceinline__ void store_vals(char* p, const float (&x)[E]) {
+  uint32_t w[E * sizeof(T) / 4];
 #pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<f32x4*>(p + 4 * i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-  } else {
-    uint32_t w[E / 2];
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-    if constexpr (E == 8) *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(w);
-    else *reinterpret_cast<u32x2*>(p) = *reinterpret_cast<const u32x2*>(w);
+  for (int i = 0; i < (int)(E * sizeof(T) / 4); ++i) {
+    if constexpr (std::is_same<T, float>::value) w[i] = __float_as_uint(x[i]);
+    else w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
   }
+  store_words(p, w);
 }
 
 template <typename T, int D>
@@ -106,10 +108,10 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(QkNormRotaryParams 
   const HeadsView in = is_v ? P.v : is_k ? P.k : P.q, to = is_v ? P.vo : is_k ? P.ko : P.qo;
   const int h = is_v ? head - P.hq - P.hkv : is_k ? head - P.hq : head;
   const char* src = in.p + n * in.row + h * in.head + part * E * (int)sizeof(T);
-  float lo[E], hi[E];
+  uint32_t lo_words[E * sizeof(T) / 4], hi_words[E * sizeof(T) / 4];
   if (live) {
-    load_vals<T, E>(src, lo);
-    load_vals<T, E>(src + kHalfBytes, hi);
+    load_words(src, lo_words);
+    load_words(src + kHalfBytes, hi_words);
   }
   if (lane < D / 2) {
     const uint64_t turns = P.table[2 * lane];
@@ -124,11 +126,14 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(QkNormRotaryParams 
   const int64_t row = head < P.hq || !P.rows ? n : P.rows[n];
   if (head >= P.hq && (row < 0 || row >= P.out_rows)) return;
   char* dst = to.p + row * to.row + h * to.head + part * E * (int)sizeof(T);
-  if (is_v) {
-    store_vals<T, E>(dst, lo);
-    store_vals<T, E>(dst + kHalfBytes, hi);
+  if (is_v) {                                 // as bits: a conversion there and back would change a signalling NaN
+    store_words(dst, lo_words);
+    store_words(dst + kHalfBytes, hi_words);
     return;
   }
+  float lo[E], hi[E];
+  values_of<T, E>(lo_words, lo);
+  values_of<T, E>(hi_words, hi);
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
@@ -137,9 +142,12 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(QkNormRotaryParams 
   ss += __shfl_xor(ss, 4);
   const float r = 1.0f / sqrtf(ss * (1.0f / D) + P.eps);
   const float* w = (is_k ? P.kw : P.qw) + part * E;
+  uint32_t wl_words[E], wh_words[E];
+  load_words(reinterpret_cast<const char*>(w), wl_words);
+  load_words(reinterpret_cast<const char*>(w + D / 2), wh_words);
   float wl[E], wh[E], yl[E], yh[E];
-  load_vals<float, E>(reinterpret_cast<const char*>(w), wl);
-  load_vals<float, E>(reinterpret_cast<const char*>(w + D / 2), wh);
+  values_of<float, E>(wl_words, wl);
+  values_of<float, E>(wh_words, wh);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const f32x2 cs = cs_all[wave][part * E + i];

@@ -147,3 +147,20 @@ def test_nothing_is_taken_from_what_a_workspace_held(ops, monkeypatch, dtype, D)
         assert len(held) == i + 1 and torch.equal(got.isnan(), w.isnan()) and torch.equal(got.nan_to_num(7.0), w.nan_to_num(7.0)), i
     for i, w in enumerate(want):
         assert w.isnan().any() == (i in (2, 4)), i
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_go_to_the_cache_bit_for_bit(ops, dtype, D):
+    """Every bf16 there is (for fp32: with further bits behind), signalling NaN among them."""
+    n, hkv = 65536 // D // 2, 2
+    b = torch.arange(65536, dtype=torch.int32)
+    b = (b - (b >= 32768).int() * 65536).to(torch.int16) if dtype == BF else ((b << 16) + 0x4321 * (b % 3 > 0)).to(torch.int32)
+    v = b.view(n, hkv, D).view(dtype).to(DEV)
+    vc, kc = torch.zeros_like(v), torch.zeros_like(v)
+    rows = torch.randperm(n, generator=torch.Generator().manual_seed(1)).to(DEV)
+    ops.qk_norm_rotary(rand((n, 4, D), dtype, 1), rand((n, hkv, D), dtype, 2), v, torch.ones(D, device=DEV), torch.ones(D, device=DEV),
+                       torch.arange(n, dtype=torch.int32, device=DEV), ops.TextRotary(D, 1e4, (D // 2, 0, 0), False, DEV), k_cache=kc,
+                       v_cache=vc, rows=rows)
+    word = torch.int16 if dtype == BF else torch.int32
+    assert torch.equal(vc[rows].view(word), v.view(word))
