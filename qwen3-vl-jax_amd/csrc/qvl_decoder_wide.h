@@ -237,7 +237,10 @@ template <int D> struct WideUnit {
   }
   static __device__ __forceinline__ void run_all(const AttnParams& P, const Unit& u, W& A, W& B, int row0, char* smem, int t0, int t1) {
     run(P, u, A, B, row0, smem, t0, t1);
-    const auto good = [&](const W& w) { return w.finite() && w.core.row_sum() < kMostSum && (w.m != -INFINITY || w.lim <= t0 * kBN); };
+    const auto good = [&](const W& w) {
+      const float l = w.core.row_sum();         // (an exchange between lanes: every lane takes part)
+      return w.finite() & (l < kMostSum) & (w.m != -INFINITY || w.lim <= t0 * kBN);
+    };
     const bool ok = good(A) & good(B);
     if (__builtin_expect(__syncthreads_or(!ok), 0)) run_safe(P, u, A, B, smem, t0, t1);
   }
