@@ -19,7 +19,8 @@
  *   - head_dim 64 or 128, bf16 or fp32. Sums, softmax statistics and norms are held in fp32 in both; outputs are
  *     rounded once.
  *   - Offsets are 64-bit: a cache may be larger than 4 GiB. Counts of tokens, tokens x (num_heads / num_kv_heads) and keys
- *     of a sequence stay below 2^30, heads below 4096 (QVL_ERR_UNSUPPORTED; lengths that lie on the device: NaN).
+ *     of a sequence stay below 2^30, heads below 4096, sequences and groups of a decode call below 65536 (QVL_ERR_UNSUPPORTED;
+ *     lengths that lie on the device: NaN).
  *   - What a call computes depends on its inputs alone, bit for bit: no atomics, and parts are joined in a fixed order.
  */
 #ifndef QVL_DECODER_H

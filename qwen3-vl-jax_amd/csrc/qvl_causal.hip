@@ -4,8 +4,8 @@
 // For a row of scores s_j = scale q . k_j over the keys it sees, out = sum_j w_j v_j / sum_j w_j with w_j = 2^(s_j log2 e - m), m
 // a maximum carried along: one pass over keys and values, nothing of the size rows x keys in memory. The rows of a tile are
 // the heads of a group token by token, so that a key/value tile in LDS serves them all. Bound by the matrix cores and the
-// exponentials beside them: 16411 tokens, 32/8 heads of 128, bf16: 2.05 ms here, 1.87 ms (1180 TFLOP/s) in tiles of 256, at
-// the power limit (a large matrix product reaches 1404); fp32, on fp32 matrix instructions: 2000 tokens 313 us, 105 TFLOP/s
+// exponentials beside them: 16411 tokens, 32/8 heads of 128, bf16: 2.06 ms here, 1.87 ms (1180 TFLOP/s) in tiles of 256, at
+// the power limit (a large matrix product reaches 1404); fp32, on fp32 matrix instructions: 2000 tokens 307 us, 107 TFLOP/s
 // (a large product: 154).
 #include "qvl_decoder_core.h"
 

@@ -9,13 +9,13 @@
 // there. (One line over heads too, its runs at unlike places: 438 us.) A job, a tile of a sequence's rows, that lies in one
 // run is finished there; one that crosses runs leaves parts, which a second launch joins.
 //
-// 96 sequences of up to 7900 keys, 32/8 heads of 128, bf16: 320 us, 4.9 TB/s; one of 9001 keys: 14 us and 5.5 for the join.
+// 96 sequences of up to 7900 keys, 32/8 heads of 128, bf16: 322 us, 4.9 TB/s; one of 9001 keys: 14 us and 5.5 for the join.
 //
 // With prefixes the tokens of a group are the rows of one more problem, the prefix's keys for all of them at once, 128 (32)
 // rows a workgroup and the keys in parts; the sequences' own keys are parts beside them, and one join covers both. (Tiles of
 // 256 rows for the prefix, then the own keys and the join in a second launch: 160 us, not 147, for 256 sequences on 24007
 // keys: the own keys, bound by memory, no longer run beside the prefix, bound by the matrix cores.)
-// 48 sequences after 9216 shared keys 28.5 us, 256 after 24007 146 us.
+// 48 sequences after 9216 shared keys 28 us, 256 after 24007 144 us.
 #include "qvl_decoder_core.h"
 
 namespace qvl {
@@ -482,14 +482,14 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   const int64_t cus = gemm_device_cus(), slots = cus * (dtype == QVL_DTYPE_F32 && head_dim == 128 ? 1 : 2);
   D = DecodePlan{};
   // fp32 is bound by its matrix products (32 rows: 8192 cycles a block of 32 keys), so few rows take tiles of 16: 16/8 heads of
-  // 128, 96 sequences of up to 5700 keys 396 us, not 473 (2.2 GB: 5.7 TB/s), one of 9000 25, not 31; 18 sequences after
-  // prefixes of 2000 to 4000 keys, 3 tokens each, 31, not 45
+  // 128, 96 sequences of up to 5760 keys 419 us, not 478 (2.3 GB: 5.4 TB/s), one of 9000 26, not 32; nine times two sequences
+  // after prefixes of 2000 to 4000 keys, 3 tokens each, 47, not 93
   const int64_t own_rows = (rows + std::max<int64_t>(n_seqs, 1) - 1) / std::max<int64_t>(n_seqs, 1);   // a sequence's, in the mean
   D.few = dtype == QVL_DTYPE_F32 && own_rows <= 16 && (n_groups == 0 || rows <= 16 * n_groups);
   D.tile = D.few ? 16 : 32;
   if (n_groups == 0) {
     // A run for each compute unit where that leaves it at most 40 blocks, else for each slot (8 heads: one sequence of 9001 keys
-    // 19 us and not 24, of 31000 32.5 and not 34.5; 16 of up to 8000 61.6 and not 69); no more than give each wave a block,
+    // 20 us and not 25, of 31000 33.5 and not 37; 16 of up to 8000 62.5 and not 72); no more than give each wave a block,
     // nor fewer than there are jobs.
     const int64_t tiles = std::max<int64_t>((own_rows + D.tile - 1) / D.tile, 1);
     const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + 31) / 32);
@@ -507,8 +507,8 @@ static int decode_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64
   D.prefix_tiles = (int)std::max<int64_t>(std::min((rows + tile - 1) / tile, (mean + tile - 1) / tile * (n_groups > 1 ? 2 : 1)), 1);
   D.own_parts = split_parts(max_len, n_seqs * num_kv_heads, slots, D.own_chunk);
   // About one unit on the prefixes for each compute unit, beside units on the sequences' own keys (one for each slot: 192
-  // rows on 9216 keys 36 us, not 30; 1024 on 24007 145, not 140). Tiles that groups of unlike size may leave empty
-  // count half: twice 1024 rows 231 us, not 328.
+  // rows on 9216 keys 36 us, not 30; 1024 on 24007 141, not 133). Tiles that groups of unlike size may leave empty
+  // count half: twice 1024 rows 228 us, not 336.
   const int64_t busy = std::min(n_groups * D.prefix_tiles, (rows + tile - 1) / tile + n_groups / 2) * num_kv_heads;
   D.prefix_parts = split_parts(max_prefix, busy, cus + busy / 8, D.prefix_chunk);
   D.units = (int64_t)num_kv_heads * (n_groups * D.prefix_parts * D.prefix_tiles + n_seqs * D.own_parts);

@@ -179,7 +179,7 @@ std::vector<Job> deal(const std::vector<Job>& jobs, const Kernel& K) {
     load[lo] += moved;
   }
   // The first workgroups go to one slot of each compute unit, the next to the second: those in reverse, so that a long job
-  // shares its compute unit with a short one (1181 tokens, 16/8 heads of 128, fp32: 70 us and not 76).
+  // shares its compute unit with a short one (1181 tokens, 16/8 heads of 128, fp32: 66 us and not 73).
   const int64_t cus = std::max<int64_t>(K.cus / kAttnQueues, 1);
   for (auto& q : queue)
     for (int64_t s = 1; s < K.slots / K.cus; s += 2)

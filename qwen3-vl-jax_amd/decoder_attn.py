@@ -303,7 +303,7 @@ def _scale(scale, head_dim: int) -> float:
 def causal_attention(q, k, v, plan: CausalPlan, *, scale: Optional[float] = None, out=None):
     """softmax(scale q k^T) v of a packed prefill: q [N, Hq, D] holds the plan's new tokens one sequence after the other
     (rows past them are left as they are in `out`), k and v [R, Hkv, D] the caches (or the prompt's own keys and values).
-    Token t of a sequence sees its keys up to itself; scale defaults to D^-0.5."""
+    Token t of a sequence sees its keys up to itself; scale defaults to D^-0.5. `out`, here and below, lies over no input."""
     like = _like(q)
     views, ov, out = _attention_views(q, k, v, out, like)
     N, Hq, D = q.shape
