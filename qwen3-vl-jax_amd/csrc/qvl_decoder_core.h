@@ -46,8 +46,9 @@ __device__ __forceinline__ float across_halves(float x) {
 // are two runs of 4, so V^T is read by two transposing reads of 4 keys (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16
 // values, and each gets a column). The weights are rounded to bf16 for that product, the type of the instruction's operands:
 // outputs are 1.7e-3 to 2.3e-3 off, 1.3e-3 to 1.7e-3 of which is their own rounding; weights in two bf16 parts would take the
-// rest away for half as many matrix instructions again, in kernels bound by those. The row sums are plain fp32 additions of the weights before their rounding: a dot
-// instruction that adds two rounded ones waits for the matrix cores (52 cycles beside a product of 32).
+// rest away for half as many matrix instructions again, in kernels bound by those. The row sums are plain fp32 additions of
+// the weights before their rounding: a dot instruction that adds two rounded ones waits for the matrix cores (52 cycles
+// beside a product of 32).
 // 16-byte chunks are XOR-swizzled by the row so that neither read meets a bank twice: 16 rows of one chunk for K, 4 rows
 // of 64 bytes for V.
 template <typename T, int D> struct Core;
