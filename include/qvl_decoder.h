@@ -8,6 +8,8 @@
  *                                               keys it had before; grouped heads
  *   qvl_decode_attention                        a few new tokens of each sequence over its cache; sequences may come in
  *                                               groups that share a prefix, which is read once for the whole group
+ *   qvl_paged_append, qvl_paged_unpack,         a cache in pages and 4 bits a value: new tokens' keys and values into it (norm and
+ *   qvl_paged_attention                         rotation on the way), read back as rows, and attended to
  *
  * The conventions of qvl_vision.h hold (streams, no allocation, error codes, thread safety). Beside them:
  *   - q, k, v, out and the caches are views [rows, heads, head_dim] of one dtype: element (r, h, d) lies at
@@ -111,6 +113,57 @@ int qvl_decode_attention(void* stream, int32_t dtype,
                          void* d_out, int64_t out_row_stride, int64_t out_head_stride,
                          int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                          void* d_workspace, size_t workspace_bytes);
+
+/* A cache in pages of `page_rows` tokens (a power of two, 16 to 4096), 4 bits a value. A head's values go in groups of 64; of a group
+ * x the scale is s = bf16(fp32(max|x| / 6)) (rounded to nearest even, twice) and each value becomes the number nearest to |x| / s of 0,
+ * .5, 1, 1.5, 2, 3, 4, 6 (a tie goes to 0, 1, 2 or 4) with x's sign, and stands for s times it. A group with a NaN or an infinity, or whose
+ * scale is beyond bf16, stands for NaN. The bytes of a page are this library's own; qvl_paged_cache_size tells how many a cache of
+ * n_pages takes (64-byte aligned; any content until tokens are written).
+ * Token t of sequence i lies in page d_page_table[i * table_stride + t / page_rows], slot t % page_rows. Sequences may share pages.
+ * An entry outside [0, n_pages) is no page: what would be written there is dropped, what would be read there is NaN. */
+int qvl_paged_cache_size(int64_t n_pages, int32_t page_rows, int32_t num_kv_heads, int32_t head_dim, size_t* bytes);
+
+/* Keys and values of new tokens into their pages. Sequence i brings tokens [d_cu_q[i], d_cu_q[i+1]) of k and v (NULL: token i,
+ * n_tokens == n_seqs) and has d_k_len[i] tokens with them: the last one's t is d_k_len[i] - 1. Tokens of no sequence, and those whose t
+ * is negative or beyond the table, are dropped. With q, the norm and rotation of qvl_qk_norm_rotary run on the way: q to q_out (rows
+ * of no sequence are left as they are) as there, k to 4 bits; k's norm, rotation and codes are formed in fp64. q NULL: k goes to 4 bits as it is, and
+ * q_norm, k_norm, eps, positions, table, q_out and num_heads are not looked at. q_out may be q. A slot that two tokens of
+ * a call are given holds any mixture of the two. */
+int qvl_paged_append(void* stream, int32_t dtype,
+                     const void* d_q, int64_t q_row_stride, int64_t q_head_stride,
+                     const void* d_k, int64_t k_row_stride, int64_t k_head_stride,
+                     const void* d_v, int64_t v_row_stride, int64_t v_head_stride,
+                     const float* d_q_norm, const float* d_k_norm, double eps,
+                     const int32_t* d_positions, int64_t pos_stride, const uint64_t* d_table,
+                     void* d_cache, int64_t n_pages, int32_t page_rows,
+                     const int32_t* d_page_table, int64_t table_width, int64_t table_stride,
+                     const int32_t* d_cu_q, int64_t n_seqs, const int32_t* d_k_len,
+                     void* d_q_out, int64_t qo_row_stride, int64_t qo_head_stride,
+                     int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/* Tokens d_first[i] <= t < d_k_len[i] (NULL: from 0) of each sequence read back as rows of k and v, token t's as row
+ * d_k_start[i] + t - d_first[i], rounded to dtype once. Rows outside [0, out_rows) are dropped. max_len: the most tokens of a
+ * sequence that the launch is laid out for; more are still right. */
+int qvl_paged_unpack(void* stream, int32_t dtype, const void* d_cache, int64_t n_pages, int32_t page_rows,
+                     const int32_t* d_page_table, int64_t table_width, int64_t table_stride, int64_t n_seqs,
+                     const int32_t* d_first, const int32_t* d_k_len, int64_t max_len, const int64_t* d_k_start,
+                     void* d_k, int64_t k_row_stride, int64_t k_head_stride,
+                     void* d_v, int64_t v_row_stride, int64_t v_head_stride, int64_t out_rows,
+                     int32_t num_kv_heads, int32_t head_dim);
+
+/* Attention of new tokens over the pages: qvl_decode_attention (without prefixes) of the values that the pages stand for. The tokens of
+ * a sequence with more tokens than its line of the table has room for, or fewer than none, come out NaN, and so does a token that sees a
+ * key in no page. What pages hold behind a sequence's last key never enters its output. */
+int qvl_paged_attention_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t max_len, int32_t num_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, size_t* bytes);
+int qvl_paged_attention(void* stream, int32_t dtype,
+                        const void* d_q, int64_t q_row_stride, int64_t q_head_stride,
+                        const void* d_cache, int64_t n_pages, int32_t page_rows,
+                        const int32_t* d_page_table, int64_t table_width, int64_t table_stride,
+                        const int32_t* d_cu_q, int64_t n_seqs, const int32_t* d_k_len, int64_t max_len, float scale,
+                        void* d_out, int64_t out_row_stride, int64_t out_head_stride,
+                        int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                        void* d_workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -84,6 +84,7 @@ class VisionMetadataDev(C.Structure):
 
 
 _view = [_p, _i64, _i64]   # a [rows, heads, head_dim] view: pointer, row and head stride
+_pages = [_p, _i64, _i32, _p, _i64, _i64]   # a paged cache: pointer, pages, rows a page; the page table, its width and row stride
 _pi64 = C.POINTER(_i64)
 
 # name -> (restype, argtypes); every function in include/qvl_vision.h and include/qvl_decoder.h
@@ -162,6 +163,12 @@ SIGNATURES = {
     "qvl_decode_workspace_size": (C.c_int, [_i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
     "qvl_decode_attention": (C.c_int, [_p, _i32, *_view, *_view, *_view, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
                                        _i64, _f32, *_view, _i64, _i32, _i32, _i32, _p, _sz]),
+    "qvl_paged_cache_size": (C.c_int, [_i64, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "qvl_paged_append": (C.c_int, [_p, _i32, *_view, *_view, *_view, _p, _p, C.c_double, _p, _i64, _p, *_pages, _p, _i64, _p,
+                                   *_view, _i64, _i32, _i32, _i32]),
+    "qvl_paged_unpack": (C.c_int, [_p, _i32, *_pages, _i64, _p, _p, _i64, _p, *_view, *_view, _i64, _i32, _i32]),
+    "qvl_paged_attention_workspace_size": (C.c_int, [_i64, _i64, _i64, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "qvl_paged_attention": (C.c_int, [_p, _i32, *_view, *_pages, _p, _i64, _p, _i64, _f32, *_view, _i64, _i32, _i32, _i32, _p, _sz]),
 }
 
 
