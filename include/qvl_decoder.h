@@ -10,6 +10,7 @@
  *                                               groups that share a prefix, which is read once for the whole group
  *   qvl_paged_append, qvl_paged_unpack,         a cache in pages and 4 bits a value: new tokens' keys and values into it (norm and
  *   qvl_paged_attention                         rotation on the way), read back as rows, and attended to
+ *   qvl_sample_tokens                           the next token of rows of logits: temperature, top-k, top-p, min-p
  *
  * The conventions of qvl_vision.h hold (streams, no allocation, error codes, thread safety). Beside them:
  *   - q, k, v, out and the caches are views [rows, heads, head_dim] of one dtype: element (r, h, d) lies at
@@ -164,6 +165,17 @@ int qvl_paged_attention(void* stream, int32_t dtype,
                         void* d_out, int64_t out_row_stride, int64_t out_head_stride,
                         int64_t n_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                         void* d_workspace, size_t workspace_bytes);
+
+/* The next token of each row of logits [n_rows, vocab] (fp32 or bf16, rows `row_stride` elements apart, vocab at most 2^18), to out[row].
+ * With z = (x - max x) / T the weight of a token is W = round(2^44 e^z), formed in fp64. In the order of falling logits (equal ones: rising
+ * index) the first top_k are kept (<= 0: all); of them those before which less than top_p of their sum of weights lies (not < 1: all); of
+ * them those whose W is no less than min_p 2^44 (not > 0: all). The token is the first index at which the sum of the kept weights up to it is over
+ * u times the sum of all (u of [0, 1); others count as 0, or as just below 1). T <= 0 or NaN, top_k 1, top_p <= 0 and min_p > 1: the first in the
+ * order. A row with NaN or +infinity, or of -infinities alone, gives -1; tokens of -infinity are never chosen.
+ * Each setting is fp32 (top_k int32) [n_rows] on the device, or, where that is NULL, the value that follows it for all rows. */
+int qvl_sample_tokens(void* stream, int32_t dtype, const void* d_logits, int64_t row_stride, int64_t n_rows, int64_t vocab,
+                      const float* d_u, const float* d_temperature, float temperature, const int32_t* d_top_k, int32_t top_k,
+                      const float* d_top_p, float top_p, const float* d_min_p, float min_p, int64_t* d_out);
 
 #ifdef __cplusplus
 }
