@@ -89,7 +89,7 @@ template <typename R, int E> __device__ __forceinline__ uint32_t codes_of(const 
   for (int i = 0; i < E; ++i) {
     const R a = fabs(x[i]);
     const uint32_t c = (uint32_t)(a > (R)0.25 * s) + (a >= (R)0.75 * s) + (a > (R)1.25 * s) + (a >= (R)1.75 * s) + (a > (R)2.5 * s) +
-                       (a >= (R)3.5 * s) + (a > (R)5 * s) + (x[i] < 0 ? 8u : 0u);
+                       (a >= (R)3.5 * s) + (a > (R)5 * s) + (__builtin_signbit(x[i]) ? 8u : 0u);
     w |= c << (4 * i);
   }
   return w;
