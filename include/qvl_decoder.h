@@ -172,10 +172,13 @@ int qvl_paged_attention(void* stream, int32_t dtype,
  * them those whose W is no less than min_p 2^44 (not > 0: all). The token is the first index at which the sum of the kept weights up to it is over
  * u times the sum of all (u of [0, 1); others count as 0, or as just below 1). T <= 0 or NaN, top_k 1, top_p <= 0 and min_p > 1: the first in the
  * order. A row with NaN or +infinity, or of -infinities alone, gives -1; tokens of -infinity are never chosen.
- * Each setting is fp32 (top_k int32) [n_rows] on the device, or, where that is NULL, the value that follows it for all rows. */
+ * Each setting is fp32 (top_k int32) [n_rows] on the device, or, where that is NULL, the value that follows it for all rows.
+ * The workspace (qvl_sample_workspace_size; 16-byte aligned) holds the rows' histograms: calls that overlap need one each. */
+int qvl_sample_workspace_size(int64_t n_rows, size_t* bytes);
 int qvl_sample_tokens(void* stream, int32_t dtype, const void* d_logits, int64_t row_stride, int64_t n_rows, int64_t vocab,
                       const float* d_u, const float* d_temperature, float temperature, const int32_t* d_top_k, int32_t top_k,
-                      const float* d_top_p, float top_p, const float* d_min_p, float min_p, int64_t* d_out);
+                      const float* d_top_p, float top_p, const float* d_min_p, float min_p, int64_t* d_out,
+                      void* d_workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -169,7 +169,8 @@ SIGNATURES = {
     "qvl_paged_unpack": (C.c_int, [_p, _i32, *_pages, _i64, _p, _p, _i64, _p, *_view, *_view, _i64, _i32, _i32]),
     "qvl_paged_attention_workspace_size": (C.c_int, [_i64, _i64, _i64, _i32, _i32, _i32, C.POINTER(_sz)]),
     "qvl_paged_attention": (C.c_int, [_p, _i32, *_view, *_pages, _p, _i64, _p, _i64, _f32, *_view, _i64, _i32, _i32, _i32, _p, _sz]),
-    "qvl_sample_tokens": (C.c_int, [_p, _i32, _p, _i64, _i64, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p]),
+    "qvl_sample_workspace_size": (C.c_int, [_i64, C.POINTER(_sz)]),
+    "qvl_sample_tokens": (C.c_int, [_p, _i32, _p, _i64, _i64, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p, _p, _sz]),
 }
 
 

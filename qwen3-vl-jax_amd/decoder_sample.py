@@ -7,10 +7,12 @@ row gives depends on its logits, its settings and its random number alone, bit f
 """
 from __future__ import annotations
 
+import ctypes as C
+import functools
 import math
 
 from . import capi
-from .decoder_attn import _elsewhere, _forward_ad, _no_gradient, _qdtype, _stream, _torch, _written
+from .decoder_attn import _elsewhere, _forward_ad, _no_gradient, _qdtype, _stream, _torch, _workspace, _written
 
 
 def _setting(value, what: str, rows: int, device, dtype, low, high):
@@ -32,6 +34,13 @@ def _setting(value, what: str, rows: int, device, dtype, low, high):
     if not low <= value <= high or not math.isfinite(value):
         raise ValueError(f"{what} {value}: a number from {low:g}" + (f" to {high:g}" if math.isfinite(high) else ""))
     return None, value
+
+
+@functools.lru_cache(maxsize=256)
+def _sample_bytes(rows: int) -> int:
+    nb = C.c_size_t()
+    capi.check(capi.load().qvl_sample_workspace_size(rows, C.byref(nb)), "qvl_sample_workspace_size")
+    return nb.value
 
 
 def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
@@ -67,7 +76,10 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     if _elsewhere(device):
         with torch.cuda.device(device):
             return sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, out=out)
+    nb = _sample_bytes(B)
+    ws = _workspace(nb, logits)
     capi.check(capi.load().qvl_sample_tokens(_stream(device), dt, logits.data_ptr(), logits.stride(0) if B > 1 else 0, B, V,
-                                             u.data_ptr(), *settings, out.data_ptr()), "qvl_sample_tokens")
+                                             u.data_ptr(), *settings, out.data_ptr(), None if ws is None else ws.data_ptr(), nb),
+               "qvl_sample_tokens")
     _written()((out,))
     return out
