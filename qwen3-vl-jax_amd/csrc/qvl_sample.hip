@@ -20,7 +20,7 @@
 namespace qvl {
 
 constexpr int kBins = 1536, kSegment = 1024, kMaxSegments = 256, kList = 4096, kShare = 1024;   // kShare: a workgroup's of the list
-constexpr int kSort = 1024;
+constexpr int kSort = 1024, kFew = 128;       // tokens that are sorted, and that are sorted without a look at parts of their bin
 constexpr int kRowsAtOnce = 1024;            // rows that share a workspace
 constexpr double kUnit = 17592186044416.0;   // 2^44
 
@@ -49,7 +49,8 @@ struct SampleParams {
 };
 
 struct Settings {
-  double t, p, floor, u;                     // floor: the least weight
+  double t, p, u;
+  uint64_t floor;                            // the least weight that min-p keeps
   int k;                                     // 0: no top-k
   bool greedy, nucleus;
 };
@@ -63,7 +64,7 @@ __device__ __forceinline__ Settings settings_of(const SampleParams& P, int64_t r
   s.u = P.u[row];
   if (!(s.u >= 0)) s.u = 0;
   s.nucleus = s.p < 1;
-  s.floor = min_p > 0 ? min_p * kUnit : 0;
+  s.floor = min_p > 0 ? (uint64_t)ceil(min(min_p, 2.0) * kUnit) : 0;
   // the first token in the order alone; elsewhere the rules keep it by themselves
   s.greedy = !(s.t > 0) || s.k == 1 || s.p <= 0 || min_p > 1;
   return s;
@@ -121,7 +122,7 @@ struct Weigher {
     e = __builtin_fma(e, r, c);
     e = __builtin_fma(e, r, 1.0);
     e *= table[bin & 31];
-    e = __hiloint2double(__double2hiint(e) - ((bin >> 5) << 20), __double2loint(e));   // 2^-4 at least
+    e = __hiloint2double(__double2hiint(e) - ((bin & ~31) << 15), __double2loint(e));   // 2^(bin / 32) less: 2^-4 at least
     // (plus 2^52: rounded to a whole number, which the low bits then hold)
     return (uint64_t)__double_as_longlong(e + 0x1p52) & 0xfffffffffffffull;
   }
@@ -164,46 +165,84 @@ template <typename T> struct Segment {
   }
 };
 
-// Inclusive sums over the workgroup of NT threads; `waves`: NT / 64 words of LDS. Ends with a barrier that frees them. (Loops that stay
-// loops here and in the choice: code that runs once is paid by its length, as a workgroup waits for each line of it.)
+// v of the lane that DPP control CTRL names, 0 where there is none (or where MASK leaves the row out).
+template <int CTRL, int MASK = 0xf> __device__ __forceinline__ uint64_t dpp_or_zero(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, MASK, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, MASK, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
+}
+// Inclusive sums over the wave: within rows of 16 lanes, then each row's last lane to the next row, then the first half's to the second.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v += dpp_or_zero<0x111>(v);
+  v += dpp_or_zero<0x112>(v);
+  v += dpp_or_zero<0x114>(v);
+  v += dpp_or_zero<0x118>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);
+  v += dpp_or_zero<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+// The smallest over the wave, in its last lane: ~v's largest, so that lanes that are none count as 0.
+__device__ __forceinline__ uint64_t wave_min(uint64_t v) {
+  v = ~v;
+  v = max(v, dpp_or_zero<0x111>(v));
+  v = max(v, dpp_or_zero<0x112>(v));
+  v = max(v, dpp_or_zero<0x114>(v));
+  v = max(v, dpp_or_zero<0x118>(v));
+  v = max(v, dpp_or_zero<0x142, 0xa>(v));
+  v = max(v, dpp_or_zero<0x143, 0xc>(v));
+  return last_lane(~v);
+}
+
+// Inclusive sums over the workgroup of NT threads; `waves`: NT / 64 words of LDS. Ends with a barrier that frees them. (Short code here
+// and in the choice: what runs once is paid by its length, as a workgroup waits for each line of it.)
 template <int NT> __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* waves, uint64_t& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 1
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t o = __shfl_up((unsigned long long)v, d);
-    v += lane >= d ? o : 0;
-  }
-  if (lane == 63) waves[wave] = v;
+  const int wave = threadIdx.x >> 6;
+  v = wave_scan(v);
+  if ((threadIdx.x & 63) == 63) waves[wave] = v;
   __syncthreads();
-  uint64_t before = 0;
+  uint64_t w[NT / 64], before = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) w[i] = waves[i];
   total = 0;
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < NT / 64; ++i) {
-    before += i < wave ? waves[i] : 0;
-    total += waves[i];
+    before = i == wave ? total : before;
+    total += w[i];
   }
   __syncthreads();
   return v + before;
 }
 
-// Runs f(x, index) for the elements of segments [s0, s1), and after(segment) behind each.
-template <typename T, int NT, typename F, typename G>
-__device__ __forceinline__ void over_segments(const char* row, int vocab, int s0, int s1, F&& f, G&& after) {
-  for (int s = s0 + (int)(threadIdx.x >> 6); s < s1; s += NT / 64) {
-    Segment<T> g;
-    g.load(row, vocab, s);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f(g.x[i], s * kSegment + Segment<T>::index(i));
-    after(s);
+// The elements of segments [s0, s1), every NT / 64th to a wave, a segment's loads ahead of the work on the one before; the first ones are
+// under way once the walk is made.
+template <typename T, int NT> struct Walk {
+  const char* row;
+  int vocab, s, s1;
+  Segment<T> g;
+  __device__ __forceinline__ Walk(const char* row, int vocab, int s0, int s1) : row(row), vocab(vocab), s(s0 + (int)(threadIdx.x >> 6)), s1(s1) {
+    if (s < s1) g.load(row, vocab, s);
   }
-}
+  // f(x, index) for each, after(segment) behind each
+  template <typename F, typename G> __device__ __forceinline__ void run(F&& f, G&& after) {
+    for (; s < s1; s += NT / 64) {
+      Segment<T> next;
+      if (s + NT / 64 < s1) next.load(row, vocab, s + NT / 64);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(g.x[i], s * kSegment + Segment<T>::index(i));
+      after(s);
+      g = next;
+    }
+  }
+};
 
 // The smallest place of a row; over the workgroup of NT threads.
 template <int NT> __device__ __forceinline__ uint64_t first_place(const SampleRow& r, int segments, uint64_t* waves) {
   uint64_t m = ~0ull;
   for (int i = threadIdx.x; i < segments; i += NT) m = min(m, r.tops[i]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = min(m, (uint64_t)__shfl_xor((unsigned long long)m, d));
+  m = wave_min(m);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
   __syncthreads();
 #pragma unroll
@@ -231,16 +270,14 @@ __global__ __launch_bounds__(256) void sample_tops_kernel(SampleParams P, int pe
   const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
   uint32_t key = ~0u;
   int at = 0;
-  over_segments<T, 256>(row, P.vocab, s0, s1, [&](float x, int index) {
+  Walk<T, 256>(row, P.vocab, s0, s1).run([&](float x, int index) {
     const uint32_t k = key_of(x);
     if (k < key) {
       key = k;
       at = index;
     }
   }, [&](int s) {
-    uint64_t m = (uint64_t)key << 32 | (uint32_t)at;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = min(m, (uint64_t)__shfl_xor((unsigned long long)m, d));
+    const uint64_t m = wave_min((uint64_t)key << 32 | (uint32_t)at);
     if ((threadIdx.x & 63) == 0) r.tops[s] = m;
     key = ~0u;
     at = 0;
@@ -256,13 +293,14 @@ __global__ __launch_bounds__(256) void sample_histogram_kernel(SampleParams P, i
   const int64_t at = P.first + (int64_t)blockIdx.y;
   const Settings st = settings_of(P, at);
   if (st.greedy || (st.k == 0 && !st.nucleus)) return;
+  const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
+  Walk<T, 256> walk(P.x + at * P.row, P.vocab, s0, s1);
   fill_table(table);
   for (int i = threadIdx.x; i < kBins; i += 256) hist[i] = 0;
   const uint64_t first = first_place<256>(r, P.segments, waves);
   if (no_token(first)) return;
   const Weigher weigh = weigher_of(first, st, table);
-  const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
-  over_segments<T, 256>(P.x + at * P.row, P.vocab, s0, s1, [&](float x, int) {
+  walk.run([&](float x, int) {
     int bin;
     if (st.k > 0) {
       double rest;
@@ -283,14 +321,11 @@ struct Cut {
   int bin;
   uint64_t before, whole;
 };
-template <typename F> __device__ __forceinline__ Cut cut_bin(const uint64_t* hist, uint64_t* waves, Cut* found, F&& enough) {
+template <typename F> __device__ __forceinline__ Cut cut_bin(const uint64_t (&h)[kBins / 256], uint64_t* waves, Cut* found, F&& enough) {
   constexpr int kPer = kBins / 256;
-  uint64_t h[kPer], own = 0, whole;
+  uint64_t own = 0, whole;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    h[j] = hist[threadIdx.x * kPer + j];
-    own += h[j];
-  }
+  for (int j = 0; j < kPer; ++j) own += h[j];
   uint64_t upto = block_scan<256>(own, waves, whole) - own;
   bool was = upto > 0 && enough(upto, whole);
 #pragma unroll
@@ -317,17 +352,21 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleParams P, int pe
   const int64_t at = P.first + (int64_t)blockIdx.y;
   const Settings st = settings_of(P, at);
   if (st.greedy) return;
+  const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
+  Walk<T, 256> walk(P.x + at * P.row, P.vocab, s0, s1);
+  uint64_t h[kBins / 256];                   // the histogram, 6 bins a thread
+#pragma unroll
+  for (int j = 0; j < kBins / 256; ++j) h[j] = r.hist[threadIdx.x * (kBins / 256) + j];
   fill_table(table);
   if (threadIdx.x == 0) n = 0;
   const uint64_t first = first_place<256>(r, P.segments, waves);
   if (no_token(first)) return;
   const Weigher weigh = weigher_of(first, st, table);
   Cut cut{kBins, 0, 0};
-  if (st.k > 0) cut = cut_bin(r.hist, waves, &found, [&](uint64_t c, uint64_t) { return c >= (uint64_t)st.k; });
-  else if (st.nucleus) cut = cut_bin(r.hist, waves, &found, [&](uint64_t w, uint64_t whole) { return !((double)w < st.p * (double)whole); });
-  const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
+  if (st.k > 0) cut = cut_bin(h, waves, &found, [&](uint64_t c, uint64_t) { return c >= (uint64_t)st.k; });
+  else if (st.nucleus) cut = cut_bin(h, waves, &found, [&](uint64_t w, uint64_t whole) { return !((double)w < st.p * (double)whole); });
   uint64_t sum = 0;
-  over_segments<T, 256>(P.x + at * P.row, P.vocab, s0, s1, [&](float x, int index) {
+  walk.run([&](float x, int index) {
     int bin;
     double rest;
     if (!weigh.bin_of(x, bin, rest) || bin > cut.bin) return;
@@ -341,13 +380,12 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleParams P, int pe
       }
     } else {
       const uint64_t w = weigh.weight(bin, rest);
-      if (!((double)w < st.floor)) sum += w;
+      sum += w < st.floor ? 0 : w;
     }
   }, [&](int s) {
     if (st.k == 0) {
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((unsigned long long)sum, d);
-      if ((threadIdx.x & 63) == 0) r.sums[s] = sum;
+      const uint64_t all = wave_scan(sum);
+      if ((threadIdx.x & 63) == 63) r.sums[s] = all;
       sum = 0;
     }
   });
@@ -439,7 +477,7 @@ template <typename F> __device__ __forceinline__ int cut_of(SampleLds& lds, int 
 // before it, `base` of them in earlier bins, is enough (the last, where none is). Where kSort share the bin, and then a 512th of it,
 // false: they are equal, or nearly.
 template <bool COUNT, typename Each, typename F>
-__device__ __forceinline__ bool cut_place(const Weigher& weigh, SampleLds& lds, int in, uint64_t base, uint64_t most, uint64_t& last, Each&& each, F&& enough) {
+__device__ __forceinline__ bool cut_place(const Weigher& weigh, SampleLds& lds, bool many, int in, uint64_t base, uint64_t most, uint64_t& last, Each&& each, F&& enough) {
   constexpr int NT = kChoosers;
   const int i = threadIdx.x;
   const auto gather = [&](int sub) {
@@ -454,8 +492,8 @@ __device__ __forceinline__ bool cut_place(const Weigher& weigh, SampleLds& lds, 
     __syncthreads();
     return lds.n;
   };
-  int n = gather(-1);
-  if (n > kSort) {
+  int n = many ? kFew + 1 : gather(-1);
+  if (n > kFew) {
     __syncthreads();
     lds.hist[i] = 0;
     __syncthreads();
@@ -544,34 +582,19 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
   uint64_t last = ~0ull;                     // the last place that is kept
   if (i < P.segments) lds.sums[i] = st.k > 0 ? 0 : sum;
   if (i == 0) lds.found[1] = 0;
-  if ((st.k > 0 || st.nucleus) && n <= kSort) {
+  if ((st.k > 0 || st.nucleus) && n <= kFew) {
     // the list sorted: with top-k all that can be kept, else the bin of top-p's cut
-    int size = 64;
-    while (size < n) size <<= 1;
-    uint64_t v[2], w[2], upto[2], part;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = j * NT + i < n ? r.list[j * NT + i] : ~0ull;
-    if (size <= NT) sort_values<1>(*reinterpret_cast<uint64_t(*)[1]>(v), size, lds.sort);
-    else sort_values<2>(v, size, lds.sort);
-    uint64_t before = st.k > 0 ? 0 : r.before, whole = st.k > 0 ? 0 : r.whole;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      int bin;
-      double rest;
-      const int at = j * NT + i;
-      w[j] = at < n && (st.k == 0 || at < st.k) && weigh.bin_of(logit_of(v[j]), bin, rest) ? weigh.weight(bin, rest) : 0;
-      if (j == 1 && size <= NT) break;
-      upto[j] = before + block_scan<NT>(w[j], lds.waves, part);
-      before += part;
-    }
-    if (st.k > 0) whole = before;
-    const double enough = st.p * (double)whole;
+    uint64_t v[1] = {i < n ? r.list[i] : ~0ull}, w = 0, part;
+    sort_values<1>(v, n <= 64 ? 64 : kFew, lds.sort);
+    int bin;
+    double rest;
+    if (i < n && (st.k == 0 || i < st.k) && weigh.bin_of(logit_of(v[0]), bin, rest)) w = weigh.weight(bin, rest);
+    const uint64_t upto = block_scan<NT>(w, lds.waves, part);
+    const double enough = st.p * (double)(st.k > 0 ? part : r.whole);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (w[j] == 0 || (st.nucleus && !((double)(upto[j] - w[j]) < enough))) continue;
-      atomicMax((unsigned long long*)&lds.found[1], (unsigned long long)v[j]);
-      if (!((double)w[j] < st.floor)) atomicAdd((unsigned long long*)&lds.sums[(uint32_t)v[j] / kSegment], (unsigned long long)w[j]);
+    if (w > 0 && !(st.nucleus && !((double)((st.k > 0 ? 0 : r.before) + upto - w) < enough))) {
+      atomicMax((unsigned long long*)&lds.found[1], (unsigned long long)v[0]);
+      if (w >= st.floor) atomicAdd((unsigned long long*)&lds.sums[(uint32_t)v[0] / kSegment], (unsigned long long)w);
     }
     __syncthreads();
     last = lds.found[1];
@@ -589,7 +612,7 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
           f(lds.list[j], bin, rest);
         }
       } else {
-        over_segments<T, NT>(row, P.vocab, 0, P.segments, [&](float x, int index) {
+        Walk<T, NT>(row, P.vocab, 0, P.segments).run([&](float x, int index) {
           int bin;
           double rest;
           if (weigh.bin_of(x, bin, rest)) f(place_of(x, index), bin, rest);
@@ -601,7 +624,7 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
     int bin = r.bin;
     if (st.k > 0) {
       const auto enough = [&](uint64_t c) { return c >= (uint64_t)st.k; };
-      if (!cut_place<true>(weigh, lds, bin, before, last, last, each, enough)) last = cut_bits<true>(weigh, lds, bin, before, last, each, enough);
+      if (!cut_place<true>(weigh, lds, false, bin, before, last, last, each, enough)) last = cut_bits<true>(weigh, lds, bin, before, last, each, enough);
     }
     if (st.nucleus) {
       if (st.k > 0) {                        // the weights of what top-k kept, by bins
@@ -623,13 +646,13 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
       const auto enough = [&](uint64_t w) { return !((double)w < st.p * (double)whole); };
       if (st.k > 0) bin = cut_of(lds, kBins, before, enough);
       const uint64_t most = last;
-      if (!cut_place<false>(weigh, lds, bin, before, most, last, each, enough)) last = cut_bits<false>(weigh, lds, bin, before, most, each, enough);
+      if (!cut_place<false>(weigh, lds, st.k == 0, bin, before, most, last, each, enough)) last = cut_bits<false>(weigh, lds, bin, before, most, each, enough);
     }
     __syncthreads();
     each([&](uint64_t place, int b, double rest) {   // without top-k the segments' sums have the bins before the cut's
       if (place > last || (st.k == 0 && b != bin)) return;
       const uint64_t w = weigh.weight(b, rest);
-      if (!((double)w < st.floor)) atomicAdd((unsigned long long*)&lds.sums[(uint32_t)place / kSegment], (unsigned long long)w);
+      if (w >= st.floor) atomicAdd((unsigned long long*)&lds.sums[(uint32_t)place / kSegment], (unsigned long long)w);
     });
   }
   __syncthreads();
@@ -653,7 +676,7 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
     double rest;
     const bool is = weigh.bin_of(x, bin, rest) && place_of(x, index + j) <= last;
     w[j] = is ? weigh.weight(bin, rest) : 0;
-    if ((double)w[j] < st.floor) w[j] = 0;
+    if (w[j] < st.floor) w[j] = 0;
   }
   const uint64_t second = lds.found[0] + block_scan<NT>(w[0] + w[1], lds.waves, whole);
   if (w[0] > 0 && (double)(second - w[1]) > t) atomicMin(&lds.token, index);
