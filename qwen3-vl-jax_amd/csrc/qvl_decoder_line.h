@@ -23,6 +23,9 @@ struct DecodeState {
   SplitJob* split;                                                      // streaming: [runs]
   int slot_rows;                                                        // streaming: rows a part's slot has
   int tile;                                                             // rows of a tile: 32, or 16 (FewWave)
+  int shift = 5;                                                        // streaming: 2^shift keys a block of the line
+  int pad = 0;                                                          // blocks that a job counts for beside its own
+  int keep = -1;                                                        // blocks of a job that stays whole; -1: a run's share
 };
 
 // A barrier for what lies in LDS alone: __syncthreads also waits until stores to memory are through (3 us of a launch of 20).
@@ -98,8 +101,8 @@ __device__ __forceinline__ bool bad_keys(const AttnParams& P, int64_t start, int
 // ---------------------------------------------------------------------------------------------
 // streaming
 // ---------------------------------------------------------------------------------------------
-// What the line holds of a sequence: its jobs (tiles of S.tile rows), and the blocks of 32 keys of each, one where there is
-// nothing to read, for the rows' zeros (or NaN).
+// What the line holds of a sequence: its jobs (tiles of S.tile rows), and the blocks of 2^S.shift keys of each, one where there is
+// nothing to read, for the rows' zeros (or NaN), and S.pad before them.
 struct Sequence {
   int64_t token0, start;
   int tokens, len, jobs, blocks;
@@ -111,7 +114,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttnParams& P, const Decod
   q.start = S.k_start ? S.k_start[seq] : 0;   // (a page table has rows of its own)
   q.len = S.k_len[seq];
   q.jobs = (int)(((int64_t)q.tokens * P.group + S.tile - 1) / S.tile);
-  q.blocks = bad_keys(P, q.start, q.len) ? 1 : max((q.len + 31) >> 5, 1);
+  q.blocks = (bad_keys(P, q.start, q.len) ? 1 : max((int)((q.len + (1ll << S.shift) - 1) >> S.shift), 1)) + S.pad;
   return q;
 }
 
@@ -147,9 +150,10 @@ __device__ __forceinline__ Sequence uniform(Sequence q) {
 // Where run i of n begins: an equal share of the line, moved to a job's end where the job is no longer than a share (or a
 // block for each wave), so that short jobs stay whole. `base`: where the jobs of the sequence that the share begins in do.
 __device__ __forceinline__ int64_t share(int64_t total, int i, int n) { return total / n * i + total % n * i / n; }
-__device__ __forceinline__ int64_t run_start(int64_t total, int64_t pos, int n, int64_t base, int blocks) {
+__device__ __forceinline__ int64_t run_start(int64_t total, int64_t pos, int n, int64_t base, int blocks, int pad, int keep) {
   const int in = (int)((pos - base) % blocks);
-  return in == 0 || blocks > max((int64_t)4, total / n) ? pos : pos - in + (2 * in < blocks ? 0 : blocks);
+  if (in <= pad) return pos - in;             // no run begins inside the padding
+  return blocks > max((int64_t)4, keep < 0 ? total / n : keep) ? pos : pos - in + (2 * in < blocks ? 0 : blocks);
 }
 
 // The line as one workgroup sees it. Up to 64 sequences: one a lane, and each wave finds its way without the others. More: a
@@ -210,7 +214,8 @@ __device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState&
         if (i == n) return (int64_t)sum;
         const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane(mine.blocks, at);
         const uint32_t in = (p - (uint32_t)__builtin_amdgcn_readlane(x - own, at)) % blocks;
-        return (int64_t)(in == 0 || blocks > max(4u, each) ? p : p - in + (2 * in < blocks ? 0 : blocks));
+        if (in <= (uint32_t)S.pad) return (int64_t)(p - in);
+        return (int64_t)(blocks > max(4u, S.keep < 0 ? each : (uint32_t)S.keep) ? p : p - in + (2 * in < blocks ? 0 : blocks));
       };
       int other = 0;
       end = start(run + 1, other);
@@ -243,7 +248,7 @@ __device__ __forceinline__ void find_run(const AttnParams& P, const DecodeState&
     const int64_t p = share(total, i, n);
     if (p >= total) return total;
     locate(P, S, L, p, per, at, first);
-    return run_start(total, p, n, first, uniform(sequence_of(P, S, at).blocks));
+    return run_start(total, p, n, first, uniform(sequence_of(P, S, at).blocks), S.pad, S.keep);
   };
   int other = 0;
   int64_t other_base = 0;

@@ -18,23 +18,21 @@
 namespace qvl {
 
 // x rounded to `PARTS` bf16 parts, the largest first (PARTS 3: exact).
-template <int PARTS, int N> __device__ __forceinline__ void bf16_parts(const float (&x)[N], bf16x8 (&out)[PARTS]) {
-  static_assert(N == 8, "an operand");
-  float rest[8];
+template <int PARTS, int N> __device__ __forceinline__ void bf16_parts(const float (&x)[N], uint32_t (&out)[PARTS][N / 2]) {
+  float rest[N];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+  for (int j = 0; j < N; ++j) rest[j] = x[j];
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
-    u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = pack_bf16x2(rest[2 * j], rest[2 * j + 1]);
+    for (int j = 0; j < N / 2; ++j) {
+      const uint32_t w = pack_bf16x2(rest[2 * j], rest[2 * j + 1]);
+      out[p][j] = w;
       if (p + 1 < PARTS) {
-        rest[2 * j] -= bf16_lo(w[j]);
-        rest[2 * j + 1] -= bf16_hi(w[j]);
+        rest[2 * j] -= bf16_lo(w);
+        rest[2 * j + 1] -= bf16_hi(w);
       }
     }
-    out[p] = __builtin_bit_cast(bf16x8, w);
   }
 }
 
@@ -50,47 +48,85 @@ __device__ __forceinline__ f32x4 product(const bf16x8& a, const bf16x8& b, const
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-template <typename T, int D> struct PagedCore {
+// The lane `BY` lanes on in its row of 16 (round).
+template <int BY> __device__ __forceinline__ float turned(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + BY, 0xf, 0xf, false));
+}
+
+// A step of a wave: kTiles tiles of 16 keys, ROWS rows. Where the rows are 8 or 4, the 16 columns of a product hold 2 or 4 copies of
+// them, and copy c (columns ROWS c on) keeps the scores of tile c alone: the scores of 2 or 4 tiles lie in the registers of one, and the
+// softmax and the scales take a half or a quarter of the instructions. In the second product each copy's weights meet its own tile (the
+// others' are masked), so that the copies hold sums over different keys, which finish() adds.
+template <typename T, int D, int ROWS> struct PagedCore {
   using B = PageBlock<D>;
-  static constexpr int kRows = 16, kParts = std::is_same<T, float>::value ? 3 : 1, kG = B::kGroups, kSteps = D / 32, kDB = D / 16;
-  static constexpr int kWords = D / 32;        // words of K, of V and of either's scales that a lane has of 16 keys
-  bf16x8 q[kSteps][kParts];                    // step 2 g + s (D = 64: s): the dims of group g in piece 2 quad + s
+  static constexpr int kRows = ROWS, kPack = 16 / ROWS, kTiles = kPack == 4 ? 4 : 2, kSets = kTiles / kPack;
+  static constexpr int kParts = std::is_same<T, float>::value ? 3 : 1, kG = B::kGroups, kDB = D / 16;
+  static constexpr int kWords = D / 32;        // words of K, of V and of either's scales that a lane has of a tile
+  bf16x8 q[D / 32][kParts];                    // step 2 g + s (D = 64: s): the dims of group g in piece 2 quad + s
   f32x4 o[kDB];                                // D = 128: dims 64 (db / 4) + 4 r + db % 4, r = 4 quad + i; D = 64: 4 r + db
   float l;
 
   static __device__ __forceinline__ int quad() { return (threadIdx.x & 63) >> 4; }
+  static __device__ __forceinline__ int copy() { return (threadIdx.x & 15) / ROWS; }
   __device__ __forceinline__ void init(const char* qrow) {
     constexpr int E = D / 16;
     const T* x = reinterpret_cast<const T*>(qrow);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int d = (2 * quad() + s) * E;
-      float lo[E], hi[E];
+      float lo[8], hi[8];                      // D = 64: both halves in the first
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         lo[j] = (float)x[d + j];
-        hi[j] = (float)x[D / 2 + d + j];
+        (D == 128 ? hi[j] : lo[E + j]) = (float)x[D / 2 + d + j];
       }
-      if constexpr (D == 128) {
-        bf16_parts<kParts>(lo, q[s]);
-        bf16_parts<kParts>(hi, q[2 + s]);
-      } else {
-        const float both[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        bf16_parts<kParts>(both, q[s]);
-      }
+      set(q[s], lo);
+      if constexpr (D == 128) set(q[2 + s], hi);
     }
 #pragma unroll
     for (auto& y : o) y = f32x4{0.f, 0.f, 0.f, 0.f};
     l = 0.f;
+  }
+  static __device__ __forceinline__ void set(bf16x8 (&to)[kParts], const float (&x)[8]) {
+    uint32_t w[kParts][4];
+    bf16_parts<kParts>(x, w);
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) to[p] = __builtin_bit_cast(bf16x8, u32x4{w[p][0], w[p][1], w[p][2], w[p][3]});
   }
   __device__ __forceinline__ void rescale(float a) {
 #pragma unroll
     for (auto& y : o) y *= a;
     l *= a;
   }
+  // the copies' sums, in all of them
+  __device__ __forceinline__ void finish() {
+    if constexpr (kPack > 1) {
+      const auto add = [](float& x) {
+        x += turned<8>(x);
+        if constexpr (kPack == 4) x += turned<4>(x);
+      };
+#pragma unroll
+      for (auto& y : o)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = y[i];
+          add(x);
+          y[i] = x;
+        }
+      add(l);
+    }
+  }
   __device__ __forceinline__ float row_sum() const {
     const float x = l + __shfl_xor(l, 16);
     return x + __shfl_xor(x, 32);
+  }
+  static __device__ __forceinline__ float row_max(float x) {
+    if constexpr (kPack > 1) x = fmaxf(x, turned<8>(x));
+    if constexpr (kPack == 4) x = fmaxf(x, turned<4>(x));
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
   }
   template <typename F> __device__ __forceinline__ void each4(F&& f) const {
 #pragma unroll
@@ -99,152 +135,187 @@ template <typename T, int D> struct PagedCore {
       for (int i = 0; i < 4; ++i) f(64 * g + 16 * quad() + 4 * i, f32x4{o[4 * g][i], o[4 * g + 1][i], o[4 * g + 2][i], o[4 * g + 3][i]});
   }
 
-  // What a lane holds of 16 keys.
-  struct Keys {
-    uint32_t k[kWords], v[kWords], ks[kWords], vs[kWords];
-    static __device__ __forceinline__ void load(uint32_t (&w)[kWords], const char* p) {
-      if constexpr (kWords == 4) *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(p);
-      else *reinterpret_cast<u32x2*>(w) = *reinterpret_cast<const u32x2*>(p);
-    }
-    __device__ __forceinline__ void load(const char* block) {
-      const int r = threadIdx.x & 15;
-      load(k, block + B::k_piece(r, 2 * quad()));
-      load(v, block + B::v_word(4 * quad(), r));
-      load(ks, block + B::k_scale(4 * quad()));
-      load(vs, block + B::v_scale(4 * quad()));
-    }
-    // scale of token i of the quad, group g
-    static __device__ __forceinline__ float scale(const uint32_t (&w)[kWords], int i, int g) {
-      const int at = i * kG + g;
-      return at & 1 ? bf16_hi(w[at >> 1]) : bf16_lo(w[at >> 1]);
-    }
-  };
+  // A lane's words out of a place of the ring (below): codes of a tile's K, of its V, the scales of the quad's four tokens.
+  using Words = uint32_t[kWords];
+  static __device__ __forceinline__ void load(Words& w, const char* p) {
+    if constexpr (kWords == 4) *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(p);
+    else *reinterpret_cast<u32x2*>(w) = *reinterpret_cast<const u32x2*>(p);
+  }
+  static __device__ __forceinline__ void load_k(Words& w, const char* place) {
+    const int lane = threadIdx.x & 63;
+    load(w, place + (D == 128 ? lane * 16 : (quad() >> 1) * 256 + (lane & 15) * 16 + (quad() & 1) * 8));
+  }
+  static __device__ __forceinline__ void load_v(Words& w, const char* place) { load(w, place + B::kCodes + (threadIdx.x & 63) * kWords * 4); }
+  template <bool V> static __device__ __forceinline__ void load_scales(Words& w, const char* place) {
+    load(w, place + 2 * B::kCodes + (V ? B::kScales : 0) + quad() * kWords * 4);
+  }
+  // of token i of the quad, group g
+  static __device__ __forceinline__ float scale(const Words& w, int i, int g) {
+    const int at = i * kG + g;
+    return at & 1 ? bf16_hi(w[at >> 1]) : bf16_lo(w[at >> 1]);
+  }
 
-  __device__ __forceinline__ f32x4 scores(const Keys& x) const {
-    f32x4 s;
+  // The scores of a step whose first place is `mem`: s[set][i] is key 16 (kPack set + copy) + 4 quad + i.
+  __device__ __forceinline__ void scores(const char* mem, int place, f32x4 (&s)[kSets]) const {
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int set = 0; set < kSets; ++set) {
+      f32x4 sum[kG];
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const bf16x8 k = numbers8(x.k[kG * st + g]);
+      for (int c = 0; c < kPack; ++c) {
+        Words k;
+        load_k(k, mem + (set * kPack + c) * place);
 #pragma unroll
-        for (int p = kParts - 1; p >= 0; --p) acc = product(k, q[2 * g + st][p], acc);
+        for (int g = 0; g < kG; ++g) {
+          f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const bf16x8 x = numbers8(k[kG * st + g]);
+#pragma unroll
+            for (int p = kParts - 1; p >= 0; --p) acc = product(x, q[2 * g + st][p], acc);
+          }
+          if (c == 0) sum[g] = acc;
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[g][i] = copy() == c ? acc[i] : sum[g][i];
+        }
       }
+      Words sc;
+      load_scales<false>(sc, mem + (set * kPack + copy()) * place);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float sc = Keys::scale(x.ks, i, g);
-        s[i] = g == 0 ? sc * acc[i] : __builtin_fmaf(sc, acc[i], s[i]);
+        s[set][i] = scale(sc, i, 0) * sum[0][i];
+        if constexpr (kG == 2) s[set][i] = __builtin_fmaf(scale(sc, i, 1), sum[1][i], s[set][i]);
       }
     }
-    return s;
   }
 
   // bytes whose low nibble is a code of a and whose high one is b's of the same dim: the even dims, the odd ones
   static __device__ __forceinline__ uint32_t even_pairs(uint32_t a, uint32_t b) { return (a & 0x0f0f0f0fu) | (b << 4 & 0xf0f0f0f0u); }
   static __device__ __forceinline__ uint32_t odd_pairs(uint32_t a, uint32_t b) { return (a >> 4 & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u); }
 
-  // o += V^T P^T of two blocks of 16 keys, weights w (scaled below); `seen`: a bit for each key that the row sees, where EDGE
-  template <bool EDGE> __device__ __forceinline__ void values(const Keys (&x)[2], const f32x4 (&w)[2], uint32_t seen) {
-    uint32_t even[2][2], odd[2][2];            // [block][tokens (0, 1), (2, 3)]
+  // o += V^T P^T of the step, weights w (V's scales come in here); `seen`: a bit for each key of the lane that the row sees, where EDGE.
+  // `read` runs once the step's places are read.
+  template <bool EDGE, typename F>
+  __device__ __forceinline__ void values(const char* mem, int place, const f32x4 (&w)[kSets], uint32_t seen, F&& read) {
+    Words sc[kSets], v[kTiles];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      l += (w[b][0] + w[b][1]) + (w[b][2] + w[b][3]);
-      if constexpr (D == 128) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          even[b][h] = even_pairs(x[b].v[2 * h], x[b].v[2 * h + 1]);
-          odd[b][h] = odd_pairs(x[b].v[2 * h], x[b].v[2 * h + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {          // two tokens a word: the second's codes are 16 bits on
-          even[b][h] = even_pairs(x[b].v[h], x[b].v[h] >> 16);
-          odd[b][h] = odd_pairs(x[b].v[h], x[b].v[h] >> 16);
-        }
-      }
+    for (int set = 0; set < kSets; ++set) {
+      load_scales<true>(sc[set], mem + (set * kPack + copy()) * place);
+      l += (w[set][0] + w[set][1]) + (w[set][2] + w[set][3]);
     }
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      float p[8];
+    for (int t = 0; t < kTiles; ++t) load_v(v[t], mem + t * place);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    read();
+    uint32_t p[kSets][kG][kParts][2];          // weights times scales, bf16
+#pragma unroll
+    for (int set = 0; set < kSets; ++set)
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = w[set][i] * scale(sc[set], i, g);
+          if (EDGE) x[i] = (seen >> (4 * set + i)) & 1 ? x[i] : 0.f;   // an unseen key's scale may be anything
+        }
+        bf16_parts<kParts>(x, p[set][g]);
+      }
+#pragma unroll
+    for (int pair = 0; pair < kTiles / 2; ++pair) {
+      uint32_t even[2][2], odd[2][2];          // [tile][tokens (0, 1), (2, 3)]
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[4 * b + i] = w[b][i] * Keys::scale(x[b].vs, i, g);
-          if (EDGE) p[4 * b + i] = (seen >> (4 * b + i)) & 1 ? p[4 * b + i] : 0.f;   // an unseen key's scale may be anything
+        for (int h = 0; h < 2; ++h) {
+          // (D = 64: two tokens a word, the second's codes 16 bits on)
+          const uint32_t x = D == 128 ? v[2 * pair + b][(2 * h) % kWords] : v[2 * pair + b][h];
+          const uint32_t y = D == 128 ? v[2 * pair + b][(2 * h + 1) % kWords] : v[2 * pair + b][h] >> 16;
+          even[b][h] = even_pairs(x, y);
+          odd[b][h] = odd_pairs(x, y);
         }
-      bf16x8 pw[kParts];
-      bf16_parts<kParts>(p, pw);
-      auto add = [&](int db, uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
-        const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{a0, a1, b0, b1});
 #pragma unroll
-        for (int q = kParts - 1; q >= 0; --q) o[db] = product(v, pw[q], o[db]);
-      };
-      if (g == 0) {                            // bytes 0 and 1: dims 4 r + (0, 1), (2, 3) of the first group
-        add(0, numbers<0>(even[0][0]), numbers<0>(even[0][1]), numbers<0>(even[1][0]), numbers<0>(even[1][1]));
-        add(1, numbers<0>(odd[0][0]), numbers<0>(odd[0][1]), numbers<0>(odd[1][0]), numbers<0>(odd[1][1]));
-        add(2, numbers<1>(even[0][0]), numbers<1>(even[0][1]), numbers<1>(even[1][0]), numbers<1>(even[1][1]));
-        add(3, numbers<1>(odd[0][0]), numbers<1>(odd[0][1]), numbers<1>(odd[1][0]), numbers<1>(odd[1][1]));
-      } else {
-        add(4, numbers<2>(even[0][0]), numbers<2>(even[0][1]), numbers<2>(even[1][0]), numbers<2>(even[1][1]));
-        add(5, numbers<2>(odd[0][0]), numbers<2>(odd[0][1]), numbers<2>(odd[1][0]), numbers<2>(odd[1][1]));
-        add(6, numbers<3>(even[0][0]), numbers<3>(even[0][1]), numbers<3>(even[1][0]), numbers<3>(even[1][1]));
-        add(7, numbers<3>(odd[0][0]), numbers<3>(odd[0][1]), numbers<3>(odd[1][0]), numbers<3>(odd[1][1]));
+      for (int g = 0; g < kG; ++g) {
+        bf16x8 pw[kParts];
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) {
+          u32x4 x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int tile = 2 * pair + j / 2;
+            x[j] = p[tile / kPack][g][n][j & 1] & (kPack == 1 || copy() == tile % kPack ? ~0u : 0u);
+          }
+          pw[n] = __builtin_bit_cast(bf16x8, x);
+        }
+        const auto add = [&](int db, uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+          const bf16x8 x = __builtin_bit_cast(bf16x8, u32x4{a0, a1, b0, b1});
+#pragma unroll
+          for (int n = kParts - 1; n >= 0; --n) o[db] = product(x, pw[n], o[db]);
+        };
+        if (g == 0) {                          // bytes 0 and 1: dims 4 r + (0, 1), (2, 3) of the first group
+          add(0, numbers<0>(even[0][0]), numbers<0>(even[0][1]), numbers<0>(even[1][0]), numbers<0>(even[1][1]));
+          add(1, numbers<0>(odd[0][0]), numbers<0>(odd[0][1]), numbers<0>(odd[1][0]), numbers<0>(odd[1][1]));
+          add(2, numbers<1>(even[0][0]), numbers<1>(even[0][1]), numbers<1>(even[1][0]), numbers<1>(even[1][1]));
+          add(3, numbers<1>(odd[0][0]), numbers<1>(odd[0][1]), numbers<1>(odd[1][0]), numbers<1>(odd[1][1]));
+        } else {
+          add(kDB - 4, numbers<2>(even[0][0]), numbers<2>(even[0][1]), numbers<2>(even[1][0]), numbers<2>(even[1][1]));
+          add(kDB - 3, numbers<2>(odd[0][0]), numbers<2>(odd[0][1]), numbers<2>(odd[1][0]), numbers<2>(odd[1][1]));
+          add(kDB - 2, numbers<3>(even[0][0]), numbers<3>(even[0][1]), numbers<3>(even[1][0]), numbers<3>(even[1][1]));
+          add(kDB - 1, numbers<3>(odd[0][0]), numbers<3>(odd[0][1]), numbers<3>(odd[1][0]), numbers<3>(odd[1][1]));
+        }
       }
     }
   }
 };
 
-// One wave: 16 rows over blocks of 32 keys.
-template <typename T, int D> struct PagedWave : RowState<PagedCore<T, D>> {
-  using C = PagedCore<T, D>;
-  using Keys = typename C::Keys;
+// One wave: its rows over steps of keys.
+template <typename T, int D, int ROWS> struct PagedWave : RowState<PagedCore<T, D, ROWS>> {
+  using C = PagedCore<T, D, ROWS>;
   using RowState<C>::core;
   using RowState<C>::lim;
   using RowState<C>::lim_lo;
 
-  // 32 keys from kb on; bad: which of the two blocks of 16 lies in a page outside the cache (its keys' scores are NaN)
-  template <bool EDGE> __device__ __forceinline__ void step(const Keys (&x)[2], int kb, float scale, int bad) {
-    f32x4 s[2];
+  // The step of key kb on, in places from mem on; bad: which of its tiles lie in a page outside the cache (their keys' scores are NaN).
+  template <bool EDGE, typename F> __device__ __forceinline__ void step(const char* mem, int place, int kb, float scale, uint32_t bad, F&& read) {
+    f32x4 s[C::kSets];
     uint32_t seen = 0;
+    core.scores(mem, place, s);
+    float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = core.scores(x[b]);
+    for (int set = 0; set < C::kSets; ++set) {
+      const int tile = set * C::kPack + C::copy();
+      if (bad != 0 && (bad >> tile & 1)) s[set] = f32x4{NAN, NAN, NAN, NAN};
+      if (EDGE) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[b][i] *= scale;
-        if (bad & (1 << b)) s[b][i] = NAN;
-        if (EDGE) {
-          const bool in = kb + 16 * b + 4 * C::quad() + i < lim;
-          seen |= (in ? 1u : 0u) << (4 * b + i);
-          s[b][i] = in ? s[b][i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          const bool in = kb + 16 * tile + 4 * C::quad() + i < lim;
+          seen |= (in ? 1u : 0u) << (4 * set + i);
+          s[set][i] = in ? s[set][i] : -INFINITY;
         }
       }
+      mx = fmaxf(fmaxf(mx, s[set][0]), s[set][1]);
+      mx = fmaxf(fmaxf(mx, s[set][2]), s[set][3]);
     }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    this->cover(mx);
+    this->cover(C::row_max(mx) * scale);
     const float shift = this->shift();
-    f32x4 w[2];
+    f32x4 w[C::kSets];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int set = 0; set < C::kSets; ++set)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[b][i] = __builtin_amdgcn_exp2f(s[b][i] + shift);
-    core.template values<EDGE>(x, w, seen);
+      for (int i = 0; i < 4; ++i) w[set][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[set][i], scale, shift));
+    core.template values<EDGE>(mem, place, w, seen, read);
   }
 };
 
-// Where a wave's blocks of 16 keys lie: of its next 32 steps' 64 blocks, one a lane.
-template <int D> struct PageWalk {
+// Where a wave's tiles lie: of its next steps' 64 tiles, one a lane.
+template <int D, int TILES> struct PageWalk {
+  static constexpr int kSteps = 64 / TILES;
   const Pages& pages;
   int64_t seq;
-  int kvh, last;                               // the last block of 16 that holds a key
-  const char* at;                              // the lane's block; NULL: its page is none
-  __device__ __forceinline__ void look(int t) {   // steps t, t + 4, ..., of two blocks each
+  int kvh, last;                               // the last tile that holds a key
+  const char* at;                              // the lane's tile; NULL: its page is none
+  __device__ __forceinline__ void look(int t) {   // steps t, t + 4, ...
     const int lane = threadIdx.x & 63;
-    const int b = min(2 * (t + 4 * (lane >> 1)) + (lane & 1), last);
+    const int b = (int)min((int64_t)TILES * (t + 4 * (lane / TILES)) + lane % TILES, (int64_t)last);
     const int page = pages.page(seq, b >> (pages.shift - 4));
     at = page < 0 ? nullptr : pages.block<D>(page, kvh, b << 4);
   }
@@ -254,89 +325,127 @@ template <int D> struct PageWalk {
   }
 };
 
-// A workgroup's four waves over blocks [t0, t1) of 32 keys, every fourth to a wave, a step's loads one step ahead.
-template <typename T, int D>
-__device__ __forceinline__ void paged_run(const AttnParams& P, const Pages& pages, int seq, const Unit& u, PagedWave<T, D>& w, int t0, int t1) {
-  using Keys = typename PagedCore<T, D>::Keys;
+// 4 bytes per lane, global -> LDS, as dma16.
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" :: "v"(voff), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
+// A wave's own ring of steps in LDS, filled by DMA kDepth steps ahead, so that a step's loads take no registers (with a step's loads one
+// step ahead in registers the loop's copies of them waited for them). Steps of 64 keys go one ahead: 70 KB of a CU are under way, and
+// with twice that memory gives less (a plain read of 415 MB: 6.5 TB/s with 32 KB of a CU under way, 5.2 with 256; 12 sequences of 32000
+// keys 87 us, not 92). A place is a block as it lies in memory, but for K, whose 16-byte pieces go where their lane reads them, 256
+// bytes a quad: 64 lanes then meet in no bank.
+template <int D, int TILES> struct Ring {
+  using B = PageBlock<D>;
+  static constexpr int kDepth = TILES == 4 ? 1 : 2, kPlace = 2 * B::kCodes + 256, kStep = TILES * kPlace, kWave = kDepth * kStep;
+  static constexpr int kLoads = TILES * (D == 128 ? 3 : 2);    // a step's
+  uint32_t lds;
+  const char* mem;
+  __device__ __forceinline__ explicit Ring(char* smem) {
+    mem = smem + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWave;
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr_of(mem));
+  }
+  // tile b of the step that takes place `at`
+  __device__ __forceinline__ void fill(int at, int b, const char* block) const {
+    const uint32_t lane = threadIdx.x & 63, to = lds + at * kStep + b * kPlace;
+    // (no page: a range of nothing, which reads nothing)
+    const u32x4 rsrc = rsrc_words(block, block ? B::kBytes : 0);
+    if constexpr (D == 128) {
+      dma16(rsrc, (lane & 15) * 64 + (lane >> 4) * 16, 0, to);
+      dma16(rsrc, B::kCodes + lane * 16, 0, to + B::kCodes);
+    } else {
+      dma16(rsrc, lane < 32 ? (lane & 15) * 32 + (lane >> 4) * 16 : lane * 16, 0, to);
+    }
+    dma4(rsrc, 2 * B::kCodes + lane * 4, to + 2 * B::kCodes);   // the scales; the lanes behind them read nothing
+  }
+};
+
+// A workgroup's four waves over steps [t0, t1), every fourth to a wave.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ void paged_run(const AttnParams& P, const Pages& pages, int seq, const Unit& u, PagedWave<T, D, ROWS>& w, char* smem, int t0, int t1) {
+  constexpr int kTiles = PagedCore<T, D, ROWS>::kTiles;
+  using R = Ring<D, kTiles>;
+  using Walk = PageWalk<D, kTiles>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int t = t0 + wave;
-  if (t >= t1) return;
-  PageWalk<D> walk{pages, seq, u.kvh, (u.len - 1) >> 4, nullptr};
-  Keys x[2][2];
-  int bad[2], n = 0;
-  auto fetch = [&](int t, Keys (&y)[2], int& out) {
-    if ((n & 31) == 0) walk.look(t);
-    out = 0;
+  if (t < t1) {
+    const R ring(smem);
+    Walk walk{pages, seq, u.kvh, (u.len - 1) >> 4, nullptr};
+    int n = 0;
+    uint32_t bad = 0;                          // kTiles bits for each step under way
+    const auto fetch = [&] {                   // step n of the wave (behind the last one, the last again)
+      if (n % Walk::kSteps == 0) walk.look(t0 + wave + 4 * n);
+      bad >>= kTiles;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const char* block = walk.block(2 * (n & 31) + b);
-      if (block) y[b].load(block);
-      else {
-        out |= 1 << b;
-        y[b] = Keys{};
+      for (int b = 0; b < kTiles; ++b) {
+        const char* block = walk.block(kTiles * (n % Walk::kSteps) + b);
+        ring.fill(n % R::kDepth, b, block);
+        if (!block) bad |= 1u << (kTiles * (R::kDepth - 1) + b);
       }
+      ++n;
+    };
+#pragma unroll
+    for (int i = 0; i < R::kDepth; ++i) fetch();
+    for (int at = 0; t < t1; t += 4, at = at + 1 == R::kDepth ? 0 : at + 1) {
+      wait_loads<R::kLoads * (R::kDepth - 1)>();
+      const char* mem = ring.mem + at * R::kStep;
+      const int kb = t * 16 * kTiles;
+      const uint32_t now = bad & ((1u << kTiles) - 1);
+      if (kb + 16 * kTiles > w.lim_lo) w.template step<true>(mem, R::kPlace, kb, P.scale, now, fetch);
+      else w.template step<false>(mem, R::kPlace, kb, P.scale, now, fetch);
     }
-    ++n;
-  };
-  auto use = [&](int t, const Keys (&y)[2], int out) {
-    if (t * 32 + 32 > w.lim_lo) w.template step<true>(y, t * 32, P.scale, out);
-    else w.template step<false>(y, t * 32, P.scale, out);
-  };
-  fetch(t, x[0], bad[0]);
-  for (;;) {
-    if (t + 4 < t1) fetch(t + 4, x[1], bad[1]);
-    use(t, x[0], bad[0]);
-    if ((t += 4) >= t1) break;
-    if (t + 4 < t1) fetch(t + 4, x[0], bad[0]);
-    use(t, x[1], bad[1]);
-    if ((t += 4) >= t1) break;
+    wait_loads<0>();                           // the join takes the ring's memory
   }
+  w.core.finish();
 }
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_stream_kernel(AttnParams P, DecodeState S, Pages pages) {
-  using W = PagedWave<T, D>;
-  __shared__ __attribute__((aligned(16))) char smem[kJoinBytes<T, D, 16>];
-  __shared__ Line L;
+  using W = PagedWave<T, D, ROWS>;
+  constexpr int kLds = std::max({kJoinBytes<T, D, ROWS>, 4 * Ring<D, W::C::kTiles>::kWave, (int)sizeof(Line)});
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  Line& L = *reinterpret_cast<Line*>(smem);    // (before the ring is)
   const int run = blockIdx.x / P.hkv, kvh = blockIdx.x % P.hkv;
   int64_t total, pos, end, base = 0;
   int n, seq = 0;
   Sequence q;
   find_run(P, S, L, run, gridDim.x / P.hkv, total, n, pos, end, seq, base, q);
+  lds_barrier();
   SplitJob joined{};
   while (pos < end) {
-    const int blocks = q.blocks;
-    const int64_t own = (int64_t)q.jobs * blocks;
+    const int cost = q.blocks;                 // of a job: S.pad and its blocks
+    const int64_t own = (int64_t)q.jobs * cost;
     if (pos >= base + own) {           // the next sequence (jobs == 0: it has no rows)
       base += own;
       q = uniform(sequence_of(P, S, ++seq));
       continue;
     }
     const int64_t into = pos - base;
-    const int job = (int)(into / blocks), b0 = (int)(into % blocks);
-    const int b1 = (int)min((int64_t)blocks, b0 + (end - pos));
+    const int job = (int)(into / cost), c0 = (int)(into % cost), c1 = (int)min((int64_t)cost, c0 + (end - pos));
+    const int b0 = max(c0 - S.pad, 0), b1 = c1 - S.pad;
     const Unit u{nullptr, nullptr, q.len, q.len - q.tokens + 1, q.token0, q.tokens * P.group, job * W::kRows, kvh};
     const int n_rows = min(W::kRows, u.rows - u.row0);
-    const bool whole = b0 == 0 && b1 == blocks;
+    const bool whole = c0 == 0 && c1 == cost;
     if (bad_keys(P, 0, u.len)) {
       for (int i = threadIdx.x; i < n_rows * (D / 4); i += 256)
         store4<T>(out_row<T, D>(P, u, u.row0 + i / (D / 4)), i % (D / 4) * 4, f32x4{NAN, NAN, NAN, NAN});
     } else {
       W w;
       w.init(P, u, u.row0);
-      paged_run<T, D>(P, pages, seq, u, w, b0, min(b1, (u.len + 31) >> 5));
-      const int64_t slot = ((int64_t)(2 * run + (b0 == 0)) * P.hkv + kvh) * S.slot_rows;
-      join_waves<T, D>(P, u, w, smem, u.row0, b0 * 32, !whole, [&](int r) { return slot + r; });
+      paged_run<T, D, ROWS>(P, pages, seq, u, w, smem, b0, min(b1, (int)((u.len + (1ll << S.shift) - 1) >> S.shift)));
+      const int64_t slot = ((int64_t)(2 * run + (c0 == 0)) * P.hkv + kvh) * S.slot_rows;
+      join_waves<T, D>(P, u, w, smem, u.row0, b0 << S.shift, !whole, [&](int r) { return slot + r; });
     }
-    if (b0 > 0 && b1 == blocks) {
-      // the run that holds the job's first block: the last whose share begins there or before
-      const int64_t first = pos - b0;
+    if (c0 > 0 && c1 == cost) {
+      // the run that holds the job's first block: the last whose share begins there, in its padding or before
+      const int64_t first = pos - c0 + S.pad;
       int w0 = (int)min((int64_t)((float)first / (float)total * n), (int64_t)run);
       while (w0 > 0 && share(total, w0, n) > first) --w0;
       while (w0 < run && share(total, w0 + 1, n) <= first) ++w0;
       joined = SplitJob{u.token0, u.rows, u.row0, w0, run - w0 + 1};
     }
-    pos += b1 - b0;
+    pos += c1 - c0;
   }
   if (threadIdx.x == 0 && kvh == 0) S.split[run] = joined;
 }
@@ -356,7 +465,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams P, DecodeSta
 
 // How a launch is laid out: from the sizes alone, so that the workspace can be told beforehand.
 struct PagedPlan {
-  int runs, slot_rows;
+  int runs, slot_rows, tile;
   size_t part_rows, split_bytes;
 };
 
@@ -369,10 +478,12 @@ static int paged_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64_
   if (num_heads > kItemMaxHeads || n_tokens > kItemMaxLen || rows > kItemMaxLen) return set_error(QVL_ERR_UNSUPPORTED, "%s: sizes", what);
   D = PagedPlan{};
   const int64_t slots = (int64_t)gemm_device_cus() * 2;
-  const int64_t own_rows = (rows + std::max<int64_t>(n_seqs, 1) - 1) / std::max<int64_t>(n_seqs, 1);
-  const int64_t tiles = std::max<int64_t>((own_rows + 15) / 16, 1), jobs = n_seqs * tiles, blocks = jobs * ((max_len + 31) / 32);
+  const int64_t own_rows = (rows + std::max<int64_t>(n_seqs, 1) - 1) / std::max<int64_t>(n_seqs, 1);   // a sequence's, in the mean
+  D.tile = own_rows <= 4 ? 4 : own_rows <= 8 ? 8 : 16;
+  const int64_t tiles = std::max<int64_t>((own_rows + D.tile - 1) / D.tile, 1), keys = D.tile == 4 ? 64 : 32;
+  const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + keys - 1) / keys);
   D.runs = (int)std::max<int64_t>(std::min(slots / num_kv_heads, std::max((blocks + 3) / 4, jobs)), 1);
-  D.slot_rows = (int)std::min<int64_t>(16, std::max<int64_t>(rows, 1));
+  D.slot_rows = (int)std::min<int64_t>(D.tile, std::max<int64_t>(rows, 1));
   D.part_rows = (size_t)D.runs * num_kv_heads * 2 * D.slot_rows;
   D.split_bytes = round_up(D.runs * sizeof(SplitJob), 16);
   return QVL_OK;
@@ -424,8 +535,27 @@ int qvl_paged_attention(void* stream, int32_t dtype, const void* q, int64_t q_ro
   S.n_seqs = (int)n_seqs;
   S.split = (SplitJob*)workspace;
   S.slot_rows = plan.slot_rows;
-  S.tile = 16;
-  QVL_ATTN_LAUNCH(paged_stream_kernel, dim3((unsigned)(plan.runs * num_kv_heads)), P, S, pages);
+  S.tile = plan.tile;
+  S.shift = plan.tile == 4 ? 6 : 5;
+  // what a job costs beside its keys (rows, first loads, join), and jobs that are not worth a part: 96 sequences of up to 7900 keys
+  // 93 us, not 122 without either
+  S.pad = 12;
+  S.keep = 24;
+  const dim3 grid((unsigned)(plan.runs * num_kv_heads));
+#define QVL_PAGED(T, D)                                                                                                              \
+  do {                                                                                                                               \
+    if (plan.tile == 4) hipLaunchKernelGGL((paged_stream_kernel<T, D, 4>), grid, dim3(256), 0, (hipStream_t)stream, P, S, pages);    \
+    else if (plan.tile == 8) hipLaunchKernelGGL((paged_stream_kernel<T, D, 8>), grid, dim3(256), 0, (hipStream_t)stream, P, S, pages); \
+    else hipLaunchKernelGGL((paged_stream_kernel<T, D, 16>), grid, dim3(256), 0, (hipStream_t)stream, P, S, pages);                  \
+  } while (0)
+  if (dtype == QVL_DTYPE_BF16) {
+    if (head_dim == 128) QVL_PAGED(bf16, 128);
+    else QVL_PAGED(bf16, 64);
+  } else {
+    if (head_dim == 128) QVL_PAGED(float, 128);
+    else QVL_PAGED(float, 64);
+  }
+#undef QVL_PAGED
   QVL_TRY_RC(check_launch("paged_stream"));
   if (plan.runs == 1) return QVL_OK;
   QVL_ATTN_LAUNCH(paged_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)plan.slot_rows), P, S);
