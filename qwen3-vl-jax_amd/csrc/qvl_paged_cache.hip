@@ -2,9 +2,9 @@
 // way (the formulas of qvl_text_rotary.hip), and pages read back as rows.
 //
 // A group x of 64 values: s = bf16(fp32(max|x| / 6)), and for each value the number nearest to |x| / s; a tie goes to the even code. A
-// code is a step function: an error of one rounding next to a border moves it by a whole step. So it is decided exactly: a value that is stored as it
-// came is compared with s times the borders, which are exact in fp32, and a normalised and rotated key is formed in fp64 (sines and
-// cosines too), so that what the cache holds does not depend on the order of a sum. fp64 runs at fp32's rate here, and only keys need it.
+// code is a step function: an error of one rounding next to a border moves it by a whole step. So it is decided exactly for a value that
+// is stored as it came, and a normalised and rotated key is formed in fp64 (sines and cosines too), so that what the cache holds does
+// not depend on the order of a sum. fp64 runs at fp32's rate here, and only keys need it.
 //
 // Bound by memory: each value is read once, q and 4.25 bits a value of k and v are written. Eight lanes hold a head, as in
 // qvl_text_rotary.hip, and a wave eight heads of one token and one kind (q, k or v), so that no wave takes two paths; the four waves of a
@@ -40,10 +40,22 @@ __device__ __forceinline__ void sincos_turns64(uint64_t f, double& c, double& s)
   c = ((quarter + 1) & 2) ? -b : b;
 }
 
-// The sequence that row n is a token of: cu[i] <= n < cu[i + 1]; -1: of none. 64 entries at a time.
-__device__ __forceinline__ int sequence_at(const int32_t* cu, int n_seqs, int64_t n) {
+// The sequence that row n is a token of (cu[i] <= n < cu[i + 1]; -1: of none), and the token's place in it. Up to 63 sequences are looked
+// at by a lane each, their lengths on the way; more 64 at a time.
+__device__ __forceinline__ int place_of(const int32_t* cu, const int32_t* k_len, int n_seqs, int64_t n, int64_t& t) {
   const int lane = threadIdx.x & 63;
+  if (!cu) {
+    t = (int64_t)k_len[n] - 1;
+    return (int)n;
+  }
   int lo = 0, size = n_seqs + 1;
+  if (size <= 64) {
+    const int first = cu[min(lane, n_seqs)], length = k_len[min(lane, n_seqs - 1)];
+    const int seq = __popcll(__builtin_amdgcn_ballot_w64(lane < size && first <= n)) - 1;
+    if (seq < 0 || seq >= n_seqs) return -1;
+    t = (int64_t)__builtin_amdgcn_readlane(length, seq) - (__builtin_amdgcn_readlane(first, seq + 1) - n);
+    return seq;
+  }
   for (;;) {
     const int step = (size + 63) >> 6, at = lane * step;
     const bool in = at < size && cu[lo + at] <= n;
@@ -51,46 +63,96 @@ __device__ __forceinline__ int sequence_at(const int32_t* cu, int n_seqs, int64_
     if (c == 0) return -1;
     lo += (c - 1) * step;
     size = min(step, size - (c - 1) * step);
-    if (step == 1) return lo < n_seqs ? lo : -1;
+    if (step == 1) break;
   }
+  if (lo >= n_seqs) return -1;
+  t = (int64_t)k_len[lo] - (cu[lo + 1] - n);
+  return lo;
 }
 
-// The 8 lanes of a head: the largest |x| (infinite where a value is infinite or NaN).
-template <typename R, int E> __device__ __forceinline__ R largest(const R (&x)[E], R m) {
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const R a = fabs(x[i]);
-    m = a < (R)INFINITY ? (a > m ? a : m) : (R)INFINITY;
-  }
-  return m;
+// v of the lane that DPP control CTRL names.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+  return __hiloint2double((int)dpp<CTRL>((uint32_t)__double2hiint(v)), (int)dpp<CTRL>((uint32_t)__double2loint(v)));
 }
-template <typename R> __device__ __forceinline__ R over_head(R m) {
+// Over the 8 lanes of a head: neighbours, neighbouring pairs, the halves mirrored.
+template <typename R, typename F> __device__ __forceinline__ R over_head(R v, F&& f) {
+  v = f(v, dpp<0xb1>(v));
+  v = f(v, dpp<0x4e>(v));
+  return f(v, dpp<0x141>(v));
+}
+
+// max|x| / 6 of a group of which each of a head's lanes holds E values (N = 2: and E more), rounded to fp32; not finite where a value is not.
+// The bits of fp32 values order as their absolute values do, infinities and NaN above all.
+template <int E, int N> __device__ __forceinline__ float sixth(const float (&x)[N][E]) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) {
-    const R o = __shfl_xor(m, d);
-    m = o > m ? o : m;
-  }
-  return m;
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < E; ++i) m = max(m, __float_as_uint(x[n][i]) & 0x7fffffffu);
+  return __uint_as_float(over_head(m, [](uint32_t a, uint32_t b) { return max(a, b); })) / 6.0f;
+}
+template <int E, int N> __device__ __forceinline__ float sixth(const double (&x)[N][E]) {
+  double m = 0, wrong = 0;                     // wrong: NaN where a value is not finite
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      m = fmax(m, fabs(x[n][i]));
+      wrong = __builtin_fma(x[n][i], 0.0, wrong);
+    }
+  m = over_head(m, [](double a, double b) { return fmax(a, b); });
+  wrong = over_head(wrong, [](double a, double b) { return a + b; });
+  return (float)((m + wrong) / 6.0);
 }
 
 // The group's scale as bf16 bits, NaN where the group holds what is not finite (or is beyond it).
-template <typename R> __device__ __forceinline__ uint32_t scale_bits(R m) {
-  float s = (float)(m / (R)6);
+__device__ __forceinline__ uint32_t scale_bits(float s) {
   asm volatile("" : "+v"(s));   // rounded to fp32 first: the compiler makes one rounding of the two (7 of 288000 groups differ)
   const uint32_t b = pack_bf16x2(s, 0.f) & 0xffffu;
   return b < 0x7f80u ? b : 0x7fc0u;
 }
 
-// The codes of E values, 4 bits each.
-template <typename R, int E> __device__ __forceinline__ uint32_t codes_of(const R (&x)[E], uint32_t scale) {
-  const R s = (R)__uint_as_float(scale << 16);
+// The codes of E values x of a group of that scale, 4 bits each: x / s to the nearest of the numbers by the conversion to e2m1 (ties to
+// the even code, beyond 6 to 6), from an fp32 quotient that lies on a border between two codes only where x / s does.
+// fp32: the quotient rounded to nearest is such a one (s has 8 bits and a border 3, so x / s that is not a border differs from it by 2^-24 of it
+// or more); q = x (1/s), then its remainder times 1/s added, is rounded so, 1/s being. Far from the ends of the exponents, that is: tiny
+// groups are brought up by 2^64 first.
+template <int E> __device__ __forceinline__ uint32_t codes_of(const float (&x)[E], uint32_t scale) {
+  float s = __uint_as_float(scale << 16);
+  const float up = s < 0x1p-60f ? 0x1p64f : 1.0f;
+  s *= up;
+  const float inverse = s > 0.f ? 1.0f / s : 0.f;
   uint32_t w = 0;
+  float q[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const R a = fabs(x[i]);
-    const uint32_t c = (uint32_t)(a > (R)0.25 * s) + (a >= (R)0.75 * s) + (a > (R)1.25 * s) + (a >= (R)1.75 * s) + (a > (R)2.5 * s) +
-                       (a >= (R)3.5 * s) + (a > (R)5 * s) + (__builtin_signbit(x[i]) ? 8u : 0u);
-    w |= c << (4 * i);
+    const float a = x[i] * up, q0 = a * inverse;
+    q[i] = __builtin_fmaf(-__builtin_fmaf(q0, s, -a), inverse, q0);   // (zeros keep their sign)
+  }
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
+  if constexpr (E == 8) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
+  }
+  return w;
+}
+// fp64: cut to the upper word's 20 bits, the last of them set where anything was cut off, the quotient is exact in fp32.
+template <int E> __device__ __forceinline__ uint32_t codes_of(const double (&x)[E], uint32_t scale) {
+  const double s = (double)__uint_as_float(scale << 16), inverse = s > 0 ? 1.0 / s : 0.0;
+  uint32_t w = 0;
+  float q[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const double t = x[i] * inverse;
+    q[i] = (float)__hiloint2double(__double2hiint(t) | (int)min((uint32_t)__double2loint(t), 1u), 0);
+  }
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
+  if constexpr (E == 8) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
   }
   return w;
 }
@@ -132,21 +194,23 @@ template <int D, bool K> __device__ __forceinline__ void store_codes(char* block
 }
 
 template <int D, bool K, typename R, int E>
-__device__ __forceinline__ void pack_head(char* block, int token, int p, const R (&lo)[E], const R (&hi)[E]) {
+__device__ __forceinline__ void pack_head(char* block, int token, int p, const R (&x)[2][E]) {
   uint32_t sl, sh;
   if constexpr (D == 128) {
-    sl = scale_bits(over_head(largest(lo, (R)0)));
-    sh = scale_bits(over_head(largest(hi, (R)0)));
+    const R lo[1][E] = {{x[0][0], x[0][1], x[0][2], x[0][3], x[0][4], x[0][5], x[0][6], x[0][7]}};
+    const R hi[1][E] = {{x[1][0], x[1][1], x[1][2], x[1][3], x[1][4], x[1][5], x[1][6], x[1][7]}};
+    sl = scale_bits(sixth<E, 1>(lo));
+    sh = scale_bits(sixth<E, 1>(hi));
   } else {
-    sl = sh = scale_bits(over_head(largest(hi, largest(lo, (R)0))));
+    sl = sh = scale_bits(sixth<E, 2>(x));
   }
-  store_codes<D, K>(block, token, p, codes_of(lo, sl), codes_of(hi, sh), sl, sh);
+  store_codes<D, K>(block, token, p, codes_of<E>(x[0], sl), codes_of<E>(x[1], sh), sl, sh);
 }
 
 template <typename T, int D, bool ROTATE>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams P) {
   constexpr int E = D / 16;                   // values of each half a lane holds
-  constexpr int kHalfBytes = D / 2 * (int)sizeof(T);
+  constexpr int kWords = E * (int)sizeof(T) / 4, kHalfBytes = D / 2 * (int)sizeof(T);
   __shared__ double cs_all[4][D / 2][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = lane & 7;
   const int64_t n = (int64_t)(blockIdx.x / (uint32_t)P.chunks) * 4 + wave;
@@ -157,27 +221,42 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams P) 
   const bool live = h < (is_q ? P.hq : P.hkv);
   const HeadsView in = is_q ? P.q : is_k ? P.k : P.v;
   const char* src = in.p + n * in.row + h * in.head + part * E * (int)sizeof(T);
-  uint32_t lo_words[E * sizeof(T) / 4], hi_words[E * sizeof(T) / 4];
+  // everything that a lane reads is asked for before the first of it is waited for
+  uint32_t lo_words[kWords], hi_words[kWords];
   if (live) {
     load_words(src, lo_words);
     load_words(src + kHalfBytes, hi_words);
   }
-  const int seq = P.cu_q ? sequence_at(P.cu_q, P.n_seqs, n) : (int)n;
+  const bool turn = ROTATE && (is_q || is_k);
+  uint64_t turns = 0, axis = 0;
+  int32_t pos[3] = {0, 0, 0};
+  float w[2][E];
+  if (turn) {
+    const int f = min(lane, D / 2 - 1);
+    turns = P.table[2 * f];
+    axis = P.table[2 * f + 1];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) pos[i] = P.pos[i * P.pos_stride + n];
+    const float* weights = (is_q ? P.qw : P.kw) + part * E;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      w[0][i] = weights[i];
+      w[1][i] = weights[D / 2 + i];
+    }
+  }
+  int64_t t;
+  const int seq = place_of(P.cu_q, P.k_len, P.n_seqs, n, t);
   if (seq < 0) return;
   char* block = nullptr;
-  int token = 0;
   if (!is_q) {
-    const int64_t end = P.cu_q ? P.cu_q[seq + 1] : n + 1, t = (int64_t)P.k_len[seq] - (end - n);
     const int page = t < 0 ? -1 : P.pages.page(seq, t >> P.pages.shift);
     if (page < 0) return;
     block = P.pages.block<D>(page, min(h, P.hkv - 1), (int)t);
-    token = (int)t & 15;
   }
-  if constexpr (ROTATE) {
-    if (lane < D / 2 && (is_q || is_k)) {
-      const uint64_t turns = P.table[2 * lane];
-      const int axis = (int)min(P.table[2 * lane + 1], (uint64_t)2);
-      const uint64_t angle = (uint64_t)(int64_t)P.pos[axis * P.pos_stride + n] * turns;
+  const int token = (int)t & 15;
+  if (turn) {
+    const uint64_t angle = (uint64_t)(int64_t)(axis == 0 ? pos[0] : axis == 1 ? pos[1] : pos[2]) * turns;
+    if (lane < D / 2) {
       if (is_q) {
         float c, s;
         sincos_turns(angle, c, s);
@@ -189,7 +268,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams P) 
     __builtin_amdgcn_wave_barrier();            // the wave's own LDS: written and read in its program order
   }
   if (!live) return;
-  float lo[E], hi[E];
+  float x[2][E];
+  float(&lo)[E] = x[0], (&hi)[E] = x[1];
   values_of<T, E>(lo_words, lo);
   values_of<T, E>(hi_words, hi);
   if constexpr (ROTATE) {
@@ -205,7 +285,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams P) 
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const f32x2 cs = reinterpret_cast<const f32x2*>(cs_all[wave])[part * E + i];
-        const float a = lo[i] * r * P.qw[part * E + i], b = hi[i] * r * P.qw[D / 2 + part * E + i];
+        const float a = lo[i] * r * w[0][i], b = hi[i] * r * w[1][i];
         yl[i] = a * cs.x - b * cs.y;
         yh[i] = b * cs.x + a * cs.y;
       }
@@ -218,24 +298,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams P) 
       double ss = 0;
 #pragma unroll
       for (int i = 0; i < E; ++i) ss += (double)lo[i] * lo[i] + (double)hi[i] * hi[i];
-      ss += __shfl_xor(ss, 1);
-      ss += __shfl_xor(ss, 2);
-      ss += __shfl_xor(ss, 4);
+      ss = over_head(ss, [](double a, double b) { return a + b; });
       const double r = 1.0 / sqrt(ss * (1.0 / D) + P.eps);
-      double yl[E], yh[E];
+      double y[2][E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const double c = cs_all[wave][part * E + i][0], s = cs_all[wave][part * E + i][1];
-        const double a = lo[i] * r * P.kw[part * E + i], b = hi[i] * r * P.kw[D / 2 + part * E + i];
-        yl[i] = a * c - b * s;
-        yh[i] = b * c + a * s;
+        const double a = lo[i] * r * w[0][i], b = hi[i] * r * w[1][i];
+        y[0][i] = a * c - b * s;
+        y[1][i] = b * c + a * s;
       }
-      pack_head<D, true>(block, token, part, yl, yh);
+      pack_head<D, true>(block, token, part, y);
       return;
     }
   }
-  if (is_k) pack_head<D, true>(block, token, part, lo, hi);
-  else pack_head<D, false>(block, token, part, lo, hi);
+  if (is_k) pack_head<D, true>(block, token, part, x);
+  else pack_head<D, false>(block, token, part, x);
 }
 
 // A block of 16 tokens and one head a wave, 8 tokens at a time, 8 lanes a token; the lanes' codes lie as the append wrote them.
