@@ -361,32 +361,35 @@ template <int D, int TILES> struct Ring {
   }
 };
 
-// A workgroup's four waves over steps [t0, t1), every fourth to a wave.
+// A workgroup's four waves over steps [t0, t1), every fourth to a wave. The first steps are under way before the rows are read.
 template <typename T, int D, int ROWS>
 __device__ __forceinline__ void paged_run(const AttnParams& P, const Pages& pages, int seq, const Unit& u, PagedWave<T, D, ROWS>& w, char* smem, int t0, int t1) {
   constexpr int kTiles = PagedCore<T, D, ROWS>::kTiles;
   using R = Ring<D, kTiles>;
   using Walk = PageWalk<D, kTiles>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int t = t0 + wave;
-  if (t < t1) {
-    const R ring(smem);
-    Walk walk{pages, seq, u.kvh, (u.len - 1) >> 4, nullptr};
-    int n = 0;
-    uint32_t bad = 0;                          // kTiles bits for each step under way
-    const auto fetch = [&] {                   // step n of the wave (behind the last one, the last again)
-      if (n % Walk::kSteps == 0) walk.look(t0 + wave + 4 * n);
-      bad >>= kTiles;
+  int t = t0 + wave, n = 0;
+  const bool any = t < t1;
+  const R ring(smem);
+  Walk walk{pages, seq, u.kvh, (u.len - 1) >> 4, nullptr};
+  uint32_t bad = 0;                            // kTiles bits for each step under way
+  const auto fetch = [&] {                     // step n of the wave (behind the last one, the last again)
+    if (n % Walk::kSteps == 0) walk.look(t0 + wave + 4 * n);
+    bad >>= kTiles;
 #pragma unroll
-      for (int b = 0; b < kTiles; ++b) {
-        const char* block = walk.block(kTiles * (n % Walk::kSteps) + b);
-        ring.fill(n % R::kDepth, b, block);
-        if (!block) bad |= 1u << (kTiles * (R::kDepth - 1) + b);
-      }
-      ++n;
-    };
+    for (int b = 0; b < kTiles; ++b) {
+      const char* block = walk.block(kTiles * (n % Walk::kSteps) + b);
+      ring.fill(n % R::kDepth, b, block);
+      if (!block) bad |= 1u << (kTiles * (R::kDepth - 1) + b);
+    }
+    ++n;
+  };
+  if (any) {
 #pragma unroll
     for (int i = 0; i < R::kDepth; ++i) fetch();
+  }
+  w.init(P, u, u.row0);
+  if (any) {
     for (int at = 0; t < t1; t += 4, at = at + 1 == R::kDepth ? 0 : at + 1) {
       wait_loads<R::kLoads * (R::kDepth - 1)>();
       const char* mem = ring.mem + at * R::kStep;
@@ -432,7 +435,6 @@ __global__ __launch_bounds__(256, 2) void paged_stream_kernel(AttnParams P, Deco
         store4<T>(out_row<T, D>(P, u, u.row0 + i / (D / 4)), i % (D / 4) * 4, f32x4{NAN, NAN, NAN, NAN});
     } else {
       W w;
-      w.init(P, u, u.row0);
       paged_run<T, D, ROWS>(P, pages, seq, u, w, smem, b0, min(b1, (int)((u.len + (1ll << S.shift) - 1) >> S.shift)));
       const int64_t slot = ((int64_t)(2 * run + (c0 == 0)) * P.hkv + kvh) * S.slot_rows;
       join_waves<T, D>(P, u, w, smem, u.row0, b0 << S.shift, !whole, [&](int r) { return slot + r; });
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams P, DecodeSta
 
 // How a launch is laid out: from the sizes alone, so that the workspace can be told beforehand.
 struct PagedPlan {
-  int runs, slot_rows, tile;
+  int runs, slot_rows, tile, join_rows;   // join_rows: workgroups that share a job's rows in the join
   size_t part_rows, split_bytes;
 };
 
@@ -484,6 +486,8 @@ static int paged_plan(const char* what, int64_t n_tokens, int64_t n_seqs, int64_
   const int64_t jobs = n_seqs * tiles, blocks = jobs * ((max_len + keys - 1) / keys);
   D.runs = (int)std::max<int64_t>(std::min(slots / num_kv_heads, std::max((blocks + 3) / 4, jobs)), 1);
   D.slot_rows = (int)std::min<int64_t>(D.tile, std::max<int64_t>(rows, 1));
+  // up to 8 parts a workgroup joins 8 rows at once; with more a row each, so that its parts come in one trip to memory
+  D.join_rows = D.runs <= 8 * jobs ? (D.slot_rows + 7) / 8 : D.slot_rows;
   D.part_rows = (size_t)D.runs * num_kv_heads * 2 * D.slot_rows;
   D.split_bytes = round_up(D.runs * sizeof(SplitJob), 16);
   return QVL_OK;
@@ -558,7 +562,7 @@ int qvl_paged_attention(void* stream, int32_t dtype, const void* q, int64_t q_ro
 #undef QVL_PAGED
   QVL_TRY_RC(check_launch("paged_stream"));
   if (plan.runs == 1) return QVL_OK;
-  QVL_ATTN_LAUNCH(paged_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)plan.slot_rows), P, S);
+  QVL_ATTN_LAUNCH(paged_join_kernel, dim3((unsigned)plan.runs, (unsigned)num_kv_heads, (unsigned)plan.join_rows), P, S);
   return check_launch("paged_join");
 }
 

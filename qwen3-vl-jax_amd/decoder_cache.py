@@ -37,31 +37,34 @@ class PagedCache:
                    "qvl_paged_cache_size")
         self.page_bytes = nb.value // self.n_pages if self.n_pages else 0
         torch = _torch()
-        self.data = torch.zeros((self.n_pages, self.page_bytes), dtype=torch.uint8, device=_device(device))
+        self._data = torch.zeros((self.n_pages, self.page_bytes), dtype=torch.uint8, device=_device(device))
+        self._where = self._data.device
+        self._args = (self._data.data_ptr(), self.n_pages, self.page_rows)
+
+    @property
+    def data(self):
+        return self._data
 
 
 def _pages(cache: PagedCache, page_table, k_len, like, heads: Optional[int] = None):
     """The cache, the page table and the sequences' lengths as the entries take them: (cache and table arguments, number of
     sequences, k_len's pointer)."""
-    data = cache.data
-    if data.device != like[1]:
-        raise ValueError(f"the cache on {data.device}, q on {like[1]}")
-    if data.dtype != _torch().uint8 or data.shape != (cache.n_pages, cache.page_bytes) or not data.is_contiguous():
-        raise ValueError(f"the cache's data must be contiguous uint8 [{cache.n_pages}, {cache.page_bytes}]")
+    if cache._where != like[1]:
+        raise ValueError(f"the cache on {cache._where}, q on {like[1]}")
     if like[2] != cache.head_dim:
         raise ValueError(f"head_dim {like[2]}, the cache has {cache.head_dim}")
     if heads is not None and heads != cache.num_kv_heads:
         raise ValueError(f"{heads} key/value heads, the cache has {cache.num_kv_heads}")
-    shape = page_table.shape
-    if len(shape) != 2 or (page_table.stride(1) != 1 and shape[1] > 1):
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"page_table must be [sequences, pages] with a contiguous last axis, not {tuple(shape)}")
-    if page_table.dtype != _torch().int32:
+    int32 = _torch().int32
+    if page_table.dtype != int32:
         raise TypeError(f"page_table is {page_table.dtype}, expected torch.int32")
     if page_table.device != like[1]:
         raise ValueError(f"page_table on {page_table.device}, q on {like[1]}")
     n = shape[0]
-    return ((data.data_ptr(), cache.n_pages, cache.page_rows, page_table.data_ptr(), shape[1], page_table.stride(0) if n > 1 else 0),
-            n, _word(k_len, "k_len", like, _torch().int32, (n,)))
+    return ((*cache._args, page_table.data_ptr(), shape[1], stride[0] if n > 1 else 0), n, _word(k_len, "k_len", like, int32, (n,)))
 
 
 def _cu(cu_q, like, n_seqs: int, n_tokens: int):
