@@ -12,8 +12,10 @@
 // entries times a short polynomial and a power of two, in fp64 (an fp32 weight would be off by 2^20 of its units).
 //
 // Four launches, each over (share of the vocabulary, row) but the last, which is over rows: the largest logits, the histogram, the
-// list with the sums of segments of 1024 tokens, the choice. Bound by reading the logits, three times where there is a cut, the second
-// and third time from a cache; for few rows by the launches.
+// list with the sums of segments of 1024 tokens, the choice. The logits are read three times where there is a cut, the second and third
+// time from a cache. 256 rows of 151936, fp32, by top-p: 35 us for the largest (4.5 TB/s), 46 for the histogram (30 instructions a logit, most
+// of them for its weight: 76 % of the units' time), 37 for the list, 13 for the choice. One row: 3.3 + 4.7 + 5.3 + 7.6 us; a row whose
+// cut goes over it again in the last launch 170 to 210.
 #include "qvl_decoder.h"
 #include "qvl_kernels.h"
 
@@ -21,6 +23,7 @@ namespace qvl {
 
 constexpr int kBins = 1536, kSegment = 1024, kMaxSegments = 256, kList = 4096, kShare = 1024;   // kShare: a workgroup's of the list
 constexpr int kSort = 1024, kFew = 128;       // tokens that are sorted, and that are sorted without a look at parts of their bin
+constexpr int kSome = 512;                   // of a segment's 1024 tokens: up to which the list's pass packs those that it weighs
 constexpr int kRowsAtOnce = 1024;            // rows that share a workspace
 constexpr double kUnit = 17592186044416.0;   // 2^44
 
@@ -126,6 +129,11 @@ struct Weigher {
     // (plus 2^52: rounded to a whole number, which the low bits then hold)
     return (uint64_t)__double_as_longlong(e + 0x1p52) & 0xfffffffffffffull;
   }
+  // A number that no logit of bins up to `bin` lies below: the border, less what its own sums and its rounding to fp32 may be off by.
+  __device__ __forceinline__ float least(int bin) const {
+    const double down = (bin + 0.5) / scale;
+    return (float)(top - down - (fabs(top) + down) * 0x1p-22);
+  }
   __device__ __forceinline__ bool operator()(float x, int& bin, uint64_t& w) const {
     double r;
     if (!bin_of(x, bin, r)) return false;
@@ -225,16 +233,22 @@ template <typename T, int NT> struct Walk {
   __device__ __forceinline__ Walk(const char* row, int vocab, int s0, int s1) : row(row), vocab(vocab), s(s0 + (int)(threadIdx.x >> 6)), s1(s1) {
     if (s < s1) g.load(row, vocab, s);
   }
-  // f(x, index) for each, after(segment) behind each
-  template <typename F, typename G> __device__ __forceinline__ void run(F&& f, G&& after) {
+  // f(values, segment) for each segment of the wave
+  template <typename F> __device__ __forceinline__ void segments(F&& f) {
     for (; s < s1; s += NT / 64) {
       Segment<T> next;
       if (s + NT / 64 < s1) next.load(row, vocab, s + NT / 64);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f(g.x[i], s * kSegment + Segment<T>::index(i));
-      after(s);
+      f(g.x, s);
       g = next;
     }
+  }
+  // f(x, index) for each, after(segment) behind each
+  template <typename F, typename G> __device__ __forceinline__ void run(F&& f, G&& after) {
+    segments([&](const float (&x)[16], int s) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(x[i], s * kSegment + Segment<T>::index(i));
+      after(s);
+    });
   }
 };
 
@@ -345,6 +359,7 @@ template <typename F> __device__ __forceinline__ Cut cut_bin(const uint64_t (&h)
 template <typename T>
 __global__ __launch_bounds__(256) void sample_list_kernel(SampleParams P, int per) {
   __shared__ uint64_t waves[4], list[kShare];
+  __shared__ f32x2 kept[4][kSome];
   __shared__ double table[32];
   __shared__ Cut found;
   __shared__ uint32_t n, base;
@@ -366,7 +381,7 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleParams P, int pe
   if (st.k > 0) cut = cut_bin(h, waves, &found, [&](uint64_t c, uint64_t) { return c >= (uint64_t)st.k; });
   else if (st.nucleus) cut = cut_bin(h, waves, &found, [&](uint64_t w, uint64_t whole) { return !((double)w < st.p * (double)whole); });
   uint64_t sum = 0;
-  walk.run([&](float x, int index) {
+  const auto take = [&](float x, int index) {
     int bin;
     double rest;
     if (!weigh.bin_of(x, bin, rest) || bin > cut.bin) return;
@@ -382,7 +397,32 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleParams P, int pe
       const uint64_t w = weigh.weight(bin, rest);
       sum += w < st.floor ? 0 : w;
     }
-  }, [&](int s) {
+  };
+  // Most cuts leave few of a segment: those are put side by side first, and their weights formed 64 at a time (256 rows by top-p: 37 us,
+  // not 54; where more than half are left, or there is no cut, all in their places)
+  const float least = weigh.least(min(cut.bin, kBins - 1));
+  f32x2* const some = kept[threadIdx.x >> 6];
+  walk.segments([&](const float (&x)[16], int s) {
+    int left = cut.bin < kBins ? 0 : kSome + 1;
+    if (left == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) left += __popcll(__builtin_amdgcn_ballot_w64(x[i] >= least));
+    if (left <= kSome) {
+      int upto = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(x[i] >= least);
+        const int to = upto + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+        if (x[i] >= least) some[to] = f32x2{x[i], __uint_as_float((uint32_t)(s * kSegment + Segment<T>::index(i)))};
+        upto += __popcll(lanes);
+      }
+      __builtin_amdgcn_wave_barrier();         // the wave's own LDS: written and read in its program order
+      for (int j = threadIdx.x & 63; j < left; j += 64) take(some[j].x, (int)__float_as_uint(some[j].y));
+      __builtin_amdgcn_wave_barrier();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) take(x[i], s * kSegment + Segment<T>::index(i));
+    }
     if (st.k == 0) {
       const uint64_t all = wave_scan(sum);
       if ((threadIdx.x & 63) == 63) r.sums[s] = all;
@@ -539,6 +579,25 @@ __device__ __forceinline__ bool cut_place(const Weigher& weigh, SampleLds& lds, 
   return true;
 }
 
+// A thread's additions to sums in LDS: what follows in the same one is added up first, as equal logits do for four levels below (a row of
+// 151936 of them: 760 us a call, not 1110). Where sums change all the time, as in the other passes, it costs more than it saves.
+struct Sums {
+  uint64_t* to;
+  int entry = 0;
+  uint64_t sum = 0;
+  __device__ __forceinline__ void put() {
+    if (sum > 0) atomicAdd((unsigned long long*)&to[entry], (unsigned long long)sum);
+  }
+  __device__ __forceinline__ void add(int e, uint64_t w) {
+    if (e != entry) {
+      put();
+      entry = e;
+      sum = 0;
+    }
+    sum += w;
+  }
+};
+
 // The same whatever the bin holds, 8 bits of the place at a time.
 template <bool COUNT, typename Each, typename F>
 __device__ __forceinline__ uint64_t cut_bits(const Weigher& weigh, SampleLds& lds, int in, uint64_t base, uint64_t most, Each&& each, F&& enough) {
@@ -549,10 +608,12 @@ __device__ __forceinline__ uint64_t cut_bits(const Weigher& weigh, SampleLds& ld
     __syncthreads();
     lds.hist[threadIdx.x] = 0;
     __syncthreads();
+    Sums sums{lds.hist};
     each([&](uint64_t place, int bin, double rest) {
       if (bin == in && place <= most && (level == 0 || (place >> above) == (prefix >> above)))
-        atomicAdd((unsigned long long*)&lds.hist[(place >> shift) & 255], (unsigned long long)(COUNT ? 1 : weigh.weight(bin, rest)));
+        sums.add((int)(place >> shift) & 255, COUNT ? 1 : weigh.weight(bin, rest));
     });
+    sums.put();
     __syncthreads();
     prefix |= (uint64_t)cut_of(lds, kChoosers, base, enough) << shift;
   }
