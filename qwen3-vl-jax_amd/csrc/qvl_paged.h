@@ -5,8 +5,8 @@
 // they are; scales are applied to their sums (K) or to the weights (V) in fp32.
 //
 // A page holds `page_rows` tokens head by head, in blocks of 16 tokens. A block is laid out as the products' operands lie in the lanes
-// of a wave (a lane is row or column r = lane % 16 of an operand and quad = lane / 16), so that a lane's share of K, and of V, is one
-// load and neither passes through LDS:
+// of a wave (a lane is row or column r = lane % 16 of an operand and quad = lane / 16), so that a lane's share of K, and of V, is
+// one read:
 //   K       token by token: 8 pieces of D / 8 values; piece p holds the codes of dims [pE, pE + E) and [D/2 + pE, D/2 + pE + E),
 //           E = D / 16. The lane of token r takes pieces 2 quad and 2 quad + 1.
 //   V       [4 quads][16 r][4 tokens][D / 16 codes]: of tokens 4 quad + i the dims 4r + j and (D = 128) 64 + 4r + j, j < 4
