@@ -10,8 +10,8 @@
 // K and V come by DMA into a ring in LDS of each wave's own (Ring): the loop has no barrier. Codes become bf16 by one conversion for two of
 // them; V's are nibbles of one token in a row, and four bit operations turn 16 of two tokens into pairs.
 //
-// 96 sequences of 1 to 7900 keys, 32/8 heads of 128, bf16: 87 us and 5.5 for the join, 4.8 TB/s of cache; 24 instead of 12 sequences of
-// 32000 keys take 72 us more, 5.8 TB/s. One of 9001: 12.0 and 5.5 us, a chain of the state, a page's number, a tile, and the join.
+// 96 sequences of 1 to 7900 keys, 32/8 heads of 128, bf16: 85 us and 5.5 for the join, 4.9 TB/s of cache; 24 instead of 12 sequences of
+// 32000 keys take 72 us more, 5.8 TB/s. One of 9001: 11.6 and 5.5 us, a chain of the state, a page's number, a tile, and the join.
 // MFMA is busy 13 % of the time, VALU 43 %, and waves wait 57 % of theirs.
 //
 // fp32: q and the weights are split in three bf16 parts (24 bits); the codes are exact, so three products give the fp32 one.
