@@ -13,8 +13,8 @@
 //
 // Four launches, each over (share of the vocabulary, row) but the last, which is over rows: the largest logits, the histogram, the
 // list with the sums of segments of 1024 tokens, the choice. The logits are read three times where there is a cut, the second and third
-// time from a cache. 256 rows of 151936, fp32, by top-p: 35 us for the largest (4.5 TB/s), 46 for the histogram (30 instructions a logit, most
-// of them for its weight: 76 % of the units' time), 37 for the list, 13 for the choice. One row: 3.3 + 4.7 + 5.3 + 7.6 us; a row whose
+// time from a cache. 256 rows of 151936, fp32, by top-p: 33 us for the largest (4.7 TB/s), 46 for the histogram (30 instructions a logit, most
+// of them for its weight: 76 % of the units' time), 37 for the list, 13 for the choice. One row: 3.2 + 4.7 + 5.3 + 7.6 us; a row whose
 // cut goes over it again in the last launch 170 to 210.
 #include "qvl_decoder.h"
 #include "qvl_kernels.h"
@@ -282,19 +282,18 @@ __global__ __launch_bounds__(256) void sample_tops_kernel(SampleParams P, int pe
   for (int i = blockIdx.x * 256 + threadIdx.x; i < kBins; i += gridDim.x * 256) r.hist[i] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) r.n = 0;
   const int s0 = blockIdx.x * per, s1 = min(s0 + per, P.segments);
-  uint32_t key = ~0u;
-  int at = 0;
-  Walk<T, 256>(row, P.vocab, s0, s1).run([&](float x, int index) {
-    const uint32_t k = key_of(x);
-    if (k < key) {
-      key = k;
-      at = index;
+  Walk<T, 256>(row, P.vocab, s0, s1).segments([&](const float (&x)[16], int s) {
+    float most = -INFINITY;                  // (a lane of nothing more: whichever of its tokens, none can be chosen)
+    int at = 0;
+    bool wrong = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      wrong = wrong || x[i] != x[i];
+      at = x[i] > most ? i : at;
+      most = x[i] > most ? x[i] : most;
     }
-  }, [&](int s) {
-    const uint64_t m = wave_min((uint64_t)key << 32 | (uint32_t)at);
+    const uint64_t m = wave_min(place_of(wrong ? NAN : most, s * kSegment + Segment<T>::index(at)));
     if ((threadIdx.x & 63) == 0) r.tops[s] = m;
-    key = ~0u;
-    at = 0;
   });
 }
 
@@ -784,7 +783,8 @@ int qvl_sample_tokens(void* stream, int32_t dtype, const void* logits, int64_t r
   for (int64_t first = 0; first < n_rows; first += kRowsAtOnce) {
     const int64_t rows = std::min<int64_t>(n_rows - first, kRowsAtOnce);
     P.first = (int)first;
-    // a segment a wave, or as many as make some 2048 workgroups of four waves
+    // a segment a wave, or as many as make some 2048 workgroups of four waves: all that the GPU holds (256 rows: the three
+    // launches take 117 to 119 us, 117 with 1024 and 136 with 512)
     const int shares = (int)std::max<int64_t>(std::min<int64_t>((P.segments + 3) / 4, 2048 / rows), 1);
     const int per = (P.segments + shares - 1) / shares;
     const dim3 grid((unsigned)((P.segments + per - 1) / per), (unsigned)rows);
