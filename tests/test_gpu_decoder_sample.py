@@ -181,3 +181,17 @@ def test_out_and_streams(sample):
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
     assert sample(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("settings", [dict(top_p=0.6), dict(top_p=0.999), dict(top_k=1500), dict(top_k=2700, top_p=0.7), dict(top_p=0.9, min_p=0.5)])
+@pytest.mark.parametrize("unit", [1.0, 1e30, 1e-37])
+def test_cuts_that_leave_some_of_each_segment(sample, dtype, settings, unit):
+    """Segments of 1024 tokens of which from none to all reach the cut, also where logits and temperature are far from 1."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.full((9 * 1024 + 37,), -12.0)
+    for segment, left in enumerate((513, 0, 1, 64, 512, 65, 1024, 511, 63)):
+        at = segment * 1024 + torch.randperm(1024, generator=g)[:left]
+        x[at] = torch.rand(left, generator=g)
+    x = (x * unit).to(dtype).to(DEV)[None].repeat(24, 1)
+    check(sample, x, torch.rand(24, generator=g).to(DEV), temperature=unit, **settings)
