@@ -64,8 +64,9 @@ __device__ __forceinline__ Settings settings_of(const SampleParams& P, int64_t r
   s.p = P.top_p ? P.top_p[row] : P.top_p1;
   const double min_p = P.min_p ? P.min_p[row] : P.min_p1;
   s.k = max(P.top_k ? P.top_k[row] : P.top_k1, 0);
-  s.u = P.u[row];
-  if (!(s.u >= 0)) s.u = 0;
+  // (beyond 1: the largest double below it, whose product with any sum, rounded, stays below that sum: it is half to one unit of its last place less)
+  const double u = P.u[row];
+  s.u = u >= 0 ? min(u, 1 - 0x1p-53) : 0;
   s.nucleus = s.p < 1;
   s.floor = min_p > 0 ? (uint64_t)ceil(min(min_p, 2.0) * kUnit) : 0;
   // the first token in the order alone; elsewhere the rules keep it by themselves
@@ -717,10 +718,13 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
   }
   __syncthreads();
   // the segment whose kept weights reach u times all, and the token in it
+  if (i == 0) {
+    lds.n = 0;
+    lds.found[0] = 0;
+  }
   uint64_t total;
   const uint64_t own = i < P.segments ? lds.sums[i] : 0, upto = block_scan<NT>(own, lds.waves, total);
-  double t = st.u * (double)total;
-  if (!(t < (double)total)) t = (double)(total - 1);
+  const double t = st.u * (double)total;
   if ((double)upto > t && !((double)(upto - own) > t)) {
     lds.n = i;
     lds.found[0] = upto - own;

@@ -195,3 +195,26 @@ def test_cuts_that_leave_some_of_each_segment(sample, dtype, settings, unit):
         x[at] = torch.rand(left, generator=g)
     x = (x * unit).to(dtype).to(DEV)[None].repeat(24, 1)
     check(sample, x, torch.rand(24, generator=g).to(DEV), temperature=unit, **settings)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [513, 600, 3001, 151936, 262144])
+@pytest.mark.parametrize("spread", [0.0, 0.01])
+def test_random_numbers_of_one_and_more_on_flat_rows(sample, dtype, vocab, spread):
+    """What is not below 1 counts as just below it, and takes the kept token of the highest index, also where the weights' sum is far
+    beyond 2^53 (512 equal tokens reach it) and one less than it is the same double."""
+    x, _ = logits(1, vocab, dtype, vocab, spread)
+    row = x[0].double().cpu().numpy()
+    order = np.lexsort((np.arange(vocab), -row))
+    w = [int(v) for v in np.rint(np.exp(row - row.max()) * 2.0 ** 44)]   # (Python's integers: sums up to 2^62)
+    for settings in (dict(), dict(top_p=0.9), dict(top_k=511), dict(min_p=0.5), dict(top_k=vocab // 2 + 1, top_p=0.75), dict(top_p=0.5, min_p=0.25)):
+        kept = order[:settings.get("top_k", vocab)].tolist()
+        if "top_p" in settings:
+            whole, upto, n = sum(w[i] for i in kept), 0, 0
+            while n < len(kept) and upto < float(np.float32(settings["top_p"])) * whole:
+                upto += w[kept[n]]
+                n += 1
+            kept = kept[:n]
+        u = torch.tensor([1.0, 7.0, float("inf"), 0.0, -1.0, float("nan")], device=DEV)
+        got = sample(x.expand(6, vocab), u, **settings).tolist()
+        assert got == [max(kept)] * 3 + [min(kept)] * 3, settings
