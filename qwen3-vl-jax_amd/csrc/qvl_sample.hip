@@ -746,7 +746,8 @@ __global__ __launch_bounds__(kChoosers) void sample_choose_kernel(SampleParams P
   if (w[0] > 0 && (double)(second - w[1]) > t) atomicMin(&lds.token, index);
   else if (w[1] > 0 && (double)second > t) atomicMin(&lds.token, index + 1);
   __syncthreads();
-  if (i == 0) *out = lds.token;
+  // (were no weight kept, the first place: whoever looks the token up finds one)
+  if (i == 0) *out = lds.token != 0x7fffffff ? lds.token : (int64_t)(uint32_t)first;
 }
 
 }  // namespace qvl

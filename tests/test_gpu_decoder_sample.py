@@ -1,4 +1,6 @@
 """GPU tests of sample_tokens against a plain form in float64 and whole numbers."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -218,3 +220,40 @@ def test_random_numbers_of_one_and_more_on_flat_rows(sample, dtype, vocab, sprea
         u = torch.tensor([1.0, 7.0, float("inf"), 0.0, -1.0, float("nan")], device=DEV)
         got = sample(x.expand(6, vocab), u, **settings).tolist()
         assert got == [max(kept)] * 3 + [min(kept)] * 3, settings
+
+
+def on_borders(temperature, count, seed):
+    """(top, x) of float32 whose distance in 32nds of a power of two, (top - x) 32 / (T ln 2), lies between two whole numbers: in the middle
+    once the product is rounded, a little to one side of it before, and so that the two would come to different ones."""
+    rng, found = np.random.default_rng(seed), []
+    scale = np.float64(32 / 0.69314718055994530942) / np.float64(np.float32(temperature))
+    while len(found) < count:
+        half = int(rng.integers(1, 500)) + 0.5
+        top = np.float32(half / scale)
+        x = np.float32(np.float64(top) - half / scale)
+        d = np.float64(top) - np.float64(x)
+        side = Fraction(float(d)) * Fraction(float(scale)) - Fraction(half)
+        if x != 0 and d * scale == half and side != 0 and np.rint(half) != half + (0.5 if side > 0 else -0.5):
+            found.append((float(top), float(x)))
+    return found
+
+
+def border_rows(temperature, copies, seed):
+    """Rows of one top, `copies` tokens at its border and lower ones, in any order, and a top-p that falls among the copies."""
+    rng, rows, top_p = np.random.default_rng(seed), [], []
+    for top, x in on_borders(temperature, 24, seed):
+        row = np.concatenate([[top], np.full(copies, x), top - 16.5 * temperature - rng.random(40)])
+        rows.append(row[rng.permutation(len(row))])
+        w = np.exp((x - top) / temperature) * copies
+        top_p.append((1 + w * 0.55) / (1 + w))
+    return torch.tensor(np.array(rows), dtype=F32, device=DEV), torch.tensor(top_p, dtype=F32, device=DEV)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 2.0])
+@pytest.mark.parametrize("copies", [1, 3, 200, 5000])
+def test_no_token_outside_the_vocabulary(sample, temperature, copies):
+    x, top_p = border_rows(temperature, copies, 3)
+    for u in (0.0, 0.5, 0.99, 1.0):
+        for settings in (dict(top_p=top_p), dict(top_k=1 + (copies + 1) // 2), dict(top_k=2 + copies, top_p=top_p)):
+            got = sample(x, torch.full((len(x),), u, device=DEV), temperature=temperature, **settings)
+            assert int(got.min()) >= 0 and int(got.max()) < x.shape[1]
