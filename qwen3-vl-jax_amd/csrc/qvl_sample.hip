@@ -109,10 +109,11 @@ struct Weigher {
   double top, scale;                         // 32 / (T ln 2)
   const double* table;                       // LDS: 2^(44 - j / 32)
   // The bin is y to the nearest whole number, which the sum with 3 2^51 leaves in its low bits: a conversion takes four times an
-  // addition's time. Products and sums are joined by hand, so that every pass over the row comes to the same bins and weights.
+  // addition's time. Products and sums are joined by hand, so that every pass over the row comes to the same bins and weights: left to the
+  // compiler, one pass rounded the product before the sum and the next did not, and a token on a bin's border was in two of them or in none.
   __device__ __forceinline__ bool bin_of(float x, int& bin, double& rest) const {
     const double d = top - (double)x, y = d * scale;
-    const double whole = y + 0x1.8p52;
+    const double whole = __builtin_fma(d, scale, 0x1.8p52);
     bin = (int)__double2loint(whole);
     rest = __builtin_fma(d, scale, -(whole - 0x1.8p52));
     return y < kBins - 1;

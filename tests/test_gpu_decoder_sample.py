@@ -257,3 +257,16 @@ def test_no_token_outside_the_vocabulary(sample, temperature, copies):
         for settings in (dict(top_p=top_p), dict(top_k=1 + (copies + 1) // 2), dict(top_k=2 + copies, top_p=top_p)):
             got = sample(x, torch.full((len(x),), u, device=DEV), temperature=temperature, **settings)
             assert int(got.min()) >= 0 and int(got.max()) < x.shape[1]
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 2.0])
+@pytest.mark.parametrize("copies", [1, 3, 200, 5000])
+def test_logits_on_the_border_of_two_bins(sample, temperature, copies):
+    """Every pass over a row has to come to the same bin, or tokens at the cut are lost or counted twice."""
+    x, top_p = border_rows(temperature, copies, 3)
+    for u in (0.02, 0.47, 0.73, 0.9, 0.97):
+        us = torch.full((len(x),), u, device=DEV)
+        for settings in (dict(top_p=top_p), dict(top_k=1 + (copies + 1) // 2), dict(top_k=2 + copies, top_p=top_p), dict(top_p=0.999, min_p=1e-5)):
+            check(sample, x, us, temperature=temperature, **settings)
+    pair = torch.tensor([[1.7003766, -4.748171e-08]], device=DEV)        # 78 and a half, 5e-15 more
+    check(sample, pair, torch.tensor([0.97], device=DEV), top_p=0.9)
