@@ -38,8 +38,6 @@ class PagedCache:
         self.page_bytes = nb.value // self.n_pages if self.n_pages else 0
         torch = _torch()
         self._data = torch.zeros((self.n_pages, self.page_bytes), dtype=torch.uint8, device=_device(device))
-        self._where = self._data.device
-        self._args = (self._data.data_ptr(), self.n_pages, self.page_rows)
 
     @property
     def data(self):
@@ -49,8 +47,11 @@ class PagedCache:
 def _pages(cache: PagedCache, page_table, k_len, like, heads: Optional[int] = None):
     """The cache, the page table and the sequences' lengths as the entries take them: (cache and table arguments, number of
     sequences, k_len's pointer)."""
-    if cache._where != like[1]:
-        raise ValueError(f"the cache on {cache._where}, q on {like[1]}")
+    data = cache._data
+    if data.device != like[1]:
+        raise ValueError(f"the cache on {data.device}, q on {like[1]}")
+    if data.shape != (cache.n_pages, cache.page_bytes) or not data.is_contiguous():
+        raise ValueError(f"the cache's data {tuple(data.shape)} is not its {cache.n_pages} pages of {cache.page_bytes} bytes any more")
     if like[2] != cache.head_dim:
         raise ValueError(f"head_dim {like[2]}, the cache has {cache.head_dim}")
     if heads is not None and heads != cache.num_kv_heads:
@@ -64,7 +65,9 @@ def _pages(cache: PagedCache, page_table, k_len, like, heads: Optional[int] = No
     if page_table.device != like[1]:
         raise ValueError(f"page_table on {page_table.device}, q on {like[1]}")
     n = shape[0]
-    return ((*cache._args, page_table.data_ptr(), shape[1], stride[0] if n > 1 else 0), n, _word(k_len, "k_len", like, int32, (n,)))
+    # (data's address with every call: a copy of the cache has pages of its own)
+    return ((data.data_ptr(), cache.n_pages, cache.page_rows, page_table.data_ptr(), shape[1], stride[0] if n > 1 else 0), n,
+            _word(k_len, "k_len", like, int32, (n,)))
 
 
 def _cu(cu_q, like, n_seqs: int, n_tokens: int):

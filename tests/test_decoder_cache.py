@@ -257,3 +257,38 @@ def test_sample_host_refusals(ops, pkg):
             (lambda: s(x, u, out=torch.zeros(2)), TypeError), (lambda: s(x, u, out=torch.zeros(3, dtype=torch.int64)), ValueError)]:
         with pytest.raises(error):
             call()
+
+
+def test_copies_of_a_cache_have_pages_of_their_own(ops):
+    """Deep copies, pickled ones and a cache whose data got other memory: every call takes the address that data has then."""
+    import copy
+    import pickle
+    c, (table, lens) = cache_of(ops), state()
+    q, k = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
+    where = {"qvl_paged_append": 17, "qvl_paged_attention": 5, "qvl_paged_unpack": 2}    # the cache among the arguments
+
+    def addresses(c):
+        ops.calls.clear()
+        ops.append_paged(k, k, c, table, lens)
+        ops.paged_attention(q, c, table, lens, max_len=1)
+        ops.unpack_paged(c, table, lens, torch.zeros(3, dtype=torch.int64), k.clone(), k.clone(), max_len=1)
+        assert [name for name, _ in ops.calls] == list(where)
+        return {a[where[name]] for name, a in ops.calls}
+
+    others = [c, copy.deepcopy(c), pickle.loads(pickle.dumps(c))]
+    for x in others:
+        assert addresses(x) == {x.data.data_ptr()}
+    assert len({x.data.data_ptr() for x in others}) == 3
+    assert addresses(copy.copy(c)) == {c.data.data_ptr()}                # (a shallow copy is the same pages)
+    c.data.data = c.data.clone()
+    assert addresses(c) == {c.data.data_ptr()}
+
+
+def test_data_that_is_not_the_caches_pages_is_refused(ops):
+    table, lens = state()
+    k = torch.zeros(3, 2, 64)
+    for other in (lambda d: d[:3], lambda d: d.reshape(-1), lambda d: d.t().contiguous().t(), lambda d: d[:, :64].contiguous()):
+        c = cache_of(ops)
+        c.data.data = other(c.data)
+        with pytest.raises(ValueError, match="pages"):
+            ops.append_paged(k, k, c, table, lens)

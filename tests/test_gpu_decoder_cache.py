@@ -568,3 +568,16 @@ def test_prompts_then_tokens(ops, pkg, dtype):
             assert_attention(out[i:i + 1], attention_ref(qr[i:i + 1], k32[a:b], v32[a:b], word([lens[i]]), D ** -0.5), lens[i])
         token = choose(out, 1 + step)
     choose(prompt([lens[0] + 1, lens[1] + 30], [1, 30], torch.cat([token[:1], torch.arange(30, device=DEV)])), 9)
+
+
+def test_a_copied_cache_is_written_and_read_alone(ops):
+    import copy
+    chats, k, v = filled(ops, [40, 7], 16, 2, 64, seed=11)
+    q = rand((2, 4, 64), BF, 9, 1.4)
+    attend = lambda cache: ops.paged_attention(q, cache, chats.table, chats.k_len, max_len=40)
+    before, out = chats.cache.data.clone(), attend(chats.cache)
+    other = copy.deepcopy(chats.cache)
+    assert torch.equal(bits(attend(other)), bits(out))
+    ops.append_paged(rand((47, 2, 64), BF, 3), rand((47, 2, 64), BF, 4), other, chats.table, chats.k_len, cu_q=word([0, 40, 47]))
+    assert torch.equal(chats.cache.data, before) and not torch.equal(other.data, before)
+    assert torch.equal(bits(attend(chats.cache)), bits(out)) and not torch.equal(bits(attend(other)), bits(out))
