@@ -327,17 +327,17 @@ __global__ __launch_bounds__(256) void paged_unpack_kernel(Pages pages, const in
   constexpr int E = D / 16;
   const int lane = threadIdx.x & 63, p = lane & 7, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.y, seq = blockIdx.z;
-  const int64_t first = first_ ? max(first_[seq], 0) : 0, row0 = k_start[seq];
-  // tokens whose rows lie in [0, out_rows)
-  if (row0 >= out_rows || row0 < -(int64_t)0x7fffffff) return;
-  const int64_t from = first + max(-row0, (int64_t)0), end = min((int64_t)k_len[seq], first + out_rows - row0);
+  const int64_t first = first_ ? first_[seq] : 0, row0 = k_start[seq];
+  // tokens whose rows lie in [0, out_rows); token t's is t + shift (first and t have 32 bits)
+  if (row0 >= out_rows || row0 < -((int64_t)1 << 32)) return;
+  const int64_t shift = row0 - first, from = max(max(first, (int64_t)0), -shift), end = min((int64_t)k_len[seq], out_rows - shift);
   for (int64_t b = (from >> 4) + blockIdx.x * 4 + wave; b * 16 < end; b += gridDim.x * 4) {
     const int page = pages.page(seq, b >> (pages.shift - 4));
     const char* block = pages.block<D>(max(page, 0), h, (int)(b << 4));
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int token = half * 8 + (lane >> 3);
-      const int64_t t = b * 16 + token, row = row0 + t - first;
+      const int64_t t = b * 16 + token, row = t + shift;
       if (t < from || t >= end) continue;
       uint32_t codes[2][2] = {}, scales[2] = {0x7fc07fc0u, 0x7fc07fc0u};   // [k, v][lo, hi]; a page of none: NaN
       if (page < 0) {

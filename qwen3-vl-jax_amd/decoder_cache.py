@@ -147,7 +147,8 @@ def append_paged(k, v, cache: PagedCache, page_table, k_len, *, cu_q=None):
 
 def unpack_paged(cache: PagedCache, page_table, k_len, k_start, k, v, *, max_len: int, first=None):
     """The keys and values that pages stand for, as rows of k and v [R, Hkv, D]: tokens first[i] (int32; None: 0) to k_len[i] of
-    sequence i from row k_start[i] (int64) on, rounded to their dtype once. Rows outside [0, R) are dropped, tokens in no page are NaN.
+    sequence i, token t as row k_start[i] + t - first[i] (k_start int64; of a negative first the tokens before 0 are none), rounded to
+    their dtype once. Rows outside [0, R) are dropped, tokens in no page are NaN.
     max_len, the most tokens of a sequence, only lays the launch out. Returns (k, v)."""
     torch = _torch()
     like = _like(k)

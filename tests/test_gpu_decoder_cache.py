@@ -581,3 +581,27 @@ def test_a_copied_cache_is_written_and_read_alone(ops):
     ops.append_paged(rand((47, 2, 64), BF, 3), rand((47, 2, 64), BF, 4), other, chats.table, chats.k_len, cu_q=word([0, 40, 47]))
     assert torch.equal(chats.cache.data, before) and not torch.equal(other.data, before)
     assert torch.equal(bits(attend(chats.cache)), bits(out)) and not torch.equal(bits(attend(other)), bits(out))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_unpack_from_before_a_sequence(ops, dtype):
+    """A negative first counts rows as any other does: token t's row is k_start + t - first, and tokens before 0 are none."""
+    hkv, D, lengths = 2, 64, [20, 33, 5, 40]
+    chats = Chats(ops, lengths, 16, hkv, D, seed=12)
+    chats.fill(rand((98, hkv, D), F32, 1), rand((98, hkv, D), F32, 2))
+    want = chats.rows(dtype)
+    first, start, R = [-3, -17, -(2 ** 31), 2], [0, 10, -(2 ** 31) + 70, 80], 110
+    for hint in (1, 40):
+        got = [torch.full((R, hkv, D), 5.0, dtype=dtype, device=DEV) for _ in range(2)]
+        ops.unpack_paged(chats.cache, chats.table, chats.k_len, word(start, torch.int64), *got, max_len=hint, first=word(first))
+        for x, w in zip(got, want):
+            ref = torch.full((R, hkv, D), 5.0, dtype=dtype, device=DEV)
+            ref[3:23] = w[:20]
+            ref[27:60] = w[20:53]
+            ref[70:75] = w[53:58]
+            ref[80:110] = w[58 + 2:58 + 32]
+            assert torch.equal(bits(x), bits(ref))
+    far = [torch.full((R, hkv, D), 5.0, dtype=dtype, device=DEV) for _ in range(2)]   # rows all before 0, or all behind the last
+    ops.unpack_paged(chats.cache, chats.table, chats.k_len, word([-60, -2 ** 62, 2 ** 62, R - 2], torch.int64), *far, max_len=40,
+                     first=word([-3, -(2 ** 31), -(2 ** 31), -3]))
+    assert all(bool((x == 5).all()) for x in far)
