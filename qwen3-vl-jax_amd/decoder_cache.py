@@ -128,7 +128,9 @@ def qk_norm_rotary_paged(q, k, v, q_norm, k_norm, positions, rotary: TextRotary,
 
 def append_paged(k, v, cache: PagedCache, page_table, k_len, *, cu_q=None):
     """Keys and values [N, Hkv, D] of new tokens into their pages as they are (a prefill's, rotated already, or those of a cache of
-    rows); the sequences' state as in `qk_norm_rotary_paged`. Values that `unpack_paged` gave in float32 come back bit for bit."""
+    rows); the sequences' state as in `qk_norm_rotary_paged`. Values that `unpack_paged` gave in float32 come back bit
+    for bit where a group's scale is 0, NaN or a normal number (2^-126 on) and six times it a float32: not for groups whose largest value is
+    under 6 2^-126 or over 3.38e38, which may come out as other multiples, zeros or, from the top, infinities that come back as NaN."""
     like = _like(k)
     N, Hkv, D = k.shape
     kv, vv = _heads_view(k, "k", like), _heads_view(v, "v", like, Hkv)

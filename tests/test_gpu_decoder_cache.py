@@ -605,3 +605,34 @@ def test_unpack_from_before_a_sequence(ops, dtype):
     ops.unpack_paged(chats.cache, chats.table, chats.k_len, word([-60, -2 ** 62, 2 ** 62, R - 2], torch.int64), *far, max_len=40,
                      first=word([-3, -(2 ** 31), -(2 ** 31), -3]))
     assert all(bool((x == 5).all()) for x in far)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_was_read_back_comes_back_at_the_ends_of_the_range(ops, D):
+    """Float32 values that pages stand for, appended again, come back from the smallest normal scale to the last whose sixfold is
+    a float32; zeros and NaN too. Beyond, groups stand for what the formula says, and the header promises no more."""
+    low, high = 2.0 ** -126, torch.tensor(0x7e2a, dtype=torch.int16).view(BF).double().item()   # the next bf16 above: 6 s > 2^128
+    assert 6 * high < torch.finfo(F32).max < 6 * high * (1 + 2.0 ** -7)
+    tops = [6 * low, 6 * low * (1 - 2.0 ** -10), 6 * low * 1.5, 6 * low * (1 + 2.0 ** -7), 6 * high, 6 * high * (1 - 2.0 ** -10), 3 * high, 0.0,
+            float("nan")]
+    x = rand((len(tops), 2, D), F32, 13).double().clamp(-1, 1)
+    x[:, :, ::64] = 1.0
+    x = (x * torch.tensor(tops, dtype=torch.float64, device=DEV)[:, None, None]).float()
+    chats = Chats(ops, [len(tops)], 16, 2, D)
+    chats.fill(x, -x)
+    k, v = chats.rows()
+    want = packed(x)[0]
+    assert torch.equal(k.double().nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(k.isnan(), want.isnan())
+    assert torch.equal(bits(v[:-1]), bits(-k[:-1])) and bool(k[:-1].isfinite().all())
+    chats.fill(k, v)
+    for again, x in zip(chats.rows(), (k, v)):
+        assert torch.equal(bits(again[:-1]), bits(x[:-1])) and bool(again[-1].isnan().all())
+    # the ends beyond: 3e-40 has a scale of the smallest subnormal, half of which is a tie; 3.4e38 rounds up to a scale whose sixfold is none
+    y = torch.tensor([3e-40, 3.4e38], device=DEV)[:, None, None].expand(2, 2, D).contiguous()
+    far = Chats(ops, [2], 16, 2, D)
+    far.fill(y, y)
+    k, v = far.rows()
+    assert torch.equal(k[0].double(), packed(y[:1])[0][0]) and bool((k[1] == float("inf")).all())
+    far.fill(k, v)
+    k, v = far.rows()
+    assert bool((k[0] == 0).all()) and bool(k[1].isnan().all())
