@@ -636,3 +636,17 @@ def test_what_was_read_back_comes_back_at_the_ends_of_the_range(ops, D):
     far.fill(k, v)
     k, v = far.rows()
     assert bool((k[0] == 0).all()) and bool(k[1].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("hq,hkv,D,new", [(8, 2, 128, 1), (8, 2, 64, 3)])
+@pytest.mark.parametrize("n,at", [(65, 64), (257, 100), (1100, 0)])
+def test_many_sequences_of_which_one_is_long(ops, dtype, hq, hkv, D, new, n, at):
+    """More sequences than lanes, than threads, than either: jobs that stay whole beside one that is cut over many runs."""
+    lengths = [new + (29 * i) % 150 for i in range(n)]
+    lengths[at] = 5000
+    chats, k, v = filled(ops, lengths, 32, hkv, D, [new] * n, seed=14)
+    q = rand((n * new, hq, D), dtype, 9, 1.4)
+    out = ops.paged_attention(q, chats.cache, chats.table, chats.k_len, max_len=5000, cu_q=chats.cu_q)
+    check_attention(out, chats, q, k, v, D ** -0.5)
+    assert torch.equal(bits(ops.paged_attention(q, chats.cache, chats.table, chats.k_len, max_len=5000, cu_q=chats.cu_q)), bits(out))
