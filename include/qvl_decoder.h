@@ -120,7 +120,8 @@ int qvl_decode_attention(void* stream, int32_t dtype,
  * x the scale is s = bf16(fp32(max|x| / 6)) (rounded to nearest even, twice) and each value becomes the number nearest to |x| / s of 0,
  * .5, 1, 1.5, 2, 3, 4, 6 (a tie goes to 0, 1, 2 or 4) with x's sign, and stands for s times it. A group with a NaN or an infinity, or whose
  * scale is beyond bf16, stands for NaN. What a group stands for in fp32 gives the same group again where s is 0, NaN or normal and 6 s
- * finite (a subnormal s has few bits, and 6 s of values over 3.38e38 may be beyond fp32). The bytes of a page are this library's own; qvl_paged_cache_size tells how many a cache of
+ * finite (a subnormal s has few bits, and 6 s of values over 3.399e38 may be beyond fp32).
+ * The bytes of a page are this library's own; qvl_paged_cache_size tells how many a cache of
  * n_pages takes (64-byte aligned; any content until tokens are written).
  * Token t of sequence i lies in page d_page_table[i * table_stride + t / page_rows], slot t % page_rows. Sequences may share pages.
  * An entry outside [0, n_pages) is no page: what would be written there is dropped, what would be read there is NaN. */

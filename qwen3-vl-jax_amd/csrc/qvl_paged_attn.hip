@@ -545,8 +545,9 @@ int qvl_paged_attention(void* stream, int32_t dtype, const void* q, int64_t q_ro
   S.slot_rows = plan.slot_rows;
   S.tile = plan.tile;
   S.shift = plan.tile == 4 ? 6 : 5;
-  // what a job costs beside its keys (rows, first loads, join), and jobs that are not worth a part: 96 sequences of up to 7900 keys
-  // 93 us, not 122 without either
+  // what a job costs beside its keys (rows, first loads, join), and jobs that are not worth a part, in blocks: 96 sequences of up to 7900 keys
+  // 93 us, not 122 without either. Found there alone, with bf16, heads of 128 and blocks of 64 keys; with blocks of 32, heads of 64 or fp32's
+  // three products a block is another share of a job's cost, and the same counts stand unmeasured.
   S.pad = 12;
   S.keep = 24;
   const dim3 grid((unsigned)(plan.runs * num_kv_heads));

@@ -3,8 +3,8 @@
 //
 // A group x of 64 values: s = bf16(fp32(max|x| / 6)), and for each value the number nearest to |x| / s; a tie goes to the even code. A
 // code is a step function: an error of one rounding next to a border moves it by a whole step. So it is decided exactly for a value that
-// is stored as it came, and a normalised and rotated key is formed in fp64 (sines and cosines too), so that what the cache holds does
-// not depend on the order of a sum. fp64 runs at fp32's rate here, and only keys need it.
+// is stored as it came, and a normalised and rotated key is formed in fp64 (sines and cosines too), so that the order of a sum can move only
+// what lies within some 1e-15 of a border. fp64 runs at fp32's rate here, and only keys need it.
 //
 // Each value is read once, q and 4.25 bits a value of k and v are written; what keeps it from the copy's rate is the keys' fp64 (88
 // registers: 5 waves a SIMD) and the lookup of the place before the stores. 18011 tokens of 32 + 8 + 8 heads of 128, bf16: 105 us, 3.7 TB/s

@@ -82,8 +82,9 @@ def qk_norm_rotary_paged(q, k, v, q_norm, k_norm, positions, rotary: TextRotary,
                          eps: float = 1e-6, cu_q=None, q_out=None):
     """`decoder_attn.qk_norm_rotary` with keys and values to pages: sequence i's new tokens (one, token i; or tokens
     cu_q[i]..cu_q[i+1], int32 [n + 1]) are the last of its k_len[i] (int32). Returns q; q_out, if given, takes it (it may be q
-    itself). A token whose place is in no page is dropped, one of no sequence leaves its row of q_out as it is. What the pages
-    hold of a key does not depend on how sums are ordered: it is normalised, rotated and brought to 4 bits in float64."""
+    itself). A token whose place is in no page is dropped, one of no sequence leaves its row of q_out as it is. A key is
+    normalised, rotated and brought to 4 bits in float64: another order of a sum could move a code only where the quotient lies within some
+    1e-15 of a border between two."""
     torch = _torch()
     like = _like(q)
     N, Hq, D = q.shape
@@ -130,7 +131,7 @@ def append_paged(k, v, cache: PagedCache, page_table, k_len, *, cu_q=None):
     """Keys and values [N, Hkv, D] of new tokens into their pages as they are (a prefill's, rotated already, or those of a cache of
     rows); the sequences' state as in `qk_norm_rotary_paged`. Values that `unpack_paged` gave in float32 come back bit
     for bit where a group's scale is 0, NaN or a normal number (2^-126 on) and six times it a float32: not for groups whose largest value is
-    under 6 2^-126 or over 3.38e38, which may come out as other multiples, zeros or, from the top, infinities that come back as NaN."""
+    under 6 2^-126 or over 3.399e38, which may come back as other multiples, zeros or, from infinities at the top, NaN."""
     like = _like(k)
     N, Hkv, D = k.shape
     kv, vv = _heads_view(k, "k", like), _heads_view(v, "v", like, Hkv)

@@ -45,12 +45,12 @@ def _sample_bytes(rows: int) -> int:
 
 def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     """The next token (int64 [B]) of each row of logits [B, V] (float32 or bfloat16, contiguous rows, V up to 2^18), by its random
-    number u [B] (float32, uniform in [0, 1)). With z = (x - max x) / temperature a token weighs e^z, as a whole number of 2^-44. In the
-    order of falling logits (equal ones: rising index) the first top_k are kept (0: all), of them those before which less than
-    top_p of their sum lies (1: all), of them those of at least min_p times the largest weight (0: all). The token is the first whose
-    sum of kept weights up to it, by index, is over u times their whole sum. Temperature 0: the largest logit, of the lowest index.
-    Tokens of -infinity are never chosen; a row of them alone, or with a NaN or +infinity, gives -1. Each setting is a number, or a
-    tensor [B] beside the logits (float32; top_k int32)."""
+    number u [B] (float32, uniform in [0, 1); others, and NaN, count as 0 or as just below 1). With z = (x - max x) / temperature a
+    token weighs e^z, as a whole number of 2^-44. In the order of falling logits (equal ones: rising index) the first top_k are kept
+    (0: all), of them those before which less than top_p of their sum lies (1: all), of them those of at least min_p times the largest
+    weight (0: all). The token is the first whose sum of kept weights up to it, by index, is over u times their whole sum.
+    Temperature 0: the largest logit, of the lowest index. Tokens of -infinity are never chosen; a row of them alone, or with a NaN or
+    +infinity, gives -1. Each setting is a number, or a tensor [B] beside the logits (float32; top_k int32)."""
     torch = _torch()
     if len(logits.shape) != 2:
         raise ValueError(f"logits must be [rows, vocab], not {tuple(logits.shape)}")
